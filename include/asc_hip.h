@@ -437,6 +437,52 @@ int32_t asc_flash_attention_dispatch(const void* q, const void* k, const void* v
                                      int32_t head_dim, float sm_scale,
                                      int32_t causal, asc_launch_plan_t* plan);
 
+/* ---- rotary positions, and norms of queries and keys with them -------------------
+ * No reference function exists; the build defines these next to its attention.
+ * Rows of one head and token, head_dim values in a row, at
+ * data + batch * batch_stride + head * head_stride + token * seq_stride (element
+ * counts; the last dimension is contiguous). */
+typedef struct asc_rows {
+  void* data;
+  int64_t batch_stride, head_stride, seq_stride;
+} asc_rows_t;
+
+/* Pair i of the first rotary_dim values, columns (i, i + rotary_dim / 2) or,
+ * interleaved, (2 i, 2 i + 1), turns by t = position * freqs[i]:
+ *   (a, b) -> magnitude * (a cos t - b sin t, b cos t + a sin t);
+ * the columns behind them stay as they are.  The angle is taken in fp64.
+ * asc_rotary            q_out = turn(q), k_out = turn(k); backward != 0: the
+ *                       gradient, the turn by -t times magnitude.
+ * asc_qk_norm_rotary    each row x normed first: y = x w / sqrt(mean(x^2) +
+ *                       epsilon), w = q_weight or k_weight (fp32 [head_dim]).
+ * asc_qk_norm_rotary_bwd  its gradient: q and k of the forward pass, dq_out and
+ *                       dk_out the results' gradients; writes dq to q_out, dk to
+ *                       k_out and the weights' gradients (fp32 [head_dim], summed
+ *                       over all rows in a fixed order) to dq_weight, dk_weight.
+ *                       `workspace` holds asc_qk_norm_rotary_bwd_workspace bytes.
+ * dtype: ASC_DT_FLOAT32 / FLOAT16 / BFLOAT16; computed in fp32, one rounding per
+ * value.  head_dim even and at most 512.  k_heads (or q_heads) may be 0.  A result
+ * may lie in place of an input with the same strides, and nowhere else over one. */
+typedef struct asc_rotary {
+  int32_t dtype, head_dim, rotary_dim, interleaved, backward;
+  int32_t positions_int64; /* positions are int64_t (else int32_t) */
+  float magnitude, epsilon;
+  int64_t batch, q_heads, k_heads, seq;
+  asc_rows_t q, k, q_out, k_out, dq_out, dk_out;
+  const void* positions; /* of token s of sequence b: [b * batch_stride + s * seq_stride] */
+  int64_t position_batch_stride, position_seq_stride;
+  const double* freqs; /* [rotary_dim / 2] */
+  const float* q_weight;
+  const float* k_weight;
+  float* dq_weight;
+  float* dk_weight;
+} asc_rotary_t;
+int32_t asc_rotary(const asc_rotary_t* args, asc_stream_t stream);
+int32_t asc_qk_norm_rotary(const asc_rotary_t* args, asc_stream_t stream);
+int64_t asc_qk_norm_rotary_bwd_workspace(const asc_rotary_t* args);
+int32_t asc_qk_norm_rotary_bwd(const asc_rotary_t* args, void* workspace,
+                               int64_t workspace_bytes, asc_stream_t stream);
+
 /* ---- element-wise tile operations ------------------------------------------------
  * The generic kernels of the reference's operation tests, one op per launch:
  *   unary   kernel(x_ptr, z_ptr, block_length, op)

@@ -51,8 +51,23 @@ class LaunchPlan(ctypes.Structure):
         return ctypes.string_at(ctypes.addressof(self.args), self.args_size)
 
 
+class Rows(ctypes.Structure):
+    """asc_rows_t: [batch, heads, seq, head_dim] rows, the last dimension contiguous."""
+    _fields_ = [("data", _c_p), ("batch_stride", _c_i64), ("head_stride", _c_i64), ("seq_stride", _c_i64)]
+
+
+class RotaryArgs(ctypes.Structure):
+    """asc_rotary_t."""
+    _fields_ = [("dtype", _c_i32), ("head_dim", _c_i32), ("rotary_dim", _c_i32), ("interleaved", _c_i32),
+                ("backward", _c_i32), ("positions_int64", _c_i32), ("magnitude", _c_f32), ("epsilon", _c_f32),
+                ("batch", _c_i64), ("q_heads", _c_i64), ("k_heads", _c_i64), ("seq", _c_i64),
+                ("q", Rows), ("k", Rows), ("q_out", Rows), ("k_out", Rows), ("dq_out", Rows), ("dk_out", Rows),
+                ("positions", _c_p), ("position_batch_stride", _c_i64), ("position_seq_stride", _c_i64),
+                ("freqs", _c_p), ("q_weight", _c_p), ("k_weight", _c_p), ("dq_weight", _c_p), ("dk_weight", _c_p)]
+
+
 # name -> argtypes; every entry point returns int32_t (asc_reduce_f32_workspace a byte
-# count, the others a status).
+# count, the others a status), those of INT64_FUNCS an int64_t byte count.
 SIGNATURES = {
     "asc_device_info": [_c_i32, ctypes.POINTER(_c_i32), ctypes.POINTER(_c_i32), ctypes.POINTER(_c_i32),
                         ctypes.c_char_p],
@@ -97,6 +112,10 @@ SIGNATURES = {
     "asc_matmul_i8_dispatch": [_c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32,
                                ctypes.POINTER(LaunchPlan)],
     "asc_matmul_i8_plan": [_c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, ctypes.POINTER(LaunchPlan)],
+    "asc_rotary": [ctypes.POINTER(RotaryArgs), _c_p],
+    "asc_qk_norm_rotary": [ctypes.POINTER(RotaryArgs), _c_p],
+    "asc_qk_norm_rotary_bwd_workspace": [ctypes.POINTER(RotaryArgs)],
+    "asc_qk_norm_rotary_bwd": [ctypes.POINTER(RotaryArgs), _c_p, _c_i64, _c_p],
     "asc_unary_f32": [_c_i32, _c_p, _c_p, _c_i64, _c_p],
     "asc_binary": [_c_i32, _c_i32, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_f64, _c_i64, _c_p],
     "asc_where_cmp": [_c_i32, _c_i32, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_f64, _c_i64, _c_f64, _c_f64, _c_p],
@@ -109,6 +128,7 @@ SIGNATURES = {
     "asc_transpose_batched": [_c_i32, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p],
     "asc_quant_i8": [_c_i32, _c_p, _c_p, _c_f64, _c_f64, _c_i64, _c_p],
 }
+INT64_FUNCS = ("asc_qk_norm_rotary_bwd_workspace",)
 # entry points returning a C string
 STRING_FUNCS = ("asc_last_error", "asc_version")
 
@@ -137,7 +157,7 @@ def load_library(path: Optional[Path] = None) -> ctypes.CDLL:
         for name, argtypes in SIGNATURES.items():
             fn = getattr(lib, name)
             fn.argtypes = argtypes
-            fn.restype = ctypes.c_int32
+            fn.restype = _c_i64 if name in INT64_FUNCS else ctypes.c_int32
         for name in STRING_FUNCS:
             fn = getattr(lib, name)
             fn.argtypes = []

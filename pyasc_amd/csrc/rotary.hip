@@ -1,0 +1,527 @@
+// Rotary positions of queries and keys, with or without an RMS norm of each head in the same
+// pass, and the gradient of both.
+//
+// Pair (a, b) of frequency f in a token of position p turns by t = p f:
+//   a' = m (a cos t - b sin t),  b' = m (b cos t + a sin t),
+// which is linear in (a, b); its gradient is the turn by -t times m.  With the norm, r =
+// 1 / sqrt(mean(x^2) + eps) and y = turn(x r w); with g = turn^T(dy) the gradients are
+//   dw = sum over rows of g x r,   dx = r (g w - x r mean(g w x r)).
+//
+// Each value is read and written once, so HBM bounds it.  A workgroup takes a few tokens and all
+// (or a chunk of) their heads: the angles of its tokens go into LDS once, from the product of
+// position and frequency in fp64 (a far position keeps its fraction of a turn), and every head
+// reads them.  A row (one head of one token) belongs to kLanes neighbouring lanes of a wave; a lane
+// holds both values of kV pairs, so the turn needs no exchange and the norm one butterfly.
+#include "common.h"
+#include "numeric.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxTokens = 4;     // of a workgroup
+constexpr int kMaxHeadDim = 512;  // kSlots lanes' slots and the LDS tables cover it
+constexpr int kMaxParts = 1024;   // workgroups of a gradient launch: partial sums of its weights
+
+struct Rows {  // [batch, heads, seq, head_dim], the last dimension contiguous
+  const void* p;
+  int64_t batch, head, seq;
+};
+
+struct RotaryArgs {
+  Rows x[2];   // queries and keys (gradient: of the forward pass)
+  Rows dy[2];  // gradient: of the results
+  Rows out[2];
+  const float* weight[2];
+  float* parts;  // gradient: [workgroup][2][head_dim] sums of g x r
+  const void* positions;
+  int64_t pos_batch, pos_seq;
+  const double* freqs;
+  int64_t seq;
+  uint32_t units;  // batch * tiles * chunks < 2^31
+  uint32_t tiles;  // of tokens per sequence
+  uint32_t chunks;  // of heads
+  int32_t q_heads, heads, chunk_heads;
+  int32_t head_dim, pairs, tokens;
+  int32_t lanes;  // of a row, a power of two
+  int32_t pos64;
+  float sign, magnitude, epsilon, inv_dim;
+};
+
+template <typename T>
+__device__ __forceinline__ float widen(T v);
+template <>
+__device__ __forceinline__ float widen<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float widen<_Float16>(_Float16 v) { return static_cast<float>(v); }
+template <>
+__device__ __forceinline__ float widen<__bf16>(__bf16 v) { return static_cast<float>(v); }
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+  T v[V];
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void load(const T* p, float (&x)[V]) {
+  const Vec<T, V> w = *reinterpret_cast<const Vec<T, V>*>(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = widen<T>(w.v[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store(T* p, const float (&x)[V]) {
+  Vec<T, V> w;
+#pragma unroll
+  for (int i = 0; i < V; ++i) w.v[i] = static_cast<T>(x[i]);
+  *reinterpret_cast<Vec<T, V>*>(p) = w;
+}
+
+// Sum over the `lanes` (a power of two) neighbouring lanes of a row.
+__device__ __forceinline__ float row_sum(float v, int lanes) {
+  for (int d = 1; d < lanes; d <<= 1) v += __shfl_xor(v, d, 64);
+  return v;
+}
+
+// cos and sin of `rev` turns.  The fraction of a quarter turn is exact in fp64 before it is
+// rounded to fp32: the angle is off by at most 2^-27.
+__device__ __forceinline__ float2 turn_of(double rev, float sign, float magnitude) {
+  const double f = rev - rint(rev);
+  const double q = rint(f * 4.0);
+  float s, c;
+  sincospif(2.0f * static_cast<float>(f - 0.25 * q), &s, &c);
+  const int quarter = static_cast<int>(q) & 3;
+  if (quarter & 1) {
+    const float t = c;
+    c = -s;
+    s = t;
+  }
+  if (quarter & 2) {
+    c = -c;
+    s = -s;
+  }
+  return make_float2(c * magnitude, s * sign * magnitude);
+}
+
+enum Mode { kTurn, kNorm, kNormGrad };
+
+// Slots of a lane: a row has head_dim / (2 kV) of them on at most 64 lanes.
+template <int V>
+constexpr int slots_per_lane() { return V >= 4 ? 1 : (V == 2 ? 2 : 4); }
+
+template <typename T, int V, bool kInterleaved, Mode kMode>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs p) {
+  constexpr int kSlots = slots_per_lane<V>();
+  __shared__ float2 table[kMaxTokens * kMaxHeadDim / 2];
+  __shared__ float sums[kMode == kNormGrad ? 2 * kMaxHeadDim : 1];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & (p.lanes - 1);
+  const int row0 = tid / p.lanes, rows_per_pass = kThreads / p.lanes;
+  const int pair_slots = p.pairs / V, slots = p.head_dim / (2 * V);
+
+  // the two vectors of each slot: the pairs' first and second values, or two neighbours of
+  // the values behind the rotated ones
+  int c0[kSlots], c1[kSlots], at[kSlots];
+  bool live[kSlots], turned[kSlots];
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i) {
+    const int slot = lane + i * p.lanes;
+    live[i] = slot < slots;
+    turned[i] = slot < pair_slots;
+    at[i] = slot * V;
+    c0[i] = kInterleaved || !turned[i] ? slot * 2 * V : slot * V;
+    c1[i] = kInterleaved || !turned[i] ? c0[i] + V : c0[i] + p.pairs;
+  }
+  float w[2][kSlots][2][V], dw[2][kSlots][2][V];
+  if (kMode != kTurn) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          w[t][i][0][e] = live[i] && p.weight[t] ? p.weight[t][c0[i] + e] : 0.f;
+          w[t][i][1][e] = live[i] && p.weight[t] ? p.weight[t][c1[i] + e] : 0.f;
+          dw[t][i][0][e] = dw[t][i][1][e] = 0.f;
+        }
+  }
+
+  for (uint32_t unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+    const uint32_t tile = unit / p.chunks;
+    const int chunk = static_cast<int>(unit - tile * p.chunks);
+    const int64_t b = tile / p.tiles;
+    const int64_t s0 = static_cast<int64_t>(tile % p.tiles) * p.tokens;
+    const int tokens = static_cast<int>(p.seq - s0 < p.tokens ? p.seq - s0 : p.tokens);
+    __syncthreads();  // the table's last readers
+    for (int i = tid; i < tokens * p.pairs; i += kThreads) {
+      const int t = i / p.pairs, j = i - t * p.pairs;
+      const int64_t o = b * p.pos_batch + (s0 + t) * p.pos_seq;
+      const double pos = p.pos64 ? static_cast<double>(static_cast<const int64_t*>(p.positions)[o])
+                                 : static_cast<double>(static_cast<const int32_t*>(p.positions)[o]);
+      table[t * p.pairs + j] = turn_of(pos * (p.freqs[j] * 0.15915494309189533577), p.sign, p.magnitude);
+    }
+    __syncthreads();
+    const int h0 = chunk * p.chunk_heads;
+    const int n_heads = p.heads - h0 < p.chunk_heads ? p.heads - h0 : p.chunk_heads;
+    // rows: tokens fastest, so that neighbours lie together in both orders of heads and tokens
+    for (int r = row0; r < n_heads * p.tokens; r += rows_per_pass) {
+      const int t = r & (p.tokens - 1);  // a power of two
+      if (t >= tokens) continue;         // all lanes of the row
+      const int head = h0 + r / p.tokens;
+      const int kv = head >= p.q_heads;
+      const int64_t h = kv ? head - p.q_heads : head;
+      const int64_t s = s0 + t;
+      const auto at_row = [&](const Rows& m) {
+        return static_cast<const T*>(m.p) + b * m.batch + h * m.head + s * m.seq;
+      };
+      const T* x = at_row(kv ? p.x[1] : p.x[0]);
+      T* out = const_cast<T*>(at_row(kv ? p.out[1] : p.out[0]));
+      float a0[kSlots][V], a1[kSlots][V], g0[kSlots][V], g1[kSlots][V];
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) {
+        if (!live[i]) continue;
+        load<T, V>(x + c0[i], a0[i]);
+        load<T, V>(x + c1[i], a1[i]);
+      }
+      if (kMode == kNormGrad) {
+        const T* dy = at_row(kv ? p.dy[1] : p.dy[0]);
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+          if (!live[i]) continue;
+          load<T, V>(dy + c0[i], g0[i]);
+          load<T, V>(dy + c1[i], g1[i]);
+        }
+      }
+      float rms = 1.f;
+      if (kMode != kTurn) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+          if (!live[i]) continue;
+#pragma unroll
+          for (int e = 0; e < V; ++e) ss += a0[i][e] * a0[i][e] + a1[i][e] * a1[i][e];
+        }
+        rms = 1.0f / sqrtf(row_sum(ss, p.lanes) * p.inv_dim + p.epsilon);
+      }
+      // turn of one slot's vectors in place; the pairs' values lie in y0, y1, or alternate
+      const auto turn = [&](int i, float (&y0)[V], float (&y1)[V]) {
+        if (!turned[i]) return;
+        const float2* cs = table + t * p.pairs + at[i];
+        if (kInterleaved && V > 1) {
+#pragma unroll
+          for (int e = 0; e < V; e += 2) {
+            const float2 u = cs[e / 2], v = cs[V / 2 + e / 2];
+            const float u0 = y0[e], u1 = y0[e + 1], v0 = y1[e], v1 = y1[e + 1];
+            y0[e] = u0 * u.x - u1 * u.y;
+            y0[e + 1] = u1 * u.x + u0 * u.y;
+            y1[e] = v0 * v.x - v1 * v.y;
+            y1[e + 1] = v1 * v.x + v0 * v.y;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float2 c = cs[e];
+            const float u = y0[e], v = y1[e];
+            y0[e] = u * c.x - v * c.y;
+            y1[e] = v * c.x + u * c.y;
+          }
+        }
+      };
+      if (kMode == kNormGrad) {
+        float along = 0.f;  // sum of g w x r
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+          if (!live[i]) continue;
+          turn(i, g0[i], g1[i]);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            a0[i][e] *= rms;
+            a1[i][e] *= rms;
+            const float d0 = g0[i][e] * a0[i][e], d1 = g1[i][e] * a1[i][e];
+            if (kv) {
+              dw[1][i][0][e] += d0;
+              dw[1][i][1][e] += d1;
+            } else {
+              dw[0][i][0][e] += d0;
+              dw[0][i][1][e] += d1;
+            }
+            g0[i][e] *= kv ? w[1][i][0][e] : w[0][i][0][e];
+            g1[i][e] *= kv ? w[1][i][1][e] : w[0][i][1][e];
+            along += g0[i][e] * a0[i][e] + g1[i][e] * a1[i][e];
+          }
+        }
+        along = row_sum(along, p.lanes) * p.inv_dim;
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+          if (!live[i]) continue;
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            a0[i][e] = rms * (g0[i][e] - a0[i][e] * along);
+            a1[i][e] = rms * (g1[i][e] - a1[i][e] * along);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+          if (!live[i]) continue;
+          if (kMode == kNorm) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              a0[i][e] = a0[i][e] * rms * (kv ? w[1][i][0][e] : w[0][i][0][e]);
+              a1[i][e] = a1[i][e] * rms * (kv ? w[1][i][1][e] : w[0][i][1][e]);
+            }
+          }
+          turn(i, a0[i], a1[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) {
+        if (!live[i]) continue;
+        store<T, V>(out + c0[i], a0[i]);
+        store<T, V>(out + c1[i], a1[i]);
+      }
+    }
+  }
+
+  if (kMode == kNormGrad) {
+    // the workgroup's sums: rows of one wave by a butterfly over the lanes above the row's, then
+    // the four waves one after the other, always in the same order
+    const int wave = tid >> 6;
+    for (int i = tid; i < 2 * p.head_dim; i += kThreads) sums[i] = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            for (int d = p.lanes; d < 64; d <<= 1) dw[t][i][c][e] += __shfl_xor(dw[t][i][c][e], d, 64);
+          }
+    for (int turn = 0; turn < kThreads / 64; ++turn) {
+      __syncthreads();
+      if (wave != turn || (tid & 63) >= p.lanes) continue;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+          if (!live[i]) continue;
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            sums[t * p.head_dim + c0[i] + e] += dw[t][i][0][e];
+            sums[t * p.head_dim + c1[i] + e] += dw[t][i][1][e];
+          }
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < 2 * p.head_dim; i += kThreads) {
+      p.parts[static_cast<int64_t>(blockIdx.x) * 2 * p.head_dim + i] = sums[i];
+    }
+  }
+}
+
+// dw[t][c] = sum over workgroups of parts[.][t][c], in fp64 (the sum itself is short).  One
+// workgroup per 16 columns: 16 rows of threads take every 16th part.
+__global__ void __launch_bounds__(256) weight_sums_kernel(const float* parts, int n_parts, int head_dim, float* dq,
+                                                          float* dk) {
+  __shared__ double acc[16][17];
+  const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+  const int col = blockIdx.x * 16 + c;
+  double s = 0.0;
+  if (col < 2 * head_dim) {
+    for (int i = r; i < n_parts; i += 16) s += parts[static_cast<int64_t>(i) * 2 * head_dim + col];
+  }
+  acc[r][c] = s;
+  __syncthreads();
+  if (r != 0 || col >= 2 * head_dim) return;
+  for (int i = 1; i < 16; ++i) s += acc[i][c];
+  float* out = col < head_dim ? dq : dk;
+  if (out != nullptr) out[col < head_dim ? col : col - head_dim] = static_cast<float>(s);
+}
+
+template <typename T, int V, Mode kMode>
+void launch(bool interleaved, dim3 grid, hipStream_t stream, const RotaryArgs& p) {
+  if (interleaved) {
+    hipLaunchKernelGGL((rotary_kernel<T, V, true, kMode>), grid, dim3(kThreads), 0, stream, p);
+  } else {
+    hipLaunchKernelGGL((rotary_kernel<T, V, false, kMode>), grid, dim3(kThreads), 0, stream, p);
+  }
+}
+
+template <typename T, Mode kMode>
+void launch_vec(int vec, bool interleaved, dim3 grid, hipStream_t stream, const RotaryArgs& p) {
+  if constexpr (sizeof(T) == 2) {
+    if (vec == 8) return launch<T, 8, kMode>(interleaved, grid, stream, p);
+  }
+  if (vec == 4) return launch<T, 4, kMode>(interleaved, grid, stream, p);
+  if (vec == 2) return launch<T, 2, kMode>(interleaved, grid, stream, p);
+  return launch<T, 1, kMode>(interleaved, grid, stream, p);
+}
+
+int64_t token_tiles(const asc_rotary_t& a) { return asc::ceil_div(a.seq, kMaxTokens); }
+
+// Workgroups of a gradient launch, as its workspace counts them: at most kMaxParts, each with a
+// share of the token tiles.
+int64_t grad_parts(const asc_rotary_t& a) {
+  const int64_t n = a.batch * token_tiles(a);
+  return n < kMaxParts ? n : kMaxParts;
+}
+
+int32_t check(const asc_rotary_t* a, const char* what, Mode mode) {
+  ASC_REQUIRE(a, ASC_ERR_INVALID_ARG, "%s: null arguments", what);
+  ASC_REQUIRE(a->dtype == ASC_DT_FLOAT32 || a->dtype == ASC_DT_FLOAT16 || a->dtype == ASC_DT_BFLOAT16,
+              ASC_ERR_UNSUPPORTED, "%s: dtype %d not supported (float32, float16, bfloat16)", what, a->dtype);
+  ASC_REQUIRE(a->batch >= 0 && a->q_heads >= 0 && a->k_heads >= 0 && a->seq >= 0, ASC_ERR_INVALID_ARG,
+              "%s: negative shape", what);
+  ASC_REQUIRE(a->head_dim > 0 && a->head_dim % 2 == 0 && a->head_dim <= kMaxHeadDim, ASC_ERR_UNSUPPORTED,
+              "%s: head_dim %d not supported (even, at most %d)", what, a->head_dim, kMaxHeadDim);
+  ASC_REQUIRE(a->rotary_dim >= 0 && a->rotary_dim % 2 == 0 && a->rotary_dim <= a->head_dim, ASC_ERR_INVALID_ARG,
+              "%s: rotary_dim %d must be even and at most head_dim %d", what, a->rotary_dim, a->head_dim);
+  ASC_REQUIRE(a->q_heads <= 1 << 20 && a->k_heads <= 1 << 20, ASC_ERR_UNSUPPORTED, "%s: too many heads", what);
+  ASC_REQUIRE(a->seq < int64_t{1} << 31 && a->batch < int64_t{1} << 31 &&
+                  a->batch * token_tiles(*a) < int64_t{1} << 31,
+              ASC_ERR_UNSUPPORTED, "%s: batch %lld x seq %lld too large", what, static_cast<long long>(a->batch),
+              static_cast<long long>(a->seq));
+  ASC_REQUIRE(mode == kTurn || a->epsilon >= 0.f, ASC_ERR_INVALID_ARG, "%s: epsilon must not be negative", what);
+  if (a->batch == 0 || a->seq == 0 || a->q_heads + a->k_heads == 0) return ASC_OK;
+  ASC_REQUIRE(a->rotary_dim == 0 || (a->positions && a->freqs), ASC_ERR_INVALID_ARG, "%s: null positions or freqs",
+              what);
+  for (int t = 0; t < 2; ++t) {
+    if ((t ? a->k_heads : a->q_heads) == 0) continue;
+    ASC_REQUIRE((t ? a->k.data : a->q.data) && (t ? a->k_out.data : a->q_out.data), ASC_ERR_INVALID_ARG,
+                "%s: null buffer", what);
+    if (mode == kTurn) continue;
+    ASC_REQUIRE(t ? a->k_weight : a->q_weight, ASC_ERR_INVALID_ARG, "%s: null weight", what);
+    ASC_REQUIRE(mode != kNormGrad || ((t ? a->dk_out.data : a->dq_out.data) && (t ? a->dk_weight : a->dq_weight)),
+                ASC_ERR_INVALID_ARG, "%s: null gradient", what);
+  }
+  return ASC_OK;
+}
+
+// The widest vector (16 bytes at most) that every row's slots allow: both halves of a pair slot
+// and every stride and address are multiples of it.
+int vector_width(const asc_rotary_t& a, Mode mode) {
+  const int64_t size = a.dtype == ASC_DT_FLOAT32 ? 4 : 2;
+  const asc_rows_t* rows[] = {&a.q, &a.q_out, &a.dq_out, &a.k, &a.k_out, &a.dk_out};
+  for (int v = static_cast<int>(16 / size); v > 1; v /= 2) {
+    bool ok = a.rotary_dim % (2 * v) == 0 && a.head_dim % (2 * v) == 0;
+    for (int i = 0; i < 6; ++i) {
+      if ((i < 3 ? a.q_heads : a.k_heads) == 0 || (i % 3 == 2 && mode != kNormGrad)) continue;
+      ok = ok && reinterpret_cast<uintptr_t>(rows[i]->data) % (v * size) == 0 && rows[i]->batch_stride % v == 0 &&
+           rows[i]->head_stride % v == 0 && rows[i]->seq_stride % v == 0;
+    }
+    if (ok) return v;
+  }
+  return 1;
+}
+
+void sum_weights(const asc_rotary_t& a, const float* parts, int n_parts, hipStream_t stream) {
+  hipLaunchKernelGGL(weight_sums_kernel, dim3(static_cast<uint32_t>(asc::ceil_div(2 * a.head_dim, 16))), dim3(256), 0,
+                     stream, parts, n_parts, a.head_dim, a.dq_weight, a.dk_weight);
+}
+
+int32_t run(const asc_rotary_t* a, const char* what, Mode mode, float* parts, asc_stream_t stream) {
+  RotaryArgs p{};
+  const auto rows = [](const asc_rows_t& r) { return Rows{r.data, r.batch_stride, r.head_stride, r.seq_stride}; };
+  p.x[0] = rows(a->q);
+  p.x[1] = rows(a->k);
+  p.dy[0] = rows(a->dq_out);
+  p.dy[1] = rows(a->dk_out);
+  p.out[0] = rows(a->q_out);
+  p.out[1] = rows(a->k_out);
+  p.weight[0] = a->q_weight;
+  p.weight[1] = a->k_weight;
+  p.parts = parts;
+  p.positions = a->positions;
+  p.pos64 = a->positions_int64;
+  p.pos_batch = a->position_batch_stride;
+  p.pos_seq = a->position_seq_stride;
+  p.freqs = a->freqs;
+  p.seq = a->seq;
+  p.q_heads = static_cast<int32_t>(a->q_heads);
+  p.heads = static_cast<int32_t>(a->q_heads + a->k_heads);
+  p.head_dim = a->head_dim;
+  p.pairs = a->rotary_dim / 2;
+  p.sign = mode == kNormGrad || (mode == kTurn && a->backward) ? -1.f : 1.f;
+  p.magnitude = a->magnitude;
+  p.epsilon = a->epsilon;
+  p.inv_dim = 1.0f / static_cast<float>(a->head_dim);
+  const int vec = vector_width(*a, mode);
+  const int per_lane = vec >= 4 ? 1 : (vec == 2 ? 2 : 4);
+  const int slots = static_cast<int>(asc::ceil_div(a->head_dim / (2 * vec), per_lane));
+  p.lanes = 1;
+  while (p.lanes < slots) p.lanes *= 2;  // at most 64: head_dim <= 512
+  p.tokens = 1;
+  while (p.tokens < kMaxTokens && p.tokens < a->seq) p.tokens *= 2;
+  p.tiles = static_cast<uint32_t>(asc::ceil_div(a->seq, p.tokens));
+  const int64_t n_tiles = a->batch * p.tiles;
+  // Few tokens: their heads spread over workgroups of one pass each; else one workgroup for all.
+  p.chunk_heads = p.heads;
+  if (mode != kNormGrad && n_tiles < 2 * 256) {
+    const int per_pass = kThreads / p.lanes / p.tokens;
+    p.chunk_heads = per_pass < 1 ? 1 : (per_pass < p.heads ? per_pass : p.heads);
+  }
+  p.chunks = static_cast<uint32_t>(asc::ceil_div(p.heads, p.chunk_heads));
+  p.units = static_cast<uint32_t>(n_tiles * p.chunks);  // chunks > 1 only where n_tiles is small
+  int64_t blocks = p.units;
+  const int64_t most = mode == kNormGrad ? kMaxParts : int64_t{1} << 23;  // the kernel strides over the rest
+  if (blocks > most) blocks = most;
+  const dim3 grid(static_cast<uint32_t>(blocks));
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool inter = a->interleaved != 0;
+  const auto go = [&](auto tag) {
+    using T = decltype(tag);
+    if (mode == kTurn) return launch_vec<T, kTurn>(vec, inter, grid, s, p);
+    if (mode == kNorm) return launch_vec<T, kNorm>(vec, inter, grid, s, p);
+    return launch_vec<T, kNormGrad>(vec, inter, grid, s, p);
+  };
+  if (a->dtype == ASC_DT_FLOAT32) {
+    go(float{});
+  } else if (a->dtype == ASC_DT_FLOAT16) {
+    go(_Float16{});
+  } else {
+    go(__bf16{});
+  }
+  if (mode == kNormGrad) {
+    const int32_t rc = asc::check_launch(what);
+    if (rc != ASC_OK) return rc;
+    sum_weights(*a, parts, static_cast<int>(blocks), s);
+  }
+  return asc::check_launch(what);
+}
+
+bool empty(const asc_rotary_t& a) { return a.batch == 0 || a.seq == 0 || a.q_heads + a.k_heads == 0; }
+
+}  // namespace
+
+extern "C" int32_t asc_rotary(const asc_rotary_t* args, asc_stream_t stream) {
+  const int32_t rc = check(args, "asc_rotary", kTurn);
+  if (rc != ASC_OK || empty(*args)) return rc;
+  return run(args, "asc_rotary", kTurn, nullptr, stream);
+}
+
+extern "C" int32_t asc_qk_norm_rotary(const asc_rotary_t* args, asc_stream_t stream) {
+  const int32_t rc = check(args, "asc_qk_norm_rotary", kNorm);
+  if (rc != ASC_OK || empty(*args)) return rc;
+  return run(args, "asc_qk_norm_rotary", kNorm, nullptr, stream);
+}
+
+extern "C" int64_t asc_qk_norm_rotary_bwd_workspace(const asc_rotary_t* args) {
+  if (check(args, "asc_qk_norm_rotary_bwd_workspace", kTurn) != ASC_OK || empty(*args)) return 0;
+  return grad_parts(*args) * 2 * args->head_dim * static_cast<int64_t>(sizeof(float));
+}
+
+extern "C" int32_t asc_qk_norm_rotary_bwd(const asc_rotary_t* args, void* workspace, int64_t workspace_bytes,
+                                          asc_stream_t stream) {
+  const int32_t rc = check(args, "asc_qk_norm_rotary_bwd", kNormGrad);
+  if (rc != ASC_OK) return rc;
+  if (empty(*args)) {  // no rows: the weights' gradients are zeros
+    if (args->dq_weight == nullptr && args->dk_weight == nullptr) return ASC_OK;
+    sum_weights(*args, nullptr, 0, static_cast<hipStream_t>(stream));
+    return asc::check_launch("asc_qk_norm_rotary_bwd");
+  }
+  const int64_t need = grad_parts(*args) * 2 * args->head_dim * static_cast<int64_t>(sizeof(float));
+  ASC_REQUIRE(workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 4 == 0,
+              ASC_ERR_INVALID_ARG, "asc_qk_norm_rotary_bwd: the workspace must hold %lld bytes",
+              static_cast<long long>(need));
+  return run(args, "asc_qk_norm_rotary_bwd", kNormGrad, static_cast<float*>(workspace), stream);
+}

@@ -8,6 +8,7 @@ GPU.  Launches are asynchronous on ``stream`` (default: torch's current stream).
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Any, Optional
 
 import torch
@@ -581,6 +582,211 @@ def flash_attention_dispatch(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     _native.call("asc_flash_attention_dispatch", *_attention_args(q, k, v, o, sm_scale, causal, lse),
                  ctypes.byref(plan))
     return plan
+
+
+# ------------------------------------------------------------------- rotary positions, q/k norms
+
+ROTARY_SCALINGS = (None, "linear", "ntk", "yarn")
+MAX_ROTARY_HEAD_DIM = 512
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _here(t: torch.Tensor, name: str) -> torch.Tensor:
+    """A tensor of the current device, the one that launches go to."""
+    _device_tensor(t, name)
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"'{name}' is on {t.device}, but the current device is cuda:{torch.cuda.current_device()}")
+    return t
+
+
+def _bhsd(t: torch.Tensor, name: str, dtype: torch.dtype, shape: Optional[tuple] = None,
+          written: bool = False) -> torch.Tensor:
+    """A [batch, heads, seq, head_dim] operand of any strides whose last dimension is contiguous.
+    A tensor that is written must hold every element at a place of its own."""
+    _here(t, name)
+    if t.dtype != dtype:
+        raise TypeError(f"'{name}' must be {dtype}, got {t.dtype}")
+    if t.dim() != 4 or (shape is not None and tuple(t.shape) != shape):
+        raise ValueError(f"'{name}' must be {list(shape) if shape else '[batch, heads, seq, head_dim]'}, "
+                         f"got {tuple(t.shape)}")
+    if t.shape[3] > 1 and t.stride(3) != 1:
+        raise ValueError(f"the last dimension of '{name}' must be contiguous")
+    if written and not t.is_contiguous():
+        span = 0  # of the dimensions so far, from the innermost
+        for stride, size in sorted((t.stride(i), t.shape[i]) for i in range(4) if t.shape[i] > 1):
+            if stride <= span:
+                raise ValueError(f"'{name}' is written but its elements overlap (strides {t.stride()})")
+            span += stride * (size - 1)
+    return t
+
+
+def _rows(t: Optional[torch.Tensor]) -> "_native.Rows":
+    if t is None:
+        return _native.Rows()
+    s = t.stride()
+    return _native.Rows(t.data_ptr(), s[0], s[1], s[2])
+
+
+def _workspace(nbytes: int, handle: int, device: torch.device, what: str) -> torch.Tensor:
+    """``nbytes`` for the launches of one call on stream ``handle``, as workspace_on's.  Under a
+    capture that torch does not know of the memory would go to others before the replays: refused."""
+    t = workspace_on(handle, nbytes, torch.uint8, device)
+    if torch.cuda.is_current_stream_capturing() and not _held_by_a_graph(t):
+        raise RuntimeError(f"{what} needs a workspace: capture it with torch.cuda.graph")
+    return t
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
+                       original_length: Optional[int] = None, device: Any = None) -> tuple:
+    """The angle per position of each of the rotary_dim / 2 pairs (float64, on ``device``, default
+    the current one), base^(-2 i / rotary_dim), and the factor on the rotated values
+    (``magnitude`` of rotary and qk_norm_rotary).  ``scaling`` extends a context of
+    ``original_length`` tokens ``factor`` times:
+
+    - "linear": every frequency divided by the factor;
+    - "ntk": a larger base, base * factor^(rotary_dim / (rotary_dim - 2)), which leaves the first
+      pair as it is and divides the last one's frequency by the factor;
+    - "yarn": pairs that turn at least 32 times in the original length keep their frequency, those
+      that turn less than once are divided by the factor, in between linearly in the number of
+      turns; the magnitude is 0.1 ln(factor) + 1 (Peng et al., arXiv:2309.00071, sections 3.2-3.4)."""
+    rotary_dim = int(rotary_dim)
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be positive and even, got {rotary_dim}")
+    if scaling not in ROTARY_SCALINGS:
+        raise ValueError(f"unknown scaling {scaling!r}; expected one of {ROTARY_SCALINGS}")
+    if not base > 0 or not factor > 0:
+        raise ValueError(f"base and factor must be positive, got {base} and {factor}")
+    if scaling == "ntk":
+        if rotary_dim == 2:
+            raise ValueError("ntk scaling needs more than one pair")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    freqs = base ** (torch.arange(rotary_dim // 2, dtype=torch.float64) * (-2.0 / rotary_dim))
+    magnitude = 1.0
+    if scaling == "linear":
+        freqs = freqs / factor
+    elif scaling == "yarn":
+        if original_length is None or original_length <= 0:
+            raise ValueError("yarn scaling needs the original_length")
+        turns = freqs * (original_length / (2 * math.pi))
+        keep = ((turns - 1.0) / (32.0 - 1.0)).clamp(0.0, 1.0)
+        freqs = freqs * keep + freqs / factor * (1.0 - keep)
+        if factor > 1:
+            magnitude = 0.1 * math.log(factor) + 1.0
+    return freqs.to("cuda" if device is None else device), magnitude
+
+
+def _rotary_args(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor,
+                 q_out: torch.Tensor, k_out: Optional[torch.Tensor], interleaved: bool,
+                 magnitude: float) -> "_native.RotaryArgs":
+    """Checks what the three rotary calls share."""
+    if not isinstance(q, torch.Tensor):
+        raise TypeError(f"'q' must be a torch.Tensor, got {type(q).__name__}")
+    if q.dtype not in _FLOATS:
+        raise TypeError(f"'q' has unsupported dtype {q.dtype}; expected one of {sorted(map(str, _FLOATS))}")
+    _bhsd(q, "q", q.dtype)
+    batch, heads, seq, head_dim = q.shape
+    if head_dim % 2 or not 0 < head_dim <= MAX_ROTARY_HEAD_DIM:
+        raise ValueError(f"head_dim {head_dim} not supported (even, at most {MAX_ROTARY_HEAD_DIM})")
+    _bhsd(q_out, "q_out", q.dtype, tuple(q.shape), written=True)
+    if (k is None) != (k_out is None):
+        raise ValueError("k and its result must be given together")
+    pairs = [(q, q_out)]
+    if k is not None:
+        _bhsd(k, "k", q.dtype)
+        _bhsd(k, "k", q.dtype, (batch, k.shape[1], seq, head_dim))
+        _bhsd(k_out, "k_out", q.dtype, tuple(k.shape), written=True)
+        pairs.append((k, k_out))
+    for x, y in pairs:
+        if x.data_ptr() == y.data_ptr() and x.stride() != y.stride() and x.numel():
+            raise ValueError("a result in place of its input must have the input's strides")
+    _here(positions, "positions")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
+    if tuple(positions.shape) not in ((seq,), (batch, seq)):
+        raise ValueError(f"positions must be [seq] or [batch, seq] = {(batch, seq)}, got {tuple(positions.shape)}")
+    _contiguous(_here(freqs, "freqs"), "freqs")
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or 2 * freqs.shape[0] > head_dim:
+        raise ValueError(f"freqs must be float64 with at most head_dim / 2 = {head_dim // 2} elements")
+    a = _native.RotaryArgs()
+    a.dtype, a.head_dim, a.rotary_dim = _DTYPE_CODES[q.dtype], head_dim, 2 * freqs.shape[0]
+    a.interleaved, a.positions_int64, a.magnitude = bool(interleaved), positions.dtype == torch.int64, magnitude
+    a.batch, a.q_heads, a.k_heads, a.seq = batch, heads, 0 if k is None else k.shape[1], seq
+    a.q, a.k, a.q_out, a.k_out = _rows(q), _rows(k), _rows(q_out), _rows(k_out)
+    a.positions, a.freqs = positions.data_ptr(), freqs.data_ptr()
+    a.position_batch_stride = positions.stride(0) if positions.dim() == 2 else 0
+    a.position_seq_stride = positions.stride(-1)
+    return a
+
+
+def _head_weight(w: torch.Tensor, name: str, head_dim: int) -> int:
+    _contiguous(_here(w, name), name)
+    if w.dtype != torch.float32 or tuple(w.shape) != (head_dim,):
+        raise ValueError(f"'{name}' must be float32 [{head_dim}], got {w.dtype} {tuple(w.shape)}")
+    return w.data_ptr()
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor,
+           q_out: torch.Tensor, k_out: Optional[torch.Tensor], interleaved: bool = False, magnitude: float = 1.0,
+           backward: bool = False, stream: Any = None) -> None:
+    """Rotary positions of queries and keys ([batch, heads, seq, head_dim] of any strides, k with
+    its own number of heads or None) in one launch: pair i of the first 2 * len(freqs) columns,
+    (i, i + len(freqs)) or, ``interleaved``, (2 i, 2 i + 1), turns by positions * freqs[i] and is
+    multiplied by ``magnitude``; the other columns are copied.  ``backward`` gives the gradient:
+    the turn the other way.  A result may lie in place of its input."""
+    a = _rotary_args(q, k, positions, freqs, q_out, k_out, interleaved, magnitude)
+    a.backward = bool(backward)
+    _native.call("asc_rotary", ctypes.byref(a), _stream(stream))
+
+
+def qk_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: torch.Tensor,
+                   k_weight: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor,
+                   q_out: torch.Tensor, k_out: Optional[torch.Tensor], epsilon: float, interleaved: bool = False,
+                   magnitude: float = 1.0, stream: Any = None) -> None:
+    """rotary after an RMS norm of each head: x / sqrt(mean(x^2) + epsilon) * weight, the weights
+    float32 [head_dim]."""
+    a = _rotary_args(q, k, positions, freqs, q_out, k_out, interleaved, magnitude)
+    _norm_args(a, k, q_weight, k_weight, epsilon)
+    _native.call("asc_qk_norm_rotary", ctypes.byref(a), _stream(stream))
+
+
+def _norm_args(a: "_native.RotaryArgs", k: Optional[torch.Tensor], q_weight: torch.Tensor,
+               k_weight: Optional[torch.Tensor], epsilon: float) -> None:
+    if not epsilon >= 0:
+        raise ValueError(f"epsilon must not be negative, got {epsilon}")
+    a.epsilon = epsilon
+    a.q_weight = _head_weight(q_weight, "q_weight", a.head_dim)
+    if k is not None:
+        a.k_weight = _head_weight(k_weight, "k_weight", a.head_dim)
+
+
+def qk_norm_rotary_bwd(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q: torch.Tensor,
+                       k: Optional[torch.Tensor], q_weight: torch.Tensor, k_weight: Optional[torch.Tensor],
+                       positions: torch.Tensor, freqs: torch.Tensor, dq: torch.Tensor, dk: Optional[torch.Tensor],
+                       dq_weight: torch.Tensor, dk_weight: Optional[torch.Tensor], epsilon: float,
+                       interleaved: bool = False, magnitude: float = 1.0, stream: Any = None) -> None:
+    """The gradient of qk_norm_rotary: from the results' gradients and its inputs, the gradients
+    of q and k (dq may lie in place of dq_out or q) and of the weights (float32 [head_dim], summed
+    over all rows in a fixed order)."""
+    a = _rotary_args(q, k, positions, freqs, dq, dk, interleaved, magnitude)
+    _norm_args(a, k, q_weight, k_weight, epsilon)
+    _bhsd(dq_out, "dq_out", q.dtype, tuple(q.shape))
+    results = [(dq_out, dq)]
+    a.dq_out = _rows(dq_out)
+    a.dq_weight = _head_weight(dq_weight, "dq_weight", a.head_dim)
+    if k is not None:
+        if dk_out is None:
+            raise ValueError("dk_out must be given with k")
+        _bhsd(dk_out, "dk_out", q.dtype, tuple(k.shape))
+        results.append((dk_out, dk))
+        a.dk_out = _rows(dk_out)
+        a.dk_weight = _head_weight(dk_weight, "dk_weight", a.head_dim)
+    for x, y in results:
+        if x.data_ptr() == y.data_ptr() and x.stride() != y.stride() and x.numel():
+            raise ValueError("a result in place of its input must have the input's strides")
+    handle = _stream(stream)
+    nbytes = _native.load_library().asc_qk_norm_rotary_bwd_workspace(ctypes.byref(a))
+    workspace = _workspace(nbytes, handle, q.device, "qk_norm_rotary_bwd") if nbytes else None
+    _native.call("asc_qk_norm_rotary_bwd", ctypes.byref(a), workspace.data_ptr() if nbytes else 0, nbytes, handle)
 
 
 # ------------------------------------------------------------------ element-wise tile operations

@@ -483,6 +483,50 @@ int64_t asc_qk_norm_rotary_bwd_workspace(const asc_rotary_t* args);
 int32_t asc_qk_norm_rotary_bwd(const asc_rotary_t* args, void* workspace,
                                int64_t workspace_bytes, asc_stream_t stream);
 
+/* ---- attention over other keys than the queries' own ------------------------------
+ * No reference function exists; the build defines these next to its attention.
+ * q and o: rows of q_heads heads and q_len queries per sequence; query head i reads
+ * key / value head i / (q_heads / kv_heads).  o = softmax(q k^T * sm_scale) v over
+ * the keys a query attends, fp32 statistics; lse (may be NULL) receives their
+ * natural log-sum-exp, fp32 [batch, q_heads, q_len].  A query without keys gets
+ * zeros, and -inf for its lse.  float16 and bfloat16, head_dim 64 or 128, sm_scale >
+ * 0; bases 16-byte aligned and strides multiples of 8 elements (ASC_ERR_ALIGNMENT);
+ * keys and values within 64 GiB.
+ * asc_cross_attention_fwd  keys 0 .. kv_lengths[b] - 1 of sequence b (kv_lengths
+ *                          NULL: all kv_len).
+ * asc_tree_attention       first the cached keys, as above, from k and v; with a
+ *                          block_table key j lies in page block_table[b][j /
+ *                          page_size], row j % page_size (k and v: num_pages "batches"
+ *                          of page_size rows; kv_len: table width * page_size).  Then
+ *                          drafted key j (of q_len) where tree_mask[b][query][j] is not
+ *                          0 (NULL: j <= query).  draft_lengths (may be NULL): drafted
+ *                          tokens of sequence b; the queries behind them are not
+ *                          written.
+ * A length outside the cache, or a page outside it that a length reaches, is not
+ * followed: the sequence's results are NaN.
+ * `workspace` holds the entry's _workspace bytes, 16-byte aligned (0: NULL allowed). */
+typedef struct asc_attention {
+  int32_t dtype, head_dim;
+  float sm_scale;
+  int32_t page_size;
+  int64_t batch, q_heads, kv_heads, q_len, kv_len, num_pages;
+  asc_rows_t q, o, k, v, k_draft, v_draft;
+  float* lse;
+  const int32_t* kv_lengths;
+  const int32_t* draft_lengths;
+  const int32_t* block_table;
+  int64_t table_stride;
+  const uint8_t* tree_mask;
+  int64_t mask_batch_stride, mask_row_stride;
+  asc_rows_t d_o, dq, dk, dv; /* asc_cross_attention_bwd */
+} asc_attention_t;
+int64_t asc_cross_attention_fwd_workspace(const asc_attention_t* args);
+int32_t asc_cross_attention_fwd(const asc_attention_t* args, void* workspace,
+                                int64_t workspace_bytes, asc_stream_t stream);
+int64_t asc_tree_attention_workspace(const asc_attention_t* args);
+int32_t asc_tree_attention(const asc_attention_t* args, void* workspace,
+                           int64_t workspace_bytes, asc_stream_t stream);
+
 /* ---- element-wise tile operations ------------------------------------------------
  * The generic kernels of the reference's operation tests, one op per launch:
  *   unary   kernel(x_ptr, z_ptr, block_length, op)

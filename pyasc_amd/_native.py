@@ -66,6 +66,16 @@ class RotaryArgs(ctypes.Structure):
                 ("freqs", _c_p), ("q_weight", _c_p), ("k_weight", _c_p), ("dq_weight", _c_p), ("dk_weight", _c_p)]
 
 
+class AttentionArgs(ctypes.Structure):
+    """asc_attention_t."""
+    _fields_ = [("dtype", _c_i32), ("head_dim", _c_i32), ("sm_scale", _c_f32), ("page_size", _c_i32),
+                ("batch", _c_i64), ("q_heads", _c_i64), ("kv_heads", _c_i64), ("q_len", _c_i64), ("kv_len", _c_i64),
+                ("num_pages", _c_i64), ("q", Rows), ("o", Rows), ("k", Rows), ("v", Rows), ("k_draft", Rows),
+                ("v_draft", Rows), ("lse", _c_p), ("kv_lengths", _c_p), ("draft_lengths", _c_p),
+                ("block_table", _c_p), ("table_stride", _c_i64), ("tree_mask", _c_p), ("mask_batch_stride", _c_i64),
+                ("mask_row_stride", _c_i64), ("d_o", Rows), ("dq", Rows), ("dk", Rows), ("dv", Rows)]
+
+
 # name -> argtypes; every entry point returns int32_t (asc_reduce_f32_workspace a byte
 # count, the others a status), those of INT64_FUNCS an int64_t byte count.
 SIGNATURES = {
@@ -116,6 +126,10 @@ SIGNATURES = {
     "asc_qk_norm_rotary": [ctypes.POINTER(RotaryArgs), _c_p],
     "asc_qk_norm_rotary_bwd_workspace": [ctypes.POINTER(RotaryArgs)],
     "asc_qk_norm_rotary_bwd": [ctypes.POINTER(RotaryArgs), _c_p, _c_i64, _c_p],
+    "asc_cross_attention_fwd_workspace": [ctypes.POINTER(AttentionArgs)],
+    "asc_cross_attention_fwd": [ctypes.POINTER(AttentionArgs), _c_p, _c_i64, _c_p],
+    "asc_tree_attention_workspace": [ctypes.POINTER(AttentionArgs)],
+    "asc_tree_attention": [ctypes.POINTER(AttentionArgs), _c_p, _c_i64, _c_p],
     "asc_unary_f32": [_c_i32, _c_p, _c_p, _c_i64, _c_p],
     "asc_binary": [_c_i32, _c_i32, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_f64, _c_i64, _c_p],
     "asc_where_cmp": [_c_i32, _c_i32, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_f64, _c_i64, _c_f64, _c_f64, _c_p],
@@ -128,7 +142,8 @@ SIGNATURES = {
     "asc_transpose_batched": [_c_i32, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p],
     "asc_quant_i8": [_c_i32, _c_p, _c_p, _c_f64, _c_f64, _c_i64, _c_p],
 }
-INT64_FUNCS = ("asc_qk_norm_rotary_bwd_workspace",)
+INT64_FUNCS = ("asc_qk_norm_rotary_bwd_workspace", "asc_cross_attention_fwd_workspace",
+               "asc_tree_attention_workspace")
 # entry points returning a C string
 STRING_FUNCS = ("asc_last_error", "asc_version")
 

@@ -81,18 +81,39 @@ __device__ __forceinline__ uint32_t v_off(int row, int col) {
   return static_cast<uint32_t>(row * (D * 2) + (((col >> 3) ^ vswz<D>(row)) << 4) + ((col & 7) << 1));
 }
 
-__device__ __forceinline__ f32x16 mfma_bf16(u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
-                                                 0, 0);
-}
-
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// Two fp32 -> packed bf16 pair, RNE (one v_cvt_pk_bf16_f32).
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, bf16x2));
-}
+// The 16-bit element types: their product and the rounding of two fp32 values to a packed pair
+// (RNE; one v_cvt_pk_bf16_f32 for bf16).  kTileSumLimit: largest sum of one lane's unnormalised
+// probabilities over a key tile (32 values) before the reference point is moved.  It bounds every
+// exp2 value, which must not overflow the type.  kLift: how far below a tile's largest score (log2)
+// the reference point is put.  fp16 ends at 2^-24, so its probabilities start from 2^8: keys down to
+// 2^-22 of the largest one keep all their bits, and 32 of the largest stay below the limit.
+struct Bf16 {
+  static constexpr float kTileSumLimit = 65536.0f;
+  static constexpr float kLift = 0.0f;
+  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, bf16x2));
+  }
+};
+struct F16 {
+  static constexpr float kTileSumLimit = 32768.0f;
+  static constexpr float kLift = 8.0f;
+  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, f16x2));
+  }
+};
 
 // LDS byte address of a pointer into a __shared__ array.
 __device__ __forceinline__ uint32_t lds_addr(const uint8_t* p) {
@@ -136,16 +157,13 @@ __device__ __forceinline__ float other_half(float v) {
   return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
 }
 
-// Largest sum of one lane's unnormalised probabilities over a key tile (32
-// values) before the reference point is moved: bounds every exp2 value by 2^16.
-constexpr float kTileSumLimit = 65536.0f;
-
 // Per-wave state of the attention kernel.  A wave owns QB blocks of 32 queries
 // (32*QB queries); a workgroup of kWaves waves owns 32*QB*kWaves.  Every K or V
 // operand a wave reads from LDS feeds QB MFMAs, one per query block, so LDS
-// read traffic per MFMA falls as 1/QB.
-template <int D, int kWaves, int QB>
+// read traffic per MFMA falls as 1/QB.  E is the element type.
+template <int D, int kWaves, int QB, class E = Bf16>
 struct FaState {
+  using Element = E;
   static constexpr int kQ = 32 * QB;              // queries per wave
   static constexpr int kChunks = D / 8;           // 16-byte chunks per row
   static constexpr int kTileBytes = BKV * D * 2;  // one K or V tile
@@ -250,7 +268,7 @@ struct FaState {
       lds_wait(a[r], r + kWin <= kReads ? kWin - 1 : kReads - 1 - r);
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
-        s[qb][r / kKSteps] = mfma_bf16(a[r], qreg[qb][r % kKSteps], s[qb][r / kKSteps]);
+        s[qb][r / kKSteps] = E::mfma(a[r], qreg[qb][r % kKSteps], s[qb][r / kKSteps]);
       }
       if (r + kWin < kReads) {
         a[r + kWin] = lds_read_b128(base + kaddr[(r + kWin) % kKSteps], ((r + kWin) / kKSteps) * 32 * (D * 2));
@@ -267,7 +285,7 @@ struct FaState {
     const float e1 = __builtin_amdgcn_exp2f(fmaf(sp[kb][8 * u + 2 * w + 1], scale_log2, neg_m));
     rs += e0;
     rs += e1;
-    pb[kb][u][w] = pack_bf16(e0, e1);
+    pb[kb][u][w] = E::pack(e0, e1);
   }
 
   // The clean step's two streams in one: S^T = K Q^T of the next tile (into s, as
@@ -301,7 +319,7 @@ struct FaState {
       lds_wait(a[r], r + kWin <= kReads ? kWin - 1 : kReads - 1 - r);
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
-        s[qb][r / kKSteps] = mfma_bf16(a[r], qreg[qb][r % kKSteps], s[qb][r / kKSteps]);
+        s[qb][r / kKSteps] = E::mfma(a[r], qreg[qb][r % kKSteps], s[qb][r / kKSteps]);
       }
 #pragma unroll
       for (int t = 0; t < kPer; ++t) {
@@ -335,14 +353,15 @@ struct FaState {
   }
 
   // Tile max of the raw scores of one query block over both lane halves, times
-  // scale_log2 (sm_scale > 0, so the max of the scaled scores is the scaled max).
+  // scale_log2 (sm_scale > 0, so the max of the scaled scores is the scaled max), less
+  // the type's lift.
   __device__ __forceinline__ float tile_max(const f32x16 (&s)[2]) const {
     float mt = -INFINITY;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[kb][r]);
-    return fmaxf(mt, other_half(mt)) * scale_log2;
+    return fmaxf(mt, other_half(mt)) * scale_log2 - E::kLift;
   }
 
   // The reference point of query block qb moves up to the tile max mt wherever
@@ -375,7 +394,7 @@ struct FaState {
           const float e1 = __builtin_amdgcn_exp2f(fmaf(s[kb][8 * u + 2 * w + 1], scale_log2, neg_m));
           rs += e0;
           rs += e1;
-          pb[kb][u][w] = pack_bf16(e0, e1);
+          pb[kb][u][w] = E::pack(e0, e1);
         }
     return rs;
   }
@@ -404,7 +423,7 @@ struct FaState {
       lds_wait(a[r], 2 * (r + kWin <= kOps ? kWin - 1 : kOps - 1 - r));
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
-        acc_o[qb][r / 4] = mfma_bf16(a[r], pb[qb][(r % 4) >> 1][r & 1], acc_o[qb][r / 4]);
+        acc_o[qb][r / 4] = E::mfma(a[r], pb[qb][(r % 4) >> 1][r & 1], acc_o[qb][r / 4]);
       }
       if (r + kWin < kOps) a[r + kWin] = vt_read(base, r + kWin);
     }
@@ -457,7 +476,7 @@ __device__ __forceinline__ void fa_step(FaState<D, kWaves, QB>& st, int j, int n
   if (act) {
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
-      if (__builtin_amdgcn_ballot_w64(rs[qb] > kTileSumLimit) != 0) {
+      if (__builtin_amdgcn_ballot_w64(rs[qb] > Bf16::kTileSumLimit) != 0) {
         st.raise(qb, st.tile_max(sc[qb]));
         rs[qb] = st.probs(qb, sc[qb], pb[qb]);
       }
@@ -659,8 +678,8 @@ __device__ __forceinline__ void fa_fwd_body(const FaArgs& p) {
       for (int rq = 0; rq < 4; ++rq) {
         const int d = db * 32 + rq * 8 + h * 4;
         u32x2 w;
-        w[0] = pack_bf16(st.acc_o[qb][db][rq * 4 + 0] * inv_l, st.acc_o[qb][db][rq * 4 + 1] * inv_l);
-        w[1] = pack_bf16(st.acc_o[qb][db][rq * 4 + 2] * inv_l, st.acc_o[qb][db][rq * 4 + 3] * inv_l);
+        w[0] = Bf16::pack(st.acc_o[qb][db][rq * 4 + 0] * inv_l, st.acc_o[qb][db][rq * 4 + 1] * inv_l);
+        w[1] = Bf16::pack(st.acc_o[qb][db][rq * 4 + 2] * inv_l, st.acc_o[qb][db][rq * 4 + 3] * inv_l);
         *reinterpret_cast<u32x2*>(os_ + k_off<D>(row, d >> 3) + (d & 7) * 2) = w;
       }
     }
@@ -778,7 +797,7 @@ __device__ __forceinline__ void fa_split_body(const FaArgs& p) {
     for (int qb = 0; qb < QB; ++qb) {
       if (j == wave) st.raise(qb, st.tile_max(s[qb]));
       float rs = st.probs(qb, s[qb], pb[qb]);
-      if (__builtin_amdgcn_ballot_w64(rs > kTileSumLimit) != 0) {
+      if (__builtin_amdgcn_ballot_w64(rs > Bf16::kTileSumLimit) != 0) {
         st.raise(qb, st.tile_max(s[qb]));
         rs = st.probs(qb, s[qb], pb[qb]);
       }
@@ -847,7 +866,7 @@ __device__ __forceinline__ void fa_split_body(const FaArgs& p) {
     if (q0 + row < S) {
       u32x4 w;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = pack_bf16(o[2 * e] * inv_l, o[2 * e + 1] * inv_l);
+      for (int e = 0; e < 4; ++e) w[e] = Bf16::pack(o[2 * e] * inv_l, o[2 * e + 1] * inv_l);
       *reinterpret_cast<u32x4*>(p.o + head_off + static_cast<int64_t>(q0 + row) * D + ch * 8) = w;
       if (p.lse != nullptr && ch == 0) p.lse[bh * S + q0 + row] = (m + __log2f(l_run)) * 0.69314718055994530942f;
     }

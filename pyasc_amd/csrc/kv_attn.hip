@@ -1,0 +1,236 @@
+// Attention over cached keys: asc_cross_attention_fwd (an encoder's states, of another length than
+// the queries) and asc_tree_attention (a cache in pages or in one piece, and drafted tokens behind
+// it).  The device code is kv_attn_kernels.h; here are the checks, the choice of the kernel and of
+// the split of the keys, and the workspace of the splits.
+#include "kv_attn_host.h"
+#include "kv_attn_kernels.h"
+
+namespace {
+
+using asc::kv::KvArgs;
+using asc::kv::Narrow;
+using asc::kv::Strides;
+using asc::kv::Wide;
+
+// Each kernel for a head_dim, an element type, and with (tree) or without pages and drafted keys.
+template <int D, class E, bool kTree>
+__global__ void __launch_bounds__(Wide<D>::kWaves * 64, Wide<D>::kWgPerCu) kv_wide(KvArgs p) {
+  asc::kv::kv_wide_body<D, E, kTree>(p);
+}
+template <int D, class E, bool kTree>
+__global__ void __launch_bounds__(Narrow<D>::kWaves * 64, Narrow<D>::kWgPerCu) kv_narrow(KvArgs p) {
+  asc::kv::kv_narrow_body<D, E, kTree>(p);
+}
+template <int D, class E>
+__global__ void __launch_bounds__(256) kv_join(KvArgs p) {
+  asc::kv::kv_join_body<D, E>(p);
+}
+
+struct Launch {
+  KvArgs p{};
+  bool wide = false;
+  int64_t blocks = 0;  // 0: nothing to launch
+  int64_t rows_all = 0;
+};
+
+constexpr int kMaxSplits = 64;
+constexpr int kCus = 256;
+
+// How the rows of one key / value head are taken, and over how many workgroups their keys are
+// split.  Up to 32 rows go to kv_narrow, more to kv_wide.
+void plan(Launch& L, const asc_attention_t& a) {
+  KvArgs& p = L.p;
+  L.wide = p.rows > Narrow<64>::kRows;
+  const int rows = L.wide ? (a.head_dim == 64 ? Wide<64>::kRows : Wide<128>::kRows) : Narrow<64>::kRows;
+  p.row_blocks = static_cast<int>(asc::ceil_div(p.rows, rows));
+  const int64_t shares = a.batch * a.kv_heads * p.row_blocks;
+  const int64_t slots = kCus * (a.head_dim == 64 ? 2 : 1);
+  const int64_t tiles = asc::ceil_div(p.capacity, asc::fa::BKV) + (p.k_draft ? asc::ceil_div(p.n_q, asc::fa::BKV) : 0);
+  const int64_t least = L.wide ? 4 : 8;  // tiles of a split
+  int64_t splits = shares >= slots ? 1 : 2 * slots / shares;
+  if (splits > tiles / least) splits = tiles / least;
+  if (splits > kMaxSplits) splits = kMaxSplits;
+  p.splits = splits < 1 ? 1 : static_cast<int>(splits);
+  p.units = static_cast<uint32_t>(a.batch * a.kv_heads * p.splits);
+  L.rows_all = a.batch * a.kv_heads * p.rows;
+  L.blocks = asc::ceil_div(p.units, 8) * 8 * p.row_blocks;
+}
+
+int64_t workspace_of(const Launch& L, int head_dim) {
+  if (L.blocks == 0 || L.p.splits == 1) return 0;
+  return L.rows_all * L.p.splits * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+}
+
+int32_t strides_of(const asc_rows_t& r, int64_t batch, int64_t heads, int64_t rows, int head_dim, const char* what,
+                   Strides& s) {
+  ASC_REQUIRE(((r.batch_stride | r.head_stride | r.seq_stride) & 7) == 0 && asc::aligned16(r.data), ASC_ERR_ALIGNMENT,
+              "%s: keys and values must be 16-byte aligned, with strides that are multiples of 8", what);
+  ASC_REQUIRE(r.batch_stride >= 0 && r.head_stride >= 0 && r.seq_stride >= 0, ASC_ERR_INVALID_ARG,
+              "%s: negative stride", what);
+  // the place of a row in 32 bits of 16 bytes; the last value marks none.  Each term is checked
+  // before they are added: none overflows 64 bits
+  constexpr int64_t limit = (int64_t{1} << 32) - 64;
+  const auto term = [](int64_t n, int64_t stride) {
+    return n <= 1 || stride == 0 ? 0 : (stride / 8 > limit / (n - 1) ? limit : (n - 1) * (stride / 8));
+  };
+  ASC_REQUIRE(term(batch, r.batch_stride) + term(heads, r.head_stride) + term(rows, r.seq_stride) + head_dim / 8 <= limit,
+              ASC_ERR_UNSUPPORTED, "%s: keys and values span more than 64 GiB", what);
+  // a dimension of one element is not stepped over, whatever its stride
+  s.batch = batch > 1 ? static_cast<uint32_t>(r.batch_stride / 8) : 0;
+  s.head = heads > 1 ? static_cast<uint32_t>(r.head_stride / 8) : 0;
+  s.seq = rows > 1 ? static_cast<uint32_t>(r.seq_stride / 8) : 0;
+  return ASC_OK;
+}
+
+int32_t make(const asc_attention_t* a, bool tree, const char* what, Launch& L) {
+  int32_t rc = asc::kv::check_shape(a, what);
+  if (rc != ASC_OK) return rc;
+  if (a->batch == 0 || a->q_heads == 0 || a->q_len == 0) return ASC_OK;
+  ASC_REQUIRE(asc::kv::row_operand(a->q) && asc::kv::row_operand(a->o), ASC_ERR_ALIGNMENT,
+              "%s: q and o must be 16-byte aligned, with strides that are multiples of 8", what);
+  ASC_REQUIRE(a->q.data && a->o.data, ASC_ERR_INVALID_ARG, "%s: null buffer", what);
+  KvArgs& p = L.p;
+  p.q = static_cast<const uint16_t*>(a->q.data);
+  p.o = static_cast<uint16_t*>(a->o.data);
+  p.lse = a->lse;
+  p.q_batch = a->q.batch_stride;
+  p.q_head = a->q.head_stride;
+  p.q_seq = a->q.seq_stride;
+  p.o_batch = a->o.batch_stride;
+  p.o_head = a->o.head_stride;
+  p.o_seq = a->o.seq_stride;
+  p.kv_heads = static_cast<int32_t>(a->kv_heads);
+  p.group = static_cast<int32_t>(a->q_heads / a->kv_heads);
+  p.n_q = static_cast<int32_t>(a->q_len);
+  p.rows = p.group * p.n_q;
+  p.capacity = static_cast<int32_t>(a->kv_len);
+  p.lengths = a->kv_lengths;
+  p.scale_log2 = a->sm_scale * 1.4426950408889634f;
+  const bool paged = tree && a->block_table != nullptr;
+  if (a->kv_len > 0) {
+    ASC_REQUIRE(a->k.data && a->v.data, ASC_ERR_INVALID_ARG, "%s: null buffer", what);
+    p.k = static_cast<const uint8_t*>(a->k.data);
+    p.v = static_cast<const uint8_t*>(a->v.data);
+    const int64_t batch = paged ? a->num_pages : a->batch, rows = paged ? a->page_size : a->kv_len;
+    if (paged) {
+      ASC_REQUIRE(a->page_size >= 1 && a->page_size < 1 << 30 && a->num_pages >= 1 &&
+                      a->num_pages < int64_t{1} << 31 && a->table_stride >= 0,
+                  ASC_ERR_INVALID_ARG, "%s: invalid pages (%d rows, %lld pages)", what, a->page_size,
+                  static_cast<long long>(a->num_pages));
+      p.table = a->block_table;
+      p.table_stride = a->table_stride;
+      p.num_pages = static_cast<uint32_t>(a->num_pages);
+      p.page_size = static_cast<uint32_t>(a->page_size);
+      // key / page_size = key * magic >> (31 + shift) for keys below 2^31, 2^shift >= page_size
+      while ((uint32_t{1} << p.page_shift) < p.page_size) ++p.page_shift;
+      p.page_magic = static_cast<uint32_t>(((uint64_t{1} << (31 + p.page_shift)) + p.page_size - 1) / p.page_size);
+    }
+    rc = strides_of(a->k, batch, a->kv_heads, rows, a->head_dim, what, p.ks);
+    if (rc == ASC_OK) rc = strides_of(a->v, batch, a->kv_heads, rows, a->head_dim, what, p.vs);
+    if (rc != ASC_OK) return rc;
+  }
+  if (tree) {
+    ASC_REQUIRE(a->k_draft.data && a->v_draft.data, ASC_ERR_INVALID_ARG, "%s: null drafted keys or values", what);
+    p.k_draft = static_cast<const uint8_t*>(a->k_draft.data);
+    p.v_draft = static_cast<const uint8_t*>(a->v_draft.data);
+    rc = strides_of(a->k_draft, a->batch, a->kv_heads, a->q_len, a->head_dim, what, p.kds);
+    if (rc == ASC_OK) rc = strides_of(a->v_draft, a->batch, a->kv_heads, a->q_len, a->head_dim, what, p.vds);
+    if (rc != ASC_OK) return rc;
+    p.draft_lengths = a->draft_lengths;
+    p.mask = a->tree_mask;
+    p.mask_batch = a->mask_batch_stride;
+    p.mask_row = a->mask_row_stride;
+  }
+  plan(L, *a);
+  ASC_REQUIRE(L.blocks < int64_t{1} << 22, ASC_ERR_UNSUPPORTED,
+              "%s: %lld workgroups exceed the launch grid limit", what, static_cast<long long>(L.blocks));
+  return ASC_OK;
+}
+
+template <int D, class E>
+void launch(const Launch& L, bool tree, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(L.blocks));
+  if (L.wide) {
+    hipLaunchKernelGGL((tree ? kv_wide<D, E, true> : kv_wide<D, E, false>), grid, dim3(Wide<D>::kWaves * 64), 0, stream,
+                       L.p);
+  } else {
+    hipLaunchKernelGGL((tree ? kv_narrow<D, E, true> : kv_narrow<D, E, false>), grid, dim3(Narrow<D>::kWaves * 64), 0,
+                       stream, L.p);
+  }
+  if (L.p.splits == 1) return;
+  hipLaunchKernelGGL((kv_join<D, E>), dim3(static_cast<uint32_t>(asc::ceil_div(L.rows_all * (D / 8), 256))), dim3(256),
+                     0, stream, L.p);
+}
+
+int32_t run(const asc_attention_t* a, bool tree, const char* what, void* workspace, int64_t workspace_bytes,
+            asc_stream_t stream) {
+  Launch L;
+  const int32_t rc = make(a, tree, what, L);
+  if (rc != ASC_OK || L.blocks == 0) return rc;
+  const int64_t need = workspace_of(L, a->head_dim);
+  ASC_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && asc::aligned16(workspace)), ASC_ERR_INVALID_ARG,
+              "%s: the workspace must hold %lld bytes, 16-byte aligned", what, static_cast<long long>(need));
+  if (need != 0) {
+    L.p.part_o = static_cast<float*>(workspace);
+    L.p.part_ml = L.p.part_o + L.rows_all * L.p.splits * a->head_dim;
+  }
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool f16 = a->dtype == ASC_DT_FLOAT16;
+  if (a->head_dim == 64) {
+    f16 ? launch<64, asc::fa::F16>(L, tree, s) : launch<64, asc::fa::Bf16>(L, tree, s);
+  } else {
+    f16 ? launch<128, asc::fa::F16>(L, tree, s) : launch<128, asc::fa::Bf16>(L, tree, s);
+  }
+  return asc::check_launch(what);
+}
+
+int64_t workspace(const asc_attention_t* a, bool tree, const char* what) {
+  Launch L;
+  return make(a, tree, what, L) == ASC_OK ? workspace_of(L, a->head_dim) : 0;
+}
+
+}  // namespace
+
+namespace asc {
+namespace kv {
+
+bool row_operand(const asc_rows_t& r) {
+  return aligned16(r.data) && ((r.batch_stride | r.head_stride | r.seq_stride) & 7) == 0;
+}
+
+int32_t check_shape(const asc_attention_t* a, const char* what) {
+  ASC_REQUIRE(a, ASC_ERR_INVALID_ARG, "%s: null arguments", what);
+  ASC_REQUIRE(a->dtype == ASC_DT_FLOAT16 || a->dtype == ASC_DT_BFLOAT16, ASC_ERR_UNSUPPORTED,
+              "%s: dtype %d not supported (float16, bfloat16)", what, a->dtype);
+  ASC_REQUIRE(a->head_dim == 64 || a->head_dim == 128, ASC_ERR_UNSUPPORTED, "%s: head_dim %d not supported (64, 128)",
+              what, a->head_dim);
+  ASC_REQUIRE(a->batch >= 0 && a->q_heads >= 0 && a->kv_heads >= 0 && a->q_len >= 0 && a->kv_len >= 0,
+              ASC_ERR_INVALID_ARG, "%s: negative shape", what);
+  ASC_REQUIRE(a->q_heads == 0 || (a->kv_heads > 0 && a->q_heads % a->kv_heads == 0), ASC_ERR_INVALID_ARG,
+              "%s: %lld query heads cannot share %lld key / value heads", what, static_cast<long long>(a->q_heads),
+              static_cast<long long>(a->kv_heads));
+  ASC_REQUIRE(a->sm_scale > 0.f, ASC_ERR_INVALID_ARG, "%s: sm_scale must be positive", what);
+  // rows of one key / value head, keys of one sequence and workgroups stay below 2^30, 2^30 and 2^22
+  ASC_REQUIRE(a->batch < 1 << 20 && a->q_heads < 1 << 20 && a->q_len < 1 << 30 && a->kv_len < 1 << 30 &&
+                  a->batch * a->q_heads < 1 << 20 &&
+                  (a->kv_heads == 0 || a->q_heads / a->kv_heads * a->q_len < 1 << 30),
+              ASC_ERR_UNSUPPORTED, "%s: shape too large", what);
+  return ASC_OK;
+}
+
+}  // namespace kv
+}  // namespace asc
+
+extern "C" int64_t asc_cross_attention_fwd_workspace(const asc_attention_t* args) {
+  return workspace(args, false, "asc_cross_attention_fwd_workspace");
+}
+extern "C" int32_t asc_cross_attention_fwd(const asc_attention_t* args, void* ws, int64_t ws_bytes,
+                                           asc_stream_t stream) {
+  return run(args, false, "asc_cross_attention_fwd", ws, ws_bytes, stream);
+}
+extern "C" int64_t asc_tree_attention_workspace(const asc_attention_t* args) {
+  return workspace(args, true, "asc_tree_attention_workspace");
+}
+extern "C" int32_t asc_tree_attention(const asc_attention_t* args, void* ws, int64_t ws_bytes, asc_stream_t stream) {
+  return run(args, true, "asc_tree_attention", ws, ws_bytes, stream);
+}

@@ -1,0 +1,742 @@
+// Attention of query rows over the keys of a cache, with another number of keys than queries, shared
+// key / value heads, per-sequence lengths, pages, and drafted tokens behind the cache: the device
+// code of asc_cross_attention_fwd and asc_tree_attention.
+//
+// The queries that share a key / value head are its rows: row r is query r % n_q of the head's
+// query head r / n_q.  A row's keys are the sequence's cached ones, all of them, and then the
+// drafted ones that the tree mask names; o = sum_j p_j v_j / sum_j p_j with p_j = exp(s_j - m).
+//
+// The tile products, the probabilities and the moving reference point are FaState's.  What
+// differs is where a tile's rows lie: lane l of a wave works out the place of the tile's key l (in
+// units of 16 bytes: a page of the table and a row in it, or a row of the sequence), and each
+// direct-to-LDS load takes the places of its rows from those lanes.  Rows past the last key come
+// from a row of zeros, so nothing behind a sequence is read, whatever it holds.
+//
+//  - kv_wide: a workgroup owns up to 32 rows per wave and streams the keys once for all of them,
+//    through rings of three LDS stages as fa_fwd_body.
+//  - kv_narrow: up to 32 rows; the workgroup's four waves take every fourth tile each.
+// Either way the keys may also be split over workgroups; kv_join adds the parts up.
+#pragma once
+
+#include "flash_attn_kernels.h"
+
+namespace asc {
+namespace kv {
+
+using fa::BKV;
+using fa::f32x16;
+using fa::FaState;
+using fa::other_half;
+using fa::u32x2;
+using fa::u32x4;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+struct Strides {  // in units of 16 bytes
+  uint32_t batch, head, seq;  // batch: of a page where there is a table
+};
+
+struct KvArgs {
+  const uint16_t* q;
+  uint16_t* o;
+  float* lse;  // [batch, q_heads, n_q] or null
+  int64_t q_batch, q_head, q_seq, o_batch, o_head, o_seq;  // elements
+  const uint8_t* k;
+  const uint8_t* v;
+  const uint8_t* k_draft;  // null: no drafted keys
+  const uint8_t* v_draft;
+  Strides ks, vs, kds, vds;
+  const int32_t* lengths;        // [batch] or null: capacity
+  const int32_t* draft_lengths;  // [batch] or null: n_q
+  const int32_t* table;          // [batch, table_stride] or null
+  int64_t table_stride;
+  const uint8_t* mask;  // [batch?, n_q, n_q] or null: a chain
+  int64_t mask_batch, mask_row;
+  float* part_o;   // [rows of all heads][splits][D], unnormalised
+  float* part_ml;  // [rows of all heads][splits][2]: reference point (log2), sum
+  uint32_t num_pages, page_size, page_magic, page_shift;
+  int32_t capacity;  // keys a sequence can have
+  int32_t kv_heads, group, n_q, rows, row_blocks, splits;
+  uint32_t units;  // batch * kv_heads * splits
+  float scale_log2;
+};
+
+// Place of a tile's row that has no key, and the row read instead.
+constexpr uint32_t kNone = 0xffffffffu;
+static __device__ const u32x4 kZeroRow[16] = {};
+
+// One workgroup's share: a sequence's key / value head, a block of its rows, a range of its tiles.
+struct Share {
+  int b, head, row0, split;
+  bool live;
+};
+
+// Workgroup i runs on XCD i % 8.  The row blocks of one share of keys run on one XCD one after the
+// other: they read the same keys through its L2.
+__device__ __forceinline__ Share share_of(const KvArgs& p) {
+  const uint32_t slot = blockIdx.x >> 3;
+  const uint32_t per = slot / p.row_blocks;
+  const uint32_t unit = per * 8 + (blockIdx.x & 7);
+  Share s;
+  s.live = unit < p.units;
+  const uint32_t bh = unit / p.splits;
+  s.split = static_cast<int>(unit - bh * p.splits);
+  s.b = static_cast<int>(bh / p.kv_heads);
+  s.head = static_cast<int>(bh - static_cast<uint32_t>(s.b) * p.kv_heads);
+  s.row0 = static_cast<int>(slot - per * p.row_blocks);
+  return s;
+}
+
+// kTree: there may be a table of pages, drafted keys and a mask over them.
+template <int D, int kWaves, class E, bool kTree>
+struct KvState : FaState<D, kWaves, 1, E> {
+  using Base = FaState<D, kWaves, 1, E>;
+  using Base::col;
+  using Base::h;
+  using Base::kKSteps;
+  using Base::kLoadsPerWave;
+  using Base::kRowsPerLoad;
+  using Base::kTileBytes;
+  using Base::lane;
+  using Base::wave;
+
+  int len, drafts;     // cached and drafted keys of the sequence
+  int cached;          // tiles of cached keys; the drafted ones follow in tiles of their own
+  int query;           // this lane's query (of n_q), or -1: no row
+  const int32_t* table;
+  uint32_t table_id;   // fetched entry of the tile after the next
+  uint32_t k0, v0, kd0, vd0;  // the sequence's first row (16-byte units)
+  const uint8_t* mask;
+  bool poison;         // a page or a length outside the cache: the rows' results are NaN
+
+  __device__ __forceinline__ void init(const KvArgs& p, const Share& s) {
+    const int n = p.lengths ? p.lengths[s.b] : p.capacity;
+    poison = n < 0 || n > p.capacity;
+    len = n < 0 ? 0 : (n > p.capacity ? p.capacity : n);
+    drafts = 0;
+    if constexpr (kTree) {
+      const int d = p.draft_lengths ? p.draft_lengths[s.b] : p.n_q;
+      poison = poison || d < 0 || d > p.n_q;
+      drafts = d < 0 ? 0 : (d > p.n_q ? p.n_q : d);
+    }
+    cached = (len + BKV - 1) / BKV;
+    const bool paged = kTree && p.table != nullptr;
+    k0 = s.head * p.ks.head + (paged ? 0 : s.b * p.ks.batch);
+    v0 = s.head * p.vs.head + (paged ? 0 : s.b * p.vs.batch);
+    if constexpr (kTree) {
+      table = paged ? p.table + s.b * p.table_stride : nullptr;
+      kd0 = s.head * p.kds.head + s.b * p.kds.batch;
+      vd0 = s.head * p.vds.head + s.b * p.vds.batch;
+      mask = p.mask ? p.mask + s.b * p.mask_batch : nullptr;
+      table_id = 0;
+    }
+
+    constexpr int kLanesPerRow = 64 / kRowsPerLoad;
+    const int rr = lane / kLanesPerRow, pos = lane % kLanesPerRow;
+#pragma unroll
+    for (int i = 0; i < Base::kKOffs; ++i) {
+      const int row = kRowsPerLoad * ((wave * kLoadsPerWave + i) & 3) + rr;
+      this->voff_k[i] = (pos ^ fa::kswz<D>(row)) << 4;
+    }
+    this->voff_v = (pos ^ fa::vswz<D>(rr)) << 4;
+#pragma unroll
+    for (int kk = 0; kk < kKSteps; ++kk) this->kaddr[kk] = fa::k_off<D>(col, kk * 2 + h);
+    const int g_lane = lane & 15;
+    const int tr_col = ((lane >> 4) & 1) * 16 + (g_lane & 3) * 4;
+#pragma unroll
+    for (int db = 0; db < Base::kDBlocks; ++db) {
+      this->vaddr[db] = fa::v_off<D>(h * 4 + (g_lane >> 2), db * 32 + tr_col);
+    }
+  }
+
+  __device__ __forceinline__ int tiles() const { return cached + (drafts + BKV - 1) / BKV; }
+
+  // Asks for the table entry of tile j's key of this lane, a tile ahead of its use.
+  __device__ __forceinline__ void fetch(const KvArgs& p, int j) {
+    if constexpr (!kTree) return;
+    if (table == nullptr || j >= cached) return;
+    const int key = min(j * BKV + lane, len - 1);
+    // key / page_size: the magic's error, below page_size, times key stays under 2^(31 + shift)
+    const uint32_t page =
+        static_cast<uint32_t>((static_cast<uint64_t>(key) * p.page_magic) >> (31 + p.page_shift));
+    table_id = static_cast<uint32_t>(table[page]);
+  }
+
+  // Places of tile j's keys, one per lane (of its table entry fetched before).
+  __device__ __forceinline__ void places(const KvArgs& p, int j, uint32_t& ik, uint32_t& iv) {
+    if constexpr (!kTree) {
+      const int key = j * BKV + lane;
+      ik = key < len ? k0 + key * p.ks.seq : kNone;
+      iv = key < len ? v0 + key * p.vs.seq : kNone;
+      return;
+    }
+    if (j < cached) {
+      const int key = j * BKV + lane;
+      if (table != nullptr) {
+        const uint32_t at = min(key, len - 1);
+        const uint32_t page = static_cast<uint32_t>((static_cast<uint64_t>(at) * p.page_magic) >> (31 + p.page_shift));
+        const uint32_t row = at - page * p.page_size;
+        uint32_t id = table_id;
+        const bool bad = id >= p.num_pages;
+        poison = poison || __builtin_amdgcn_ballot_w64(bad) != 0;
+        if (bad) id = 0;
+        ik = k0 + id * p.ks.batch + row * p.ks.seq;
+        iv = v0 + id * p.vs.batch + row * p.vs.seq;
+      } else {
+        ik = k0 + key * p.ks.seq;
+        iv = v0 + key * p.vs.seq;
+      }
+      if (key >= len) ik = iv = kNone;
+    } else {
+      const int key = (j - cached) * BKV + lane;
+      ik = key < drafts ? kd0 + key * p.kds.seq : kNone;
+      iv = key < drafts ? vd0 + key * p.vds.seq : kNone;
+    }
+  }
+
+  // Tile j of K (kIsV false) or V, whose rows' places the lanes hold, into one LDS stage.
+  template <bool kIsV>
+  __device__ __forceinline__ void load(const KvArgs& p, uint8_t* dst, int j, uint32_t places) const {
+    const uint8_t* base = kIsV ? p.v : p.k;
+    if (kTree && j >= cached) base = kIsV ? p.v_draft : p.k_draft;
+    const bool whole = (j + 1) * BKV <= len;
+    int wave_lds = wave * (kLoadsPerWave * 1024);
+    asm volatile("" : "+s"(wave_lds));
+    constexpr int kLanesPerRow = 64 / kRowsPerLoad;
+    const int rr = lane / kLanesPerRow;
+#pragma unroll
+    for (int i = 0; i < kLoadsPerWave; ++i) {
+      const int row = kRowsPerLoad * (wave * kLoadsPerWave + i) + rr;
+      const uint32_t at =
+          static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(row * 4, static_cast<int>(places)));
+      const uint8_t* src = base + static_cast<uint64_t>(at) * 16;
+      if (!whole) src = at == kNone ? reinterpret_cast<const uint8_t*>(kZeroRow) : src;
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)(src + (kIsV ? this->voff_v : this->voff_k[i & 3])),
+          (__attribute__((address_space(3))) void*)(dst + wave_lds + i * 1024), 16, 0, 0);
+    }
+  }
+
+  __device__ __forceinline__ bool needs_mask(int j) const { return (j + 1) * BKV > len; }
+
+  // Scores of tile j: -inf for keys that the lane's row does not attend.
+  __device__ __forceinline__ void hide(const KvArgs& p, f32x16 (&s)[1][2], int j) const {
+    if (!kTree || j < cached) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if (j * BKV + kb * 32 + (r >> 2) * 8 + h * 4 + (r & 3) >= len) s[0][kb][r] = -INFINITY;
+        }
+      return;
+    }
+    // one bit per score register pair of blocks, gathered in a loop: unrolled, its addresses and
+    // the wave's accumulators would not fit the registers
+    const int first = (j - cached) * BKV + h * 4;
+    const uint8_t* row = mask ? mask + static_cast<int64_t>(query < 0 ? 0 : query) * p.mask_row : nullptr;
+    uint32_t seen = 0;
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {  // four keys of register group i % 4 of block i / 4
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = first + i * 8 + e;
+        const bool on = row ? row[min(key, p.n_q - 1)] != 0 : key <= query;
+        seen |= (on && key < drafts && query >= 0 ? 1u : 0u) << (i * 4 + e);
+      }
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        if (!((seen >> (kb * 16 + r)) & 1)) s[0][kb][r] = -INFINITY;
+      }
+  }
+
+  // A row that has had no key yet has no reference point: it takes the tile's.
+  __device__ __forceinline__ void first_point(const f32x16 (&s)[1][2]) {
+    if (__builtin_amdgcn_ballot_w64(this->m_run[0] == -INFINITY) != 0) this->raise(0, this->tile_max(s[0]));
+  }
+
+  // Whether a value of the V tile is infinite or NaN.
+  __device__ __forceinline__ bool has_infinite(const uint8_t* vs) const {
+    constexpr uint32_t kExp = __is_same(E, fa::Bf16) ? 0x7f80u : 0x7c00u;
+    bool found = false;
+    for (int i = 0; i < kTileBytes / 1024; ++i) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(vs + i * 1024 + lane * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        found = found || (w[e] & kExp) == kExp || ((w[e] >> 16) & kExp) == kExp;
+      }
+    }
+    return __builtin_amdgcn_ballot_w64(found) != 0;
+  }
+
+  // O^T += V^T P^T without the keys of probability zero: a drafted token that a row does not attend
+  // may hold infinities or NaN, and 0 times those is not 0.  Rare, so one key after the other.
+  __device__ __forceinline__ void pv_attended(const uint8_t* vs, const u32x4 (&pb)[2][2]) {
+    typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+#pragma unroll 1
+    for (int key = 0; key < BKV; ++key) {
+      // key 32 kb + 16 u + 8 w2 + 4 half + 2 w1 + e lies in half `half`, word 2 w2 + w1 of pb[kb][u]
+      uint32_t word = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int at = ((key >> 5) << 3) + (((key >> 4) & 1) << 2) + (((key >> 3) & 1) << 1) + ((key >> 1) & 1);
+        if (at == i) word = pb[i >> 3][(i >> 2) & 1][i & 3];
+      }
+      uint32_t bits = (key & 1) ? word >> 16 : word & 0xffffu;
+      const uint32_t theirs = __builtin_bit_cast(uint32_t, other_half(__builtin_bit_cast(float, bits)));
+      if (((key >> 2) & 1) != h) bits = theirs;
+      const float prob = to_float(static_cast<uint16_t>(bits));
+#pragma unroll
+      for (int db = 0; db < Base::kDBlocks; ++db)
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq) {
+          const u16x4 x = *reinterpret_cast<const u16x4*>(vs + fa::v_off<D>(key, db * 32 + rq * 8 + h * 4));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float value = prob == 0.f ? 0.f : to_float(x[e]);
+            this->acc_o[0][db][rq * 4 + e] = fmaf(prob, value, this->acc_o[0][db][rq * 4 + e]);
+          }
+        }
+    }
+  }
+  static __device__ __forceinline__ float to_float(uint16_t bits) {
+    return __is_same(E, fa::Bf16) ? bf16_to_f32(bits) : f16_to_f32(bits);
+  }
+
+  // O^T += V^T P^T of tile j.
+  __device__ __forceinline__ void add_values(const uint8_t* vs, const u32x4 (&pb)[1][2][2], int j) {
+    if (kTree && j >= cached && has_infinite(vs)) {
+      pv_attended(vs, pb[0]);
+    } else {
+      this->pv(vs, pb);
+    }
+  }
+
+  // This lane's row of the block: its query and where its output and statistics lie.
+  __device__ __forceinline__ void set_query(const KvArgs& p, const Share& s, int row, int64_t& q_at) {
+    query = -1;
+    q_at = 0;
+    if (row < p.rows) {
+      const int g = row / p.n_q;
+      query = row - g * p.n_q;
+      q_at = s.b * p.q_batch + static_cast<int64_t>(s.head * p.group + g) * p.q_head + query * p.q_seq;
+    }
+  }
+
+  __device__ __forceinline__ void load_query(const KvArgs& p, int64_t q_at) {
+#pragma unroll
+    for (int ks = 0; ks < kKSteps; ++ks) {
+      this->qreg[0][ks] = u32x4{0, 0, 0, 0};
+      if (query >= 0) this->qreg[0][ks] = *reinterpret_cast<const u32x4*>(p.q + q_at + ks * 16 + h * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < Base::kDBlocks; ++i) this->acc_o[0][i] = f32x16{};
+    this->m_run[0] = -INFINITY;
+    this->l_part[0] = 0.f;
+    this->scale_log2 = p.scale_log2;
+  }
+};
+
+// Output row `row` of the share: its query and head, false where nothing is written.
+__device__ __forceinline__ bool out_row(const KvArgs& p, const Share& s, int row, int written, int64_t& o_at,
+                                        int64_t& lse_at) {
+  if (row >= p.rows) return false;
+  const int g = row / p.n_q, query = row - g * p.n_q;
+  if (query >= written) return false;
+  const int64_t head = s.head * p.group + g;
+  o_at = s.b * p.o_batch + head * p.o_head + query * p.o_seq;
+  lse_at = (static_cast<int64_t>(s.b) * p.kv_heads * p.group + head) * p.n_q + query;
+  return true;
+}
+
+// Queries of sequence b that are written: those behind its drafted tokens are left as they were.
+__device__ __forceinline__ int written_of(const KvArgs& p, int b) {
+  return p.k_draft && p.draft_lengths ? p.draft_lengths[b] : p.n_q;
+}
+
+// 0 for a row without keys; NaN stays NaN.
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.0f / l; }
+
+__device__ __forceinline__ float lse_of(float m, float l) { return (m + __log2f(l)) * 0.69314718055994530942f; }
+
+// One pipeline step for tile j of [.., end), as fa_step: on entry LDS holds K_{j+1} and V_j, sc the
+// masked scores of tile j.  iv2: places of V_{j+2}; the table entry of tile j+3 has been fetched.
+// kGuard false: tiles j+1 .. j+3 exist and tile j+1 is whole.
+template <bool kGuard, class St>
+__device__ __forceinline__ void kv_step(St& st, const KvArgs& p, int j, int end, uint8_t* ring, int c, bool act,
+                                        uint32_t& iv2, f32x16 (&sc)[1][2], f32x16 (&sn)[1][2]) {
+  constexpr int T = St::kTileBytes;
+  constexpr int L = St::kLoadsPerWave;
+  const int c1 = c == 2 ? 0 : c + 1;
+  const int c2 = c == 0 ? 2 : c - 1;
+  const bool has_next = !kGuard || j + 1 < end;
+  const bool load_v = !kGuard || j + 2 < end;
+  const bool load_k = !kGuard || j + 3 < end;
+  uint32_t ik3 = 0, iv3 = 0;
+  if (load_k) {
+    st.places(p, j + 3, ik3, iv3);
+    st.fetch(p, j + 4);
+  }
+  if (load_v) st.template load<true>(p, ring + (3 + c2) * T, j + 2, iv2);
+  if (load_k) st.template load<false>(p, ring + c * T, j + 3, ik3);
+  iv2 = iv3;
+  u32x4 pb[1][2][2];
+  float rs[1];
+  if (!kGuard || act) {
+    st.first_point(sc);
+    if constexpr (kGuard) {
+      rs[0] = st.probs(0, sc[0], pb[0]);
+    } else {
+      st.scores_probs(ring + c1 * T, sn, sc, pb, rs);
+    }
+    if (__builtin_amdgcn_ballot_w64(rs[0] > St::Element::kTileSumLimit) != 0) {
+      st.raise(0, st.tile_max(sc[0]));
+      rs[0] = st.probs(0, sc[0], pb[0]);
+    }
+    st.l_part[0] += rs[0];
+    if (kGuard) {
+      st.add_values(ring + (3 + c) * T, pb, j);
+      if (has_next) {
+        st.scores(ring + c1 * T, sn);
+        if (st.needs_mask(j + 1)) st.hide(p, sn, j + 1);
+      }
+    } else {
+      st.pv(ring + (3 + c) * T, pb);
+    }
+  }
+  if (load_v && load_k) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * L) : "memory");
+  } else if (load_v || load_k) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(L) : "memory");
+  } else {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  }
+  asm volatile("s_barrier" ::: "memory");
+}
+
+template <int D>
+struct Wide {
+  static constexpr int kWaves = D == 128 ? 8 : 4, kWgPerCu = D == 128 ? 1 : 2;
+  static constexpr int kRows = 32 * kWaves;
+};
+
+template <int D, class E, bool kTree>
+__device__ __forceinline__ void kv_wide_body(const KvArgs& p) {
+  constexpr int kWaves = Wide<D>::kWaves;
+  using St = KvState<D, kWaves, E, kTree>;
+  constexpr int T = St::kTileBytes;
+  constexpr int L = St::kLoadsPerWave;
+  constexpr int kThreads = kWaves * 64;
+  constexpr int kChunks = D / 8;
+  __shared__ __attribute__((aligned(16))) uint8_t ring[6 * T];
+
+  Share s = share_of(p);
+  if (!s.live) return;
+  s.row0 *= Wide<D>::kRows;
+  St st;
+  const int tid = threadIdx.x;
+  if (kWaves == 8 && (tid >> 6) < 4) __builtin_amdgcn_s_setprio(1);
+  st.lane = tid & 63;
+  st.wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  st.col = st.lane & 31;
+  st.h = st.lane >> 5;
+  st.init(p, s);
+  const int wave_row = s.row0 + st.wave * 32;
+  const bool act = wave_row < p.rows;
+  int64_t q_at;
+  st.set_query(p, s, wave_row + st.col, q_at);
+  st.load_query(p, q_at);
+
+  const int total = st.tiles();
+  const int per = (total + p.splits - 1) / p.splits;
+  const int begin = min(total, s.split * per), end = min(total, begin + per);
+  if (begin < end) {
+    uint32_t ik, iv0, iv1 = 0, iv2 = 0;
+    const auto place = [&](int j, uint32_t& iv) {  // K_j goes out; its values' places stay
+      st.fetch(p, j);
+      st.places(p, j, ik, iv);
+    };
+    place(begin, iv0);
+    st.template load<false>(p, ring, begin, ik);
+    st.template load<true>(p, ring + 3 * T, begin, iv0);
+    if (begin + 1 < end) {
+      place(begin + 1, iv1);
+      st.template load<false>(p, ring + T, begin + 1, ik);
+      st.template load<true>(p, ring + 4 * T, begin + 1, iv1);
+    }
+    if (begin + 2 < end) {
+      place(begin + 2, iv2);
+      st.template load<false>(p, ring + 2 * T, begin + 2, ik);
+      st.fetch(p, begin + 3);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * L) : "memory");
+    } else if (begin + 1 < end) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    asm volatile("s_barrier" ::: "memory");
+    f32x16 sa[1][2], sb[1][2];
+    st.scores(ring, sa);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    asm volatile("s_barrier" ::: "memory");
+    if (st.needs_mask(begin)) st.hide(p, sa, begin);
+    const int clean = st.len / BKV;  // whole tiles; the drafted ones are masked
+    int j = begin, c = 0;
+    if (act) {
+      for (; j + 4 < min(clean, end); j += 2) {
+        kv_step<false>(st, p, j, end, ring, c, true, iv2, sa, sb);
+        c = c == 2 ? 0 : c + 1;
+        kv_step<false>(st, p, j + 1, end, ring, c, true, iv2, sb, sa);
+        c = c == 2 ? 0 : c + 1;
+      }
+    }
+    for (; j < end; j += 2) {
+      kv_step<true>(st, p, j, end, ring, c, act, iv2, sa, sb);
+      c = c == 2 ? 0 : c + 1;
+      if (j + 1 < end) kv_step<true>(st, p, j + 1, end, ring, c, act, iv2, sb, sa);
+      c = c == 2 ? 0 : c + 1;
+    }
+  }
+
+  float l_run = st.l_part[0] + other_half(st.l_part[0]);
+  if (st.poison) l_run = __builtin_nanf("");
+  const int written = written_of(p, s.b);
+  if (p.splits > 1) {
+    // the unnormalised part, from registers: lane (row, half h) holds d = 32 db + 8 rq + 4 h + 0..3
+    const int row = wave_row + st.col;
+    if (row < p.rows) {
+      const int64_t at =
+          ((static_cast<int64_t>(s.b) * p.kv_heads + s.head) * p.rows + row) * p.splits + s.split;
+      if (st.h == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(st.m_run[0], l_run);
+      if (begin < end) {
+#pragma unroll
+        for (int db = 0; db < St::kDBlocks; ++db)
+#pragma unroll
+          for (int rq = 0; rq < 4; ++rq) {
+            const f32x16& a = st.acc_o[0][db];
+            *reinterpret_cast<f32x4*>(p.part_o + at * D + db * 32 + rq * 8 + st.h * 4) =
+                f32x4{a[rq * 4], a[rq * 4 + 1], a[rq * 4 + 2], a[rq * 4 + 3]};
+          }
+      }
+    }
+    return;
+  }
+  // rows of the block through the rings (no load is in flight): 64 rows per stage
+  const float inv = inverse_sum(l_run);
+  {
+    const int brow = st.wave * 32 + st.col;
+    uint8_t* os = ring + (brow >> 6) * T;
+#pragma unroll
+    for (int db = 0; db < St::kDBlocks; ++db)
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        const f32x16& a = st.acc_o[0][db];
+        u32x2 w;
+        w[0] = E::pack(a[rq * 4] * inv, a[rq * 4 + 1] * inv);
+        w[1] = E::pack(a[rq * 4 + 2] * inv, a[rq * 4 + 3] * inv);
+        *reinterpret_cast<u32x2*>(os + fa::k_off<D>(brow & 63, db * 4 + rq) + st.h * 8) = w;
+      }
+    int64_t o_at, lse_at;
+    if (p.lse != nullptr && st.h == 0 && out_row(p, s, s.row0 + brow, written, o_at, lse_at)) {
+      p.lse[lse_at] = lse_of(st.m_run[0], l_run);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < Wide<D>::kRows * kChunks / kThreads; ++i) {
+    const int cc = tid + kThreads * i;
+    const int row = cc / kChunks, ch = cc % kChunks;
+    int64_t o_at, lse_at;
+    if (!out_row(p, s, s.row0 + row, written, o_at, lse_at)) continue;
+    *reinterpret_cast<u32x4*>(p.o + o_at + ch * 8) =
+        *reinterpret_cast<const u32x4*>(ring + (row >> 6) * T + fa::k_off<D>(row & 63, ch));
+  }
+}
+
+template <int D>
+struct Narrow {
+  static constexpr int kWaves = 4, kWgPerCu = D == 64 ? 2 : 1;
+  static constexpr int kRows = 32;
+};
+
+template <int D, class E, bool kTree>
+__device__ __forceinline__ void kv_narrow_body(const KvArgs& p) {
+  using St = KvState<D, 1, E, kTree>;
+  constexpr int kWaves = Narrow<D>::kWaves;
+  constexpr int T = St::kTileBytes;
+  constexpr int L = St::kLoadsPerWave;
+  constexpr int kRow = D * 4;
+  static_assert(Narrow<D>::kRows * kRow <= 2 * T, "a wave's part reuses its tiles");
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves * 2 * T];
+  __shared__ float stats[2][kWaves][Narrow<D>::kRows];
+
+  Share s = share_of(p);
+  if (!s.live) return;
+  s.row0 *= Narrow<D>::kRows;
+  St st;
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  uint8_t* kring = lds + wave * 2 * T;
+  uint8_t* vring = kring + T;
+  st.lane = tid & 63;
+  st.wave = 0;
+  st.col = st.lane & 31;
+  st.h = st.lane >> 5;
+  st.init(p, s);
+  int64_t q_at;
+  st.set_query(p, s, s.row0 + st.col, q_at);
+  st.load_query(p, q_at);
+
+  const int total = st.tiles();
+  const int per = (total + p.splits - 1) / p.splits;
+  const int begin = min(total, s.split * per), end = min(total, begin + per);
+  uint32_t ik = 0, iv = 0, iv_next = 0;
+  if (begin + wave < end) {
+    st.fetch(p, begin + wave);
+    st.places(p, begin + wave, ik, iv);
+    st.template load<false>(p, kring, begin + wave, ik);
+    st.template load<true>(p, vring, begin + wave, iv);
+    st.fetch(p, begin + wave + kWaves);
+  }
+  for (int j = begin + wave; j < end; j += kWaves) {
+    const bool next = j + kWaves < end;
+    // all but V_j (and a table entry behind it) have landed
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");
+    f32x16 sc[1][2];
+    st.scores(kring, sc);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (next) {
+      st.places(p, j + kWaves, ik, iv_next);
+      st.template load<false>(p, kring, j + kWaves, ik);
+    }
+    if (st.needs_mask(j)) st.hide(p, sc, j);
+    st.first_point(sc);
+    u32x4 pb[1][2][2];
+    float rs = st.probs(0, sc[0], pb[0]);
+    if (__builtin_amdgcn_ballot_w64(rs > E::kTileSumLimit) != 0) {
+      st.raise(0, st.tile_max(sc[0]));
+      rs = st.probs(0, sc[0], pb[0]);
+    }
+    st.l_part[0] += rs;
+    if (next) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");  // all but K of the next tile
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    st.add_values(vring, pb, j);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (next) {
+      st.template load<true>(p, vring, j + kWaves, iv_next);
+      st.fetch(p, j + 2 * kWaves);
+    }
+  }
+
+  // the waves' parts, relative to their own reference points, through LDS
+  const auto part_off = [](int row, int c) { return row * kRow + ((c ^ (row & 15)) << 4); };
+  {
+    float l = st.l_part[0] + other_half(st.l_part[0]);
+    if (st.poison) l = __builtin_nanf("");
+    if (st.h == 0) {
+      stats[0][wave][st.col] = st.m_run[0];
+      stats[1][wave][st.col] = l;
+    }
+#pragma unroll
+    for (int db = 0; db < St::kDBlocks; ++db)
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        const f32x16& a = st.acc_o[0][db];
+        *reinterpret_cast<f32x4*>(kring + part_off(st.col, db * 8 + rq * 2 + st.h)) =
+            f32x4{a[rq * 4], a[rq * 4 + 1], a[rq * 4 + 2], a[rq * 4 + 3]};
+      }
+  }
+  __syncthreads();
+  const int written = written_of(p, s.b);
+#pragma unroll
+  for (int i = 0; i < Narrow<D>::kRows * (D / 8) / (kWaves * 64); ++i) {
+    const int cc = tid + kWaves * 64 * i;
+    const int row = cc / (D / 8), ch = cc % (D / 8);
+    if (s.row0 + row >= p.rows) continue;
+    float m = stats[0][0][row];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, stats[0][w][row]);
+    float f[kWaves], l_run = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float mw = stats[0][w][row];
+      f[w] = mw == m ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
+      l_run += f[w] * stats[1][w][row];
+    }
+    float o[8] = {};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const uint8_t* part = lds + w * 2 * T;
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(part + part_off(row, 2 * ch));
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(part + part_off(row, 2 * ch + 1));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[e] = fmaf(f[w], lo[e], o[e]);
+        o[4 + e] = fmaf(f[w], hi[e], o[4 + e]);
+      }
+    }
+    if (p.splits > 1) {
+      const int64_t at =
+          ((static_cast<int64_t>(s.b) * p.kv_heads + s.head) * p.rows + s.row0 + row) * p.splits + s.split;
+      if (ch == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m, l_run);
+      *reinterpret_cast<f32x4*>(p.part_o + at * D + ch * 8) = f32x4{o[0], o[1], o[2], o[3]};
+      *reinterpret_cast<f32x4*>(p.part_o + at * D + ch * 8 + 4) = f32x4{o[4], o[5], o[6], o[7]};
+      continue;
+    }
+    int64_t o_at, lse_at;
+    if (!out_row(p, s, s.row0 + row, written, o_at, lse_at)) continue;
+    const float inv = inverse_sum(l_run);
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = E::pack(o[2 * e] * inv, o[2 * e + 1] * inv);
+    *reinterpret_cast<u32x4*>(p.o + o_at + ch * 8) = w;
+    if (p.lse != nullptr && ch == 0) p.lse[lse_at] = lse_of(m, l_run);
+  }
+}
+
+// Adds up the splits of a row: D / 8 lanes per row, relative to the largest reference point.
+template <int D, class E>
+__device__ __forceinline__ void kv_join_body(const KvArgs& p) {
+  constexpr int kLanes = D / 8;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t row_all = i / kLanes;
+  const int ch = static_cast<int>(i % kLanes);
+  const int64_t bh = row_all / p.rows;
+  Share s;
+  s.b = static_cast<int>(bh / p.kv_heads);
+  s.head = static_cast<int>(bh - static_cast<int64_t>(s.b) * p.kv_heads);
+  if (bh >= static_cast<int64_t>(p.units / p.splits)) return;
+  int64_t o_at, lse_at;
+  if (!out_row(p, s, static_cast<int>(row_all - bh * p.rows), written_of(p, s.b), o_at, lse_at)) return;
+  const float* ml = p.part_ml + row_all * p.splits * 2;
+  float m = -INFINITY;
+  for (int k = 0; k < p.splits; ++k) m = fmaxf(m, ml[2 * k]);
+  float l_run = 0.f, o[8] = {};
+  for (int k = 0; k < p.splits; ++k) {
+    const float l = ml[2 * k + 1];
+    if (l == 0.f) continue;  // no keys: its part is not written
+    const float f = ml[2 * k] == m ? 1.0f : __builtin_amdgcn_exp2f(ml[2 * k] - m);
+    l_run += f * l;
+    const float* part = p.part_o + (row_all * p.splits + k) * D + ch * 8;
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(part), hi = *reinterpret_cast<const f32x4*>(part + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[e] = fmaf(f, lo[e], o[e]);
+      o[4 + e] = fmaf(f, hi[e], o[4 + e]);
+    }
+  }
+  const float inv = inverse_sum(l_run);
+  u32x4 w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = E::pack(o[2 * e] * inv, o[2 * e + 1] * inv);
+  *reinterpret_cast<u32x4*>(p.o + o_at + ch * 8) = w;
+  if (p.lse != nullptr && ch == 0) p.lse[lse_at] = lse_of(m, l_run);
+}
+
+}  // namespace kv
+}  // namespace asc

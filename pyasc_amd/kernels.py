@@ -789,6 +789,141 @@ def qk_norm_rotary_bwd(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q: 
     _native.call("asc_qk_norm_rotary_bwd", ctypes.byref(a), workspace.data_ptr() if nbytes else 0, nbytes, handle)
 
 
+# ------------------------------------------------- attention over other keys than the queries' own
+
+_HALVES = (torch.float16, torch.bfloat16)
+
+
+def _aligned_rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    """Rows that are read and written 16 bytes at a time."""
+    if t.data_ptr() % 16 or any(t.stride(i) % 8 for i in range(3) if t.shape[i] > 1):
+        raise ValueError(f"'{name}' must be 16-byte aligned, with strides that are multiples of 8 elements "
+                         f"(address {t.data_ptr():#x}, strides {t.stride()})")
+    return t
+
+
+def _wide_rows(t: torch.Tensor) -> "_native.Rows":
+    """_rows of a tensor checked by _aligned_rows: a dimension of one element is not stepped over."""
+    s = [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
+    return _native.Rows(t.data_ptr(), *s)
+
+
+def _counts(t: Optional[torch.Tensor], name: str, shape: tuple) -> int:
+    if t is None:
+        return 0
+    _contiguous(_here(t, name), name)
+    if t.dtype != torch.int32 or tuple(t.shape) != shape:
+        raise ValueError(f"'{name}' must be int32 {list(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _kv_args(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, sm_scale: float,
+             lse: Optional[torch.Tensor], pages: bool, names: tuple) -> "_native.AttentionArgs":
+    """Checks queries, keys, values and results; ``pages``: the first dimension of k is not the batch's."""
+    if not isinstance(q, torch.Tensor):
+        raise TypeError(f"'q' must be a torch.Tensor, got {type(q).__name__}")
+    if q.dtype not in _HALVES:
+        raise TypeError(f"'q' has unsupported dtype {q.dtype}; expected one of {sorted(map(str, _HALVES))}")
+    _aligned_rows(_bhsd(q, "q", q.dtype), "q")
+    batch, heads, q_len, head_dim = q.shape
+    if head_dim not in FA_HEAD_DIMS:
+        raise ValueError(f"head_dim {head_dim} not supported (supported: {FA_HEAD_DIMS})")
+    _aligned_rows(_bhsd(o, "o", q.dtype, tuple(q.shape), written=True), "o")
+    _aligned_rows(_bhsd(k, names[0], q.dtype), names[0])
+    if k.shape[3] != head_dim or (not pages and k.shape[0] != batch):
+        raise ValueError(f"'{names[0]}' {tuple(k.shape)} does not fit q {tuple(q.shape)}")
+    _aligned_rows(_bhsd(v, names[1], q.dtype, tuple(k.shape)), names[1])
+    if k.shape[1] == 0 or heads % k.shape[1]:
+        raise ValueError(f"{heads} query heads cannot share {k.shape[1]} key / value heads")
+    if not sm_scale > 0:
+        raise ValueError(f"sm_scale must be positive, got {sm_scale}")
+    a = _native.AttentionArgs()
+    a.dtype, a.head_dim, a.sm_scale = _DTYPE_CODES[q.dtype], head_dim, sm_scale
+    a.batch, a.q_heads, a.kv_heads, a.q_len, a.kv_len = batch, heads, k.shape[1], q_len, k.shape[2]
+    a.q, a.o, a.k, a.v = _wide_rows(q), _wide_rows(o), _wide_rows(k), _wide_rows(v)
+    if lse is not None:
+        _contiguous(_here(lse, "lse"), "lse")
+        if lse.dtype != torch.float32 or tuple(lse.shape) != (batch, heads, q_len):
+            raise ValueError("lse must be float32 [batch, heads, q_len]")
+        a.lse = lse.data_ptr()
+    return a
+
+
+def _attend(entry: str, a: "_native.AttentionArgs", device: torch.device, stream: Any, what: str) -> None:
+    """Calls an attention entry with the workspace that it asks for."""
+    handle = _stream(stream)
+    nbytes = getattr(_native.load_library(), entry + "_workspace")(ctypes.byref(a))
+    workspace = _workspace(nbytes, handle, device, what) if nbytes else None
+    _native.call(entry, ctypes.byref(a), workspace.data_ptr() if nbytes else 0, nbytes, handle)
+
+
+def cross_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, sm_scale: float,
+                        kv_lengths: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                        stream: Any = None) -> None:
+    """o = softmax(q k^T * sm_scale) v for float16 or bfloat16 queries [batch, heads, q_len, head_dim]
+    over keys and values [batch, kv_heads, kv_len, head_dim] (an encoder's states: any length, heads
+    a multiple of kv_heads, head_dim 64 or 128), all of any strides that are multiples of 8 elements
+    with a contiguous last dimension.  ``kv_lengths`` (int32 [batch]): the keys of each sequence;
+    what lies behind them is not read.  A sequence without keys gets zeros.  ``lse`` (float32
+    [batch, heads, q_len]) receives the log-sum-exp, -inf without keys.  A length outside
+    [0, kv_len] is not followed: its sequence's results are NaN."""
+    a = _kv_args(q, k, v, o, sm_scale, lse, False, ("k", "v"))
+    a.kv_lengths = _counts(kv_lengths, "kv_lengths", (q.shape[0],))
+    _attend("asc_cross_attention_fwd", a, q.device, stream, "cross_attention_fwd")
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cache_lengths: torch.Tensor,
+                   k_draft: torch.Tensor, v_draft: torch.Tensor, tree_mask: Optional[torch.Tensor],
+                   o: torch.Tensor, sm_scale: float, block_table: Optional[torch.Tensor] = None,
+                   draft_lengths: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                   stream: Any = None) -> None:
+    """Attention of a tree of drafted tokens (a single one: plain decoding) over a cache and
+    themselves: o = softmax(s) v with s = q k^T * sm_scale over the cached keys and the drafted ones
+    that the mask names, for float16 or bfloat16 q [batch, heads, n, head_dim].
+
+    - k_cache, v_cache: [batch, kv_heads, length, head_dim], or with ``block_table`` (int32
+      [batch, pages of a sequence]) [pages, kv_heads, page size, head_dim]: key j of sequence b
+      lies in page block_table[b, j // page_size], row j % page_size.  cache_lengths (int32
+      [batch]): the cached keys, all of which every token attends.
+    - k_draft, v_draft: [batch, kv_heads, n, head_dim], not in the cache yet.  tree_mask (bool
+      [n, n] or [batch, n, n]): whether token i attends token j (its ancestors and itself); None: a
+      chain, j <= i.  draft_lengths (int32 [batch]): tokens of each sequence, default n; the rows of
+      o and lse behind them are left as they were.
+
+    Strides and the last dimension as in cross_attention_fwd.  A token that attends nothing gets zeros
+    and an lse of -inf.  A length outside the cache, or a page outside it that a length reaches, is
+    not followed: the sequence's results are NaN."""
+    a = _kv_args(q, k_cache, v_cache, o, sm_scale, lse, block_table is not None, ("k_cache", "v_cache"))
+    batch, _, n, head_dim = q.shape
+    a.kv_lengths = _counts(_device_tensor(cache_lengths, "cache_lengths"), "cache_lengths", (batch,))
+    shape = (batch, k_cache.shape[1], n, head_dim)
+    a.k_draft = _wide_rows(_aligned_rows(_bhsd(k_draft, "k_draft", q.dtype, shape), "k_draft"))
+    a.v_draft = _wide_rows(_aligned_rows(_bhsd(v_draft, "v_draft", q.dtype, shape), "v_draft"))
+    if block_table is not None:
+        _here(block_table, "block_table")
+        if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch:
+            raise ValueError(f"'block_table' must be int32 [batch, pages], got {block_table.dtype} "
+                             f"{tuple(block_table.shape)}")
+        if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+            raise ValueError("the last dimension of 'block_table' must be contiguous")
+        a.num_pages, a.page_size = k_cache.shape[0], k_cache.shape[2]
+        a.kv_len = block_table.shape[1] * k_cache.shape[2]
+        if a.num_pages == 0 and a.kv_len:
+            raise ValueError("a cache without pages needs a block_table without columns")
+        a.block_table, a.table_stride = block_table.data_ptr(), block_table.stride(0)
+    if tree_mask is not None:
+        _here(tree_mask, "tree_mask")
+        if tree_mask.dtype != torch.bool or tuple(tree_mask.shape) not in ((n, n), (batch, n, n)):
+            raise ValueError(f"'tree_mask' must be bool [{n}, {n}] or [{batch}, {n}, {n}], got {tree_mask.dtype} "
+                             f"{tuple(tree_mask.shape)}")
+        if n > 1 and tree_mask.stride(-1) != 1:
+            raise ValueError("the last dimension of 'tree_mask' must be contiguous")
+        a.tree_mask, a.mask_row_stride = tree_mask.data_ptr(), tree_mask.stride(-2)
+        a.mask_batch_stride = tree_mask.stride(0) if tree_mask.dim() == 3 else 0
+    a.draft_lengths = _counts(draft_lengths, "draft_lengths", (batch,))
+    _attend("asc_tree_attention", a, q.device, stream, "tree_attention")
+
+
 # ------------------------------------------------------------------ element-wise tile operations
 
 UNARY_OPS = ("abs", "ceil", "cos", "cosh", "erf", "exp", "exp2", "floor", "log", "log2", "negative", "relu",

@@ -128,6 +128,8 @@ SIGNATURES = {
     "asc_qk_norm_rotary_bwd": [ctypes.POINTER(RotaryArgs), _c_p, _c_i64, _c_p],
     "asc_cross_attention_fwd_workspace": [ctypes.POINTER(AttentionArgs)],
     "asc_cross_attention_fwd": [ctypes.POINTER(AttentionArgs), _c_p, _c_i64, _c_p],
+    "asc_cross_attention_bwd_workspace": [ctypes.POINTER(AttentionArgs)],
+    "asc_cross_attention_bwd": [ctypes.POINTER(AttentionArgs), _c_p, _c_i64, _c_p],
     "asc_tree_attention_workspace": [ctypes.POINTER(AttentionArgs)],
     "asc_tree_attention": [ctypes.POINTER(AttentionArgs), _c_p, _c_i64, _c_p],
     "asc_unary_f32": [_c_i32, _c_p, _c_p, _c_i64, _c_p],
@@ -143,6 +145,7 @@ SIGNATURES = {
     "asc_quant_i8": [_c_i32, _c_p, _c_p, _c_f64, _c_f64, _c_i64, _c_p],
 }
 INT64_FUNCS = ("asc_qk_norm_rotary_bwd_workspace", "asc_cross_attention_fwd_workspace",
+               "asc_cross_attention_bwd_workspace",
                "asc_tree_attention_workspace")
 # entry points returning a C string
 STRING_FUNCS = ("asc_last_error", "asc_version")

@@ -9,7 +9,6 @@ namespace {
 
 using asc::kv::KvArgs;
 using asc::kv::Narrow;
-using asc::kv::Strides;
 using asc::kv::Wide;
 
 // Each kernel for a head_dim, an element type, and with (tree) or without pages and drafted keys.
@@ -61,27 +60,6 @@ int64_t workspace_of(const Launch& L, int head_dim) {
   return L.rows_all * L.p.splits * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
-int32_t strides_of(const asc_rows_t& r, int64_t batch, int64_t heads, int64_t rows, int head_dim, const char* what,
-                   Strides& s) {
-  ASC_REQUIRE(((r.batch_stride | r.head_stride | r.seq_stride) & 7) == 0 && asc::aligned16(r.data), ASC_ERR_ALIGNMENT,
-              "%s: keys and values must be 16-byte aligned, with strides that are multiples of 8", what);
-  ASC_REQUIRE(r.batch_stride >= 0 && r.head_stride >= 0 && r.seq_stride >= 0, ASC_ERR_INVALID_ARG,
-              "%s: negative stride", what);
-  // the place of a row in 32 bits of 16 bytes; the last value marks none.  Each term is checked
-  // before they are added: none overflows 64 bits
-  constexpr int64_t limit = (int64_t{1} << 32) - 64;
-  const auto term = [](int64_t n, int64_t stride) {
-    return n <= 1 || stride == 0 ? 0 : (stride / 8 > limit / (n - 1) ? limit : (n - 1) * (stride / 8));
-  };
-  ASC_REQUIRE(term(batch, r.batch_stride) + term(heads, r.head_stride) + term(rows, r.seq_stride) + head_dim / 8 <= limit,
-              ASC_ERR_UNSUPPORTED, "%s: keys and values span more than 64 GiB", what);
-  // a dimension of one element is not stepped over, whatever its stride
-  s.batch = batch > 1 ? static_cast<uint32_t>(r.batch_stride / 8) : 0;
-  s.head = heads > 1 ? static_cast<uint32_t>(r.head_stride / 8) : 0;
-  s.seq = rows > 1 ? static_cast<uint32_t>(r.seq_stride / 8) : 0;
-  return ASC_OK;
-}
-
 int32_t make(const asc_attention_t* a, bool tree, const char* what, Launch& L) {
   int32_t rc = asc::kv::check_shape(a, what);
   if (rc != ASC_OK) return rc;
@@ -125,16 +103,16 @@ int32_t make(const asc_attention_t* a, bool tree, const char* what, Launch& L) {
       while ((uint32_t{1} << p.page_shift) < p.page_size) ++p.page_shift;
       p.page_magic = static_cast<uint32_t>(((uint64_t{1} << (31 + p.page_shift)) + p.page_size - 1) / p.page_size);
     }
-    rc = strides_of(a->k, batch, a->kv_heads, rows, a->head_dim, what, p.ks);
-    if (rc == ASC_OK) rc = strides_of(a->v, batch, a->kv_heads, rows, a->head_dim, what, p.vs);
+    rc = asc::kv::strides_of(a->k, batch, a->kv_heads, rows, a->head_dim, what, p.ks);
+    if (rc == ASC_OK) rc = asc::kv::strides_of(a->v, batch, a->kv_heads, rows, a->head_dim, what, p.vs);
     if (rc != ASC_OK) return rc;
   }
   if (tree) {
     ASC_REQUIRE(a->k_draft.data && a->v_draft.data, ASC_ERR_INVALID_ARG, "%s: null drafted keys or values", what);
     p.k_draft = static_cast<const uint8_t*>(a->k_draft.data);
     p.v_draft = static_cast<const uint8_t*>(a->v_draft.data);
-    rc = strides_of(a->k_draft, a->batch, a->kv_heads, a->q_len, a->head_dim, what, p.kds);
-    if (rc == ASC_OK) rc = strides_of(a->v_draft, a->batch, a->kv_heads, a->q_len, a->head_dim, what, p.vds);
+    rc = asc::kv::strides_of(a->k_draft, a->batch, a->kv_heads, a->q_len, a->head_dim, what, p.kds);
+    if (rc == ASC_OK) rc = asc::kv::strides_of(a->v_draft, a->batch, a->kv_heads, a->q_len, a->head_dim, what, p.vds);
     if (rc != ASC_OK) return rc;
     p.draft_lengths = a->draft_lengths;
     p.mask = a->tree_mask;
@@ -196,6 +174,27 @@ namespace kv {
 
 bool row_operand(const asc_rows_t& r) {
   return aligned16(r.data) && ((r.batch_stride | r.head_stride | r.seq_stride) & 7) == 0;
+}
+
+int32_t strides_of(const asc_rows_t& r, int64_t batch, int64_t heads, int64_t rows, int head_dim, const char* what,
+                   Strides& s) {
+  ASC_REQUIRE(((r.batch_stride | r.head_stride | r.seq_stride) & 7) == 0 && asc::aligned16(r.data), ASC_ERR_ALIGNMENT,
+              "%s: keys and values must be 16-byte aligned, with strides that are multiples of 8", what);
+  ASC_REQUIRE(r.batch_stride >= 0 && r.head_stride >= 0 && r.seq_stride >= 0, ASC_ERR_INVALID_ARG,
+              "%s: negative stride", what);
+  // the place of a row in 32 bits of 16 bytes; the last value marks none.  Each term is checked
+  // before they are added: none overflows 64 bits
+  constexpr int64_t limit = (int64_t{1} << 32) - 64;
+  const auto term = [](int64_t n, int64_t stride) {
+    return n <= 1 || stride == 0 ? 0 : (stride / 8 > limit / (n - 1) ? limit : (n - 1) * (stride / 8));
+  };
+  ASC_REQUIRE(term(batch, r.batch_stride) + term(heads, r.head_stride) + term(rows, r.seq_stride) + head_dim / 8 <= limit,
+              ASC_ERR_UNSUPPORTED, "%s: keys and values span more than 64 GiB", what);
+  // a dimension of one element is not stepped over, whatever its stride
+  s.batch = batch > 1 ? static_cast<uint32_t>(r.batch_stride / 8) : 0;
+  s.head = heads > 1 ? static_cast<uint32_t>(r.head_stride / 8) : 0;
+  s.seq = rows > 1 ? static_cast<uint32_t>(r.seq_stride / 8) : 0;
+  return ASC_OK;
 }
 
 int32_t check_shape(const asc_attention_t* a, const char* what) {

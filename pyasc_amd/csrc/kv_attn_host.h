@@ -2,12 +2,17 @@
 #pragma once
 
 #include "common.h"
+#include "kv_attn_kernels.h"
 
 namespace asc {
 namespace kv {
 
 // The arguments' types, shapes and scale.
 int32_t check_shape(const asc_attention_t* a, const char* what);
+
+// Keys' or values' strides in units of 16 bytes, checked so that a row's place fits 32 bits.
+int32_t strides_of(const asc_rows_t& r, int64_t batch, int64_t heads, int64_t rows, int head_dim, const char* what,
+                   Strides& s);
 
 // Whether rows can be read and written in 16-byte pieces.
 bool row_operand(const asc_rows_t& r);

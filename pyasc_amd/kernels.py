@@ -818,8 +818,10 @@ def _counts(t: Optional[torch.Tensor], name: str, shape: tuple) -> int:
 
 
 def _kv_args(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, sm_scale: float,
-             lse: Optional[torch.Tensor], pages: bool, names: tuple) -> "_native.AttentionArgs":
-    """Checks queries, keys, values and results; ``pages``: the first dimension of k is not the batch's."""
+             lse: Optional[torch.Tensor], names: tuple, pages: bool = False,
+             written: bool = True) -> "_native.AttentionArgs":
+    """Checks queries, keys, values and o, a result where it is ``written``; ``pages``: the first
+    dimension of k is not the batch's."""
     if not isinstance(q, torch.Tensor):
         raise TypeError(f"'q' must be a torch.Tensor, got {type(q).__name__}")
     if q.dtype not in _HALVES:
@@ -828,7 +830,7 @@ def _kv_args(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
     batch, heads, q_len, head_dim = q.shape
     if head_dim not in FA_HEAD_DIMS:
         raise ValueError(f"head_dim {head_dim} not supported (supported: {FA_HEAD_DIMS})")
-    _aligned_rows(_bhsd(o, "o", q.dtype, tuple(q.shape), written=True), "o")
+    _aligned_rows(_bhsd(o, "o", q.dtype, tuple(q.shape), written), "o")
     _aligned_rows(_bhsd(k, names[0], q.dtype), names[0])
     if k.shape[3] != head_dim or (not pages and k.shape[0] != batch):
         raise ValueError(f"'{names[0]}' {tuple(k.shape)} does not fit q {tuple(q.shape)}")
@@ -867,9 +869,32 @@ def cross_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: to
     what lies behind them is not read.  A sequence without keys gets zeros.  ``lse`` (float32
     [batch, heads, q_len]) receives the log-sum-exp, -inf without keys.  A length outside
     [0, kv_len] is not followed: its sequence's results are NaN."""
-    a = _kv_args(q, k, v, o, sm_scale, lse, False, ("k", "v"))
+    a = _kv_args(q, k, v, o, sm_scale, lse, ("k", "v"))
     a.kv_lengths = _counts(kv_lengths, "kv_lengths", (q.shape[0],))
     _attend("asc_cross_attention_fwd", a, q.device, stream, "cross_attention_fwd")
+
+
+def cross_attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
+                        lse: torch.Tensor, dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, sm_scale: float,
+                        kv_lengths: Optional[torch.Tensor] = None, stream: Any = None) -> None:
+    """The gradients of cross_attention_fwd: from the gradient ``do`` of o, its inputs and its o and
+    lse, the gradients of q, k and v.  dk and dv are summed over the query heads that share a key /
+    value head, in a fixed order, and are zeros behind a sequence's keys.  The probabilities and the
+    scores' gradients are rounded to the inputs' type for their products; in float16 those below
+    2^-14 lose bits, so small gradients want a scaled loss."""
+    a = _kv_args(q, k, v, o, sm_scale, lse, ("k", "v"), written=False)
+    if lse is None:
+        raise TypeError("'lse' must be the forward pass's")
+    a.kv_lengths = _counts(kv_lengths, "kv_lengths", (q.shape[0],))
+    a.d_o = _wide_rows(_aligned_rows(_bhsd(do, "do", q.dtype, tuple(q.shape)), "do"))
+    inputs = {t.data_ptr() for t in (do, q, k, v, o) if t.numel()}
+    for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+        _aligned_rows(_bhsd(t, name, q.dtype, tuple(like.shape), written=True), name)
+        if t.numel() and t.data_ptr() in inputs:
+            raise ValueError(f"'{name}' must not lie in place of an input or of another result")
+        inputs.add(t.data_ptr())
+        setattr(a, name, _wide_rows(t))
+    _attend("asc_cross_attention_bwd", a, q.device, stream, "cross_attention_bwd")
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cache_lengths: torch.Tensor,
@@ -893,7 +918,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     Strides and the last dimension as in cross_attention_fwd.  A token that attends nothing gets zeros
     and an lse of -inf.  A length outside the cache, or a page outside it that a length reaches, is
     not followed: the sequence's results are NaN."""
-    a = _kv_args(q, k_cache, v_cache, o, sm_scale, lse, block_table is not None, ("k_cache", "v_cache"))
+    a = _kv_args(q, k_cache, v_cache, o, sm_scale, lse, ("k_cache", "v_cache"), pages=block_table is not None)
     batch, _, n, head_dim = q.shape
     a.kv_lengths = _counts(_device_tensor(cache_lengths, "cache_lengths"), "cache_lengths", (batch,))
     shape = (batch, k_cache.shape[1], n, head_dim)

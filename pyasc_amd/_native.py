@@ -122,16 +122,17 @@ SIGNATURES = {
     "asc_matmul_i8_dispatch": [_c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32,
                                ctypes.POINTER(LaunchPlan)],
     "asc_matmul_i8_plan": [_c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, ctypes.POINTER(LaunchPlan)],
-    "asc_rotary": [ctypes.POINTER(RotaryArgs), _c_p],
-    "asc_qk_norm_rotary": [ctypes.POINTER(RotaryArgs), _c_p],
-    "asc_qk_norm_rotary_bwd_workspace": [ctypes.POINTER(RotaryArgs)],
-    "asc_qk_norm_rotary_bwd": [ctypes.POINTER(RotaryArgs), _c_p, _c_i64, _c_p],
-    "asc_cross_attention_fwd_workspace": [ctypes.POINTER(AttentionArgs)],
-    "asc_cross_attention_fwd": [ctypes.POINTER(AttentionArgs), _c_p, _c_i64, _c_p],
-    "asc_cross_attention_bwd_workspace": [ctypes.POINTER(AttentionArgs)],
-    "asc_cross_attention_bwd": [ctypes.POINTER(AttentionArgs), _c_p, _c_i64, _c_p],
-    "asc_tree_attention_workspace": [ctypes.POINTER(AttentionArgs)],
-    "asc_tree_attention": [ctypes.POINTER(AttentionArgs), _c_p, _c_i64, _c_p],
+    # the first argument of these: a pointer to a struct, or its bytes
+    "asc_rotary": [_c_p, _c_p],
+    "asc_qk_norm_rotary": [_c_p, _c_p],
+    "asc_qk_norm_rotary_bwd_workspace": [_c_p],
+    "asc_qk_norm_rotary_bwd": [_c_p, _c_p, _c_i64, _c_p],
+    "asc_cross_attention_fwd_workspace": [_c_p],
+    "asc_cross_attention_fwd": [_c_p, _c_p, _c_i64, _c_p],
+    "asc_cross_attention_bwd_workspace": [_c_p],
+    "asc_cross_attention_bwd": [_c_p, _c_p, _c_i64, _c_p],
+    "asc_tree_attention_workspace": [_c_p],
+    "asc_tree_attention": [_c_p, _c_p, _c_i64, _c_p],
     "asc_unary_f32": [_c_i32, _c_p, _c_p, _c_i64, _c_p],
     "asc_binary": [_c_i32, _c_i32, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_f64, _c_i64, _c_p],
     "asc_where_cmp": [_c_i32, _c_i32, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_f64, _c_i64, _c_f64, _c_f64, _c_p],

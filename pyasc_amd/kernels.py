@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Any, Optional
 
 import torch
@@ -591,49 +592,79 @@ MAX_ROTARY_HEAD_DIM = 512
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
-def _here(t: torch.Tensor, name: str) -> torch.Tensor:
+_NO_ROWS = (0, 0, 0, 0)
+
+
+def _current_device() -> int:
+    c = _native._torch_c
+    return torch.cuda.current_device() if c is None else c._cuda_getDevice()
+
+
+def _here(t: torch.Tensor, name: str, device: int) -> torch.Tensor:
     """A tensor of the current device, the one that launches go to."""
-    _device_tensor(t, name)
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"'{name}' is on {t.device}, but the current device is cuda:{torch.cuda.current_device()}")
+    if not isinstance(t, torch.Tensor) or t.get_device() != device:
+        _device_tensor(t, name)
+        raise ValueError(f"'{name}' is on {t.device}, but the current device is cuda:{device}")
     return t
 
 
-def _bhsd(t: torch.Tensor, name: str, dtype: torch.dtype, shape: Optional[tuple] = None,
-          written: bool = False) -> torch.Tensor:
-    """A [batch, heads, seq, head_dim] operand of any strides whose last dimension is contiguous.
-    A tensor that is written must hold every element at a place of its own."""
-    _here(t, name)
-    if t.dtype != dtype:
+def _apart(t: torch.Tensor, name: str) -> None:
+    """Refuses a tensor to write to whose elements may share a place."""
+    span = 0  # of the dimensions so far, from the innermost
+    for stride, size in sorted((t.stride(i), t.shape[i]) for i in range(t.dim()) if t.shape[i] > 1):
+        if stride <= span:
+            raise ValueError(f"'{name}' is written but its elements overlap (strides {t.stride()})")
+        span += stride * (size - 1)
+
+
+def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: int, shape: Optional[tuple] = None,
+          written: bool = False, aligned: bool = False) -> tuple:
+    """A [batch, heads, seq, head_dim] operand whose last dimension is contiguous as asc_rows_t's
+    fields; ``aligned``: with rows that can be read and written 16 bytes at a time (16-bit elements)."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != device:
+        _here(t, name, device)
+    if t.dtype is not dtype:
         raise TypeError(f"'{name}' must be {dtype}, got {t.dtype}")
-    if t.dim() != 4 or (shape is not None and tuple(t.shape) != shape):
+    size = t.shape
+    if len(size) != 4 or (shape is not None and size != shape):
         raise ValueError(f"'{name}' must be {list(shape) if shape else '[batch, heads, seq, head_dim]'}, "
-                         f"got {tuple(t.shape)}")
-    if t.shape[3] > 1 and t.stride(3) != 1:
+                         f"got {tuple(size)}")
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1 and size[3] > 1:
         raise ValueError(f"the last dimension of '{name}' must be contiguous")
     if written and not t.is_contiguous():
-        span = 0  # of the dimensions so far, from the innermost
-        for stride, size in sorted((t.stride(i), t.shape[i]) for i in range(4) if t.shape[i] > 1):
-            if stride <= span:
-                raise ValueError(f"'{name}' is written but its elements overlap (strides {t.stride()})")
-            span += stride * (size - 1)
-    return t
+        _apart(t, name)
+    at = t.data_ptr()
+    if aligned and (at | (s0 | s1 | s2) << 1) & 15:
+        # a dimension of one element is not stepped over, whatever its stride
+        s0, s1, s2 = (s if n > 1 else 0 for s, n in zip((s0, s1, s2), size))
+        if (at | (s0 | s1 | s2) << 1) & 15:
+            raise ValueError(f"'{name}' must be 16-byte aligned, with strides that are multiples of 8 elements "
+                             f"(address {at:#x}, strides {t.stride()})")
+    return at, s0, s1, s2
 
 
-def _rows(t: Optional[torch.Tensor]) -> "_native.Rows":
-    if t is None:
-        return _native.Rows()
-    s = t.stride()
-    return _native.Rows(t.data_ptr(), s[0], s[1], s[2])
+def _vector(t: torch.Tensor, name: str, dtype: torch.dtype, device: int, shape: tuple) -> int:
+    """The address of a contiguous tensor of this type and shape."""
+    _here(t, name, device)
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"'{name}' must be a contiguous {dtype} {list(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
 
 
-def _workspace(nbytes: int, handle: int, device: torch.device, what: str) -> torch.Tensor:
-    """``nbytes`` for the launches of one call on stream ``handle``, as workspace_on's.  Under a
-    capture that torch does not know of the memory would go to others before the replays: refused."""
-    t = workspace_on(handle, nbytes, torch.uint8, device)
-    if torch.cuda.is_current_stream_capturing() and not _held_by_a_graph(t):
-        raise RuntimeError(f"{what} needs a workspace: capture it with torch.cuda.graph")
-    return t
+def _with_workspace(entry: str, args: bytes, device: torch.device, stream: Any) -> None:
+    """Calls an entry with the workspace that it asks for, from the launch stream's pool as
+    workspace_on's.  Under a capture that torch does not know of the workspace would go to others
+    before the replays: refused."""
+    handle = _stream(stream)
+    nbytes = getattr(_native.load_library(), entry + "_workspace")(args)
+    if nbytes == 0:
+        _native.call(entry, args, 0, 0, handle)
+        return
+    workspace = workspace_on(handle, nbytes, torch.uint8, device)
+    if torch.cuda.is_current_stream_capturing() and not _held_by_a_graph(workspace):
+        raise RuntimeError(f"{entry} needs a workspace: capture it with torch.cuda.graph")
+    _native.call(entry, args, workspace.data_ptr(), nbytes, handle)
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
@@ -675,54 +706,76 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
     return freqs.to("cuda" if device is None else device), magnitude
 
 
+_ROTARY = struct.Struct("@6i2f4q" + "P3q" * 6 + "P2q5P")  # asc_rotary_t
+
+
 def _rotary_args(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor,
-                 q_out: torch.Tensor, k_out: Optional[torch.Tensor], interleaved: bool,
-                 magnitude: float) -> "_native.RotaryArgs":
-    """Checks what the three rotary calls share."""
+                 q_out: torch.Tensor, k_out: Optional[torch.Tensor], interleaved: bool, magnitude: float,
+                 device: int, backward: bool = False, epsilon: float = 0.0, weights: Optional[tuple] = None,
+                 grads: Optional[tuple] = None) -> bytes:
+    """Checks the arguments of a rotary call and returns them as an asc_rotary_t.  ``weights``: those
+    of q and k; ``grads``: the gradients of the results, and of the weights."""
     if not isinstance(q, torch.Tensor):
         raise TypeError(f"'q' must be a torch.Tensor, got {type(q).__name__}")
-    if q.dtype not in _FLOATS:
-        raise TypeError(f"'q' has unsupported dtype {q.dtype}; expected one of {sorted(map(str, _FLOATS))}")
-    _bhsd(q, "q", q.dtype)
-    batch, heads, seq, head_dim = q.shape
+    dtype = q.dtype
+    if dtype not in _FLOATS:
+        raise TypeError(f"'q' has unsupported dtype {dtype}; expected one of {sorted(map(str, _FLOATS))}")
+    q_rows = _rows(q, "q", dtype, device)
+    shape = q.shape
+    batch, heads, seq, head_dim = shape
     if head_dim % 2 or not 0 < head_dim <= MAX_ROTARY_HEAD_DIM:
         raise ValueError(f"head_dim {head_dim} not supported (even, at most {MAX_ROTARY_HEAD_DIM})")
-    _bhsd(q_out, "q_out", q.dtype, tuple(q.shape), written=True)
+    out_rows = [_rows(q_out, "q_out", dtype, device, shape, written=True), _NO_ROWS]
+    in_rows, k_heads = [q_rows, _NO_ROWS], 0
     if (k is None) != (k_out is None):
         raise ValueError("k and its result must be given together")
-    pairs = [(q, q_out)]
     if k is not None:
-        _bhsd(k, "k", q.dtype)
-        _bhsd(k, "k", q.dtype, (batch, k.shape[1], seq, head_dim))
-        _bhsd(k_out, "k_out", q.dtype, tuple(k.shape), written=True)
-        pairs.append((k, k_out))
-    for x, y in pairs:
-        if x.data_ptr() == y.data_ptr() and x.stride() != y.stride() and x.numel():
-            raise ValueError("a result in place of its input must have the input's strides")
-    _here(positions, "positions")
-    if positions.dtype not in (torch.int32, torch.int64):
+        in_rows[1] = _rows(k, "k", dtype, device)
+        k_heads = k.shape[1]
+        k_shape = (batch, k_heads, seq, head_dim)
+        if k.shape != k_shape:
+            raise ValueError(f"'k' must be {list(k_shape)}, got {tuple(k.shape)}")
+        out_rows[1] = _rows(k_out, "k_out", dtype, device, k_shape, written=True)
+    w, dw, dy_rows = (0, 0), (0, 0), (_NO_ROWS, _NO_ROWS)
+    if weights is not None:
+        if not epsilon >= 0:
+            raise ValueError(f"epsilon must not be negative, got {epsilon}")
+        w = [_head_weight(weights[0], "q_weight", head_dim, device), 0]
+        if k is not None:
+            w[1] = _head_weight(weights[1], "k_weight", head_dim, device)
+    if grads is not None:
+        dy_rows = [_rows(grads[0], "dq_out", dtype, device, shape), _NO_ROWS]
+        dw = [_head_weight(grads[2], "dq_weight", head_dim, device), 0]
+        if k is not None:
+            if grads[1] is None:
+                raise ValueError("dk_out must be given with k")
+            dy_rows[1] = _rows(grads[1], "dk_out", dtype, device, k_shape)
+            dw[1] = _head_weight(grads[3], "dk_weight", head_dim, device)
+    for ins in (in_rows, dy_rows):
+        for x, y in zip(ins, out_rows):
+            if x[0] == y[0] and x != y and q.numel():
+                raise ValueError("a result in place of its input must have the input's strides")
+    _here(positions, "positions", device)
+    if positions.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
-    if tuple(positions.shape) not in ((seq,), (batch, seq)):
+    if positions.shape == (seq,):
+        steps = (0, positions.stride(0))
+    elif positions.shape == (batch, seq):
+        steps = positions.stride()
+    else:
         raise ValueError(f"positions must be [seq] or [batch, seq] = {(batch, seq)}, got {tuple(positions.shape)}")
-    _contiguous(_here(freqs, "freqs"), "freqs")
-    if freqs.dtype != torch.float64 or freqs.dim() != 1 or 2 * freqs.shape[0] > head_dim:
-        raise ValueError(f"freqs must be float64 with at most head_dim / 2 = {head_dim // 2} elements")
-    a = _native.RotaryArgs()
-    a.dtype, a.head_dim, a.rotary_dim = _DTYPE_CODES[q.dtype], head_dim, 2 * freqs.shape[0]
-    a.interleaved, a.positions_int64, a.magnitude = bool(interleaved), positions.dtype == torch.int64, magnitude
-    a.batch, a.q_heads, a.k_heads, a.seq = batch, heads, 0 if k is None else k.shape[1], seq
-    a.q, a.k, a.q_out, a.k_out = _rows(q), _rows(k), _rows(q_out), _rows(k_out)
-    a.positions, a.freqs = positions.data_ptr(), freqs.data_ptr()
-    a.position_batch_stride = positions.stride(0) if positions.dim() == 2 else 0
-    a.position_seq_stride = positions.stride(-1)
-    return a
+    _here(freqs, "freqs", device)
+    pairs = freqs.numel()
+    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or 2 * pairs > head_dim or not freqs.is_contiguous():
+        raise ValueError(f"'freqs' must be a contiguous float64 vector of at most head_dim / 2 = {head_dim // 2} elements")
+    return _ROTARY.pack(_DTYPE_CODES[dtype], head_dim, 2 * pairs, bool(interleaved), bool(backward),
+                        positions.dtype is torch.int64, magnitude, epsilon, batch, heads, k_heads, seq, *in_rows[0],
+                        *in_rows[1], *out_rows[0], *out_rows[1], *dy_rows[0], *dy_rows[1], positions.data_ptr(), *steps,
+                        freqs.data_ptr(), *w, *dw)
 
 
-def _head_weight(w: torch.Tensor, name: str, head_dim: int) -> int:
-    _contiguous(_here(w, name), name)
-    if w.dtype != torch.float32 or tuple(w.shape) != (head_dim,):
-        raise ValueError(f"'{name}' must be float32 [{head_dim}], got {w.dtype} {tuple(w.shape)}")
-    return w.data_ptr()
+def _head_weight(w: torch.Tensor, name: str, head_dim: int, device: int) -> int:
+    return _vector(w, name, torch.float32, device, (head_dim,))
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor,
@@ -733,9 +786,9 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     (i, i + len(freqs)) or, ``interleaved``, (2 i, 2 i + 1), turns by positions * freqs[i] and is
     multiplied by ``magnitude``; the other columns are copied.  ``backward`` gives the gradient:
     the turn the other way.  A result may lie in place of its input."""
-    a = _rotary_args(q, k, positions, freqs, q_out, k_out, interleaved, magnitude)
-    a.backward = bool(backward)
-    _native.call("asc_rotary", ctypes.byref(a), _stream(stream))
+    device = _current_device()
+    _native.call("asc_rotary", _rotary_args(q, k, positions, freqs, q_out, k_out, interleaved, magnitude, device,
+                                            backward), _stream(stream))
 
 
 def qk_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: torch.Tensor,
@@ -744,19 +797,9 @@ def qk_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: torch.T
                    magnitude: float = 1.0, stream: Any = None) -> None:
     """rotary after an RMS norm of each head: x / sqrt(mean(x^2) + epsilon) * weight, the weights
     float32 [head_dim]."""
-    a = _rotary_args(q, k, positions, freqs, q_out, k_out, interleaved, magnitude)
-    _norm_args(a, k, q_weight, k_weight, epsilon)
-    _native.call("asc_qk_norm_rotary", ctypes.byref(a), _stream(stream))
-
-
-def _norm_args(a: "_native.RotaryArgs", k: Optional[torch.Tensor], q_weight: torch.Tensor,
-               k_weight: Optional[torch.Tensor], epsilon: float) -> None:
-    if not epsilon >= 0:
-        raise ValueError(f"epsilon must not be negative, got {epsilon}")
-    a.epsilon = epsilon
-    a.q_weight = _head_weight(q_weight, "q_weight", a.head_dim)
-    if k is not None:
-        a.k_weight = _head_weight(k_weight, "k_weight", a.head_dim)
+    device = _current_device()
+    _native.call("asc_qk_norm_rotary", _rotary_args(q, k, positions, freqs, q_out, k_out, interleaved, magnitude,
+                                                    device, False, epsilon, (q_weight, k_weight)), _stream(stream))
 
 
 def qk_norm_rotary_bwd(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q: torch.Tensor,
@@ -767,26 +810,10 @@ def qk_norm_rotary_bwd(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q: 
     """The gradient of qk_norm_rotary: from the results' gradients and its inputs, the gradients
     of q and k (dq may lie in place of dq_out or q) and of the weights (float32 [head_dim], summed
     over all rows in a fixed order)."""
-    a = _rotary_args(q, k, positions, freqs, dq, dk, interleaved, magnitude)
-    _norm_args(a, k, q_weight, k_weight, epsilon)
-    _bhsd(dq_out, "dq_out", q.dtype, tuple(q.shape))
-    results = [(dq_out, dq)]
-    a.dq_out = _rows(dq_out)
-    a.dq_weight = _head_weight(dq_weight, "dq_weight", a.head_dim)
-    if k is not None:
-        if dk_out is None:
-            raise ValueError("dk_out must be given with k")
-        _bhsd(dk_out, "dk_out", q.dtype, tuple(k.shape))
-        results.append((dk_out, dk))
-        a.dk_out = _rows(dk_out)
-        a.dk_weight = _head_weight(dk_weight, "dk_weight", a.head_dim)
-    for x, y in results:
-        if x.data_ptr() == y.data_ptr() and x.stride() != y.stride() and x.numel():
-            raise ValueError("a result in place of its input must have the input's strides")
-    handle = _stream(stream)
-    nbytes = _native.load_library().asc_qk_norm_rotary_bwd_workspace(ctypes.byref(a))
-    workspace = _workspace(nbytes, handle, q.device, "qk_norm_rotary_bwd") if nbytes else None
-    _native.call("asc_qk_norm_rotary_bwd", ctypes.byref(a), workspace.data_ptr() if nbytes else 0, nbytes, handle)
+    device = _current_device()
+    args = _rotary_args(q, k, positions, freqs, dq, dk, interleaved, magnitude, device, False, epsilon,
+                        (q_weight, k_weight), (dq_out, dk_out, dq_weight, dk_weight))
+    _with_workspace("asc_qk_norm_rotary_bwd", args, q.device, stream)
 
 
 # ------------------------------------------------- attention over other keys than the queries' own
@@ -794,69 +821,35 @@ def qk_norm_rotary_bwd(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q: 
 _HALVES = (torch.float16, torch.bfloat16)
 
 
-def _aligned_rows(t: torch.Tensor, name: str) -> torch.Tensor:
-    """Rows that are read and written 16 bytes at a time."""
-    if t.data_ptr() % 16 or any(t.stride(i) % 8 for i in range(3) if t.shape[i] > 1):
-        raise ValueError(f"'{name}' must be 16-byte aligned, with strides that are multiples of 8 elements "
-                         f"(address {t.data_ptr():#x}, strides {t.stride()})")
-    return t
+_ATTENTION = struct.Struct("@iifi6q" + "P3q" * 6 + "4PqP2q" + "P3q" * 4)  # asc_attention_t
+_NO_GRADS = _NO_ROWS * 4
+_NO_TREE = (0, 0, 0, 0, 0, 0)  # draft_lengths, block_table and its stride, tree_mask and its strides
 
 
-def _wide_rows(t: torch.Tensor) -> "_native.Rows":
-    """_rows of a tensor checked by _aligned_rows: a dimension of one element is not stepped over."""
-    s = [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
-    return _native.Rows(t.data_ptr(), *s)
-
-
-def _counts(t: Optional[torch.Tensor], name: str, shape: tuple) -> int:
-    if t is None:
-        return 0
-    _contiguous(_here(t, name), name)
-    if t.dtype != torch.int32 or tuple(t.shape) != shape:
-        raise ValueError(f"'{name}' must be int32 {list(shape)}, got {t.dtype} {tuple(t.shape)}")
-    return t.data_ptr()
-
-
-def _kv_args(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, sm_scale: float,
-             lse: Optional[torch.Tensor], names: tuple, pages: bool = False,
-             written: bool = True) -> "_native.AttentionArgs":
-    """Checks queries, keys, values and o, a result where it is ``written``; ``pages``: the first
-    dimension of k is not the batch's."""
+def _kv_rows(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, sm_scale: float, device: int,
+             names: tuple, pages: bool = False, written: bool = True) -> tuple:
+    """Checks queries, keys, values and o, a result where it is ``written``, and returns their rows;
+    ``pages``: the first dimension of k is not the batch's."""
     if not isinstance(q, torch.Tensor):
         raise TypeError(f"'q' must be a torch.Tensor, got {type(q).__name__}")
-    if q.dtype not in _HALVES:
-        raise TypeError(f"'q' has unsupported dtype {q.dtype}; expected one of {sorted(map(str, _HALVES))}")
-    _aligned_rows(_bhsd(q, "q", q.dtype), "q")
-    batch, heads, q_len, head_dim = q.shape
-    if head_dim not in FA_HEAD_DIMS:
-        raise ValueError(f"head_dim {head_dim} not supported (supported: {FA_HEAD_DIMS})")
-    _aligned_rows(_bhsd(o, "o", q.dtype, tuple(q.shape), written), "o")
-    _aligned_rows(_bhsd(k, names[0], q.dtype), names[0])
-    if k.shape[3] != head_dim or (not pages and k.shape[0] != batch):
-        raise ValueError(f"'{names[0]}' {tuple(k.shape)} does not fit q {tuple(q.shape)}")
-    _aligned_rows(_bhsd(v, names[1], q.dtype, tuple(k.shape)), names[1])
-    if k.shape[1] == 0 or heads % k.shape[1]:
-        raise ValueError(f"{heads} query heads cannot share {k.shape[1]} key / value heads")
+    dtype = q.dtype
+    if dtype not in _HALVES:
+        raise TypeError(f"'q' has unsupported dtype {dtype}; expected one of {sorted(map(str, _HALVES))}")
+    q_rows = _rows(q, "q", dtype, device, None, False, True)
+    shape = q.shape
+    if shape[3] not in FA_HEAD_DIMS:
+        raise ValueError(f"head_dim {shape[3]} not supported (supported: {FA_HEAD_DIMS})")
+    o_rows = _rows(o, "o", dtype, device, shape, written, True)
+    k_rows = _rows(k, names[0], dtype, device, None, False, True)
+    k_shape = k.shape
+    if k_shape[3] != shape[3] or (k_shape[0] != shape[0] and not pages):
+        raise ValueError(f"'{names[0]}' {tuple(k_shape)} does not fit q {tuple(shape)}")
+    v_rows = _rows(v, names[1], dtype, device, k_shape, False, True)
+    if k_shape[1] == 0 or shape[1] % k_shape[1]:
+        raise ValueError(f"{shape[1]} query heads cannot share {k_shape[1]} key / value heads")
     if not sm_scale > 0:
         raise ValueError(f"sm_scale must be positive, got {sm_scale}")
-    a = _native.AttentionArgs()
-    a.dtype, a.head_dim, a.sm_scale = _DTYPE_CODES[q.dtype], head_dim, sm_scale
-    a.batch, a.q_heads, a.kv_heads, a.q_len, a.kv_len = batch, heads, k.shape[1], q_len, k.shape[2]
-    a.q, a.o, a.k, a.v = _wide_rows(q), _wide_rows(o), _wide_rows(k), _wide_rows(v)
-    if lse is not None:
-        _contiguous(_here(lse, "lse"), "lse")
-        if lse.dtype != torch.float32 or tuple(lse.shape) != (batch, heads, q_len):
-            raise ValueError("lse must be float32 [batch, heads, q_len]")
-        a.lse = lse.data_ptr()
-    return a
-
-
-def _attend(entry: str, a: "_native.AttentionArgs", device: torch.device, stream: Any, what: str) -> None:
-    """Calls an attention entry with the workspace that it asks for."""
-    handle = _stream(stream)
-    nbytes = getattr(_native.load_library(), entry + "_workspace")(ctypes.byref(a))
-    workspace = _workspace(nbytes, handle, device, what) if nbytes else None
-    _native.call(entry, ctypes.byref(a), workspace.data_ptr() if nbytes else 0, nbytes, handle)
+    return q_rows, o_rows, k_rows, v_rows
 
 
 def cross_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, sm_scale: float,
@@ -869,9 +862,15 @@ def cross_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: to
     what lies behind them is not read.  A sequence without keys gets zeros.  ``lse`` (float32
     [batch, heads, q_len]) receives the log-sum-exp, -inf without keys.  A length outside
     [0, kv_len] is not followed: its sequence's results are NaN."""
-    a = _kv_args(q, k, v, o, sm_scale, lse, ("k", "v"))
-    a.kv_lengths = _counts(kv_lengths, "kv_lengths", (q.shape[0],))
-    _attend("asc_cross_attention_fwd", a, q.device, stream, "cross_attention_fwd")
+    device = _current_device()
+    q_rows, o_rows, k_rows, v_rows = _kv_rows(q, k, v, o, sm_scale, device, ("k", "v"))
+    batch, heads, q_len, head_dim = q.shape
+    lse_at = 0 if lse is None else _vector(lse, "lse", torch.float32, device, (batch, heads, q_len))
+    lengths = 0 if kv_lengths is None else _vector(kv_lengths, "kv_lengths", torch.int32, device, (batch,))
+    args = _ATTENTION.pack(_DTYPE_CODES[q.dtype], head_dim, sm_scale, 0, batch, heads, k.shape[1], q_len, k.shape[2],
+                           0, *q_rows, *o_rows, *k_rows, *v_rows, *_NO_ROWS, *_NO_ROWS, lse_at, lengths, *_NO_TREE,
+                           *_NO_GRADS)
+    _with_workspace("asc_cross_attention_fwd", args, q.device, stream)
 
 
 def cross_attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
@@ -882,19 +881,25 @@ def cross_attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: t
     value head, in a fixed order, and are zeros behind a sequence's keys.  The probabilities and the
     scores' gradients are rounded to the inputs' type for their products; in float16 those below
     2^-14 lose bits, so small gradients want a scaled loss."""
-    a = _kv_args(q, k, v, o, sm_scale, lse, ("k", "v"), written=False)
-    if lse is None:
-        raise TypeError("'lse' must be the forward pass's")
-    a.kv_lengths = _counts(kv_lengths, "kv_lengths", (q.shape[0],))
-    a.d_o = _wide_rows(_aligned_rows(_bhsd(do, "do", q.dtype, tuple(q.shape)), "do"))
-    inputs = {t.data_ptr() for t in (do, q, k, v, o) if t.numel()}
-    for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-        _aligned_rows(_bhsd(t, name, q.dtype, tuple(like.shape), written=True), name)
-        if t.numel() and t.data_ptr() in inputs:
+    device = _current_device()
+    q_rows, o_rows, k_rows, v_rows = _kv_rows(q, k, v, o, sm_scale, device, ("k", "v"), written=False)
+    dtype, shape = q.dtype, q.shape
+    batch, heads, q_len, head_dim = shape
+    lse_at = _vector(lse, "lse", torch.float32, device, (batch, heads, q_len))
+    lengths = 0 if kv_lengths is None else _vector(kv_lengths, "kv_lengths", torch.int32, device, (batch,))
+    do_rows = _rows(do, "do", dtype, device, shape, False, True)
+    taken = [do_rows[0], q_rows[0], k_rows[0], v_rows[0], o_rows[0]]
+    grads = ()
+    for name, t, like in (("dq", dq, shape), ("dk", dk, k.shape), ("dv", dv, k.shape)):
+        rows = _rows(t, name, dtype, device, like, True, True)
+        if rows[0] in taken and t.numel():
             raise ValueError(f"'{name}' must not lie in place of an input or of another result")
-        inputs.add(t.data_ptr())
-        setattr(a, name, _wide_rows(t))
-    _attend("asc_cross_attention_bwd", a, q.device, stream, "cross_attention_bwd")
+        taken.append(rows[0])
+        grads += rows
+    args = _ATTENTION.pack(_DTYPE_CODES[dtype], head_dim, sm_scale, 0, batch, heads, k.shape[1], q_len, k.shape[2], 0,
+                           *q_rows, *o_rows, *k_rows, *v_rows, *_NO_ROWS, *_NO_ROWS, lse_at, lengths, *_NO_TREE,
+                           *do_rows, *grads)
+    _with_workspace("asc_cross_attention_bwd", args, q.device, stream)
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cache_lengths: torch.Tensor,
@@ -918,35 +923,46 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     Strides and the last dimension as in cross_attention_fwd.  A token that attends nothing gets zeros
     and an lse of -inf.  A length outside the cache, or a page outside it that a length reaches, is
     not followed: the sequence's results are NaN."""
-    a = _kv_args(q, k_cache, v_cache, o, sm_scale, lse, ("k_cache", "v_cache"), pages=block_table is not None)
-    batch, _, n, head_dim = q.shape
-    a.kv_lengths = _counts(_device_tensor(cache_lengths, "cache_lengths"), "cache_lengths", (batch,))
-    shape = (batch, k_cache.shape[1], n, head_dim)
-    a.k_draft = _wide_rows(_aligned_rows(_bhsd(k_draft, "k_draft", q.dtype, shape), "k_draft"))
-    a.v_draft = _wide_rows(_aligned_rows(_bhsd(v_draft, "v_draft", q.dtype, shape), "v_draft"))
+    device = _current_device()
+    q_rows, o_rows, k_rows, v_rows = _kv_rows(q, k_cache, v_cache, o, sm_scale, device, ("k_cache", "v_cache"),
+                                              pages=block_table is not None)
+    dtype = q.dtype
+    batch, heads, n, head_dim = q.shape
+    pages, kv_heads, kv_len, _ = k_cache.shape
+    lse_at = 0 if lse is None else _vector(lse, "lse", torch.float32, device, (batch, heads, n))
+    lengths = _vector(cache_lengths, "cache_lengths", torch.int32, device, (batch,))
+    drafted = 0 if draft_lengths is None else _vector(draft_lengths, "draft_lengths", torch.int32, device, (batch,))
+    shape = (batch, kv_heads, n, head_dim)
+    kd_rows = _rows(k_draft, "k_draft", dtype, device, shape, False, True)
+    vd_rows = _rows(v_draft, "v_draft", dtype, device, shape, False, True)
+    page_size, table, table_stride = 0, 0, 0
     if block_table is not None:
-        _here(block_table, "block_table")
-        if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch:
-            raise ValueError(f"'block_table' must be int32 [batch, pages], got {block_table.dtype} "
-                             f"{tuple(block_table.shape)}")
-        if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+        _here(block_table, "block_table", device)
+        size = block_table.shape
+        if block_table.dtype is not torch.int32 or len(size) != 2 or size[0] != batch:
+            raise ValueError(f"'block_table' must be int32 [batch, pages], got {block_table.dtype} {tuple(size)}")
+        table_stride, step = block_table.stride()
+        if step != 1 and size[1] > 1:
             raise ValueError("the last dimension of 'block_table' must be contiguous")
-        a.num_pages, a.page_size = k_cache.shape[0], k_cache.shape[2]
-        a.kv_len = block_table.shape[1] * k_cache.shape[2]
-        if a.num_pages == 0 and a.kv_len:
+        page_size, kv_len = kv_len, size[1] * kv_len
+        if pages == 0 and kv_len:
             raise ValueError("a cache without pages needs a block_table without columns")
-        a.block_table, a.table_stride = block_table.data_ptr(), block_table.stride(0)
+        table = block_table.data_ptr()
+    mask, mask_batch, mask_row = 0, 0, 0
     if tree_mask is not None:
-        _here(tree_mask, "tree_mask")
-        if tree_mask.dtype != torch.bool or tuple(tree_mask.shape) not in ((n, n), (batch, n, n)):
+        _here(tree_mask, "tree_mask", device)
+        size = tree_mask.shape
+        if tree_mask.dtype is not torch.bool or (size != (batch, n, n) and size != (n, n)):
             raise ValueError(f"'tree_mask' must be bool [{n}, {n}] or [{batch}, {n}, {n}], got {tree_mask.dtype} "
-                             f"{tuple(tree_mask.shape)}")
-        if n > 1 and tree_mask.stride(-1) != 1:
+                             f"{tuple(size)}")
+        *outer, mask_row, step = tree_mask.stride()
+        if step != 1 and n > 1:
             raise ValueError("the last dimension of 'tree_mask' must be contiguous")
-        a.tree_mask, a.mask_row_stride = tree_mask.data_ptr(), tree_mask.stride(-2)
-        a.mask_batch_stride = tree_mask.stride(0) if tree_mask.dim() == 3 else 0
-    a.draft_lengths = _counts(draft_lengths, "draft_lengths", (batch,))
-    _attend("asc_tree_attention", a, q.device, stream, "tree_attention")
+        mask, mask_batch = tree_mask.data_ptr(), outer[0] if outer else 0
+    args = _ATTENTION.pack(_DTYPE_CODES[dtype], head_dim, sm_scale, page_size, batch, heads, kv_heads, n, kv_len, pages,
+                           *q_rows, *o_rows, *k_rows, *v_rows, *kd_rows, *vd_rows, lse_at, lengths, drafted, table,
+                           table_stride, mask, mask_batch, mask_row, *_NO_GRADS)
+    _with_workspace("asc_tree_attention", args, q.device, stream)
 
 
 # ------------------------------------------------------------------ element-wise tile operations

@@ -160,8 +160,11 @@ __device__ __forceinline__ float other_half(float v) {
 // Per-wave state of the attention kernel.  A wave owns QB blocks of 32 queries
 // (32*QB queries); a workgroup of kWaves waves owns 32*QB*kWaves.  Every K or V
 // operand a wave reads from LDS feeds QB MFMAs, one per query block, so LDS
-// read traffic per MFMA falls as 1/QB.  E is the element type.
-template <int D, int kWaves, int QB, class E = Bf16>
+// read traffic per MFMA falls as 1/QB.  E is the element type.  kXor: one LDS address per
+// operand in place of one per chunk, the chunk's bits flipped at each read (a tile's base is a
+// multiple of its rows' size, so they carry into nothing); for kernels that hold more than
+// fa_fwd_body does.
+template <int D, int kWaves, int QB, class E = Bf16, bool kXor = false>
 struct FaState {
   using Element = E;
   static constexpr int kQ = 32 * QB;              // queries per wave
@@ -182,8 +185,8 @@ struct FaState {
   // Per-lane LDS read offsets, loop-invariant: the K swizzle of row kb*32+col
   // equals that of row col, and the V swizzle of row r0+j (r0 % 4 == 0) equals
   // that of row j, so every other term of a read address is an immediate.
-  uint32_t kaddr[kKSteps];   // K row col, chunk 2*kk+h
-  uint32_t vaddr[kDBlocks];  // V transpose read of d block db, rows 4h+j
+  uint32_t kaddr[kXor ? 1 : kKSteps];   // K row col, chunk 2*kk+h
+  uint32_t vaddr[kXor ? 1 : kDBlocks];  // V transpose read of d block db, rows 4h+j
   u32x4 qreg[QB][kKSteps];
   f32x16 acc_o[QB][kDBlocks];
   float m_run[QB];   // reference point of the scaled scores (log2 domain), <= running max
@@ -223,6 +226,17 @@ struct FaState {
     for (int db = 0; db < kDBlocks; ++db) vaddr[db] = v_off<D>(h * 4 + (g_lane >> 2), db * 32 + tr_col);
   }
 
+  // Chunk 2*kk+h of a K row is 2*kk chunks away from chunk h by its bits, as the swizzles only flip
+  // bits; d block db of a V row is 4*db chunks away.
+  __device__ __forceinline__ uint32_t k_addr(uint32_t base, int kk) const {
+    if constexpr (kXor) return (base + kaddr[0]) ^ (kk << 5);
+    return base + kaddr[kXor ? 0 : kk];
+  }
+  __device__ __forceinline__ uint32_t v_addr(uint32_t base, int db) const {
+    if constexpr (kXor) return (base + vaddr[0]) ^ (db << 6);
+    return base + vaddr[kXor ? 0 : db];
+  }
+
   // Keys k0 .. k0+63 of K (kIsV false) or V into one LDS stage.
   template <bool kIsV>
   __device__ __forceinline__ void load_tile(uint8_t* dst, int k0) const {
@@ -257,7 +271,7 @@ struct FaState {
     constexpr int kReads = 2 * kKSteps;
     u32x4 a[kReads];
 #pragma unroll
-    for (int r = 0; r < kWin; ++r) a[r] = lds_read_b128(base + kaddr[r % kKSteps], (r / kKSteps) * 32 * (D * 2));
+    for (int r = 0; r < kWin; ++r) a[r] = lds_read_b128(k_addr(base, r % kKSteps), (r / kKSteps) * 32 * (D * 2));
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       s[qb][0] = f32x16{};
@@ -271,7 +285,7 @@ struct FaState {
         s[qb][r / kKSteps] = E::mfma(a[r], qreg[qb][r % kKSteps], s[qb][r / kKSteps]);
       }
       if (r + kWin < kReads) {
-        a[r + kWin] = lds_read_b128(base + kaddr[(r + kWin) % kKSteps], ((r + kWin) / kKSteps) * 32 * (D * 2));
+        a[r + kWin] = lds_read_b128(k_addr(base, (r + kWin) % kKSteps), ((r + kWin) / kKSteps) * 32 * (D * 2));
       }
     }
   }
@@ -312,7 +326,7 @@ struct FaState {
     }
     u32x4 a[kReads];
 #pragma unroll
-    for (int r = 0; r < kWin; ++r) a[r] = lds_read_b128(base + kaddr[r % kKSteps], (r / kKSteps) * 32 * (D * 2));
+    for (int r = 0; r < kWin; ++r) a[r] = lds_read_b128(k_addr(base, r % kKSteps), (r / kKSteps) * 32 * (D * 2));
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int r = 0; r < kReads; ++r) {
@@ -327,7 +341,7 @@ struct FaState {
         prob_pair(it / 16, it % 16, sp[it / 16], neg_m[it / 16], pb[it / 16], rs[it / 16]);
       }
       if (r + kWin < kReads) {
-        a[r + kWin] = lds_read_b128(base + kaddr[(r + kWin) % kKSteps], ((r + kWin) / kKSteps) * 32 * (D * 2));
+        a[r + kWin] = lds_read_b128(k_addr(base, (r + kWin) % kKSteps), ((r + kWin) / kKSteps) * 32 * (D * 2));
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -403,8 +417,8 @@ struct FaState {
   // tile rows 16 * (r % 4) + {0, 8}, two transpose reads.
   __device__ __forceinline__ u32x4 vt_read(uint32_t base, int r) const {
     const int db = r / 4, row = (r % 4) * 16;
-    const u32x2 lo = lds_read_tr16_b64(base + vaddr[db], row * (D * 2));
-    const u32x2 hi = lds_read_tr16_b64(base + vaddr[db], (row + 8) * (D * 2));
+    const u32x2 lo = lds_read_tr16_b64(v_addr(base, db), row * (D * 2));
+    const u32x2 hi = lds_read_tr16_b64(v_addr(base, db), (row + 8) * (D * 2));
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   }
 

@@ -46,7 +46,7 @@ void plan(Launch& L, const asc_attention_t& a) {
   const int64_t slots = kCus * (a.head_dim == 64 ? 2 : 1);
   const int64_t tiles = asc::ceil_div(p.capacity, asc::fa::BKV) + (p.k_draft ? asc::ceil_div(p.n_q, asc::fa::BKV) : 0);
   const int64_t least = L.wide ? 4 : 8;  // tiles of a split
-  int64_t splits = shares >= slots ? 1 : 2 * slots / shares;
+  int64_t splits = shares >= slots ? 1 : (L.wide ? 1 : 2) * slots / shares;
   if (splits > tiles / least) splits = tiles / least;
   if (splits > kMaxSplits) splits = kMaxSplits;
   p.splits = splits < 1 ? 1 : static_cast<int>(splits);

@@ -89,8 +89,8 @@ __device__ __forceinline__ Share share_of(const KvArgs& p) {
 
 // kTree: there may be a table of pages, drafted keys and a mask over them.
 template <int D, int kWaves, class E, bool kTree>
-struct KvState : FaState<D, kWaves, 1, E> {
-  using Base = FaState<D, kWaves, 1, E>;
+struct KvState : FaState<D, kWaves, 1, E, true> {
+  using Base = FaState<D, kWaves, 1, E, true>;
   using Base::col;
   using Base::h;
   using Base::kKSteps;
@@ -104,7 +104,8 @@ struct KvState : FaState<D, kWaves, 1, E> {
   int cached;          // tiles of cached keys; the drafted ones follow in tiles of their own
   int query;           // this lane's query (of n_q), or -1: no row
   const int32_t* table;
-  uint32_t table_id;   // fetched entry of the tile after the next
+  uint8_t* ids;        // LDS, 256 bytes of this wave: the fetched entries of a tile's keys
+  uint32_t drafted;    // hidden_bits of the first drafted tile
   uint32_t k0, v0, kd0, vd0;  // the sequence's first row (16-byte units)
   const uint8_t* mask;
   bool poison;         // a page or a length outside the cache: the rows' results are NaN
@@ -128,7 +129,7 @@ struct KvState : FaState<D, kWaves, 1, E> {
       kd0 = s.head * p.kds.head + s.b * p.kds.batch;
       vd0 = s.head * p.vds.head + s.b * p.vds.batch;
       mask = p.mask ? p.mask + s.b * p.mask_batch : nullptr;
-      table_id = 0;
+      drafted = 0;
     }
 
     constexpr int kLanesPerRow = 64 / kRowsPerLoad;
@@ -139,44 +140,47 @@ struct KvState : FaState<D, kWaves, 1, E> {
       this->voff_k[i] = (pos ^ fa::kswz<D>(row)) << 4;
     }
     this->voff_v = (pos ^ fa::vswz<D>(rr)) << 4;
-#pragma unroll
-    for (int kk = 0; kk < kKSteps; ++kk) this->kaddr[kk] = fa::k_off<D>(col, kk * 2 + h);
+    this->kaddr[0] = fa::k_off<D>(col, h);
     const int g_lane = lane & 15;
     const int tr_col = ((lane >> 4) & 1) * 16 + (g_lane & 3) * 4;
-#pragma unroll
-    for (int db = 0; db < Base::kDBlocks; ++db) {
-      this->vaddr[db] = fa::v_off<D>(h * 4 + (g_lane >> 2), db * 32 + tr_col);
-    }
+    this->vaddr[0] = fa::v_off<D>(h * 4 + (g_lane >> 2), tr_col);
   }
 
   __device__ __forceinline__ int tiles() const { return cached + (drafts + BKV - 1) / BKV; }
 
-  // Asks for the table entry of tile j's key of this lane, a tile ahead of its use.
-  __device__ __forceinline__ void fetch(const KvArgs& p, int j) {
-    if constexpr (!kTree) return;
-    if (table == nullptr || j >= cached) return;
+  // Address of the table entry of tile j's key of this lane (of the last key behind it), j < cached.
+  __device__ __forceinline__ const int32_t* entry(const KvArgs& p, int j) const {
     const int key = min(j * BKV + lane, len - 1);
     // key / page_size: the magic's error, below page_size, times key stays under 2^(31 + shift)
-    const uint32_t page =
-        static_cast<uint32_t>((static_cast<uint64_t>(key) * p.page_magic) >> (31 + p.page_shift));
-    table_id = static_cast<uint32_t>(table[page]);
+    return table + static_cast<uint32_t>((static_cast<uint64_t>(key) * p.page_magic) >> (31 + p.page_shift));
+  }
+  __device__ __forceinline__ uint32_t entry_now(const KvArgs& p, int j) const {
+    if (!kTree || table == nullptr || j >= cached) return 0;
+    return static_cast<uint32_t>(*entry(p, j));
+  }
+  // Asks for tile j's entries, a tile ahead of their use, straight into LDS: a load to registers
+  // would be waited for with all loads of tiles behind it, as the compiler cannot count those
+  // past a branch.  Sent before a step's tiles, the step's own wait covers it.
+  __device__ __forceinline__ void fetch(const KvArgs& p, int j) const {
+    if (!kTree || table == nullptr || j >= cached) return;
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)entry(p, j),
+                                     (__attribute__((address_space(3))) void*)ids, 4, 0, 0);
+  }
+  __device__ __forceinline__ uint32_t fetched(int j) const {
+    if (!kTree || table == nullptr || j >= cached) return 0;
+    uint32_t r;
+    asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(r) : "v"(fa::lds_addr(ids) + lane * 4) : "memory");
+    return r;
   }
 
-  // Places of tile j's keys, one per lane (of its table entry fetched before).
-  __device__ __forceinline__ void places(const KvArgs& p, int j, uint32_t& ik, uint32_t& iv) {
-    if constexpr (!kTree) {
-      const int key = j * BKV + lane;
-      ik = key < len ? k0 + key * p.ks.seq : kNone;
-      iv = key < len ? v0 + key * p.vs.seq : kNone;
-      return;
-    }
-    if (j < cached) {
-      const int key = j * BKV + lane;
-      if (table != nullptr) {
+  // Places of tile j's keys, one per lane, of its table entry.
+  __device__ __forceinline__ void places(const KvArgs& p, int j, uint32_t id, uint32_t& ik, uint32_t& iv) {
+    const int key = (j < cached ? j : j - cached) * BKV + lane;
+    if (!kTree || j < cached) {
+      if (kTree && table != nullptr) {
         const uint32_t at = min(key, len - 1);
         const uint32_t page = static_cast<uint32_t>((static_cast<uint64_t>(at) * p.page_magic) >> (31 + p.page_shift));
         const uint32_t row = at - page * p.page_size;
-        uint32_t id = table_id;
         const bool bad = id >= p.num_pages;
         poison = poison || __builtin_amdgcn_ballot_w64(bad) != 0;
         if (bad) id = 0;
@@ -188,7 +192,6 @@ struct KvState : FaState<D, kWaves, 1, E> {
       }
       if (key >= len) ik = iv = kNone;
     } else {
-      const int key = (j - cached) * BKV + lane;
       ik = key < drafts ? kd0 + key * p.kds.seq : kNone;
       iv = key < drafts ? vd0 + key * p.vds.seq : kNone;
     }
@@ -197,8 +200,12 @@ struct KvState : FaState<D, kWaves, 1, E> {
   // Tile j of K (kIsV false) or V, whose rows' places the lanes hold, into one LDS stage.
   template <bool kIsV>
   __device__ __forceinline__ void load(const KvArgs& p, uint8_t* dst, int j, uint32_t places) const {
-    const uint8_t* base = kIsV ? p.v : p.k;
-    if (kTree && j >= cached) base = kIsV ? p.v_draft : p.k_draft;
+    uint64_t base = reinterpret_cast<uint64_t>(kIsV ? p.v : p.k);
+    if constexpr (kTree) {
+      uint64_t draft = reinterpret_cast<uint64_t>(kIsV ? p.v_draft : p.k_draft);
+      asm("" : "+s"(base), "+s"(draft));  // selected in registers, not from a table in scratch memory
+      if (j >= cached) base = draft;
+    }
     const bool whole = (j + 1) * BKV <= len;
     int wave_lds = wave * (kLoadsPerWave * 1024);
     asm volatile("" : "+s"(wave_lds));
@@ -209,7 +216,7 @@ struct KvState : FaState<D, kWaves, 1, E> {
       const int row = kRowsPerLoad * (wave * kLoadsPerWave + i) + rr;
       const uint32_t at =
           static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(row * 4, static_cast<int>(places)));
-      const uint8_t* src = base + static_cast<uint64_t>(at) * 16;
+      const uint8_t* src = reinterpret_cast<const uint8_t*>(base + static_cast<uint64_t>(at) * 16);
       if (!whole) src = at == kNone ? reinterpret_cast<const uint8_t*>(kZeroRow) : src;
       __builtin_amdgcn_global_load_lds(
           (const __attribute__((address_space(1))) void*)(src + (kIsV ? this->voff_v : this->voff_k[i & 3])),
@@ -230,20 +237,7 @@ struct KvState : FaState<D, kWaves, 1, E> {
         }
       return;
     }
-    // one bit per score register pair of blocks, gathered in a loop: unrolled, its addresses and
-    // the wave's accumulators would not fit the registers
-    const int first = (j - cached) * BKV + h * 4;
-    const uint8_t* row = mask ? mask + static_cast<int64_t>(query < 0 ? 0 : query) * p.mask_row : nullptr;
-    uint32_t seen = 0;
-#pragma unroll 1
-    for (int i = 0; i < 8; ++i) {  // four keys of register group i % 4 of block i / 4
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = first + i * 8 + e;
-        const bool on = row ? row[min(key, p.n_q - 1)] != 0 : key <= query;
-        seen |= (on && key < drafts && query >= 0 ? 1u : 0u) << (i * 4 + e);
-      }
-    }
+    const uint32_t seen = j == cached ? drafted : draft_bits<1>(p, (j - cached) * BKV);
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -252,15 +246,47 @@ struct KvState : FaState<D, kWaves, 1, E> {
       }
   }
 
-  // A row that has had no key yet has no reference point: it takes the tile's.
-  __device__ __forceinline__ void first_point(const f32x16 (&s)[1][2]) {
-    if (__builtin_amdgcn_ballot_w64(this->m_run[0] == -INFINITY) != 0) this->raise(0, this->tile_max(s[0]));
+  // Which of the drafted keys first .. first + 63 this lane's row attends: bit 16 kb + r for score
+  // register r of block kb.  kGroups groups of four are loaded at a time: all of them ahead of
+  // the tiles, where the registers are free and the loads' time is hidden.
+  template <int kGroups>
+  __device__ __forceinline__ uint32_t draft_bits(const KvArgs& p, int first) const {
+    uint32_t seen = 0;
+    if (mask != nullptr) {
+      const uint8_t* row = mask + static_cast<int64_t>(query < 0 ? 0 : query) * p.mask_row;
+#pragma unroll 1
+      for (int i = 0; i < 8; i += kGroups) {
+        uint32_t on[4 * kGroups];
+#pragma unroll
+        for (int e = 0; e < 4 * kGroups; ++e) {
+          on[e] = row[min(first + h * 4 + (i + e / 4) * 8 + e % 4, p.n_q - 1)];
+        }
+#pragma unroll
+        for (int e = 0; e < 4 * kGroups; ++e) seen |= (on[e] != 0 ? 1u : 0u) << (i * 4 + e);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) seen |= (first + h * 4 + (e / 4) * 8 + e % 4 <= query ? 1u : 0u) << e;
+    }
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      if (first + h * 4 + (e / 4) * 8 + e % 4 >= drafts || query < 0) seen &= ~(1u << e);
+    }
+    return seen;
+  }
+
+  // Whether the reference point has to move: a lane's sum of probabilities is too large, or a row
+  // has had no key yet and so no reference point.
+  __device__ __forceinline__ bool out_of_range(float sum) const {
+    return __builtin_amdgcn_ballot_w64(sum > E::kTileSumLimit || this->m_run[0] == -INFINITY) != 0;
   }
 
   // Whether a value of the V tile is infinite or NaN.
   __device__ __forceinline__ bool has_infinite(const uint8_t* vs) const {
     constexpr uint32_t kExp = __is_same(E, fa::Bf16) ? 0x7f80u : 0x7c00u;
     bool found = false;
+    // unrolled further, its loads would not fit beside the accumulators
+#pragma unroll 1
     for (int i = 0; i < kTileBytes / 1024; ++i) {
       const u32x4 w = *reinterpret_cast<const u32x4*>(vs + i * 1024 + lane * 16);
 #pragma unroll
@@ -271,44 +297,54 @@ struct KvState : FaState<D, kWaves, 1, E> {
     return __builtin_amdgcn_ballot_w64(found) != 0;
   }
 
-  // O^T += V^T P^T without the keys of probability zero: a drafted token that a row does not attend
-  // may hold infinities or NaN, and 0 times those is not 0.  Rare, so one key after the other.
-  __device__ __forceinline__ void pv_attended(const uint8_t* vs, const u32x4 (&pb)[2][2]) {
-    typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
-#pragma unroll 1
-    for (int key = 0; key < BKV; ++key) {
-      // key 32 kb + 16 u + 8 w2 + 4 half + 2 w1 + e lies in half `half`, word 2 w2 + w1 of pb[kb][u]
-      uint32_t word = 0;
+  // O^T += V^T P^T for a tile with infinities or NaN, which a row that does not attend their key must
+  // not see: 0 times those is not 0.  The finite values are multiplied as they are, and where a row
+  // gives a positive infinity (or NaN) or a negative one (or NaN) any weight, it is added.
+  __device__ __forceinline__ void pv_infinite(const uint8_t* vs, const u32x4 (&pb)[2][2]) {
+    constexpr uint32_t kExp = __is_same(E, fa::Bf16) ? 0x7f80u : 0x7c00u;
+    constexpr uint32_t kOne = __is_same(E, fa::Bf16) ? 0x3f80u : 0x3c00u;
+    const uint32_t base = fa::lds_addr(vs);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int at = ((key >> 5) << 3) + (((key >> 4) & 1) << 2) + (((key >> 3) & 1) << 1) + ((key >> 1) & 1);
-        if (at == i) word = pb[i >> 3][(i >> 2) & 1][i & 3];
-      }
-      uint32_t bits = (key & 1) ? word >> 16 : word & 0xffffu;
-      const uint32_t theirs = __builtin_bit_cast(uint32_t, other_half(__builtin_bit_cast(float, bits)));
-      if (((key >> 2) & 1) != h) bits = theirs;
-      const float prob = to_float(static_cast<uint16_t>(bits));
+    for (int db = 0; db < Base::kDBlocks; ++db) {
+      f32x16 up = {}, down = {};
 #pragma unroll
-      for (int db = 0; db < Base::kDBlocks; ++db)
+      for (int i = 0; i < 4; ++i) {
+        u32x4 a = this->vt_read(base, db * 4 + i);
+        fa::lds_wait(a, 0);
+        u32x4 ups, downs;
 #pragma unroll
-        for (int rq = 0; rq < 4; ++rq) {
-          const u16x4 x = *reinterpret_cast<const u16x4*>(vs + fa::v_off<D>(key, db * 32 + rq * 8 + h * 4));
+        for (int w = 0; w < 4; ++w) {
+          uint32_t finite = 0, u = 0, d = 0;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float value = prob == 0.f ? 0.f : to_float(x[e]);
-            this->acc_o[0][db][rq * 4 + e] = fmaf(prob, value, this->acc_o[0][db][rq * 4 + e]);
+          for (int e = 0; e < 32; e += 16) {
+            const uint32_t bits = (a[w] >> e) & 0xffffu;
+            const bool infinite = (bits & kExp) == kExp, nan = (bits & 0x7fffu) > kExp;
+            finite |= infinite ? 0u : bits << e;
+            u |= infinite && (nan || bits < 0x8000u) ? kOne << e : 0u;
+            d |= infinite && (nan || bits >= 0x8000u) ? kOne << e : 0u;
           }
+          a[w] = finite;
+          ups[w] = u;
+          downs[w] = d;
         }
+        const u32x4 b = pb[i >> 1][i & 1];
+        this->acc_o[0][db] = E::mfma(a, b, this->acc_o[0][db]);
+        up = E::mfma(ups, b, up);
+        down = E::mfma(downs, b, down);
+        __builtin_amdgcn_sched_barrier(0);  // one operand at a time: registers
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        this->acc_o[0][db][r] += (up[r] > 0.f ? INFINITY : 0.f) + (down[r] > 0.f ? -INFINITY : 0.f);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
-  }
-  static __device__ __forceinline__ float to_float(uint16_t bits) {
-    return __is_same(E, fa::Bf16) ? bf16_to_f32(bits) : f16_to_f32(bits);
   }
 
   // O^T += V^T P^T of tile j.
   __device__ __forceinline__ void add_values(const uint8_t* vs, const u32x4 (&pb)[1][2][2], int j) {
     if (kTree && j >= cached && has_infinite(vs)) {
-      pv_attended(vs, pb[0]);
+      pv_infinite(vs, pb[0]);
     } else {
       this->pv(vs, pb);
     }
@@ -362,53 +398,51 @@ __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 
 __device__ __forceinline__ float lse_of(float m, float l) { return (m + __log2f(l)) * 0.69314718055994530942f; }
 
 // One pipeline step for tile j of [.., end), as fa_step: on entry LDS holds K_{j+1} and V_j, sc the
-// masked scores of tile j.  iv2: places of V_{j+2}; the table entry of tile j+3 has been fetched.
-// kGuard false: tiles j+1 .. j+3 exist and tile j+1 is whole.
-template <bool kGuard, class St>
+// masked scores of tile j.  iv2: places of V_{j+2}; the table entries of tile j+3 have been fetched.
+// kTail false: tile j+1 exists and is whole, and its scores are taken into sn between the
+// probabilities of tile j.  kTail true: any tile, one thing after the other, the next scores into sc.
+template <bool kTail, class St>
 __device__ __forceinline__ void kv_step(St& st, const KvArgs& p, int j, int end, uint8_t* ring, int c, bool act,
                                         uint32_t& iv2, f32x16 (&sc)[1][2], f32x16 (&sn)[1][2]) {
   constexpr int T = St::kTileBytes;
   constexpr int L = St::kLoadsPerWave;
   const int c1 = c == 2 ? 0 : c + 1;
   const int c2 = c == 0 ? 2 : c - 1;
-  const bool has_next = !kGuard || j + 1 < end;
-  const bool load_v = !kGuard || j + 2 < end;
-  const bool load_k = !kGuard || j + 3 < end;
+  const bool load_v = j + 2 < end, load_k = j + 3 < end;
   uint32_t ik3 = 0, iv3 = 0;
   if (load_k) {
-    st.places(p, j + 3, ik3, iv3);
+    st.places(p, j + 3, st.fetched(j + 3), ik3, iv3);
     st.fetch(p, j + 4);
   }
   if (load_v) st.template load<true>(p, ring + (3 + c2) * T, j + 2, iv2);
   if (load_k) st.template load<false>(p, ring + c * T, j + 3, ik3);
   iv2 = iv3;
-  u32x4 pb[1][2][2];
-  float rs[1];
-  if (!kGuard || act) {
-    st.first_point(sc);
-    if constexpr (kGuard) {
+  if (!kTail || act) {
+    u32x4 pb[1][2][2];
+    float rs[1];
+    if constexpr (kTail) {
       rs[0] = st.probs(0, sc[0], pb[0]);
     } else {
       st.scores_probs(ring + c1 * T, sn, sc, pb, rs);
     }
-    if (__builtin_amdgcn_ballot_w64(rs[0] > St::Element::kTileSumLimit) != 0) {
+    if (st.out_of_range(rs[0])) {
       st.raise(0, st.tile_max(sc[0]));
       rs[0] = st.probs(0, sc[0], pb[0]);
     }
     st.l_part[0] += rs[0];
-    if (kGuard) {
+    if constexpr (kTail) {
       st.add_values(ring + (3 + c) * T, pb, j);
-      if (has_next) {
-        st.scores(ring + c1 * T, sn);
-        if (st.needs_mask(j + 1)) st.hide(p, sn, j + 1);
+      if (j + 1 < end) {
+        st.scores(ring + c1 * T, sc);
+        if (st.needs_mask(j + 1)) st.hide(p, sc, j + 1);
       }
     } else {
       st.pv(ring + (3 + c) * T, pb);
     }
   }
-  if (load_v && load_k) {
+  if (load_k) {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * L) : "memory");
-  } else if (load_v || load_k) {
+  } else if (load_v) {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(L) : "memory");
   } else {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -431,6 +465,7 @@ __device__ __forceinline__ void kv_wide_body(const KvArgs& p) {
   constexpr int kThreads = kWaves * 64;
   constexpr int kChunks = D / 8;
   __shared__ __attribute__((aligned(16))) uint8_t ring[6 * T];
+  __shared__ __attribute__((aligned(16))) uint8_t ids[kTree ? kWaves * 256 : 16];
 
   Share s = share_of(p);
   if (!s.live) return;
@@ -442,6 +477,7 @@ __device__ __forceinline__ void kv_wide_body(const KvArgs& p) {
   st.wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   st.col = st.lane & 31;
   st.h = st.lane >> 5;
+  st.ids = ids + (kTree ? st.wave * 256 : 0);
   st.init(p, s);
   const int wave_row = s.row0 + st.wave * 32;
   const bool act = wave_row < p.rows;
@@ -453,23 +489,25 @@ __device__ __forceinline__ void kv_wide_body(const KvArgs& p) {
   const int per = (total + p.splits - 1) / p.splits;
   const int begin = min(total, s.split * per), end = min(total, begin + per);
   if (begin < end) {
-    uint32_t ik, iv0, iv1 = 0, iv2 = 0;
-    const auto place = [&](int j, uint32_t& iv) {  // K_j goes out; its values' places stay
-      st.fetch(p, j);
-      st.places(p, j, ik, iv);
-    };
-    place(begin, iv0);
-    st.template load<false>(p, ring, begin, ik);
+    uint32_t ik0, ik1 = 0, ik2 = 0, iv0, iv1 = 0, iv2 = 0;
+    {
+      const uint32_t id0 = st.entry_now(p, begin);
+      const uint32_t id1 = begin + 1 < end ? st.entry_now(p, begin + 1) : 0;
+      const uint32_t id2 = begin + 2 < end ? st.entry_now(p, begin + 2) : 0;
+      st.places(p, begin, id0, ik0, iv0);
+      if (begin + 1 < end) st.places(p, begin + 1, id1, ik1, iv1);
+      if (begin + 2 < end) st.places(p, begin + 2, id2, ik2, iv2);
+    }
+    if (begin + 3 < end) st.fetch(p, begin + 3);
+    st.template load<false>(p, ring, begin, ik0);
     st.template load<true>(p, ring + 3 * T, begin, iv0);
     if (begin + 1 < end) {
-      place(begin + 1, iv1);
-      st.template load<false>(p, ring + T, begin + 1, ik);
+      st.template load<false>(p, ring + T, begin + 1, ik1);
       st.template load<true>(p, ring + 4 * T, begin + 1, iv1);
     }
+    if (begin + 2 < end) st.template load<false>(p, ring + 2 * T, begin + 2, ik2);
+    if (kTree && begin <= st.cached && st.cached < end) st.drafted = st.template draft_bits<8>(p, 0);
     if (begin + 2 < end) {
-      place(begin + 2, iv2);
-      st.template load<false>(p, ring + 2 * T, begin + 2, ik);
-      st.fetch(p, begin + 3);
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * L) : "memory");
     } else if (begin + 1 < end) {
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");
@@ -482,20 +520,19 @@ __device__ __forceinline__ void kv_wide_body(const KvArgs& p) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     asm volatile("s_barrier" ::: "memory");
     if (st.needs_mask(begin)) st.hide(p, sa, begin);
-    const int clean = st.len / BKV;  // whole tiles; the drafted ones are masked
+    if (act) st.m_run[0] = st.tile_max(sa[0]);  // nothing to rescale yet
     int j = begin, c = 0;
     if (act) {
-      for (; j + 4 < min(clean, end); j += 2) {
+      const int whole = min(end, st.len / BKV);
+      for (; j + 2 < whole; j += 2) {
         kv_step<false>(st, p, j, end, ring, c, true, iv2, sa, sb);
         c = c == 2 ? 0 : c + 1;
         kv_step<false>(st, p, j + 1, end, ring, c, true, iv2, sb, sa);
         c = c == 2 ? 0 : c + 1;
       }
     }
-    for (; j < end; j += 2) {
-      kv_step<true>(st, p, j, end, ring, c, act, iv2, sa, sb);
-      c = c == 2 ? 0 : c + 1;
-      if (j + 1 < end) kv_step<true>(st, p, j + 1, end, ring, c, act, iv2, sb, sa);
+    for (; j < end; ++j) {
+      kv_step<true>(st, p, j, end, ring, c, act, iv2, sa, sa);
       c = c == 2 ? 0 : c + 1;
     }
   }
@@ -571,6 +608,7 @@ __device__ __forceinline__ void kv_narrow_body(const KvArgs& p) {
   static_assert(Narrow<D>::kRows * kRow <= 2 * T, "a wave's part reuses its tiles");
   __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves * 2 * T];
   __shared__ float stats[2][kWaves][Narrow<D>::kRows];
+  __shared__ __attribute__((aligned(16))) uint8_t ids[kTree ? kWaves * 256 : 16];
 
   Share s = share_of(p);
   if (!s.live) return;
@@ -584,6 +622,7 @@ __device__ __forceinline__ void kv_narrow_body(const KvArgs& p) {
   st.wave = 0;
   st.col = st.lane & 31;
   st.h = st.lane >> 5;
+  st.ids = ids + (kTree ? wave * 256 : 0);
   st.init(p, s);
   int64_t q_at;
   st.set_query(p, s, s.row0 + st.col, q_at);
@@ -594,28 +633,30 @@ __device__ __forceinline__ void kv_narrow_body(const KvArgs& p) {
   const int begin = min(total, s.split * per), end = min(total, begin + per);
   uint32_t ik = 0, iv = 0, iv_next = 0;
   if (begin + wave < end) {
-    st.fetch(p, begin + wave);
-    st.places(p, begin + wave, ik, iv);
+    st.places(p, begin + wave, st.entry_now(p, begin + wave), ik, iv);
+    if (begin + wave + kWaves < end) st.fetch(p, begin + wave + kWaves);
     st.template load<false>(p, kring, begin + wave, ik);
     st.template load<true>(p, vring, begin + wave, iv);
-    st.fetch(p, begin + wave + kWaves);
+    if (kTree && st.cached >= begin + wave && st.cached < end && (st.cached - begin - wave) % kWaves == 0) {
+      st.drafted = st.template draft_bits<8>(p, 0);
+    }
   }
   for (int j = begin + wave; j < end; j += kWaves) {
     const bool next = j + kWaves < end;
-    // all but V_j (and a table entry behind it) have landed
+    // all but V_j have landed
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");
     f32x16 sc[1][2];
     st.scores(kring, sc);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (next) {
-      st.places(p, j + kWaves, ik, iv_next);
+      st.places(p, j + kWaves, st.fetched(j + kWaves), ik, iv_next);
       st.template load<false>(p, kring, j + kWaves, ik);
     }
     if (st.needs_mask(j)) st.hide(p, sc, j);
-    st.first_point(sc);
+    if (j == begin + wave) st.m_run[0] = st.tile_max(sc[0]);  // nothing to rescale yet
     u32x4 pb[1][2][2];
     float rs = st.probs(0, sc[0], pb[0]);
-    if (__builtin_amdgcn_ballot_w64(rs > E::kTileSumLimit) != 0) {
+    if (st.out_of_range(rs)) {
       st.raise(0, st.tile_max(sc[0]));
       rs = st.probs(0, sc[0], pb[0]);
     }
@@ -628,8 +669,8 @@ __device__ __forceinline__ void kv_narrow_body(const KvArgs& p) {
     st.add_values(vring, pb, j);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (next) {
+      if (j + 2 * kWaves < end) st.fetch(p, j + 2 * kWaves);
       st.template load<true>(p, vring, j + kWaves, iv_next);
-      st.fetch(p, j + 2 * kWaves);
     }
   }
 

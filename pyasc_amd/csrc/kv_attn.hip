@@ -33,18 +33,18 @@ struct Launch {
 };
 
 constexpr int kMaxSplits = 64;
-constexpr int kCus = 256;
+constexpr int64_t kCus = 256;
 
-// How the rows of one key / value head are taken, and over how many workgroups their keys are
-// split.  Up to 32 rows go to kv_narrow, more to kv_wide.
+// How the rows of one key / value head are taken: up to 32 of them by kv_narrow, more by kv_wide.
+// Where they are too few workgroups to fill the chip twice, the keys are split too.
 void plan(Launch& L, const asc_attention_t& a) {
   KvArgs& p = L.p;
   L.wide = p.rows > Narrow<64>::kRows;
   const int rows = L.wide ? (a.head_dim == 64 ? Wide<64>::kRows : Wide<128>::kRows) : Narrow<64>::kRows;
   p.row_blocks = static_cast<int>(asc::ceil_div(p.rows, rows));
+  const int64_t tiles = asc::ceil_div(p.capacity, asc::fa::BKV) + (p.k_draft ? asc::ceil_div(p.n_q, asc::fa::BKV) : 0);
   const int64_t shares = a.batch * a.kv_heads * p.row_blocks;
   const int64_t slots = kCus * (a.head_dim == 64 ? 2 : 1);
-  const int64_t tiles = asc::ceil_div(p.capacity, asc::fa::BKV) + (p.k_draft ? asc::ceil_div(p.n_q, asc::fa::BKV) : 0);
   const int64_t least = L.wide ? 4 : 8;  // tiles of a split
   int64_t splits = shares >= slots ? 1 : (L.wide ? 1 : 2) * slots / shares;
   if (splits > tiles / least) splits = tiles / least;
@@ -55,9 +55,10 @@ void plan(Launch& L, const asc_attention_t& a) {
   L.blocks = asc::ceil_div(p.units, 8) * 8 * p.row_blocks;
 }
 
+// Bytes of the parts: their values, statistics and flags.
 int64_t workspace_of(const Launch& L, int head_dim) {
   if (L.blocks == 0 || L.p.splits == 1) return 0;
-  return L.rows_all * L.p.splits * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+  return L.p.units * (static_cast<int64_t>(L.p.rows) * (head_dim + 2) + 1) * static_cast<int64_t>(sizeof(float));
 }
 
 int32_t make(const asc_attention_t* a, bool tree, const char* what, Launch& L) {
@@ -77,6 +78,7 @@ int32_t make(const asc_attention_t* a, bool tree, const char* what, Launch& L) {
   p.o_batch = a->o.batch_stride;
   p.o_head = a->o.head_stride;
   p.o_seq = a->o.seq_stride;
+  p.batch = static_cast<int32_t>(a->batch);
   p.kv_heads = static_cast<int32_t>(a->kv_heads);
   p.group = static_cast<int32_t>(a->q_heads / a->kv_heads);
   p.n_q = static_cast<int32_t>(a->q_len);
@@ -118,6 +120,7 @@ int32_t make(const asc_attention_t* a, bool tree, const char* what, Launch& L) {
     p.mask = a->tree_mask;
     p.mask_batch = a->mask_batch_stride;
     p.mask_row = a->mask_row_stride;
+    p.mask_words = a->q_len % 4 == 0 && ((reinterpret_cast<uintptr_t>(p.mask) | p.mask_batch | p.mask_row) & 3) == 0;
   }
   plan(L, *a);
   ASC_REQUIRE(L.blocks < int64_t{1} << 22, ASC_ERR_UNSUPPORTED,
@@ -150,7 +153,8 @@ int32_t run(const asc_attention_t* a, bool tree, const char* what, void* workspa
               "%s: the workspace must hold %lld bytes, 16-byte aligned", what, static_cast<long long>(need));
   if (need != 0) {
     L.p.part_o = static_cast<float*>(workspace);
-    L.p.part_ml = L.p.part_o + L.rows_all * L.p.splits * a->head_dim;
+    L.p.part_ml = L.p.part_o + L.p.units * static_cast<int64_t>(L.p.rows) * a->head_dim;
+    L.p.infinite = reinterpret_cast<int32_t*>(L.p.part_ml + L.p.units * static_cast<int64_t>(L.p.rows) * 2);
   }
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const bool f16 = a->dtype == ASC_DT_FLOAT16;

@@ -50,11 +50,18 @@ struct GradArgs {
   float scale, scale_log2, inv_scale;
 };
 
-__device__ __forceinline__ Share grad_share(uint32_t blocks, uint32_t splits, uint32_t units, uint32_t kv_heads) {
+// One workgroup's share: a sequence's key / value head, a block of the rows (keys) that it sums into,
+// and which split of what it streams.
+struct GradShare {
+  int b, head, row0, split;
+  bool live;
+};
+// As share_of: the blocks of one split run on one XCD one after the other.
+__device__ __forceinline__ GradShare grad_share(uint32_t blocks, uint32_t splits, uint32_t units, uint32_t kv_heads) {
   const uint32_t slot = blockIdx.x >> 3;
   const uint32_t per = slot / blocks;
   const uint32_t unit = per * 8 + (blockIdx.x & 7);
-  Share s;
+  GradShare s;
   s.live = unit < units;
   const uint32_t bh = unit / splits;
   s.split = static_cast<int>(unit - bh * splits);
@@ -226,7 +233,7 @@ __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
   constexpr int kLoads = 2 * (kKeys / T::kRowsPerLoad / kWaves);  // of K and V, per wave and tile
   __shared__ __attribute__((aligned(16))) uint8_t ring[6 * kTile];  // K stages 0-2, V stages 3-5
 
-  const Share s = grad_share(p.q_blocks, p.q_splits, p.q_units, p.kv_heads);
+  const GradShare s = grad_share(p.q_blocks, p.q_splits, p.q_units, p.kv_heads);
   if (!s.live) return;
   T t;
   t.init(threadIdx.x);
@@ -349,7 +356,7 @@ __device__ __forceinline__ void grad_kv_body(const GradArgs& p) {
   __shared__ __attribute__((aligned(16))) uint8_t ring[6 * kTile];  // Q stages 0-2, dO stages 3-5
   __shared__ __attribute__((aligned(16))) float values[3][2 * kRows];  // -lse / scale and -delta of a tile
 
-  const Share s = grad_share(p.kv_blocks, p.kv_splits, p.kv_units, p.kv_heads);
+  const GradShare s = grad_share(p.kv_blocks, p.kv_splits, p.kv_units, p.kv_heads);
   if (!s.live) return;
   T t;
   t.init(threadIdx.x);

@@ -52,12 +52,15 @@ struct KvArgs {
   int64_t table_stride;
   const uint8_t* mask;  // [batch?, n_q, n_q] or null: a chain
   int64_t mask_batch, mask_row;
-  float* part_o;   // [rows of all heads][splits][D], unnormalised
-  float* part_ml;  // [rows of all heads][splits][2]: reference point (log2), sum
+  int32_t mask_words;  // the mask's rows can be read four bytes at a time
+  float* part_o;   // [unit][rows][D], unnormalised
+  float* part_ml;  // [unit][rows][2]: reference point (log2), sum
+  int32_t* infinite;  // [unit]: whether its drafted values hold infinities or NaN
   uint32_t num_pages, page_size, page_magic, page_shift;
   int32_t capacity;  // keys a sequence can have
-  int32_t kv_heads, group, n_q, rows, row_blocks, splits;
-  uint32_t units;  // batch * kv_heads * splits
+  int32_t batch, kv_heads, group, n_q, rows, row_blocks;
+  int32_t splits;  // of each sequence's keys
+  uint32_t units;  // batch * splits * kv_heads
   float scale_log2;
 };
 
@@ -65,32 +68,48 @@ struct KvArgs {
 constexpr uint32_t kNone = 0xffffffffu;
 static __device__ const u32x4 kZeroRow[16] = {};
 
-// One workgroup's share: a sequence's key / value head, a block of its rows, a range of its tiles.
+// Cached keys of sequence b and its drafted ones; bad: a length outside what the call can hold.
+__device__ __forceinline__ int clamped(int n, int most, bool& bad) {
+  bad = bad || n < 0 || n > most;
+  return n < 0 ? 0 : (n > most ? most : n);
+}
+template <bool kTree>
+__device__ __forceinline__ void keys_of(const KvArgs& p, int b, int& len, int& drafts, bool& bad) {
+  len = clamped(p.lengths ? p.lengths[b] : p.capacity, p.capacity, bad);
+  drafts = 0;
+  if constexpr (kTree) drafts = clamped(p.draft_lengths ? p.draft_lengths[b] : p.n_q, p.n_q, bad);
+}
+
+// One workgroup's share: a sequence's key / value head, a block of its rows, a split of its keys;
+// `unit` is where its part goes.
 struct Share {
   int b, head, row0, split;
+  uint32_t unit;
   bool live;
 };
 
-// Workgroup i runs on XCD i % 8.  The row blocks of one share of keys run on one XCD one after the
+// Workgroup i runs on XCD i % 8.  The row blocks of one range of keys run on one XCD one after the
 // other: they read the same keys through its L2.
+//
+// A sequence's keys may be split over workgroups, each with an even share of its tiles.
 __device__ __forceinline__ Share share_of(const KvArgs& p) {
   const uint32_t slot = blockIdx.x >> 3;
   const uint32_t per = slot / p.row_blocks;
-  const uint32_t unit = per * 8 + (blockIdx.x & 7);
   Share s;
-  s.live = unit < p.units;
-  const uint32_t bh = unit / p.splits;
-  s.split = static_cast<int>(unit - bh * p.splits);
-  s.b = static_cast<int>(bh / p.kv_heads);
-  s.head = static_cast<int>(bh - static_cast<uint32_t>(s.b) * p.kv_heads);
+  s.unit = per * 8 + (blockIdx.x & 7);
+  s.live = s.unit < p.units;
   s.row0 = static_cast<int>(slot - per * p.row_blocks);
+  const uint32_t range = s.unit / p.kv_heads;
+  s.head = static_cast<int>(s.unit - range * p.kv_heads);
+  s.b = static_cast<int>(range / p.splits);
+  s.split = static_cast<int>(range - static_cast<uint32_t>(s.b) * p.splits);
   return s;
 }
 
 // kTree: there may be a table of pages, drafted keys and a mask over them.
 template <int D, int kWaves, class E, bool kTree>
-struct KvState : FaState<D, kWaves, 1, E, true> {
-  using Base = FaState<D, kWaves, 1, E, true>;
+struct KvState : FaState<D, kWaves, 1, E, kTree> {
+  using Base = FaState<D, kWaves, 1, E, kTree>;
   using Base::col;
   using Base::h;
   using Base::kKSteps;
@@ -104,26 +123,27 @@ struct KvState : FaState<D, kWaves, 1, E, true> {
   int cached;          // tiles of cached keys; the drafted ones follow in tiles of their own
   int query;           // this lane's query (of n_q), or -1: no row
   const int32_t* table;
+  int* infinite;       // LDS, one of each wave: 1 where it has loaded infinite or NaN drafted values
+  int wave_of;         // in the workgroup
   uint8_t* ids;        // LDS, 256 bytes of this wave: the fetched entries of a tile's keys
-  uint32_t drafted;    // hidden_bits of the first drafted tile
+  uint32_t drafted;    // mask_bits of the first drafted tile
   uint32_t k0, v0, kd0, vd0;  // the sequence's first row (16-byte units)
+  uint32_t k_step, v_step;    // from row to row
+  bool even;                  // whole tiles lie in one piece, within 2 GiB of it
   const uint8_t* mask;
   bool poison;         // a page or a length outside the cache: the rows' results are NaN
 
   __device__ __forceinline__ void init(const KvArgs& p, const Share& s) {
-    const int n = p.lengths ? p.lengths[s.b] : p.capacity;
-    poison = n < 0 || n > p.capacity;
-    len = n < 0 ? 0 : (n > p.capacity ? p.capacity : n);
-    drafts = 0;
-    if constexpr (kTree) {
-      const int d = p.draft_lengths ? p.draft_lengths[s.b] : p.n_q;
-      poison = poison || d < 0 || d > p.n_q;
-      drafts = d < 0 ? 0 : (d > p.n_q ? p.n_q : d);
-    }
+    poison = false;
+    keys_of<kTree>(p, s.b, len, drafts, poison);
+    if (kTree) infinite[wave_of] = 0;
     cached = (len + BKV - 1) / BKV;
     const bool paged = kTree && p.table != nullptr;
     k0 = s.head * p.ks.head + (paged ? 0 : s.b * p.ks.batch);
     v0 = s.head * p.vs.head + (paged ? 0 : s.b * p.vs.batch);
+    k_step = p.ks.seq;
+    v_step = p.vs.seq;
+    even = (!paged || p.page_size % BKV == 0) && max(k_step, v_step) < (1u << 31) / (16 * BKV);
     if constexpr (kTree) {
       table = paged ? p.table + s.b * p.table_stride : nullptr;
       kd0 = s.head * p.kds.head + s.b * p.kds.batch;
@@ -140,10 +160,13 @@ struct KvState : FaState<D, kWaves, 1, E, true> {
       this->voff_k[i] = (pos ^ fa::kswz<D>(row)) << 4;
     }
     this->voff_v = (pos ^ fa::vswz<D>(rr)) << 4;
-    this->kaddr[0] = fa::k_off<D>(col, h);
+    constexpr int kK = kTree ? 1 : kKSteps, kV = kTree ? 1 : Base::kDBlocks;
+#pragma unroll
+    for (int kk = 0; kk < kK; ++kk) this->kaddr[kk] = fa::k_off<D>(col, kk * 2 + h);
     const int g_lane = lane & 15;
     const int tr_col = ((lane >> 4) & 1) * 16 + (g_lane & 3) * 4;
-    this->vaddr[0] = fa::v_off<D>(h * 4 + (g_lane >> 2), tr_col);
+#pragma unroll
+    for (int db = 0; db < kV; ++db) this->vaddr[db] = fa::v_off<D>(h * 4 + (g_lane >> 2), db * 32 + tr_col);
   }
 
   __device__ __forceinline__ int tiles() const { return cached + (drafts + BKV - 1) / BKV; }
@@ -211,6 +234,25 @@ struct KvState : FaState<D, kWaves, 1, E, true> {
     asm volatile("" : "+s"(wave_lds));
     constexpr int kLanesPerRow = 64 / kRowsPerLoad;
     const int rr = lane / kLanesPerRow;
+    if (whole && even) {
+      // rows at a fixed distance from the tile's first: one scalar base and an offset per lane
+      const uint32_t first = __builtin_amdgcn_readfirstlane(places);
+      base += static_cast<uint64_t>(first) * 16;
+      const uint32_t stride = (kIsV ? v_step : k_step) * 16;
+#pragma unroll
+      for (int i = 0; i < kLoadsPerWave; ++i) {
+        const uint32_t row = kRowsPerLoad * (wave * kLoadsPerWave + i);
+        const uint32_t off = rr * stride + (kIsV ? this->voff_v : this->voff_k[i & 3]);
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)(reinterpret_cast<const uint8_t*>(base + row * stride) + off),
+            (__attribute__((address_space(3))) void*)(dst + wave_lds + i * 1024), 16, 0, 0);
+      }
+      return;
+    }
+    if (kTree && kIsV && j >= cached) {
+      load_drafted_values(base, dst + wave_lds, places);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < kLoadsPerWave; ++i) {
       const int row = kRowsPerLoad * (wave * kLoadsPerWave + i) + rr;
@@ -222,6 +264,31 @@ struct KvState : FaState<D, kWaves, 1, E, true> {
           (const __attribute__((address_space(1))) void*)(src + (kIsV ? this->voff_v : this->voff_k[i & 3])),
           (__attribute__((address_space(3))) void*)(dst + wave_lds + i * 1024), 16, 0, 0);
     }
+  }
+
+  // Drafted values go through registers: infinities and NaN become zeros, because 0 times those is
+  // not 0 and a row must not see the values of a token that it does not attend.  The rows that
+  // attend it get them back at the end (add_infinite).
+  __device__ __forceinline__ void load_drafted_values(uint64_t base, uint8_t* dst, uint32_t places) const {
+    constexpr uint32_t kExp = __is_same(E, fa::Bf16) ? 0x7f80u : 0x7c00u;
+    const int rr = lane / (64 / kRowsPerLoad);
+    bool found = false;
+#pragma unroll 4
+    for (int i = 0; i < kLoadsPerWave; ++i) {
+      const int row = kRowsPerLoad * (wave * kLoadsPerWave + i) + rr;
+      const uint32_t at =
+          static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(row * 4, static_cast<int>(places)));
+      u32x4 w = {0, 0, 0, 0};
+      if (at != kNone) w = *reinterpret_cast<const u32x4*>(base + static_cast<uint64_t>(at) * 16 + this->voff_v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool low = (w[e] & kExp) == kExp, high = (w[e] >> 16 & kExp) == kExp;
+        found = found || low || high;
+        w[e] &= (low ? 0xffff0000u : ~0u) & (high ? 0xffffu : ~0u);
+      }
+      *reinterpret_cast<u32x4*>(dst + i * 1024 + lane * 16) = w;
+    }
+    if (__builtin_amdgcn_ballot_w64(found) != 0) infinite[wave_of] = 1;
   }
 
   __device__ __forceinline__ bool needs_mask(int j) const { return (j + 1) * BKV > len; }
@@ -237,7 +304,12 @@ struct KvState : FaState<D, kWaves, 1, E, true> {
         }
       return;
     }
-    const uint32_t seen = j == cached ? drafted : draft_bits<1>(p, (j - cached) * BKV);
+    uint32_t seen = drafted;
+    if (j > cached) {
+      uint32_t words[8];
+      mask_words(p, (j - cached) * BKV, words);
+      seen = mask_bits((j - cached) * BKV, words);
+    }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -247,30 +319,42 @@ struct KvState : FaState<D, kWaves, 1, E, true> {
   }
 
   // Which of the drafted keys first .. first + 63 this lane's row attends: bit 16 kb + r for score
-  // register r of block kb.  kGroups groups of four are loaded at a time: all of them ahead of
-  // the tiles, where the registers are free and the loads' time is hidden.
-  template <int kGroups>
-  __device__ __forceinline__ uint32_t draft_bits(const KvArgs& p, int first) const {
-    uint32_t seen = 0;
-    if (mask != nullptr) {
-      const uint8_t* row = mask + static_cast<int64_t>(query < 0 ? 0 : query) * p.mask_row;
-#pragma unroll 1
-      for (int i = 0; i < 8; i += kGroups) {
-        uint32_t on[4 * kGroups];
+  // register r of block kb, keys 32 kb + 8 (r / 4) + 4 h + r % 4, so four bytes of the mask's row
+  // each.  The words are asked for ahead of the tiles.
+  __device__ __forceinline__ void mask_words(const KvArgs& p, int first, uint32_t (&words)[8]) const {
+    if (mask == nullptr) return;
+    const uint8_t* row = mask + static_cast<int64_t>(query < 0 ? 0 : query) * p.mask_row;
+    if (p.mask_words) {
 #pragma unroll
-        for (int e = 0; e < 4 * kGroups; ++e) {
-          on[e] = row[min(first + h * 4 + (i + e / 4) * 8 + e % 4, p.n_q - 1)];
-        }
-#pragma unroll
-        for (int e = 0; e < 4 * kGroups; ++e) seen |= (on[e] != 0 ? 1u : 0u) << (i * 4 + e);
+      for (int i = 0; i < 8; ++i) {
+        const int key = first + (i >> 2) * 32 + (i & 3) * 8 + h * 4;
+        words[i] = *reinterpret_cast<const uint32_t*>(row + min(key, p.n_q - 4));
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 32; ++e) seen |= (first + h * 4 + (e / 4) * 8 + e % 4 <= query ? 1u : 0u) << e;
-    }
+      for (int i = 0; i < 8; ++i) {
+        words[i] = 0;
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      if (first + h * 4 + (e / 4) * 8 + e % 4 >= drafts || query < 0) seen &= ~(1u << e);
+        for (int e = 0; e < 4; ++e) {
+          const int key = first + (i >> 2) * 32 + (i & 3) * 8 + h * 4 + e;
+          words[i] |= static_cast<uint32_t>(row[min(key, p.n_q - 1)]) << (8 * e);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ uint32_t mask_bits(int first, const uint32_t (&words)[8]) const {
+    uint32_t seen = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int key = first + (i >> 2) * 32 + (i & 3) * 8 + h * 4;
+      uint32_t w = words[i];  // four flags in the lowest bits of its bytes, then next to each other
+      w = (w | w >> 4) & 0x0f0f0f0fu;
+      w = (w | w >> 2) & 0x03030303u;
+      w = (w | w >> 1) & 0x01010101u;
+      w = w * 0x10204080u >> 28;
+      if (mask == nullptr) w = (1u << min(max(query + 1 - key, 0), 4)) - 1;  // a chain: keys <= query
+      const int left = query < 0 ? 0 : min(max(drafts - key, 0), 4);
+      seen |= (w & ((1u << left) - 1)) << (4 * i);
     }
     return seen;
   }
@@ -279,75 +363,6 @@ struct KvState : FaState<D, kWaves, 1, E, true> {
   // has had no key yet and so no reference point.
   __device__ __forceinline__ bool out_of_range(float sum) const {
     return __builtin_amdgcn_ballot_w64(sum > E::kTileSumLimit || this->m_run[0] == -INFINITY) != 0;
-  }
-
-  // Whether a value of the V tile is infinite or NaN.
-  __device__ __forceinline__ bool has_infinite(const uint8_t* vs) const {
-    constexpr uint32_t kExp = __is_same(E, fa::Bf16) ? 0x7f80u : 0x7c00u;
-    bool found = false;
-    // unrolled further, its loads would not fit beside the accumulators
-#pragma unroll 1
-    for (int i = 0; i < kTileBytes / 1024; ++i) {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(vs + i * 1024 + lane * 16);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        found = found || (w[e] & kExp) == kExp || ((w[e] >> 16) & kExp) == kExp;
-      }
-    }
-    return __builtin_amdgcn_ballot_w64(found) != 0;
-  }
-
-  // O^T += V^T P^T for a tile with infinities or NaN, which a row that does not attend their key must
-  // not see: 0 times those is not 0.  The finite values are multiplied as they are, and where a row
-  // gives a positive infinity (or NaN) or a negative one (or NaN) any weight, it is added.
-  __device__ __forceinline__ void pv_infinite(const uint8_t* vs, const u32x4 (&pb)[2][2]) {
-    constexpr uint32_t kExp = __is_same(E, fa::Bf16) ? 0x7f80u : 0x7c00u;
-    constexpr uint32_t kOne = __is_same(E, fa::Bf16) ? 0x3f80u : 0x3c00u;
-    const uint32_t base = fa::lds_addr(vs);
-#pragma unroll
-    for (int db = 0; db < Base::kDBlocks; ++db) {
-      f32x16 up = {}, down = {};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        u32x4 a = this->vt_read(base, db * 4 + i);
-        fa::lds_wait(a, 0);
-        u32x4 ups, downs;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t finite = 0, u = 0, d = 0;
-#pragma unroll
-          for (int e = 0; e < 32; e += 16) {
-            const uint32_t bits = (a[w] >> e) & 0xffffu;
-            const bool infinite = (bits & kExp) == kExp, nan = (bits & 0x7fffu) > kExp;
-            finite |= infinite ? 0u : bits << e;
-            u |= infinite && (nan || bits < 0x8000u) ? kOne << e : 0u;
-            d |= infinite && (nan || bits >= 0x8000u) ? kOne << e : 0u;
-          }
-          a[w] = finite;
-          ups[w] = u;
-          downs[w] = d;
-        }
-        const u32x4 b = pb[i >> 1][i & 1];
-        this->acc_o[0][db] = E::mfma(a, b, this->acc_o[0][db]);
-        up = E::mfma(ups, b, up);
-        down = E::mfma(downs, b, down);
-        __builtin_amdgcn_sched_barrier(0);  // one operand at a time: registers
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        this->acc_o[0][db][r] += (up[r] > 0.f ? INFINITY : 0.f) + (down[r] > 0.f ? -INFINITY : 0.f);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-
-  // O^T += V^T P^T of tile j.
-  __device__ __forceinline__ void add_values(const uint8_t* vs, const u32x4 (&pb)[1][2][2], int j) {
-    if (kTree && j >= cached && has_infinite(vs)) {
-      pv_infinite(vs, pb[0]);
-    } else {
-      this->pv(vs, pb);
-    }
   }
 
   // This lane's row of the block: its query and where its output and statistics lie.
@@ -397,6 +412,42 @@ __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 
 
 __device__ __forceinline__ float lse_of(float m, float l) { return (m + __log2f(l)) * 0.69314718055994530942f; }
 
+template <class E>
+__device__ __forceinline__ u32x4 pack8(const float (&o)[8], float scale) {
+  u32x4 w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = E::pack(o[2 * e] * scale, o[2 * e + 1] * scale);
+  return w;
+}
+template <class E>
+__device__ __forceinline__ void unpack(const u32x4& w, float (&o)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint16_t bits = static_cast<uint16_t>(w[e / 2] >> (e % 2 * 16));
+    o[e] = __is_same(E, fa::Bf16) ? bf16_to_f32(bits) : f16_to_f32(bits);
+  }
+}
+
+// What the infinities and NaN among the drafted values that a row attends add to eight of its
+// results: rare, so one key after the other.
+template <class E>
+__device__ __forceinline__ void add_infinite(const KvArgs& p, int b, int head, int query, int ch, float (&o)[8]) {
+  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+  bool bad = false;
+  const int drafts = clamped(p.draft_lengths ? p.draft_lengths[b] : p.n_q, p.n_q, bad);
+  const uint8_t* mask = p.mask ? p.mask + b * p.mask_batch + query * p.mask_row : nullptr;
+  const uint8_t* v = p.v_draft + (static_cast<uint64_t>(b) * p.vds.batch + static_cast<uint64_t>(head) * p.vds.head) * 16;
+  for (int key = 0; key < drafts; ++key) {
+    if (!(mask ? mask[key] != 0 : key <= query)) continue;
+    const u16x8 x = *reinterpret_cast<const u16x8*>(v + static_cast<uint64_t>(key) * p.vds.seq * 16 + ch * 16);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float f = __is_same(E, fa::Bf16) ? bf16_to_f32(x[e]) : f16_to_f32(x[e]);
+      if (!(fabsf(f) < INFINITY)) o[e] += f;
+    }
+  }
+}
+
 // One pipeline step for tile j of [.., end), as fa_step: on entry LDS holds K_{j+1} and V_j, sc the
 // masked scores of tile j.  iv2: places of V_{j+2}; the table entries of tile j+3 have been fetched.
 // kTail false: tile j+1 exists and is whole, and its scores are taken into sn between the
@@ -430,14 +481,12 @@ __device__ __forceinline__ void kv_step(St& st, const KvArgs& p, int j, int end,
       rs[0] = st.probs(0, sc[0], pb[0]);
     }
     st.l_part[0] += rs[0];
+    st.pv(ring + (3 + c) * T, pb);
     if constexpr (kTail) {
-      st.add_values(ring + (3 + c) * T, pb, j);
       if (j + 1 < end) {
         st.scores(ring + c1 * T, sc);
         if (st.needs_mask(j + 1)) st.hide(p, sc, j + 1);
       }
-    } else {
-      st.pv(ring + (3 + c) * T, pb);
     }
   }
   if (load_k) {
@@ -466,6 +515,7 @@ __device__ __forceinline__ void kv_wide_body(const KvArgs& p) {
   constexpr int kChunks = D / 8;
   __shared__ __attribute__((aligned(16))) uint8_t ring[6 * T];
   __shared__ __attribute__((aligned(16))) uint8_t ids[kTree ? kWaves * 256 : 16];
+  __shared__ int infinite[kWaves];
 
   Share s = share_of(p);
   if (!s.live) return;
@@ -478,6 +528,8 @@ __device__ __forceinline__ void kv_wide_body(const KvArgs& p) {
   st.col = st.lane & 31;
   st.h = st.lane >> 5;
   st.ids = ids + (kTree ? st.wave * 256 : 0);
+  st.infinite = infinite;
+  st.wave_of = st.wave;
   st.init(p, s);
   const int wave_row = s.row0 + st.wave * 32;
   const bool act = wave_row < p.rows;
@@ -490,6 +542,10 @@ __device__ __forceinline__ void kv_wide_body(const KvArgs& p) {
   const int begin = min(total, s.split * per), end = min(total, begin + per);
   if (begin < end) {
     uint32_t ik0, ik1 = 0, ik2 = 0, iv0, iv1 = 0, iv2 = 0;
+    // the mask's words are asked for with the table's entries, ahead of the tiles
+    const bool drafted = kTree && begin <= st.cached && st.cached < end;
+    uint32_t words[8] = {};
+    if (drafted) st.mask_words(p, 0, words);
     {
       const uint32_t id0 = st.entry_now(p, begin);
       const uint32_t id1 = begin + 1 < end ? st.entry_now(p, begin + 1) : 0;
@@ -506,7 +562,7 @@ __device__ __forceinline__ void kv_wide_body(const KvArgs& p) {
       st.template load<true>(p, ring + 4 * T, begin + 1, iv1);
     }
     if (begin + 2 < end) st.template load<false>(p, ring + 2 * T, begin + 2, ik2);
-    if (kTree && begin <= st.cached && st.cached < end) st.drafted = st.template draft_bits<8>(p, 0);
+    if (drafted) st.drafted = st.mask_bits(0, words);
     if (begin + 2 < end) {
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * L) : "memory");
     } else if (begin + 1 < end) {
@@ -540,12 +596,20 @@ __device__ __forceinline__ void kv_wide_body(const KvArgs& p) {
   float l_run = st.l_part[0] + other_half(st.l_part[0]);
   if (st.poison) l_run = __builtin_nanf("");
   const int written = written_of(p, s.b);
+  const auto any_infinite = [&] {
+    int any = 0;
+    for (int w = 0; w < kWaves; ++w) any |= infinite[w];
+    return any;
+  };
   if (p.splits > 1) {
+    if constexpr (kTree) {
+      __syncthreads();
+      if (tid == 0) p.infinite[s.unit] = any_infinite();
+    }
     // the unnormalised part, from registers: lane (row, half h) holds d = 32 db + 8 rq + 4 h + 0..3
     const int row = wave_row + st.col;
     if (row < p.rows) {
-      const int64_t at =
-          ((static_cast<int64_t>(s.b) * p.kv_heads + s.head) * p.rows + row) * p.splits + s.split;
+      const int64_t at = static_cast<int64_t>(s.unit) * p.rows + row;
       if (st.h == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(st.m_run[0], l_run);
       if (begin < end) {
 #pragma unroll
@@ -581,14 +645,21 @@ __device__ __forceinline__ void kv_wide_body(const KvArgs& p) {
     }
   }
   __syncthreads();
+  const bool add = kTree && any_infinite();
 #pragma unroll
   for (int i = 0; i < Wide<D>::kRows * kChunks / kThreads; ++i) {
     const int cc = tid + kThreads * i;
     const int row = cc / kChunks, ch = cc % kChunks;
     int64_t o_at, lse_at;
     if (!out_row(p, s, s.row0 + row, written, o_at, lse_at)) continue;
-    *reinterpret_cast<u32x4*>(p.o + o_at + ch * 8) =
-        *reinterpret_cast<const u32x4*>(ring + (row >> 6) * T + fa::k_off<D>(row & 63, ch));
+    u32x4 w = *reinterpret_cast<const u32x4*>(ring + (row >> 6) * T + fa::k_off<D>(row & 63, ch));
+    if (add) {
+      float o[8];
+      unpack<E>(w, o);
+      add_infinite<E>(p, s.b, s.head, (s.row0 + row) % p.n_q, ch, o);
+      w = pack8<E>(o, 1.0f);
+    }
+    *reinterpret_cast<u32x4*>(p.o + o_at + ch * 8) = w;
   }
 }
 
@@ -609,6 +680,7 @@ __device__ __forceinline__ void kv_narrow_body(const KvArgs& p) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves * 2 * T];
   __shared__ float stats[2][kWaves][Narrow<D>::kRows];
   __shared__ __attribute__((aligned(16))) uint8_t ids[kTree ? kWaves * 256 : 16];
+  __shared__ int infinite[kWaves];
 
   Share s = share_of(p);
   if (!s.live) return;
@@ -623,6 +695,8 @@ __device__ __forceinline__ void kv_narrow_body(const KvArgs& p) {
   st.col = st.lane & 31;
   st.h = st.lane >> 5;
   st.ids = ids + (kTree ? wave * 256 : 0);
+  st.infinite = infinite;
+  st.wave_of = wave;
   st.init(p, s);
   int64_t q_at;
   st.set_query(p, s, s.row0 + st.col, q_at);
@@ -633,13 +707,15 @@ __device__ __forceinline__ void kv_narrow_body(const KvArgs& p) {
   const int begin = min(total, s.split * per), end = min(total, begin + per);
   uint32_t ik = 0, iv = 0, iv_next = 0;
   if (begin + wave < end) {
+    const bool drafted =
+        kTree && st.cached >= begin + wave && st.cached < end && (st.cached - begin - wave) % kWaves == 0;
+    uint32_t words[8] = {};
+    if (drafted) st.mask_words(p, 0, words);
     st.places(p, begin + wave, st.entry_now(p, begin + wave), ik, iv);
     if (begin + wave + kWaves < end) st.fetch(p, begin + wave + kWaves);
     st.template load<false>(p, kring, begin + wave, ik);
     st.template load<true>(p, vring, begin + wave, iv);
-    if (kTree && st.cached >= begin + wave && st.cached < end && (st.cached - begin - wave) % kWaves == 0) {
-      st.drafted = st.template draft_bits<8>(p, 0);
-    }
+    if (drafted) st.drafted = st.mask_bits(0, words);
   }
   for (int j = begin + wave; j < end; j += kWaves) {
     const bool next = j + kWaves < end;
@@ -666,7 +742,7 @@ __device__ __forceinline__ void kv_narrow_body(const KvArgs& p) {
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    st.add_values(vring, pb, j);
+    st.pv(vring, pb);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (next) {
       if (j + 2 * kWaves < end) st.fetch(p, j + 2 * kWaves);
@@ -694,6 +770,11 @@ __device__ __forceinline__ void kv_narrow_body(const KvArgs& p) {
   }
   __syncthreads();
   const int written = written_of(p, s.b);
+  int add = 0;
+  if constexpr (kTree) {
+    for (int w = 0; w < kWaves; ++w) add |= infinite[w];
+    if (p.splits > 1 && tid == 0) p.infinite[s.unit] = add;
+  }
 #pragma unroll
   for (int i = 0; i < Narrow<D>::kRows * (D / 8) / (kWaves * 64); ++i) {
     const int cc = tid + kWaves * 64 * i;
@@ -722,8 +803,7 @@ __device__ __forceinline__ void kv_narrow_body(const KvArgs& p) {
       }
     }
     if (p.splits > 1) {
-      const int64_t at =
-          ((static_cast<int64_t>(s.b) * p.kv_heads + s.head) * p.rows + s.row0 + row) * p.splits + s.split;
+      const int64_t at = static_cast<int64_t>(s.unit) * p.rows + s.row0 + row;
       if (ch == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m, l_run);
       *reinterpret_cast<f32x4*>(p.part_o + at * D + ch * 8) = f32x4{o[0], o[1], o[2], o[3]};
       *reinterpret_cast<f32x4*>(p.part_o + at * D + ch * 8 + 4) = f32x4{o[4], o[5], o[6], o[7]};
@@ -731,11 +811,8 @@ __device__ __forceinline__ void kv_narrow_body(const KvArgs& p) {
     }
     int64_t o_at, lse_at;
     if (!out_row(p, s, s.row0 + row, written, o_at, lse_at)) continue;
-    const float inv = inverse_sum(l_run);
-    u32x4 w;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = E::pack(o[2 * e] * inv, o[2 * e + 1] * inv);
-    *reinterpret_cast<u32x4*>(p.o + o_at + ch * 8) = w;
+    if (add) add_infinite<E>(p, s.b, s.head, (s.row0 + row) % p.n_q, ch, o);
+    *reinterpret_cast<u32x4*>(p.o + o_at + ch * 8) = pack8<E>(o, inverse_sum(l_run));
     if (p.lse != nullptr && ch == 0) p.lse[lse_at] = lse_of(m, l_run);
   }
 }
@@ -751,19 +828,27 @@ __device__ __forceinline__ void kv_join_body(const KvArgs& p) {
   Share s;
   s.b = static_cast<int>(bh / p.kv_heads);
   s.head = static_cast<int>(bh - static_cast<int64_t>(s.b) * p.kv_heads);
-  if (bh >= static_cast<int64_t>(p.units / p.splits)) return;
+  if (s.b >= p.batch) return;
   int64_t o_at, lse_at;
-  if (!out_row(p, s, static_cast<int>(row_all - bh * p.rows), written_of(p, s.b), o_at, lse_at)) return;
-  const float* ml = p.part_ml + row_all * p.splits * 2;
+  const int row = static_cast<int>(row_all - bh * p.rows);
+  if (!out_row(p, s, row, written_of(p, s.b), o_at, lse_at)) return;
+  const int n = p.splits, first = s.b * n;
+  const int64_t at = (static_cast<int64_t>(first) * p.kv_heads + s.head) * p.rows + row;
+  const int64_t step = static_cast<int64_t>(p.kv_heads) * p.rows;
   float m = -INFINITY;
-  for (int k = 0; k < p.splits; ++k) m = fmaxf(m, ml[2 * k]);
+  int add = 0;
+  for (int k = 0; k < n; ++k) {
+    m = fmaxf(m, p.part_ml[(at + k * step) * 2]);
+    if (p.k_draft) add |= p.infinite[(first + k) * p.kv_heads + s.head];
+  }
   float l_run = 0.f, o[8] = {};
-  for (int k = 0; k < p.splits; ++k) {
-    const float l = ml[2 * k + 1];
+  for (int k = 0; k < n; ++k) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (at + k * step) * 2);
+    const float l = ml.y;
     if (l == 0.f) continue;  // no keys: its part is not written
-    const float f = ml[2 * k] == m ? 1.0f : __builtin_amdgcn_exp2f(ml[2 * k] - m);
+    const float f = ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m);
     l_run += f * l;
-    const float* part = p.part_o + (row_all * p.splits + k) * D + ch * 8;
+    const float* part = p.part_o + (at + k * step) * D + ch * 8;
     const f32x4 lo = *reinterpret_cast<const f32x4*>(part), hi = *reinterpret_cast<const f32x4*>(part + 4);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -771,11 +856,8 @@ __device__ __forceinline__ void kv_join_body(const KvArgs& p) {
       o[4 + e] = fmaf(f, hi[e], o[4 + e]);
     }
   }
-  const float inv = inverse_sum(l_run);
-  u32x4 w;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = E::pack(o[2 * e] * inv, o[2 * e + 1] * inv);
-  *reinterpret_cast<u32x4*>(p.o + o_at + ch * 8) = w;
+  if (add) add_infinite<E>(p, s.b, s.head, row % p.n_q, ch, o);
+  *reinterpret_cast<u32x4*>(p.o + o_at + ch * 8) = pack8<E>(o, inverse_sum(l_run));
   if (p.lse != nullptr && ch == 0) p.lse[lse_at] = lse_of(m, l_run);
 }
 

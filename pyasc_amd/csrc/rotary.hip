@@ -12,13 +12,15 @@
 // position and frequency in fp64 (a far position keeps its fraction of a turn), and every head
 // reads them.  A row (one head of one token) belongs to kLanes neighbouring lanes of a wave; a lane
 // holds both values of kV pairs, so the turn needs no exchange and the norm one butterfly.
+#include <type_traits>
+
 #include "common.h"
 #include "numeric.h"
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxTokens = 4;     // of a workgroup
+constexpr int kMaxTokens = 8;     // of a workgroup at a time
 constexpr int kMaxHeadDim = 512;  // kSlots lanes' slots and the LDS tables cover it
 constexpr int kMaxParts = 1024;   // workgroups of a gradient launch: partial sums of its weights
 
@@ -62,8 +64,11 @@ struct alignas(sizeof(T) * V) Vec {
 };
 
 template <typename T, int V>
-__device__ __forceinline__ void load(const T* p, float (&x)[V]) {
-  const Vec<T, V> w = *reinterpret_cast<const Vec<T, V>*>(p);
+__device__ __forceinline__ Vec<T, V> load(const T* p) {
+  return *reinterpret_cast<const Vec<T, V>*>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void widen(const Vec<T, V>& w, float (&x)[V]) {
 #pragma unroll
   for (int i = 0; i < V; ++i) x[i] = widen<T>(w.v[i]);
 }
@@ -75,9 +80,14 @@ __device__ __forceinline__ void store(T* p, const float (&x)[V]) {
   *reinterpret_cast<Vec<T, V>*>(p) = w;
 }
 
-// Sum over the `lanes` (a power of two) neighbouring lanes of a row.
+// Sum over the `lanes` (a power of two) neighbouring lanes of a row, by wave_sum's steps.
 __device__ __forceinline__ float row_sum(float v, int lanes) {
-  for (int d = 1; d < lanes; d <<= 1) v += __shfl_xor(v, d, 64);
+  if (lanes > 1) v += asc::dpp_mov<asc::kDppQuadXor1>(v);
+  if (lanes > 2) v += asc::dpp_mov<asc::kDppQuadXor2>(v);
+  if (lanes > 4) v += asc::dpp_mov<asc::kDppRowHalfMirror>(v);
+  if (lanes > 8) v += asc::dpp_mov<asc::kDppRowMirror>(v);
+  if (lanes > 16) v += asc::lane_xor16(v);
+  if (lanes > 32) v += asc::lane_xor32(v);
   return v;
 }
 
@@ -108,7 +118,7 @@ template <int V>
 constexpr int slots_per_lane() { return V >= 4 ? 1 : (V == 2 ? 2 : 4); }
 
 template <typename T, int V, bool kInterleaved, Mode kMode>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs p) {
+__global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
   constexpr int kSlots = slots_per_lane<V>();
   __shared__ float2 table[kMaxTokens * kMaxHeadDim / 2];
   __shared__ float sums[kMode == kNormGrad ? 2 * kMaxHeadDim : 1];
@@ -131,19 +141,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs p) {
     c0[i] = kInterleaved || !turned[i] ? slot * 2 * V : slot * V;
     c1[i] = kInterleaved || !turned[i] ? c0[i] + V : c0[i] + p.pairs;
   }
-  float w[2][kSlots][2][V], dw[2][kSlots][2][V];
-  if (kMode != kTurn) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < kSlots; ++i)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          w[t][i][0][e] = live[i] && p.weight[t] ? p.weight[t][c0[i] + e] : 0.f;
-          w[t][i][1][e] = live[i] && p.weight[t] ? p.weight[t][c1[i] + e] : 0.f;
-          dw[t][i][0][e] = dw[t][i][1][e] = 0.f;
-        }
-  }
+  float dw[2][kSlots][2][V] = {};
 
   for (uint32_t unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
     const uint32_t tile = unit / p.chunks;
@@ -162,124 +160,165 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs p) {
     __syncthreads();
     const int h0 = chunk * p.chunk_heads;
     const int n_heads = p.heads - h0 < p.chunk_heads ? p.heads - h0 : p.chunk_heads;
-    // rows: tokens fastest, so that neighbours lie together in both orders of heads and tokens
-    for (int r = row0; r < n_heads * p.tokens; r += rows_per_pass) {
-      const int t = r & (p.tokens - 1);  // a power of two
-      if (t >= tokens) continue;         // all lanes of the row
-      const int head = h0 + r / p.tokens;
-      const int kv = head >= p.q_heads;
-      const int64_t h = kv ? head - p.q_heads : head;
-      const int64_t s = s0 + t;
-      const auto at_row = [&](const Rows& m) {
-        return static_cast<const T*>(m.p) + b * m.batch + h * m.head + s * m.seq;
+    // Rows: tokens fastest, so that neighbours lie together in both orders of heads and tokens.  The
+    // next row is asked for before this one is worked on.
+    // Queries and keys one after the other, so that a row's weights and sums are fixed registers.
+    struct Row {
+      bool live;
+      int t;
+      T* out;
+      Vec<T, V> a0[kSlots], a1[kSlots], g0[kSlots], g1[kSlots];
+    };
+    const auto heads_of = [&](auto which) {
+      constexpr int kKind = decltype(which)::value;  // 0: queries, 1: keys
+      const int first = kKind == 0 ? h0 : (h0 > p.q_heads ? h0 : p.q_heads) - p.q_heads;
+      const int last = kKind == 0 ? (h0 + n_heads < p.q_heads ? h0 + n_heads : p.q_heads) : h0 + n_heads - p.q_heads;
+      const int count = (last - first) * p.tokens;  // may be negative
+      float w[kSlots][2][V];
+      if (kMode != kTurn && count > 0) {
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i)
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            w[i][0][e] = live[i] ? p.weight[kKind][c0[i] + e] : 0.f;
+            w[i][1][e] = live[i] ? p.weight[kKind][c1[i] + e] : 0.f;
+          }
+      }
+      const auto fetch = [&](int r, Row& m) {
+        m.t = r & (p.tokens - 1);  // a power of two
+        m.live = r < count && m.t < tokens;
+        if (!m.live) return;
+        const int64_t h = first + r / p.tokens;
+        const int64_t s = s0 + m.t;
+        const auto at_row = [&](const Rows& rows) {
+          return static_cast<const T*>(rows.p) + b * rows.batch + h * rows.head + s * rows.seq;
+        };
+        const T* x = at_row(p.x[kKind]);
+        m.out = const_cast<T*>(at_row(p.out[kKind]));
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+          if (!live[i]) continue;
+          m.a0[i] = load<T, V>(x + c0[i]);
+          m.a1[i] = load<T, V>(x + c1[i]);
+        }
+        if (kMode == kNormGrad) {
+          const T* dy = at_row(p.dy[kKind]);
+#pragma unroll
+          for (int i = 0; i < kSlots; ++i) {
+            if (!live[i]) continue;
+            m.g0[i] = load<T, V>(dy + c0[i]);
+            m.g1[i] = load<T, V>(dy + c1[i]);
+          }
+        }
       };
-      const T* x = at_row(kv ? p.x[1] : p.x[0]);
-      T* out = const_cast<T*>(at_row(kv ? p.out[1] : p.out[0]));
-      float a0[kSlots][V], a1[kSlots][V], g0[kSlots][V], g1[kSlots][V];
-#pragma unroll
-      for (int i = 0; i < kSlots; ++i) {
-        if (!live[i]) continue;
-        load<T, V>(x + c0[i], a0[i]);
-        load<T, V>(x + c1[i], a1[i]);
-      }
-      if (kMode == kNormGrad) {
-        const T* dy = at_row(kv ? p.dy[1] : p.dy[0]);
+      const auto work = [&](Row& m) {
+        if (!m.live) return;  // all lanes of the row
+        float a0[kSlots][V], a1[kSlots][V], g0[kSlots][V], g1[kSlots][V];
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) {
           if (!live[i]) continue;
-          load<T, V>(dy + c0[i], g0[i]);
-          load<T, V>(dy + c1[i], g1[i]);
+          widen<T, V>(m.a0[i], a0[i]);
+          widen<T, V>(m.a1[i], a1[i]);
+          if (kMode != kNormGrad) continue;
+          widen<T, V>(m.g0[i], g0[i]);
+          widen<T, V>(m.g1[i], g1[i]);
         }
-      }
-      float rms = 1.f;
-      if (kMode != kTurn) {
-        float ss = 0.f;
+        float rms = 1.f;
+        if (kMode != kTurn) {
+          float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < kSlots; ++i) {
-          if (!live[i]) continue;
+          for (int i = 0; i < kSlots; ++i) {
+            if (!live[i]) continue;
 #pragma unroll
-          for (int e = 0; e < V; ++e) ss += a0[i][e] * a0[i][e] + a1[i][e] * a1[i][e];
+            for (int e = 0; e < V; ++e) ss += a0[i][e] * a0[i][e] + a1[i][e] * a1[i][e];
+          }
+          rms = 1.0f / sqrtf(row_sum(ss, p.lanes) * p.inv_dim + p.epsilon);
         }
-        rms = 1.0f / sqrtf(row_sum(ss, p.lanes) * p.inv_dim + p.epsilon);
-      }
-      // turn of one slot's vectors in place; the pairs' values lie in y0, y1, or alternate
-      const auto turn = [&](int i, float (&y0)[V], float (&y1)[V]) {
-        if (!turned[i]) return;
-        const float2* cs = table + t * p.pairs + at[i];
-        if (kInterleaved && V > 1) {
+        // turn of one slot's vectors in place; the pairs' values lie in y0, y1, or alternate
+        const auto turn = [&](int i, float (&y0)[V], float (&y1)[V]) {
+          if (!turned[i]) return;
+          const float2* cs = table + m.t * p.pairs + at[i];
+          if (kInterleaved && V > 1) {
 #pragma unroll
-          for (int e = 0; e < V; e += 2) {
-            const float2 u = cs[e / 2], v = cs[V / 2 + e / 2];
-            const float u0 = y0[e], u1 = y0[e + 1], v0 = y1[e], v1 = y1[e + 1];
-            y0[e] = u0 * u.x - u1 * u.y;
-            y0[e + 1] = u1 * u.x + u0 * u.y;
-            y1[e] = v0 * v.x - v1 * v.y;
-            y1[e + 1] = v1 * v.x + v0 * v.y;
+            for (int e = 0; e < V; e += 2) {
+              const float2 u = cs[e / 2], v = cs[V / 2 + e / 2];
+              const float u0 = y0[e], u1 = y0[e + 1], v0 = y1[e], v1 = y1[e + 1];
+              y0[e] = u0 * u.x - u1 * u.y;
+              y0[e + 1] = u1 * u.x + u0 * u.y;
+              y1[e] = v0 * v.x - v1 * v.y;
+              y1[e + 1] = v1 * v.x + v0 * v.y;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              const float2 c = cs[e];
+              const float u = y0[e], v = y1[e];
+              y0[e] = u * c.x - v * c.y;
+              y1[e] = v * c.x + u * c.y;
+            }
+          }
+        };
+        if (kMode == kNormGrad) {
+          float along = 0.f;  // sum of g w x r
+#pragma unroll
+          for (int i = 0; i < kSlots; ++i) {
+            if (!live[i]) continue;
+            turn(i, g0[i], g1[i]);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              a0[i][e] *= rms;
+              a1[i][e] *= rms;
+              const float d0 = g0[i][e] * a0[i][e], d1 = g1[i][e] * a1[i][e];
+              dw[kKind][i][0][e] += d0;
+              dw[kKind][i][1][e] += d1;
+              g0[i][e] *= w[i][0][e];
+              g1[i][e] *= w[i][1][e];
+              along += g0[i][e] * a0[i][e] + g1[i][e] * a1[i][e];
+            }
+          }
+          along = row_sum(along, p.lanes) * p.inv_dim;
+#pragma unroll
+          for (int i = 0; i < kSlots; ++i) {
+            if (!live[i]) continue;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              a0[i][e] = rms * (g0[i][e] - a0[i][e] * along);
+              a1[i][e] = rms * (g1[i][e] - a1[i][e] * along);
+            }
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float2 c = cs[e];
-            const float u = y0[e], v = y1[e];
-            y0[e] = u * c.x - v * c.y;
-            y1[e] = v * c.x + u * c.y;
+          for (int i = 0; i < kSlots; ++i) {
+            if (!live[i]) continue;
+            if (kMode == kNorm) {
+#pragma unroll
+              for (int e = 0; e < V; ++e) {
+                a0[i][e] = a0[i][e] * rms * w[i][0][e];
+                a1[i][e] = a1[i][e] * rms * w[i][1][e];
+              }
+            }
+            turn(i, a0[i], a1[i]);
           }
+        }
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+          if (!live[i]) continue;
+          store<T, V>(m.out + c0[i], a0[i]);
+          store<T, V>(m.out + c1[i], a1[i]);
         }
       };
-      if (kMode == kNormGrad) {
-        float along = 0.f;  // sum of g w x r
-#pragma unroll
-        for (int i = 0; i < kSlots; ++i) {
-          if (!live[i]) continue;
-          turn(i, g0[i], g1[i]);
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            a0[i][e] *= rms;
-            a1[i][e] *= rms;
-            const float d0 = g0[i][e] * a0[i][e], d1 = g1[i][e] * a1[i][e];
-            if (kv) {
-              dw[1][i][0][e] += d0;
-              dw[1][i][1][e] += d1;
-            } else {
-              dw[0][i][0][e] += d0;
-              dw[0][i][1][e] += d1;
-            }
-            g0[i][e] *= kv ? w[1][i][0][e] : w[0][i][0][e];
-            g1[i][e] *= kv ? w[1][i][1][e] : w[0][i][1][e];
-            along += g0[i][e] * a0[i][e] + g1[i][e] * a1[i][e];
-          }
-        }
-        along = row_sum(along, p.lanes) * p.inv_dim;
-#pragma unroll
-        for (int i = 0; i < kSlots; ++i) {
-          if (!live[i]) continue;
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            a0[i][e] = rms * (g0[i][e] - a0[i][e] * along);
-            a1[i][e] = rms * (g1[i][e] - a1[i][e] * along);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kSlots; ++i) {
-          if (!live[i]) continue;
-          if (kMode == kNorm) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              a0[i][e] = a0[i][e] * rms * (kv ? w[1][i][0][e] : w[0][i][0][e]);
-              a1[i][e] = a1[i][e] * rms * (kv ? w[1][i][1][e] : w[0][i][1][e]);
-            }
-          }
-          turn(i, a0[i], a1[i]);
-        }
+      Row rows[2];
+      int r = row0;
+      fetch(r, rows[0]);
+      for (; r < count; r += 2 * rows_per_pass) {
+        fetch(r + rows_per_pass, rows[1]);
+        work(rows[0]);
+        fetch(r + 2 * rows_per_pass, rows[0]);
+        work(rows[1]);
       }
-#pragma unroll
-      for (int i = 0; i < kSlots; ++i) {
-        if (!live[i]) continue;
-        store<T, V>(out + c0[i], a0[i]);
-        store<T, V>(out + c1[i], a1[i]);
-      }
-    }
+    };
+    heads_of(std::integral_constant<int, 0>{});
+    heads_of(std::integral_constant<int, 1>{});
   }
 
   if (kMode == kNormGrad) {
@@ -320,22 +359,36 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs p) {
 }
 
 // dw[t][c] = sum over workgroups of parts[.][t][c], in fp64 (the sum itself is short).  One
-// workgroup per 16 columns: 16 rows of threads take every 16th part.
-__global__ void __launch_bounds__(256) weight_sums_kernel(const float* parts, int n_parts, int head_dim, float* dq,
-                                                          float* dk) {
-  __shared__ double acc[16][17];
+// workgroup per 16 columns; 64 rows of threads take every 64th part, four loads in flight each, and
+// are added up in pairs.
+constexpr int kSumRows = 64;
+__global__ void __launch_bounds__(1024) weight_sums_kernel(const float* parts, int n_parts, int head_dim, float* dq,
+                                                           float* dk) {
+  __shared__ double acc[kSumRows][17];
   const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
   const int col = blockIdx.x * 16 + c;
+  const int64_t step = 2 * head_dim;
   double s = 0.0;
   if (col < 2 * head_dim) {
-    for (int i = r; i < n_parts; i += 16) s += parts[static_cast<int64_t>(i) * 2 * head_dim + col];
+    int i = r;
+    for (; i + 3 * kSumRows < n_parts; i += 4 * kSumRows) {
+      float x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = parts[(i + k * kSumRows) * step + col];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s += x[k];
+    }
+    for (; i < n_parts; i += kSumRows) s += parts[i * step + col];
   }
   acc[r][c] = s;
   __syncthreads();
+  for (int half = kSumRows / 2; half > 0; half /= 2) {
+    if (r < half) acc[r][c] += acc[r + half][c];
+    __syncthreads();
+  }
   if (r != 0 || col >= 2 * head_dim) return;
-  for (int i = 1; i < 16; ++i) s += acc[i][c];
   float* out = col < head_dim ? dq : dk;
-  if (out != nullptr) out[col < head_dim ? col : col - head_dim] = static_cast<float>(s);
+  if (out != nullptr) out[col < head_dim ? col : col - head_dim] = static_cast<float>(acc[0][c]);
 }
 
 template <typename T, int V, Mode kMode>
@@ -349,7 +402,7 @@ void launch(bool interleaved, dim3 grid, hipStream_t stream, const RotaryArgs& p
 
 template <typename T, Mode kMode>
 void launch_vec(int vec, bool interleaved, dim3 grid, hipStream_t stream, const RotaryArgs& p) {
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (sizeof(T) == 2 && kMode != kNormGrad) {
     if (vec == 8) return launch<T, 8, kMode>(interleaved, grid, stream, p);
   }
   if (vec == 4) return launch<T, 4, kMode>(interleaved, grid, stream, p);
@@ -357,7 +410,13 @@ void launch_vec(int vec, bool interleaved, dim3 grid, hipStream_t stream, const 
   return launch<T, 1, kMode>(interleaved, grid, stream, p);
 }
 
-int64_t token_tiles(const asc_rotary_t& a) { return asc::ceil_div(a.seq, kMaxTokens); }
+// Tokens of a workgroup at a time, a power of two: as many as leave the chip four workgroups per CU.
+int tokens_of(const asc_rotary_t& a) {
+  int n = kMaxTokens;
+  while (n > 1 && (a.seq <= n / 2 || a.batch * asc::ceil_div(a.seq, n) < 1024)) n /= 2;
+  return n;
+}
+int64_t token_tiles(const asc_rotary_t& a) { return asc::ceil_div(a.seq, tokens_of(a)); }
 
 // Workgroups of a gradient launch, as its workspace counts them: at most kMaxParts, each with a
 // share of the token tiles.
@@ -397,12 +456,13 @@ int32_t check(const asc_rotary_t* a, const char* what, Mode mode) {
   return ASC_OK;
 }
 
-// The widest vector (16 bytes at most) that every row's slots allow: both halves of a pair slot
-// and every stride and address are multiples of it.
+// The widest vector (16 bytes at most; four values in a gradient launch, whose two rows in flight and
+// sums would not fit the registers of four waves per SIMD otherwise: 98 us against 46) that
+// every row's slots allow: both halves of a pair slot and every stride and address are multiples of it.
 int vector_width(const asc_rotary_t& a, Mode mode) {
   const int64_t size = a.dtype == ASC_DT_FLOAT32 ? 4 : 2;
   const asc_rows_t* rows[] = {&a.q, &a.q_out, &a.dq_out, &a.k, &a.k_out, &a.dk_out};
-  for (int v = static_cast<int>(16 / size); v > 1; v /= 2) {
+  for (int v = mode == kNormGrad ? 4 : static_cast<int>(16 / size); v > 1; v /= 2) {
     bool ok = a.rotary_dim % (2 * v) == 0 && a.head_dim % (2 * v) == 0;
     for (int i = 0; i < 6; ++i) {
       if ((i < 3 ? a.q_heads : a.k_heads) == 0 || (i % 3 == 2 && mode != kNormGrad)) continue;
@@ -415,7 +475,8 @@ int vector_width(const asc_rotary_t& a, Mode mode) {
 }
 
 void sum_weights(const asc_rotary_t& a, const float* parts, int n_parts, hipStream_t stream) {
-  hipLaunchKernelGGL(weight_sums_kernel, dim3(static_cast<uint32_t>(asc::ceil_div(2 * a.head_dim, 16))), dim3(256), 0,
+  const dim3 grid(static_cast<uint32_t>(asc::ceil_div(2 * a.head_dim, 16)));
+hipLaunchKernelGGL(weight_sums_kernel, grid, dim3(1024), 0,
                      stream, parts, n_parts, a.head_dim, a.dq_weight, a.dk_weight);
 }
 
@@ -450,8 +511,7 @@ int32_t run(const asc_rotary_t* a, const char* what, Mode mode, float* parts, as
   const int slots = static_cast<int>(asc::ceil_div(a->head_dim / (2 * vec), per_lane));
   p.lanes = 1;
   while (p.lanes < slots) p.lanes *= 2;  // at most 64: head_dim <= 512
-  p.tokens = 1;
-  while (p.tokens < kMaxTokens && p.tokens < a->seq) p.tokens *= 2;
+  p.tokens = tokens_of(*a);
   p.tiles = static_cast<uint32_t>(asc::ceil_div(a->seq, p.tokens));
   const int64_t n_tiles = a->batch * p.tiles;
   // Few tokens: their heads spread over workgroups of one pass each; else one workgroup for all.

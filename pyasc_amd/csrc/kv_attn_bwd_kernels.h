@@ -88,25 +88,20 @@ struct Tiles {
   static constexpr int kRowsPerLoad = 1024 / (D * 2), kLanesPerRow = 64 / kRowsPerLoad;
 
   int lane, wave, col, h;
-  uint32_t raddr[kKSteps];      // row operand: row col, chunk 2 * k-step + h
-  uint32_t taddr[kDBlocks][2];  // transposed operand: rows 8 w + 4 h + 0..3 of d block db
+  // One address per kind of operand; other chunks and rows are some of its bits flipped, as the
+  // places only flip bits and a block of 32 rows starts at a multiple of its size.
+  uint32_t raddr;  // row operand: row col, chunk h (k-step kk: 2 kk chunks away)
+  uint32_t taddr;  // transposed operand: rows 4 h + 0..3 (w: 8 rows, db: 4 chunks away)
 
   __device__ __forceinline__ void init(int tid) {
     lane = tid & 63;
     wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     col = lane & 31;
     h = lane >> 5;
-#pragma unroll
-    for (int kk = 0; kk < kKSteps; ++kk) raddr[kk] = tile_off<D>(col, kk * 2 + h);
+    raddr = tile_off<D>(col, h);
     const int g_lane = lane & 15;
     const int tr_col = ((lane >> 4) & 1) * 16 + (g_lane & 3) * 4;
-#pragma unroll
-    for (int db = 0; db < kDBlocks; ++db)
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const int c = db * 32 + tr_col;
-        taddr[db][w] = tile_off<D>(8 * w + 4 * h + (g_lane >> 2), c >> 3) + (c & 7) * 2;
-      }
+    taddr = tile_off<D>(4 * h + (g_lane >> 2), tr_col >> 3) + (tr_col & 7) * 2;
   }
 
   // Rows row0 .. row0 + kRows - 1 of `base` (`stride` 16-byte units apart) into an LDS tile; rows
@@ -132,10 +127,10 @@ struct Tiles {
   // x += A bx and y += B by for 32 rows of two tiles (A, B: row operands).
   __device__ __forceinline__ void products(uint32_t a_base, uint32_t b_base, const u32x4 (&bx)[kKSteps],
                                            const u32x4 (&by)[kKSteps], f32x16& x, f32x16& y) const {
-    constexpr int kWin = 4, kReads = 2 * kKSteps;
+    constexpr int kWin = 3, kReads = 2 * kKSteps;  // 4: 1% slower, for the registers
     u32x4 a[kReads];
     const auto read = [&](int r) {
-      return fa::lds_read_b128((r < kKSteps ? a_base : b_base) + raddr[r % kKSteps], 0);
+      return fa::lds_read_b128(((r < kKSteps ? a_base : b_base) + raddr) ^ (r % kKSteps << 5), 0);
     };
 #pragma unroll
     for (int r = 0; r < kWin; ++r) a[r] = read(r);
@@ -153,8 +148,9 @@ struct Tiles {
 
   // Operand (db, u) of a transposed tile: rows 16 u + 4 h + 0..3 and 16 u + 8 + 4 h + 0..3.
   __device__ __forceinline__ u32x4 transposed(uint32_t base, int db, int u) const {
-    const u32x2 lo = fa::lds_read_tr16_b64(base + taddr[db][0], u * 16 * (D * 2));
-    const u32x2 hi = fa::lds_read_tr16_b64(base + taddr[db][1], u * 16 * (D * 2));
+    const uint32_t at = (base + taddr) ^ (db << 6);
+    const u32x2 lo = fa::lds_read_tr16_b64(at, u * 16 * (D * 2));
+    const u32x2 hi = fa::lds_read_tr16_b64(at ^ (8 * D * 2 + 32), u * 16 * (D * 2));
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   }
   // acc += A^T b for 32 rows of the tile at base, b[u] holding rows 16 u ..
@@ -224,6 +220,7 @@ struct GradQ {
   static constexpr int kRows = 32 * kWaves;
   static constexpr int kKeys = 64;  // of a tile
 };
+constexpr int kExactTiles = 4;  // see grad_q_body; as many are never split
 
 template <int D, class E>
 __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
@@ -231,7 +228,7 @@ __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
   using T = Tiles<D, kWaves, E>;
   constexpr int kTile = kKeys * D * 2;
   constexpr int kLoads = 2 * (kKeys / T::kRowsPerLoad / kWaves);  // of K and V, per wave and tile
-  __shared__ __attribute__((aligned(16))) uint8_t ring[6 * kTile];  // K stages 0-2, V stages 3-5
+  __shared__ __attribute__((aligned(8192))) uint8_t ring[6 * kTile];  // K stages 0-2, V stages 3-5
 
   const GradShare s = grad_share(p.q_blocks, p.q_splits, p.q_units, p.kv_heads);
   if (!s.live) return;
@@ -257,8 +254,11 @@ __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
     t.template load<kKeys>(ring + stage * kTile, kbase, p.ks.seq, j * kKeys, len);
     t.template load<kKeys>(ring + (3 + stage) * kTile, vbase, p.vs.seq, j * kKeys, len);
   };
-  if (begin < end) load(begin, 0);
-  if (begin + 1 < end) load(begin + 1, 1);
+  const auto start = [&] {
+    if (begin < end) load(begin, 0);
+    if (begin + 1 < end) load(begin + 1, 1);
+  };
+  start();
 
   u32x4 q[T::kKSteps], d_o[T::kKSteps];
   t.own_row(at(p.q, p.qs), live, q);
@@ -285,47 +285,69 @@ __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
   // a row without keys: its probabilities are 0
   const float lse = live ? p.lse[row_at] : -INFINITY;
   const float a = lse == -INFINITY ? INFINITY : lse * p.inv_scale;
-  if (live && t.h == 0 && s.split == 0) {
-    p.neg_a[row_at] = -a;
-    p.neg_d[row_at] = -delta;
-  }
   const float neg_l2 = lse == -INFINITY ? -INFINITY : -lse * 1.4426950408889634f;
+
+  // body(tile, block, x, y) for every 32 keys: x the probabilities, y = dP
+  const auto stream = [&](auto body) {
+    int c = 0;
+    for (int j = begin; j < end; ++j) {
+      // every wave has read the stage that the tile after the next goes to: it was tile j-1's
+      if (j + 1 < end) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLoads) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      }
+      asm volatile("s_barrier" ::: "memory");
+      if (j + 2 < end) load(j + 2, c == 0 ? 2 : c - 1);
+      const uint32_t kt = fa::lds_addr(ring + c * kTile), vt = fa::lds_addr(ring + (3 + c) * kTile);
+#pragma unroll
+      for (int kb = 0; kb < kKeys / 32; ++kb) {
+        const uint32_t off = kb * 32 * D * 2;
+        f32x16 x = {}, y = {};
+        t.products(kt + off, vt + off, q, d_o, x, y);
+        if (j * kKeys + kb * 32 + 32 > len) {  // keys behind the length
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            if (j * kKeys + kb * 32 + (r >> 2) * 8 + t.h * 4 + (r & 3) >= len) x[r] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], p.scale_log2, neg_l2));
+        body(kt + off, x, y);
+      }
+      c = c == 2 ? 0 : c + 1;
+    }
+  };
+
+  // o is rounded to its type, and delta with it.  Over few keys, where o is as large as the values,
+  // that shows in the gradients (0.0026 against 0.0024 relative, bf16, 10 keys), and delta is taken
+  // as the sum of p dP in a pass of its own; over many it is left to o.
+  if (total <= kExactTiles) {
+    delta = 0.f;
+    stream([&](uint32_t, const f32x16& x, const f32x16& y) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) delta = fmaf(x[r], y[r], delta);
+    });
+    delta += other_half(delta);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    asm volatile("s_barrier" ::: "memory");  // the first tile goes where another wave may still read
+    start();
+  }
 
   f32x16 acc[T::kDBlocks];
 #pragma unroll
   for (int i = 0; i < T::kDBlocks; ++i) acc[i] = f32x16{};
-  int c = 0;
-  for (int j = begin; j < end; ++j) {
-    // every wave has read the stage that the tile after the next goes to: it was tile j-1's
-    if (j + 1 < end) {
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLoads) : "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    }
-    asm volatile("s_barrier" ::: "memory");
-    if (j + 2 < end) load(j + 2, c == 0 ? 2 : c - 1);
-    const uint32_t kt = fa::lds_addr(ring + c * kTile), vt = fa::lds_addr(ring + (3 + c) * kTile);
-#pragma unroll
-    for (int kb = 0; kb < kKeys / 32; ++kb) {
-      const uint32_t off = kb * 32 * D * 2;
-      f32x16 x = {}, y = {};
-      t.products(kt + off, vt + off, q, d_o, x, y);
-      if (j * kKeys + kb * 32 + 32 > len) {  // keys behind the length
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          if (j * kKeys + kb * 32 + (r >> 2) * 8 + t.h * 4 + (r & 3) >= len) x[r] = -INFINITY;
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], p.scale_log2, neg_l2)) * (y[r] - delta);
-      }
-      u32x4 ds[2];
-      T::pack(x, ds);
-      t.add_transposed(kt + off, ds, acc);
-    }
-    c = c == 2 ? 0 : c + 1;
+  if (live && t.h == 0 && s.split == 0) {
+    p.neg_a[row_at] = -a;
+    p.neg_d[row_at] = -delta;
   }
+  stream([&](uint32_t kt, f32x16& x, const f32x16& y) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] *= y[r] - delta;
+    u32x4 ds[2];
+    T::pack(x, ds);
+    t.add_transposed(kt, ds, acc);
+  });
   if (!live) return;
   const float scale = bad ? __builtin_nanf("") : p.scale;
   if (p.q_splits > 1) {
@@ -353,7 +375,7 @@ __device__ __forceinline__ void grad_kv_body(const GradArgs& p) {
   using T = Tiles<D, kWaves, E>;
   constexpr int kTile = kRows * D * 2;
   constexpr int kLoads = 2 * (kRows / T::kRowsPerLoad / kWaves);
-  __shared__ __attribute__((aligned(16))) uint8_t ring[6 * kTile];  // Q stages 0-2, dO stages 3-5
+  __shared__ __attribute__((aligned(8192))) uint8_t ring[6 * kTile];  // Q stages 0-2, dO stages 3-5
   __shared__ __attribute__((aligned(16))) float values[3][2 * kRows];  // -lse / scale and -delta of a tile
 
   const GradShare s = grad_share(p.kv_blocks, p.kv_splits, p.kv_units, p.kv_heads);

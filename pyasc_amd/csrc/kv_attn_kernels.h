@@ -513,7 +513,7 @@ __device__ __forceinline__ void kv_wide_body(const KvArgs& p) {
   constexpr int L = St::kLoadsPerWave;
   constexpr int kThreads = kWaves * 64;
   constexpr int kChunks = D / 8;
-  __shared__ __attribute__((aligned(16))) uint8_t ring[6 * T];
+  __shared__ __attribute__((aligned(256))) uint8_t ring[6 * T];
   __shared__ __attribute__((aligned(16))) uint8_t ids[kTree ? kWaves * 256 : 16];
   __shared__ int infinite[kWaves];
 
@@ -677,7 +677,7 @@ __device__ __forceinline__ void kv_narrow_body(const KvArgs& p) {
   constexpr int L = St::kLoadsPerWave;
   constexpr int kRow = D * 4;
   static_assert(Narrow<D>::kRows * kRow <= 2 * T, "a wave's part reuses its tiles");
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves * 2 * T];
+  __shared__ __attribute__((aligned(256))) uint8_t lds[kWaves * 2 * T];
   __shared__ float stats[2][kWaves][Narrow<D>::kRows];
   __shared__ __attribute__((aligned(16))) uint8_t ids[kTree ? kWaves * 256 : 16];
   __shared__ int infinite[kWaves];

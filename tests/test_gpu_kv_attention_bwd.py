@@ -14,18 +14,20 @@ SMALL = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}  # half the sma
 
 
 def reference(do, q, k, v, o, lse, scale, dtype):
-    """dq, dk, dv of one query head in fp64, from the forward pass's o and lse, each with its bound
-    before it is rounded to the type."""
+    """dq, dk, dv of one query head in fp64, from the forward pass's lse, each with its bound before it
+    is rounded to the type."""
     do, q, k, v, o, lse = (t.double().contiguous() for t in (do, q, k, v, o, lse))
     kt, vt = k.T.contiguous(), v.T.contiguous()
     p = torch.exp((q @ kt) * scale - lse[:, None])
     # fp32: D products per score with the largest initial value, exp2 and its argument
     rel = (q.shape[1] + 8) * 2.0 ** -23 * (float((q.abs() @ kt.abs()).amax()) * scale + float(lse.abs().amax()) + 1)
-    delta = (do * o).sum(1, keepdim=True)
     dp = do @ vt
+    delta = (p * dp).sum(1, keepdim=True)
     ds = p * (dp - delta)
-    dp_err = (q.shape[1] + 8) * 2.0 ** -23 * (do.abs() @ vt.abs() + (do * o).abs().sum(1, keepdim=True))
+    # delta may come from o, which was rounded to the type after its probabilities were
     r, small = ROUND[dtype], SMALL[dtype]
+    dp_err = (q.shape[1] + 8) * 2.0 ** -23 * (do.abs() @ vt.abs() + (do * o).abs().sum(1, keepdim=True))
+    dp_err = dp_err + (r * (do * o).abs() + (r + rel) * (do.abs() * (p @ v.abs()))).sum(1, keepdim=True)
     p_err = p * (rel + r * (1 + rel)) + small
     ds_err = (ds.abs() * rel + p * (1 + rel) * dp_err) * (1 + r) + ds.abs() * r + small
     n, m = k.shape[0], q.shape[0]

@@ -35,23 +35,51 @@ struct Launch {
 constexpr int kMaxSplits = 64;
 constexpr int64_t kCus = 256;
 
-// How the rows of one key / value head are taken: up to 32 of them by kv_narrow, more by kv_wide.
-// Where they are too few workgroups to fill the chip twice, the keys are split too.
+// One way to launch.
+struct Way {
+  int64_t row_blocks, splits;
+  double us;
+};
+
+// A way's split of the keys, where its workgroups are too few to fill the chip, and its time: rounds
+// of workgroups, each with its start and end and its longest chain of tiles, and the join.
+Way way_of(int64_t heads, int64_t row_blocks, int64_t tiles, int64_t slots, int fill, int64_t least, int waves,
+           double start, double tile) {
+  Way w{row_blocks, 1, 0.0};
+  const int64_t shares = heads * row_blocks;
+  if (shares < slots) w.splits = fill * slots / shares;
+  if (w.splits > tiles / least) w.splits = tiles / least;
+  if (w.splits > kMaxSplits) w.splits = kMaxSplits;
+  if (w.splits < 1) w.splits = 1;
+  const int64_t chain = asc::ceil_div(asc::ceil_div(tiles, w.splits), waves);
+  w.us = static_cast<double>(asc::ceil_div(shares * w.splits, slots)) * (start + tile * static_cast<double>(chain)) +
+         (w.splits > 1 ? 3.5 : 0.0);
+  return w;
+}
+
+// kv_narrow for up to 32 rows; above that, kv_narrow (whose four waves share a tile's time, but
+// which reads the keys once per 32 rows) or kv_wide, whichever the times above say is clearly shorter.
+// They were taken from kernels of 1 to 4 rounds.  kv_wide, kv_narrow (us): 128 heads, 64 rows, 500
+// keys, head_dim 64: 13.7, 7.0; 64 heads, 333 rows, 777 keys, head_dim 64: 24.0, 18.1; 8 heads, 333
+// rows, 777 keys, head_dim 128: 22.4, 13.0; 128 heads, 128 rows, 500 keys: 22.3, 19.9; 32 heads, 200
+// rows, 2000 keys: 31.8, 32.0; 64 heads, 48 rows, 4000 keys: 32.7, 36.2.
+// kv_wide's keys are split to fill the chip once (twice: 70 against 60 us for 8 sequences of 4096
+// down to 1024 keys, 64 drafted tokens, 32 / 8 heads), kv_narrow's, which HBM bounds, twice.
 void plan(Launch& L, const asc_attention_t& a) {
   KvArgs& p = L.p;
-  L.wide = p.rows > Narrow<64>::kRows;
-  const int rows = L.wide ? (a.head_dim == 64 ? Wide<64>::kRows : Wide<128>::kRows) : Narrow<64>::kRows;
-  p.row_blocks = static_cast<int>(asc::ceil_div(p.rows, rows));
+  const bool small = a.head_dim == 64;
+  const int64_t heads = a.batch * a.kv_heads, slots = small ? 2 * kCus : kCus;
   const int64_t tiles = asc::ceil_div(p.capacity, asc::fa::BKV) + (p.k_draft ? asc::ceil_div(p.n_q, asc::fa::BKV) : 0);
-  const int64_t shares = a.batch * a.kv_heads * p.row_blocks;
-  const int64_t slots = kCus * (a.head_dim == 64 ? 2 : 1);
-  const int64_t least = L.wide ? 4 : 8;  // tiles of a split
-  int64_t splits = shares >= slots ? 1 : (L.wide ? 1 : 2) * slots / shares;
-  if (splits > tiles / least) splits = tiles / least;
-  if (splits > kMaxSplits) splits = kMaxSplits;
-  p.splits = splits < 1 ? 1 : static_cast<int>(splits);
-  p.units = static_cast<uint32_t>(a.batch * a.kv_heads * p.splits);
-  L.rows_all = a.batch * a.kv_heads * p.rows;
+  const Way narrow = way_of(heads, asc::ceil_div(p.rows, Narrow<64>::kRows), tiles, slots, 2, 8, Narrow<64>::kWaves,
+                            small ? 4.5 : 5.5, small ? 1.2 : 2.0);
+  const Way wide = way_of(heads, asc::ceil_div(p.rows, small ? Wide<64>::kRows : Wide<128>::kRows), tiles, slots, 1, 4,
+                          1, small ? 8.0 : 9.0, small ? 1.6 : 2.2);
+  L.wide = p.rows > Narrow<64>::kRows && narrow.us > 0.9 * wide.us;
+  const Way& w = L.wide ? wide : narrow;
+  p.row_blocks = static_cast<int>(w.row_blocks);
+  p.splits = static_cast<int>(w.splits);
+  p.units = static_cast<uint32_t>(heads * p.splits);
+  L.rows_all = heads * p.rows;
   L.blocks = asc::ceil_div(p.units, 8) * 8 * p.row_blocks;
 }
 

@@ -80,6 +80,8 @@ void plan(Launch& L, const asc_attention_t& a) {
   p.splits = static_cast<int>(w.splits);
   p.units = static_cast<uint32_t>(heads * p.splits);
   L.rows_all = heads * p.rows;
+  p.join_groups = small ? asc::kv::JoinLanes<64>::groups_of(L.rows_all, p.splits)
+                        : asc::kv::JoinLanes<128>::groups_of(L.rows_all, p.splits);
   L.blocks = asc::ceil_div(p.units, 8) * 8 * p.row_blocks;
 }
 
@@ -167,8 +169,9 @@ void launch(const Launch& L, bool tree, hipStream_t stream) {
                        stream, L.p);
   }
   if (L.p.splits == 1) return;
-  hipLaunchKernelGGL((kv_join<D, E>), dim3(static_cast<uint32_t>(asc::ceil_div(L.rows_all * (D / 8), 256))), dim3(256),
-                     0, stream, L.p);
+  const int64_t threads = L.rows_all * (D / 8) * L.p.join_groups;
+  hipLaunchKernelGGL((kv_join<D, E>), dim3(static_cast<uint32_t>(asc::ceil_div(threads, 256))), dim3(256), 0, stream,
+                     L.p);
 }
 
 int32_t run(const asc_attention_t* a, bool tree, const char* what, void* workspace, int64_t workspace_bytes,

@@ -13,13 +13,13 @@ template <int D, class E>
 __global__ void __launch_bounds__(GradQ<D>::kWaves * 64, GradQ<D>::kWgPerCu) grad_q(GradArgs p) {
   asc::kv::grad_q_body<D, E>(p);
 }
-template <int D, class E>
+template <int D, class E, bool kPacked>
 __global__ void __launch_bounds__(GradKv<D>::kWaves * 64, GradKv<D>::kWgPerCu) grad_kv(GradArgs p) {
-  asc::kv::grad_kv_body<D, E>(p);
+  asc::kv::grad_kv_body<D, E, kPacked>(p);
 }
 template <int D, class E>
-__global__ void __launch_bounds__(256) join_grad(GradArgs p, int kind) {
-  asc::kv::join_grad_body<D, E>(p, kind);
+__global__ void __launch_bounds__(256) join_grad(GradArgs p, int kind, int groups) {
+  asc::kv::join_grad_body<D, E>(p, kind, groups);
 }
 
 constexpr int kMaxSplits = 32;
@@ -49,7 +49,10 @@ void plan(Launch& L, const asc_attention_t& a) {
   p.q_blocks = static_cast<int32_t>(asc::ceil_div(p.rows, small ? GradQ<64>::kRows : GradQ<128>::kRows));
   p.kv_blocks = static_cast<int32_t>(asc::ceil_div(a.kv_len, GradKv<64>::kKeys));
   p.q_splits = splits_of(heads * p.q_blocks, small ? kSlots : kSlots / 2, asc::ceil_div(a.kv_len, GradQ<64>::kKeys), 4);
-  p.kv_splits = splits_of(heads * p.kv_blocks, kSlots, p.group * asc::ceil_div(p.n_q, GradKv<64>::kRows), 8);
+  p.kv_splits = splits_of(heads * p.kv_blocks, kSlots,
+                          p.n_q < GradKv<64>::kRows ? asc::ceil_div(p.rows, GradKv<64>::kRows)
+                                                    : p.group * asc::ceil_div(p.n_q, GradKv<64>::kRows),
+                          8);
   p.q_units = static_cast<uint32_t>(heads * p.q_splits);
   p.kv_units = static_cast<uint32_t>(heads * p.kv_splits);
   L.q_grid = asc::ceil_div(p.q_units, 8) * 8 * p.q_blocks;
@@ -133,16 +136,20 @@ int32_t launch(const Launch& L, const char* what, hipStream_t stream) {
     const int32_t rc = asc::check_launch(what);
     if (rc != ASC_OK) return rc;
     if (L.parts_q > 0) {
-      hipLaunchKernelGGL((join_grad<D, E>), grid(asc::ceil_div(L.q_rows * (D / 8), 256)), dim3(256), 0, stream, L.p, 0);
+      const int groups = asc::kv::JoinLanes<D>::groups_of(L.q_rows, L.p.q_splits);
+      hipLaunchKernelGGL((join_grad<D, E>), grid(asc::ceil_div(L.q_rows * (D / 8) * groups, 256)), dim3(256), 0, stream,
+                         L.p, 0, groups);
     }
   }
   if (L.kv_grid > 0) {
-    hipLaunchKernelGGL((grad_kv<D, E>), grid(L.kv_grid), dim3(GradKv<D>::kWaves * 64), 0, stream, L.p);
+    const auto kernel = L.p.n_q < GradKv<D>::kRows ? grad_kv<D, E, true> : grad_kv<D, E, false>;
+    hipLaunchKernelGGL(kernel, grid(L.kv_grid), dim3(GradKv<D>::kWaves * 64), 0, stream, L.p);
     const int32_t rc = asc::check_launch(what);
     if (rc != ASC_OK) return rc;
     for (int kind = 1; kind < 3 && L.parts_kv > 0; ++kind) {
-      hipLaunchKernelGGL((join_grad<D, E>), grid(asc::ceil_div(L.kv_rows * (D / 8), 256)), dim3(256), 0, stream, L.p,
-                         kind);
+      const int groups = asc::kv::JoinLanes<D>::groups_of(L.kv_rows, L.p.kv_splits);
+      hipLaunchKernelGGL((join_grad<D, E>), grid(asc::ceil_div(L.kv_rows * (D / 8) * groups, 256)), dim3(256), 0,
+                         stream, L.p, kind, groups);
     }
   }
   return asc::check_launch(what);

@@ -105,9 +105,10 @@ struct Tiles {
   }
 
   // Rows row0 .. row0 + kRows - 1 of `base` (`stride` 16-byte units apart) into an LDS tile; rows
-  // >= n are zeros.
-  template <int kRows>
-  __device__ __forceinline__ void load(uint8_t* dst, const uint8_t* base, uint32_t stride, int row0, int n) const {
+  // >= n are zeros.  kPacked: row r is row r % per_head of head r / per_head.
+  template <int kRows, bool kPacked = false>
+  __device__ __forceinline__ void load(uint8_t* dst, const uint8_t* base, uint32_t stride, int row0, int n,
+                                       int per_head = 0, uint32_t head_stride = 0) const {
     constexpr int kLoads = kRows / kRowsPerLoad / kWaves;
     static_assert(kLoads >= 1, "a load per wave");
     int wave_lds = wave * (kLoads * 1024);
@@ -117,6 +118,11 @@ struct Tiles {
     for (int i = 0; i < kLoads; ++i) {
       const int row = kRowsPerLoad * (wave * kLoads + i) + rr;
       const uint8_t* src = base + static_cast<uint64_t>(row0 + row) * (static_cast<uint64_t>(stride) * 16);
+      if constexpr (kPacked) {
+        const uint32_t g = static_cast<uint32_t>(row0 + row) / static_cast<uint32_t>(per_head);
+        const uint32_t s = static_cast<uint32_t>(row0 + row) - g * static_cast<uint32_t>(per_head);
+        src = base + (static_cast<uint64_t>(g) * head_stride + static_cast<uint64_t>(s) * stride) * 16;
+      }
       if (row0 + row >= n) src = reinterpret_cast<const uint8_t*>(kZeroRow);
       __builtin_amdgcn_global_load_lds(
           (const __attribute__((address_space(1))) void*)(src + ((pos ^ place<D>(row)) << 4)),
@@ -369,7 +375,8 @@ struct GradKv {
   static constexpr int kRows = 32;  // of a tile
 };
 
-template <int D, class E>
+// kPacked: fewer queries than a tile has rows, so those of several heads share one.
+template <int D, class E, bool kPacked>
 __device__ __forceinline__ void grad_kv_body(const GradArgs& p) {
   constexpr int kWaves = GradKv<D>::kWaves, kRows = GradKv<D>::kRows;
   using T = Tiles<D, kWaves, E>;
@@ -389,26 +396,27 @@ __device__ __forceinline__ void grad_kv_body(const GradArgs& p) {
   const bool live = key < len;
 
   // tiles of rows: every query head of the group, its queries in tiles
-  const int per_head = (p.n_q + kRows - 1) / kRows;
-  const int total = key0 < len ? per_head * p.group : 0;
+  const int per_head = ((kPacked ? p.rows : p.n_q) + kRows - 1) / kRows;
+  const int total = key0 < len ? (kPacked ? per_head : per_head * p.group) : 0;
   const int per = (total + p.kv_splits - 1) / p.kv_splits;
   const int begin = min(total, s.split * per), end = min(total, begin + per);
-  int next_head = per_head ? begin / per_head : 0, next_tile = begin - next_head * per_head;  // of the next load
+  int next_head = per_head && !kPacked ? begin / per_head : 0, next_tile = begin - next_head * per_head;  // of the next load
   float value = 0.f;  // loaded for a tile, not yet in LDS
   const auto load = [&](int stage) {
     const uint64_t head = static_cast<uint64_t>(s.head) * p.group + next_head;
     const int row0 = next_tile * kRows;
+    const int n = kPacked ? p.rows : p.n_q;
     if (t.wave == 0) {
       const int row = row0 + t.col;
       const float* from = t.h ? p.neg_d : p.neg_a;
       value = t.h ? 0.f : -INFINITY;  // behind the queries: probability 0
-      if (row < p.n_q) value = from[(static_cast<int64_t>(s.b) * p.kv_heads * p.group + head) * p.n_q + row];
+      // the heads of a group follow each other
+      if (row < n) value = from[(static_cast<int64_t>(s.b) * p.kv_heads * p.group + head) * p.n_q + row];
     }
-    t.template load<kRows>(ring + stage * kTile, p.q + (static_cast<uint64_t>(s.b) * p.qs.batch + head * p.qs.head) * 16,
-                           p.qs.seq, row0, p.n_q);
-    t.template load<kRows>(ring + (3 + stage) * kTile,
-                           p.d_o + (static_cast<uint64_t>(s.b) * p.dos.batch + head * p.dos.head) * 16, p.dos.seq,
-                           row0, p.n_q);
+    const uint8_t* q = p.q + (static_cast<uint64_t>(s.b) * p.qs.batch + head * p.qs.head) * 16;
+    const uint8_t* d_o = p.d_o + (static_cast<uint64_t>(s.b) * p.dos.batch + head * p.dos.head) * 16;
+    t.template load<kRows, kPacked>(ring + stage * kTile, q, p.qs.seq, row0, n, p.n_q, p.qs.head);
+    t.template load<kRows, kPacked>(ring + (3 + stage) * kTile, d_o, p.dos.seq, row0, n, p.n_q, p.dos.head);
     if (++next_tile == per_head) {
       next_tile = 0;
       ++next_head;
@@ -494,32 +502,30 @@ __device__ __forceinline__ void grad_kv_body(const GradArgs& p) {
   t.store(dv, p.dv + s.b * p.dv_batch + s.head * p.dv_head + key * p.dv_seq, bad ? nan : 1.0f, zero);
 }
 
-// Adds up the parts of rows, D / 8 lanes per row.  kind 0: dq, 1: dk, 2: dv.
+// Adds up the parts of rows.  kind 0: dq, 1: dk, 2: dv.
 template <int D, class E>
-__device__ __forceinline__ void join_grad_body(const GradArgs& p, int kind) {
-  constexpr int kLanes = D / 8;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t row_all = i / kLanes;
-  const int ch = static_cast<int>(i % kLanes);
+__device__ __forceinline__ void join_grad_body(const GradArgs& p, int kind, int groups) {
   const int per_head = kind == 0 ? p.rows : p.capacity, splits = kind == 0 ? p.q_splits : p.kv_splits;
-  const int64_t bh = row_all / per_head;
+  const JoinLanes<D> at(groups);
+  const int64_t bh = at.row / per_head;
   if (bh >= static_cast<int64_t>((kind == 0 ? p.q_units : p.kv_units) / splits)) return;
-  const int row = static_cast<int>(row_all - bh * per_head);
+  const int row = static_cast<int>(at.row - bh * per_head);
   const int64_t b = bh / p.kv_heads, head = bh - b * p.kv_heads;
-  const float* part = (kind == 0 ? p.part_q : kind == 1 ? p.part_k : p.part_v) + row_all * splits * D + ch * 8;
+  const float* part = (kind == 0 ? p.part_q : kind == 1 ? p.part_k : p.part_v) + at.row * splits * D + at.ch * 8;
   float o[8] = {};
-  for (int k = 0; k < splits; ++k) {
-    const f32x4 lo = *reinterpret_cast<const f32x4*>(part + k * D), hi = *reinterpret_cast<const f32x4*>(part + k * D + 4);
+#pragma unroll 4
+  for (int k = at.group; k < splits; k += at.groups) {
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(part + k * D);
+    const f32x4 hi = *reinterpret_cast<const f32x4*>(part + k * D + 4);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       o[e] += lo[e];
       o[4 + e] += hi[e];
     }
   }
-  const float scale = kind == 2 ? 1.0f : p.scale;
-  u32x4 w;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = E::pack(o[2 * e] * scale, o[2 * e + 1] * scale);
+  for (int e = 0; e < 8; ++e) o[e] = at.reduce(o[e], [](float x, float y) { return x + y; });
+  if (at.group != 0) return;
   uint16_t* out;
   if (kind == 0) {
     const int g = row / p.n_q;
@@ -529,7 +535,7 @@ __device__ __forceinline__ void join_grad_body(const GradArgs& p, int kind) {
   } else {
     out = p.dv + b * p.dv_batch + head * p.dv_head + row * p.dv_seq;
   }
-  *reinterpret_cast<u32x4*>(out + ch * 8) = w;
+  *reinterpret_cast<u32x4*>(out + at.ch * 8) = pack8<E>(o, kind == 2 ? 1.0f : p.scale);
 }
 
 }  // namespace kv

@@ -226,7 +226,7 @@ struct GradQ {
   static constexpr int kRows = 32 * kWaves;
   static constexpr int kKeys = 64;  // of a tile
 };
-constexpr int kExactTiles = 4;  // see grad_q_body; as many are never split
+constexpr int kExactTiles = 4;  // up to as many, delta is exact (see grad_q_body)
 
 template <int D, class E>
 __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
@@ -252,7 +252,8 @@ __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
   };
 
   const int total = (len + kKeys - 1) / kKeys;
-  const int per = (total + p.q_splits - 1) / p.q_splits;
+  // few keys are not split, however many there could be: the first split sees all of them
+  const int per = total <= kExactTiles ? total : (total + p.q_splits - 1) / p.q_splits;
   const int begin = min(total, s.split * per), end = min(total, begin + per);
   const uint8_t* kbase = p.k + (static_cast<uint64_t>(s.b) * p.ks.batch + static_cast<uint64_t>(s.head) * p.ks.head) * 16;
   const uint8_t* vbase = p.v + (static_cast<uint64_t>(s.b) * p.vs.batch + static_cast<uint64_t>(s.head) * p.vs.head) * 16;

@@ -661,8 +661,14 @@ def _with_workspace(entry: str, args: bytes, device: torch.device, stream: Any) 
     if nbytes == 0:
         _native.call(entry, args, 0, 0, handle)
         return
-    workspace = workspace_on(handle, nbytes, torch.uint8, device)
-    if torch.cuda.is_current_stream_capturing() and not _held_by_a_graph(workspace):
+    if handle == _native.current_stream_handle(device.index):
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        usable = not torch.cuda.is_current_stream_capturing() or _held_by_a_graph(workspace)
+    else:
+        with torch.cuda.stream(_stream_of(handle, device)):
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            usable = not torch.cuda.is_current_stream_capturing() or _held_by_a_graph(workspace)
+    if not usable:
         raise RuntimeError(f"{entry} needs a workspace: capture it with torch.cuda.graph")
     _native.call(entry, args, workspace.data_ptr(), nbytes, handle)
 
@@ -845,6 +851,8 @@ def _kv_rows(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
     if k_shape[3] != shape[3] or (k_shape[0] != shape[0] and not pages):
         raise ValueError(f"'{names[0]}' {tuple(k_shape)} does not fit q {tuple(shape)}")
     v_rows = _rows(v, names[1], dtype, device, k_shape, False, True)
+    if written and o_rows[0] in (q_rows[0], k_rows[0], v_rows[0]) and o_rows[0]:
+        raise ValueError("'o' must not lie in place of an input")
     if k_shape[1] == 0 or shape[1] % k_shape[1]:
         raise ValueError(f"{shape[1]} query heads cannot share {k_shape[1]} key / value heads")
     if not sm_scale > 0:

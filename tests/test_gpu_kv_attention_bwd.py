@@ -121,6 +121,16 @@ def test_padded_batches(device, sq, D, dtype):
     check_run(q, k, v, do, lengths)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lengths", [[108, 193], [70, 2000], [256, 257], [1, 0]])
+def test_few_keys_where_many_could_be(device, lengths, D, dtype):
+    """The keys are split for the longest sequence there could be, and a short one's are not."""
+    g = torch.Generator(device=device).manual_seed(lengths[0])
+    q, do = rows((2, 2, 1, D), dtype, g), rows((2, 2, 1, D), dtype, g)
+    check_run(q, rows((2, 1, 2000, D), dtype, g), rows((2, 1, 2000, D), dtype, g), do, lengths)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_scores_far_below_zero(device, D):
     """exp of a padding row's score against such an lse overflows: it must not reach the sums."""

@@ -76,7 +76,7 @@ def test_null_arguments_and_small_workspaces():
     assert lib.asc_rotary(None, None) == _native.ERR_INVALID_ARG
     a = _args()
     need = lib.asc_qk_norm_rotary_bwd_workspace(ctypes.byref(a))
-    assert need == 2 * 64 * 4  # one workgroup's sums
+    assert need == 3 * 2 * 64 * 4  # the sums of a workgroup for every token
     assert lib.asc_qk_norm_rotary_bwd(ctypes.byref(a), 1024, need - 1, None) == _native.ERR_INVALID_ARG
     assert lib.asc_qk_norm_rotary_bwd(ctypes.byref(a), None, need, None) == _native.ERR_INVALID_ARG
 

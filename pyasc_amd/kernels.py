@@ -621,20 +621,24 @@ def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: int, shape: Op
           written: bool = False, aligned: bool = False) -> tuple:
     """A [batch, heads, seq, head_dim] operand whose last dimension is contiguous as asc_rows_t's
     fields; ``aligned``: with rows that can be read and written 16 bytes at a time (16-bit elements)."""
-    if not isinstance(t, torch.Tensor) or t.get_device() != device:
-        _here(t, name, device)
+    try:
+        if t.get_device() != device:
+            _here(t, name, device)
+        size = t.shape
+        if (size != shape if shape is not None else len(size) != 4):
+            raise ValueError(f"'{name}' must be {list(shape) if shape else '[batch, heads, seq, head_dim]'}, "
+                             f"got {tuple(size)}")
+        s0, s1, s2, s3 = t.stride()
+        at = t.data_ptr()
+    except AttributeError:
+        _device_tensor(t, name)  # says what it is instead of a tensor
+        raise
     if t.dtype is not dtype:
         raise TypeError(f"'{name}' must be {dtype}, got {t.dtype}")
-    size = t.shape
-    if len(size) != 4 or (shape is not None and size != shape):
-        raise ValueError(f"'{name}' must be {list(shape) if shape else '[batch, heads, seq, head_dim]'}, "
-                         f"got {tuple(size)}")
-    s0, s1, s2, s3 = t.stride()
     if s3 != 1 and size[3] > 1:
         raise ValueError(f"the last dimension of '{name}' must be contiguous")
     if written and not t.is_contiguous():
         _apart(t, name)
-    at = t.data_ptr()
     if aligned and (at | (s0 | s1 | s2) << 1) & 15:
         # a dimension of one element is not stepped over, whatever its stride
         s0, s1, s2 = (s if n > 1 else 0 for s, n in zip((s0, s1, s2), size))
@@ -731,53 +735,54 @@ def _rotary_args(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     batch, heads, seq, head_dim = shape
     if head_dim % 2 or not 0 < head_dim <= MAX_ROTARY_HEAD_DIM:
         raise ValueError(f"head_dim {head_dim} not supported (even, at most {MAX_ROTARY_HEAD_DIM})")
-    out_rows = [_rows(q_out, "q_out", dtype, device, shape, written=True), _NO_ROWS]
-    in_rows, k_heads = [q_rows, _NO_ROWS], 0
+    qo_rows = _rows(q_out, "q_out", dtype, device, shape, True)
+    k_rows = ko_rows = dq_rows = dk_rows = _NO_ROWS
+    k_heads, w_q, w_k, dw_q, dw_k = 0, 0, 0, 0, 0
     if (k is None) != (k_out is None):
         raise ValueError("k and its result must be given together")
     if k is not None:
-        in_rows[1] = _rows(k, "k", dtype, device)
-        k_heads = k.shape[1]
-        k_shape = (batch, k_heads, seq, head_dim)
-        if k.shape != k_shape:
-            raise ValueError(f"'k' must be {list(k_shape)}, got {tuple(k.shape)}")
-        out_rows[1] = _rows(k_out, "k_out", dtype, device, k_shape, written=True)
-    w, dw, dy_rows = (0, 0), (0, 0), (_NO_ROWS, _NO_ROWS)
+        k_rows = _rows(k, "k", dtype, device)
+        k_shape = k.shape
+        k_heads = k_shape[1]
+        if k_shape != (batch, k_heads, seq, head_dim):
+            raise ValueError(f"'k' must be {[batch, k_heads, seq, head_dim]}, got {tuple(k_shape)}")
+        ko_rows = _rows(k_out, "k_out", dtype, device, k_shape, True)
     if weights is not None:
         if not epsilon >= 0:
             raise ValueError(f"epsilon must not be negative, got {epsilon}")
-        w = [_head_weight(weights[0], "q_weight", head_dim, device), 0]
+        w_q = _head_weight(weights[0], "q_weight", head_dim, device)
         if k is not None:
-            w[1] = _head_weight(weights[1], "k_weight", head_dim, device)
+            w_k = _head_weight(weights[1], "k_weight", head_dim, device)
     if grads is not None:
-        dy_rows = [_rows(grads[0], "dq_out", dtype, device, shape), _NO_ROWS]
-        dw = [_head_weight(grads[2], "dq_weight", head_dim, device), 0]
+        dq_rows = _rows(grads[0], "dq_out", dtype, device, shape)
+        dw_q = _head_weight(grads[2], "dq_weight", head_dim, device)
         if k is not None:
             if grads[1] is None:
                 raise ValueError("dk_out must be given with k")
-            dy_rows[1] = _rows(grads[1], "dk_out", dtype, device, k_shape)
-            dw[1] = _head_weight(grads[3], "dk_weight", head_dim, device)
-    for ins in (in_rows, dy_rows):
-        for x, y in zip(ins, out_rows):
-            if x[0] == y[0] and x != y and q.numel():
-                raise ValueError("a result in place of its input must have the input's strides")
+            dk_rows = _rows(grads[1], "dk_out", dtype, device, k_shape)
+            dw_k = _head_weight(grads[3], "dk_weight", head_dim, device)
+    at_q, at_k = qo_rows[0], ko_rows[0]
+    if (((at_q == q_rows[0] and qo_rows != q_rows) or (at_q == dq_rows[0] and qo_rows != dq_rows)) and q.numel() or
+            ((at_k == k_rows[0] and ko_rows != k_rows) or (at_k == dk_rows[0] and ko_rows != dk_rows)) and k.numel()):
+        raise ValueError("a result in place of its input must have the input's strides")
     _here(positions, "positions", device)
-    if positions.dtype not in (torch.int64, torch.int32):
-        raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
-    if positions.shape == (seq,):
-        steps = (0, positions.stride(0))
-    elif positions.shape == (batch, seq):
-        steps = positions.stride()
+    positions_dtype, positions_shape = positions.dtype, positions.shape
+    if positions_dtype is not torch.int64 and positions_dtype is not torch.int32:
+        raise TypeError(f"positions must be int32 or int64, got {positions_dtype}")
+    if positions_shape == (batch, seq):
+        batch_step, step = positions.stride()
+    elif positions_shape == (seq,):
+        batch_step, step = 0, positions.stride(0)
     else:
-        raise ValueError(f"positions must be [seq] or [batch, seq] = {(batch, seq)}, got {tuple(positions.shape)}")
+        raise ValueError(f"positions must be [seq] or [batch, seq] = {(batch, seq)}, got {tuple(positions_shape)}")
     _here(freqs, "freqs", device)
     pairs = freqs.numel()
     if freqs.dtype is not torch.float64 or freqs.dim() != 1 or 2 * pairs > head_dim or not freqs.is_contiguous():
-        raise ValueError(f"'freqs' must be a contiguous float64 vector of at most head_dim / 2 = {head_dim // 2} elements")
+        raise ValueError(f"'freqs' must be a contiguous float64 vector of at most {head_dim // 2} elements")
     return _ROTARY.pack(_DTYPE_CODES[dtype], head_dim, 2 * pairs, bool(interleaved), bool(backward),
-                        positions.dtype is torch.int64, magnitude, epsilon, batch, heads, k_heads, seq, *in_rows[0],
-                        *in_rows[1], *out_rows[0], *out_rows[1], *dy_rows[0], *dy_rows[1], positions.data_ptr(), *steps,
-                        freqs.data_ptr(), *w, *dw)
+                        positions_dtype is torch.int64, magnitude, epsilon, batch, heads, k_heads, seq, *q_rows,
+                        *k_rows, *qo_rows, *ko_rows, *dq_rows, *dk_rows, positions.data_ptr(), batch_step, step,
+                        freqs.data_ptr(), w_q, w_k, dw_q, dw_k)
 
 
 def _head_weight(w: torch.Tensor, name: str, head_dim: int, device: int) -> int:

@@ -489,9 +489,9 @@ int32_t asc_qk_norm_rotary_bwd(const asc_rotary_t* args, void* workspace,
  * key / value head i / (q_heads / kv_heads).  o = softmax(q k^T * sm_scale) v over
  * the keys a query attends, fp32 statistics; lse (may be NULL) receives their
  * natural log-sum-exp, fp32 [batch, q_heads, q_len].  A query without keys gets
- * zeros, and -inf for its lse.  float16 and bfloat16, head_dim 64 or 128, sm_scale >
- * 0; bases 16-byte aligned and strides multiples of 8 elements (ASC_ERR_ALIGNMENT);
- * keys and values within 64 GiB.
+ * zeros, and -inf for its lse.  float16 and bfloat16, head_dim 64 or 128, sm_scale
+ * positive and finite (gradients: at least 2^-100); bases 16-byte aligned and strides
+ * multiples of 8 elements (ASC_ERR_ALIGNMENT); keys and values within 64 GiB.
  * asc_cross_attention_fwd  keys 0 .. kv_lengths[b] - 1 of sequence b (kv_lengths
  *                          NULL: all kv_len).
  * asc_tree_attention       first the cached keys, as above, from k and v; with a

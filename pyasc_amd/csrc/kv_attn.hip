@@ -2,6 +2,8 @@
 // the queries) and asc_tree_attention (a cache in pages or in one piece, and drafted tokens behind
 // it).  The device code is kv_attn_kernels.h; here are the checks, the choice of the kernel and of
 // the split of the keys, and the workspace of the splits.
+#include <cmath>
+
 #include "kv_attn_host.h"
 #include "kv_attn_kernels.h"
 
@@ -243,7 +245,8 @@ int32_t check_shape(const asc_attention_t* a, const char* what) {
   ASC_REQUIRE(a->q_heads == 0 || (a->kv_heads > 0 && a->q_heads % a->kv_heads == 0), ASC_ERR_INVALID_ARG,
               "%s: %lld query heads cannot share %lld key / value heads", what, static_cast<long long>(a->q_heads),
               static_cast<long long>(a->kv_heads));
-  ASC_REQUIRE(a->sm_scale > 0.f, ASC_ERR_INVALID_ARG, "%s: sm_scale must be positive", what);
+  ASC_REQUIRE(a->sm_scale > 0.f && a->sm_scale < INFINITY, ASC_ERR_INVALID_ARG,
+              "%s: sm_scale must be positive and finite", what);
   // rows of one key / value head, keys of one sequence and workgroups stay below 2^30, 2^30 and 2^22
   ASC_REQUIRE(a->batch < 1 << 20 && a->q_heads < 1 << 20 && a->q_len < 1 << 30 && a->kv_len < 1 << 30 &&
                   a->batch * a->q_heads < 1 << 20 &&

@@ -73,6 +73,8 @@ int64_t workspace_of(const Launch& L) {
 int32_t make(const asc_attention_t* a, const char* what, Launch& L) {
   int32_t rc = asc::kv::check_shape(a, what);
   if (rc != ASC_OK) return rc;
+  // lse / sm_scale has to stay finite: the logarithm of a count of keys is below 2^5
+  ASC_REQUIRE(a->sm_scale >= 0x1p-100f, ASC_ERR_UNSUPPORTED, "%s: sm_scale %g is below 2^-100", what, a->sm_scale);
   const bool queries = a->batch > 0 && a->q_heads > 0 && a->q_len > 0;
   const bool keys = a->batch > 0 && a->kv_heads > 0 && a->kv_len > 0;
   GradArgs& p = L.p;

@@ -476,8 +476,7 @@ int vector_width(const asc_rotary_t& a, Mode mode) {
 
 void sum_weights(const asc_rotary_t& a, const float* parts, int n_parts, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(asc::ceil_div(2 * a.head_dim, 16)));
-hipLaunchKernelGGL(weight_sums_kernel, grid, dim3(1024), 0,
-                     stream, parts, n_parts, a.head_dim, a.dq_weight, a.dk_weight);
+  hipLaunchKernelGGL(weight_sums_kernel, grid, dim3(1024), 0, stream, parts, n_parts, a.head_dim, a.dq_weight, a.dk_weight);
 }
 
 int32_t run(const asc_rotary_t* a, const char* what, Mode mode, float* parts, asc_stream_t stream) {

@@ -765,6 +765,8 @@ def _rotary_args(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     if (((at_q == q_rows[0] and qo_rows != q_rows) or (at_q == dq_rows[0] and qo_rows != dq_rows)) and q.numel() or
             ((at_k == k_rows[0] and ko_rows != k_rows) or (at_k == dk_rows[0] and ko_rows != dk_rows)) and k.numel()):
         raise ValueError("a result in place of its input must have the input's strides")
+    if at_q and at_k and (at_q in (at_k, k_rows[0], dk_rows[0]) or at_k in (q_rows[0], dq_rows[0])):
+        raise ValueError("a result of q must not lie in place of k's tensors, nor k's of q's")
     _here(positions, "positions", device)
     positions_dtype, positions_shape = positions.dtype, positions.shape
     if positions_dtype is not torch.int64 and positions_dtype is not torch.int32:
@@ -860,8 +862,8 @@ def _kv_rows(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
         raise ValueError("'o' must not lie in place of an input")
     if k_shape[1] == 0 or shape[1] % k_shape[1]:
         raise ValueError(f"{shape[1]} query heads cannot share {k_shape[1]} key / value heads")
-    if not sm_scale > 0:
-        raise ValueError(f"sm_scale must be positive, got {sm_scale}")
+    if not 0 < sm_scale < math.inf:
+        raise ValueError(f"sm_scale must be positive and finite, got {sm_scale}")
     return q_rows, o_rows, k_rows, v_rows
 
 
@@ -948,6 +950,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     shape = (batch, kv_heads, n, head_dim)
     kd_rows = _rows(k_draft, "k_draft", dtype, device, shape, False, True)
     vd_rows = _rows(v_draft, "v_draft", dtype, device, shape, False, True)
+    if o_rows[0] in (kd_rows[0], vd_rows[0]) and o_rows[0]:
+        raise ValueError("'o' must not lie in place of an input")
     page_size, table, table_stride = 0, 0, 0
     if block_table is not None:
         _here(block_table, "block_table", device)

@@ -406,3 +406,24 @@ def test_refusals(device):
     tree_refused(ValueError, "block_table", block_table=torch.zeros((2, 8), device=device).int()[:, ::2])
     tree_refused(ValueError, "without pages", kc=k[:0], block_table=table)
     tree_refused(ValueError, "draft_lengths", draft_lengths=n[:1])
+
+
+def test_refused_places_and_scales(device):
+    q = torch.zeros((2, 4, 3, 64), device=device).half()
+    k = torch.zeros((2, 4, 8, 64), device=device).half()
+    d, n = q.clone(), torch.full((2,), 8, dtype=torch.int32, device=device)
+    for kd, vd in ((d, q.clone()), (q.clone(), d)):
+        with pytest.raises(ValueError, match="in place"):
+            kernels.tree_attention(q, k, k, n, kd, vd, None, d, 0.125)
+    with pytest.raises(ValueError, match="finite"):
+        kernels.cross_attention_fwd(q, k, k, d, math.inf)
+    # the smallest scale that has a gradient: all probabilities alike, as for a scale of 0
+    v = torch.randn((2, 4, 8, 64), device=device).half()
+    do, lse = torch.randn_like(q), torch.empty((2, 4, 3), device=device)
+    kernels.cross_attention_fwd(q, k, v, d, 2.0 ** -100, lse=lse)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    kernels.cross_attention_bwd(do, q, k, v, d, lse, dq, dk, dv, 2.0 ** -100)
+    assert not dq.any() and not dk.any()
+    want = (do.double().sum(2, keepdim=True) / 8).expand(v.shape)
+    # probabilities of 1/8 are exact; sums in fp32, then a rounding
+    torch.testing.assert_close(dv.double(), want, rtol=2.0 ** -11 + 2.0 ** -20, atol=1e-6)

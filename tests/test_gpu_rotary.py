@@ -289,3 +289,20 @@ def test_refusals(device):
         kernels.qk_norm_rotary(q, None, w, None, p, freqs, out, None, epsilon=-1.0)
     with pytest.raises(ValueError, match="dk_out"):
         kernels.qk_norm_rotary_bwd(q, None, q, q, w, w, p, freqs, out, out.clone(), w, w, 1e-6)
+
+
+def test_refused_places(device):
+    q, k = torch.zeros((1, 2, 3, 64), device=device), torch.zeros((1, 2, 3, 64), device=device)
+    p, (freqs, _) = torch.arange(3, device=device), kernels.rotary_frequencies(64)
+    w = torch.ones(64, device=device)
+    other = q.clone()
+    for outs in ((k, other), (other, q), (other, other)):
+        with pytest.raises(ValueError, match="in place of k's"):
+            kernels.rotary(q, k, p, freqs, *outs)
+    dq, dk = q.clone(), k.clone()
+    for outs in ((dk, other), (other, dq)):
+        with pytest.raises(ValueError, match="in place of k's"):
+            kernels.qk_norm_rotary_bwd(dq, dk, q, k, w, w, p, freqs, *outs, w.clone(), w.clone(), 1e-6)
+    none = torch.zeros((1, 0, 3, 64), device=device)  # nothing to write: nothing to refuse
+    kernels.rotary(none, none, p, freqs, none, none)
+    kernels.rotary(none, k, p, freqs, none, k)

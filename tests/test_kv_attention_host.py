@@ -99,3 +99,14 @@ def test_nothing_to_do():
             a = _args(**kw)
             assert getattr(lib, entry + "_workspace")(ctypes.byref(a)) == 0
             assert getattr(lib, entry)(ctypes.byref(a), None, 0, None) == 0
+
+
+@pytest.mark.parametrize("entry", ENTRIES)
+def test_scales(entry):
+    a = _args(sm_scale=float("inf"))
+    assert getattr(_native.load_library(), entry)(ctypes.byref(a), AT, 1 << 40, None) == INVALID
+    assert "finite" in _native.last_error()
+    if entry == "asc_cross_attention_bwd":  # lse / sm_scale would not be finite
+        a = _args(sm_scale=2.0 ** -101)
+        assert getattr(_native.load_library(), entry)(ctypes.byref(a), AT, 1 << 40, None) == UNSUPPORTED
+        assert "2^-100" in _native.last_error()

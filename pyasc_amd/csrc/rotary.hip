@@ -125,7 +125,10 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
 
   const int tid = threadIdx.x;
   const int lane = tid & (p.lanes - 1);
+  // rows of a pass: tokens fastest, so that neighbours lie together in both orders of heads and
+  // tokens; at least as many as tokens, so a lane stays with its token and steps over heads
   const int row0 = tid / p.lanes, rows_per_pass = kThreads / p.lanes;
+  const int t = row0 & (p.tokens - 1), head0 = row0 / p.tokens, head_step = rows_per_pass / p.tokens;
   const int pair_slots = p.pairs / V, slots = p.head_dim / (2 * V);
 
   // the two vectors of each slot: the pairs' first and second values, or two neighbours of
@@ -151,31 +154,35 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
     const int tokens = static_cast<int>(p.seq - s0 < p.tokens ? p.seq - s0 : p.tokens);
     __syncthreads();  // the table's last readers
     for (int i = tid; i < tokens * p.pairs; i += kThreads) {
-      const int t = i / p.pairs, j = i - t * p.pairs;
-      const int64_t o = b * p.pos_batch + (s0 + t) * p.pos_seq;
+      const int of = i / p.pairs, j = i - of * p.pairs;
+      const int64_t o = b * p.pos_batch + (s0 + of) * p.pos_seq;
       const double pos = p.pos64 ? static_cast<double>(static_cast<const int64_t*>(p.positions)[o])
                                  : static_cast<double>(static_cast<const int32_t*>(p.positions)[o]);
-      table[t * p.pairs + j] = turn_of(pos * (p.freqs[j] * 0.15915494309189533577), p.sign, p.magnitude);
+      table[of * p.pairs + j] = turn_of(pos * (p.freqs[j] * 0.15915494309189533577), p.sign, p.magnitude);
     }
     __syncthreads();
+    float2 cs[kSlots][V];  // of this lane's token and pairs, for every head
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        cs[i][e] = t < tokens && turned[i] ? table[t * p.pairs + at[i] + e] : make_float2(1.f, 0.f);
+      }
     const int h0 = chunk * p.chunk_heads;
     const int n_heads = p.heads - h0 < p.chunk_heads ? p.heads - h0 : p.chunk_heads;
-    // Rows: tokens fastest, so that neighbours lie together in both orders of heads and tokens.  The
-    // next row is asked for before this one is worked on.
     // Queries and keys one after the other, so that a row's weights and sums are fixed registers.
+    // The next row is asked for before this one is worked on.
     struct Row {
       bool live;
-      int t;
-      T* out;
       Vec<T, V> a0[kSlots], a1[kSlots], g0[kSlots], g1[kSlots];
     };
     const auto heads_of = [&](auto which) {
       constexpr int kKind = decltype(which)::value;  // 0: queries, 1: keys
       const int first = kKind == 0 ? h0 : (h0 > p.q_heads ? h0 : p.q_heads) - p.q_heads;
       const int last = kKind == 0 ? (h0 + n_heads < p.q_heads ? h0 + n_heads : p.q_heads) : h0 + n_heads - p.q_heads;
-      const int count = (last - first) * p.tokens;  // may be negative
+      if (first >= last) return;
       float w[kSlots][2][V];
-      if (kMode != kTurn && count > 0) {
+      if (kMode != kTurn) {
 #pragma unroll
         for (int i = 0; i < kSlots; ++i)
 #pragma unroll
@@ -184,31 +191,34 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
             w[i][1][e] = live[i] ? p.weight[kKind][c1[i] + e] : 0.f;
           }
       }
-      const auto fetch = [&](int r, Row& m) {
-        m.t = r & (p.tokens - 1);  // a power of two
-        m.live = r < count && m.t < tokens;
+      const auto at_row = [&](const Rows& rows) {
+        return static_cast<const T*>(rows.p) + b * rows.batch + (first + head0) * rows.head + (s0 + t) * rows.seq;
+      };
+      const T* x = at_row(p.x[kKind]);  // of the next row to fetch, and dy
+      const T* dy = kMode == kNormGrad ? at_row(p.dy[kKind]) : nullptr;
+      T* out = const_cast<T*>(at_row(p.out[kKind]));  // of the next row to work on
+      const int64_t x_step = head_step * p.x[kKind].head, dy_step = head_step * p.dy[kKind].head,
+                    out_step = head_step * p.out[kKind].head;
+      int left = t < tokens ? last - first - head0 : 0;  // heads from the next row to fetch on
+      const auto fetch = [&](Row& m) {
+        m.live = left > 0;
+        left -= head_step;
         if (!m.live) return;
-        const int64_t h = first + r / p.tokens;
-        const int64_t s = s0 + m.t;
-        const auto at_row = [&](const Rows& rows) {
-          return static_cast<const T*>(rows.p) + b * rows.batch + h * rows.head + s * rows.seq;
-        };
-        const T* x = at_row(p.x[kKind]);
-        m.out = const_cast<T*>(at_row(p.out[kKind]));
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) {
           if (!live[i]) continue;
           m.a0[i] = load<T, V>(x + c0[i]);
           m.a1[i] = load<T, V>(x + c1[i]);
         }
+        x += x_step;
         if (kMode == kNormGrad) {
-          const T* dy = at_row(p.dy[kKind]);
 #pragma unroll
           for (int i = 0; i < kSlots; ++i) {
             if (!live[i]) continue;
             m.g0[i] = load<T, V>(dy + c0[i]);
             m.g1[i] = load<T, V>(dy + c1[i]);
           }
+          dy += dy_step;
         }
       };
       const auto work = [&](Row& m) {
@@ -232,16 +242,15 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
 #pragma unroll
             for (int e = 0; e < V; ++e) ss += a0[i][e] * a0[i][e] + a1[i][e] * a1[i][e];
           }
-          rms = 1.0f / sqrtf(row_sum(ss, p.lanes) * p.inv_dim + p.epsilon);
+          rms = rsqrtf(row_sum(ss, p.lanes) * p.inv_dim + p.epsilon);
         }
         // turn of one slot's vectors in place; the pairs' values lie in y0, y1, or alternate
         const auto turn = [&](int i, float (&y0)[V], float (&y1)[V]) {
           if (!turned[i]) return;
-          const float2* cs = table + m.t * p.pairs + at[i];
           if (kInterleaved && V > 1) {
 #pragma unroll
             for (int e = 0; e < V; e += 2) {
-              const float2 u = cs[e / 2], v = cs[V / 2 + e / 2];
+              const float2 u = cs[i][e / 2], v = cs[i][V / 2 + e / 2];
               const float u0 = y0[e], u1 = y0[e + 1], v0 = y1[e], v1 = y1[e + 1];
               y0[e] = u0 * u.x - u1 * u.y;
               y0[e + 1] = u1 * u.x + u0 * u.y;
@@ -251,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
           } else {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-              const float2 c = cs[e];
+              const float2 c = cs[i][e];
               const float u = y0[e], v = y1[e];
               y0[e] = u * c.x - v * c.y;
               y1[e] = v * c.x + u * c.y;
@@ -303,17 +312,17 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) {
           if (!live[i]) continue;
-          store<T, V>(m.out + c0[i], a0[i]);
-          store<T, V>(m.out + c1[i], a1[i]);
+          store<T, V>(out + c0[i], a0[i]);
+          store<T, V>(out + c1[i], a1[i]);
         }
+        out += out_step;
       };
       Row rows[2];
-      int r = row0;
-      fetch(r, rows[0]);
-      for (; r < count; r += 2 * rows_per_pass) {
-        fetch(r + rows_per_pass, rows[1]);
+      fetch(rows[0]);
+      for (int n = first; n < last; n += 2 * head_step) {
+        fetch(rows[1]);
         work(rows[0]);
-        fetch(r + 2 * rows_per_pass, rows[0]);
+        fetch(rows[0]);
         work(rows[1]);
       }
     };
@@ -511,6 +520,7 @@ int32_t run(const asc_rotary_t* a, const char* what, Mode mode, float* parts, as
   p.lanes = 1;
   while (p.lanes < slots) p.lanes *= 2;  // at most 64: head_dim <= 512
   p.tokens = tokens_of(*a);
+  if (p.tokens > kThreads / p.lanes) p.tokens = kThreads / p.lanes;  // both powers of two
   p.tiles = static_cast<uint32_t>(asc::ceil_div(a->seq, p.tokens));
   const int64_t n_tiles = a->batch * p.tiles;
   // Few tokens: their heads spread over workgroups of one pass each; else one workgroup for all.
@@ -522,7 +532,7 @@ int32_t run(const asc_rotary_t* a, const char* what, Mode mode, float* parts, as
   p.chunks = static_cast<uint32_t>(asc::ceil_div(p.heads, p.chunk_heads));
   p.units = static_cast<uint32_t>(n_tiles * p.chunks);  // chunks > 1 only where n_tiles is small
   int64_t blocks = p.units;
-  const int64_t most = mode == kNormGrad ? kMaxParts : int64_t{1} << 23;  // the kernel strides over the rest
+  const int64_t most = mode == kNormGrad ? grad_parts(*a) : int64_t{1} << 23;  // the kernel strides over the rest
   if (blocks > most) blocks = most;
   const dim3 grid(static_cast<uint32_t>(blocks));
   const hipStream_t s = static_cast<hipStream_t>(stream);

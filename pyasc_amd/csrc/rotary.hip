@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTokens = 8;     // of a workgroup at a time
+constexpr int kMinTokens = 4;     // where there are many: a row has at most 64 lanes
 constexpr int kMaxHeadDim = 512;  // kSlots lanes' slots and the LDS tables cover it
 constexpr int kMaxParts = 1024;   // workgroups of a gradient launch: partial sums of its weights
 
@@ -122,6 +123,7 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
   constexpr int kSlots = slots_per_lane<V>();
   __shared__ float2 table[kMaxTokens * kMaxHeadDim / 2];
   __shared__ float sums[kMode == kNormGrad ? 2 * kMaxHeadDim : 1];
+  __shared__ float weights[kMode != kTurn ? 2 * kMaxHeadDim : 1];
 
   const int tid = threadIdx.x;
   const int lane = tid & (p.lanes - 1);
@@ -145,6 +147,12 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
     c1[i] = kInterleaved || !turned[i] ? c0[i] + V : c0[i] + p.pairs;
   }
   float dw[2][kSlots][2][V] = {};
+  if (kMode != kTurn) {
+    for (int i = tid; i < 2 * p.head_dim; i += kThreads) {
+      const float* w = p.weight[i >= p.head_dim];
+      weights[i] = w ? w[i >= p.head_dim ? i - p.head_dim : i] : 0.f;
+    }
+  }
 
   for (uint32_t unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
     const uint32_t tile = unit / p.chunks;
@@ -152,6 +160,69 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
     const int64_t b = tile / p.tiles;
     const int64_t s0 = static_cast<int64_t>(tile % p.tiles) * p.tokens;
     const int tokens = static_cast<int>(p.seq - s0 < p.tokens ? p.seq - s0 : p.tokens);
+    const int h0 = chunk * p.chunk_heads;
+    const int n_heads = p.heads - h0 < p.chunk_heads ? p.heads - h0 : p.chunk_heads;
+    struct Row {
+      bool live;
+      Vec<T, V> a0[kSlots], a1[kSlots], g0[kSlots], g1[kSlots];
+    };
+    struct Heads {   // of queries or keys
+      const T* x;    // of the next row to fetch, and dy
+      const T* dy;
+      T* out;  // of the next row to work on
+      int64_t x_step, dy_step, out_step;
+      int count, left;  // of the unit; from the next row to fetch on
+    };
+    const auto heads_of = [&](auto which) {
+      constexpr int kKind = decltype(which)::value;  // 0: queries, 1: keys
+      const int first = kKind == 0 ? h0 : (h0 > p.q_heads ? h0 : p.q_heads) - p.q_heads;
+      const int last = kKind == 0 ? (h0 + n_heads < p.q_heads ? h0 + n_heads : p.q_heads) : h0 + n_heads - p.q_heads;
+      const auto at_row = [&](const Rows& rows) {
+        return static_cast<const T*>(rows.p) + b * rows.batch + (first + head0) * rows.head + (s0 + t) * rows.seq;
+      };
+      Heads m;
+      m.x = at_row(p.x[kKind]);
+      m.dy = kMode == kNormGrad ? at_row(p.dy[kKind]) : nullptr;
+      m.out = const_cast<T*>(at_row(p.out[kKind]));
+      m.x_step = head_step * p.x[kKind].head;
+      m.dy_step = head_step * p.dy[kKind].head;
+      m.out_step = head_step * p.out[kKind].head;
+      m.count = last - first;
+      m.left = t < tokens ? m.count - head0 : 0;
+      return m;
+    };
+    const auto fetch = [&](Heads& h, Row& m) {
+      m.live = h.left > 0;
+      h.left -= head_step;
+      if (!m.live) return;
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) {
+        if (!live[i]) continue;
+        m.a0[i] = load<T, V>(h.x + c0[i]);
+        m.a1[i] = load<T, V>(h.x + c1[i]);
+      }
+      h.x += h.x_step;
+      if (kMode == kNormGrad) {
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+          if (!live[i]) continue;
+          m.g0[i] = load<T, V>(h.dy + c0[i]);
+          m.g1[i] = load<T, V>(h.dy + c1[i]);
+        }
+        h.dy += h.dy_step;
+      }
+    };
+    // The first rows are asked for ahead of the table, but for the gradient's, whose registers are
+    // full.
+    constexpr bool kAhead = kMode != kNormGrad;
+    Heads heads[2];
+    Row first[2];
+    if constexpr (kAhead) {
+      heads[0] = heads_of(std::integral_constant<int, 0>{});
+      fetch(heads[0], first[0]);
+      heads[1] = heads_of(std::integral_constant<int, 1>{});
+      fetch(heads[1], first[1]);
+    }
     __syncthreads();  // the table's last readers
     for (int i = tid; i < tokens * p.pairs; i += kThreads) {
       const int of = i / p.pairs, j = i - of * p.pairs;
@@ -168,59 +239,21 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
       for (int e = 0; e < V; ++e) {
         cs[i][e] = t < tokens && turned[i] ? table[t * p.pairs + at[i] + e] : make_float2(1.f, 0.f);
       }
-    const int h0 = chunk * p.chunk_heads;
-    const int n_heads = p.heads - h0 < p.chunk_heads ? p.heads - h0 : p.chunk_heads;
     // Queries and keys one after the other, so that a row's weights and sums are fixed registers.
     // The next row is asked for before this one is worked on.
-    struct Row {
-      bool live;
-      Vec<T, V> a0[kSlots], a1[kSlots], g0[kSlots], g1[kSlots];
-    };
-    const auto heads_of = [&](auto which) {
-      constexpr int kKind = decltype(which)::value;  // 0: queries, 1: keys
-      const int first = kKind == 0 ? h0 : (h0 > p.q_heads ? h0 : p.q_heads) - p.q_heads;
-      const int last = kKind == 0 ? (h0 + n_heads < p.q_heads ? h0 + n_heads : p.q_heads) : h0 + n_heads - p.q_heads;
-      if (first >= last) return;
+    const auto rows_of = [&](auto which, Heads& h, Row& first) {
+      constexpr int kKind = decltype(which)::value;
+      if (h.count <= 0) return;
       float w[kSlots][2][V];
       if (kMode != kTurn) {
 #pragma unroll
         for (int i = 0; i < kSlots; ++i)
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            w[i][0][e] = live[i] ? p.weight[kKind][c0[i] + e] : 0.f;
-            w[i][1][e] = live[i] ? p.weight[kKind][c1[i] + e] : 0.f;
+            w[i][0][e] = live[i] ? weights[kKind * p.head_dim + c0[i] + e] : 0.f;
+            w[i][1][e] = live[i] ? weights[kKind * p.head_dim + c1[i] + e] : 0.f;
           }
       }
-      const auto at_row = [&](const Rows& rows) {
-        return static_cast<const T*>(rows.p) + b * rows.batch + (first + head0) * rows.head + (s0 + t) * rows.seq;
-      };
-      const T* x = at_row(p.x[kKind]);  // of the next row to fetch, and dy
-      const T* dy = kMode == kNormGrad ? at_row(p.dy[kKind]) : nullptr;
-      T* out = const_cast<T*>(at_row(p.out[kKind]));  // of the next row to work on
-      const int64_t x_step = head_step * p.x[kKind].head, dy_step = head_step * p.dy[kKind].head,
-                    out_step = head_step * p.out[kKind].head;
-      int left = t < tokens ? last - first - head0 : 0;  // heads from the next row to fetch on
-      const auto fetch = [&](Row& m) {
-        m.live = left > 0;
-        left -= head_step;
-        if (!m.live) return;
-#pragma unroll
-        for (int i = 0; i < kSlots; ++i) {
-          if (!live[i]) continue;
-          m.a0[i] = load<T, V>(x + c0[i]);
-          m.a1[i] = load<T, V>(x + c1[i]);
-        }
-        x += x_step;
-        if (kMode == kNormGrad) {
-#pragma unroll
-          for (int i = 0; i < kSlots; ++i) {
-            if (!live[i]) continue;
-            m.g0[i] = load<T, V>(dy + c0[i]);
-            m.g1[i] = load<T, V>(dy + c1[i]);
-          }
-          dy += dy_step;
-        }
-      };
       const auto work = [&](Row& m) {
         if (!m.live) return;  // all lanes of the row
         float a0[kSlots][V], a1[kSlots][V], g0[kSlots][V], g1[kSlots][V];
@@ -312,22 +345,32 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) {
           if (!live[i]) continue;
-          store<T, V>(out + c0[i], a0[i]);
-          store<T, V>(out + c1[i], a1[i]);
+          store<T, V>(h.out + c0[i], a0[i]);
+          store<T, V>(h.out + c1[i], a1[i]);
         }
-        out += out_step;
+        h.out += h.out_step;
       };
-      Row rows[2];
-      fetch(rows[0]);
-      for (int n = first; n < last; n += 2 * head_step) {
-        fetch(rows[1]);
-        work(rows[0]);
-        fetch(rows[0]);
-        work(rows[1]);
+      Row second;
+      for (int n = 0; n < h.count; n += 2 * head_step) {
+        fetch(h, second);
+        work(first);
+        fetch(h, first);
+        work(second);
       }
     };
-    heads_of(std::integral_constant<int, 0>{});
-    heads_of(std::integral_constant<int, 1>{});
+    if constexpr (kAhead) {
+      rows_of(std::integral_constant<int, 0>{}, heads[0], first[0]);
+      rows_of(std::integral_constant<int, 1>{}, heads[1], first[1]);
+    } else {
+      const auto fetch_and_work = [&](auto which) {
+        Heads h = heads_of(which);
+        Row m;
+        fetch(h, m);
+        rows_of(which, h, m);
+      };
+      fetch_and_work(std::integral_constant<int, 0>{});
+      fetch_and_work(std::integral_constant<int, 1>{});
+    }
   }
 
   if (kMode == kNormGrad) {
@@ -419,19 +462,21 @@ void launch_vec(int vec, bool interleaved, dim3 grid, hipStream_t stream, const 
   return launch<T, 1, kMode>(interleaved, grid, stream, p);
 }
 
-// Tokens of a workgroup at a time, a power of two: as many as leave the chip four workgroups per CU.
-int tokens_of(const asc_rotary_t& a) {
-  int n = kMaxTokens;
-  while (n > 1 && (a.seq <= n / 2 || a.batch * asc::ceil_div(a.seq, n) < 1024)) n /= 2;
+// Tokens of a workgroup at a time, a power of two of at most the rows of its pass: as many as leave
+// the chip four workgroups per CU, or one where fewer tokens would leave lanes without a head (24
+// sequences of 78 tokens, 4 and 4 heads of 128: 7.5 us, always four per CU 19.7).
+int tokens_of(const asc_rotary_t& a, int rows_per_pass) {
+  const int64_t heads = a.q_heads > a.k_heads ? a.q_heads : a.k_heads;
+  int n = rows_per_pass < kMaxTokens ? rows_per_pass : kMaxTokens;
+  while (n > 1 && (a.seq <= n / 2 || a.batch * asc::ceil_div(a.seq, n) < (n * heads <= rows_per_pass ? 256 : 1024))) {
+    n /= 2;
+  }
   return n;
 }
-int64_t token_tiles(const asc_rotary_t& a) { return asc::ceil_div(a.seq, tokens_of(a)); }
 
-// Workgroups of a gradient launch, as its workspace counts them: at most kMaxParts, each with a
-// share of the token tiles.
+// Workgroups of a gradient launch, as its workspace counts them: each has a share of the tokens.
 int64_t grad_parts(const asc_rotary_t& a) {
-  const int64_t n = a.batch * token_tiles(a);
-  return n < kMaxParts ? n : kMaxParts;
+  return a.seq >= kMaxParts || a.batch * a.seq >= kMaxParts ? kMaxParts : a.batch * a.seq;
 }
 
 int32_t check(const asc_rotary_t* a, const char* what, Mode mode) {
@@ -446,7 +491,7 @@ int32_t check(const asc_rotary_t* a, const char* what, Mode mode) {
               "%s: rotary_dim %d must be even and at most head_dim %d", what, a->rotary_dim, a->head_dim);
   ASC_REQUIRE(a->q_heads <= 1 << 20 && a->k_heads <= 1 << 20, ASC_ERR_UNSUPPORTED, "%s: too many heads", what);
   ASC_REQUIRE(a->seq < int64_t{1} << 31 && a->batch < int64_t{1} << 31 &&
-                  a->batch * token_tiles(*a) < int64_t{1} << 31,
+                  a->batch * asc::ceil_div(a->seq, kMinTokens) < int64_t{1} << 31,
               ASC_ERR_UNSUPPORTED, "%s: batch %lld x seq %lld too large", what, static_cast<long long>(a->batch),
               static_cast<long long>(a->seq));
   ASC_REQUIRE(mode == kTurn || a->epsilon >= 0.f, ASC_ERR_INVALID_ARG, "%s: epsilon must not be negative", what);
@@ -519,8 +564,7 @@ int32_t run(const asc_rotary_t* a, const char* what, Mode mode, float* parts, as
   const int slots = static_cast<int>(asc::ceil_div(a->head_dim / (2 * vec), per_lane));
   p.lanes = 1;
   while (p.lanes < slots) p.lanes *= 2;  // at most 64: head_dim <= 512
-  p.tokens = tokens_of(*a);
-  if (p.tokens > kThreads / p.lanes) p.tokens = kThreads / p.lanes;  // both powers of two
+  p.tokens = tokens_of(*a, kThreads / p.lanes);
   p.tiles = static_cast<uint32_t>(asc::ceil_div(a->seq, p.tokens));
   const int64_t n_tiles = a->batch * p.tiles;
   // Few tokens: their heads spread over workgroups of one pass each; else one workgroup for all.

@@ -306,3 +306,13 @@ def test_refused_places(device):
     none = torch.zeros((1, 0, 3, 64), device=device)  # nothing to write: nothing to refuse
     kernels.rotary(none, none, p, freqs, none, none)
     kernels.rotary(none, k, p, freqs, none, k)
+
+
+@pytest.mark.parametrize("dtype,layout", [(torch.float32, "contiguous"), (torch.bfloat16, "odd"),
+                                          (torch.float16, "fused")])
+@pytest.mark.parametrize("b,hq,hk,s,d,rot", [(3, 1, 2, 1301, 512, 512), (9, 2, 2, 901, 128, 32), (2, 5, 1, 2500, 64, 64),
+                                             (1100, 1, 1, 3, 130, 2), (1, 33, 3, 1027, 48, 16)])
+def test_many_tokens_of_few_heads(device, b, hq, hk, s, d, rot, dtype, layout):
+    # several tokens per workgroup, of fewer or more heads than its pass has rows, the last ones odd
+    test_rotary(device, b, hq, hk, s, d, rot, layout, False, dtype)
+    test_norm_and_its_gradient(device, b, hq, hk, s, d, rot, layout, True, dtype)

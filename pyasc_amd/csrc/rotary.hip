@@ -9,9 +9,15 @@
 //
 // Each value is read and written once, so HBM bounds it.  A workgroup takes a few tokens and all
 // (or a chunk of) their heads: the angles of its tokens go into LDS once, from the product of
-// position and frequency in fp64 (a far position keeps its fraction of a turn), and every head
-// reads them.  A row (one head of one token) belongs to kLanes neighbouring lanes of a wave; a lane
-// holds both values of kV pairs, so the turn needs no exchange and the norm one butterfly.
+// position and frequency in fp64 (a far position keeps its fraction of a turn).  A row (one head of
+// one token) belongs to neighbouring lanes of a wave; a lane holds both values of V pairs, so the
+// turn needs no exchange and the norm one butterfly.  A lane stays with its token: cos and sin,
+// weights and the steps of its addresses are registers over all heads (with addresses worked out
+// row by row, the norm took 74 us where it takes 63).
+//
+// bf16, 4 x 4096 tokens, 32 + 8 heads of 128: positions 60 us (5.6 TB/s), with the norm 63 (5.3), a
+// copy of the same bytes 65; the gradient 107 (4.7), its conversions and sums beside the loads.
+// fp32, half the tokens: 131, 133 and 195 us (5.1 TB/s each).
 #include <type_traits>
 
 #include "common.h"
@@ -412,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
 
 // dw[t][c] = sum over workgroups of parts[.][t][c], in fp64 (the sum itself is short).  One
 // workgroup per 16 columns; 64 rows of threads take every 64th part, four loads in flight each, and
-// are added up in pairs.
+// are added up in pairs: 4 us for 1024 parts of 2 x 64, the latency of sixteen loads in a chain of four.
 constexpr int kSumRows = 64;
 __global__ void __launch_bounds__(1024) weight_sums_kernel(const float* parts, int n_parts, int head_dim, float* dq,
                                                            float* dk) {

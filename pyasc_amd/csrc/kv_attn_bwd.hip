@@ -18,8 +18,8 @@ __global__ void __launch_bounds__(GradKv<D>::kWaves * 64, GradKv<D>::kWgPerCu) g
   asc::kv::grad_kv_body<D, E, kPacked>(p);
 }
 template <int D, class E>
-__global__ void __launch_bounds__(256) join_grad(GradArgs p, int kind, int groups) {
-  asc::kv::join_grad_body<D, E>(p, kind, groups);
+__global__ void __launch_bounds__(256) join_grad(GradArgs p) {
+  asc::kv::join_grad_body<D, E>(p);
 }
 
 constexpr int kMaxSplits = 32;
@@ -60,6 +60,14 @@ void plan(Launch& L, const asc_attention_t& a) {
   L.values = L.q_rows;
   L.parts_q = p.q_splits > 1 ? L.q_rows * p.q_splits * a.head_dim : 0;
   L.parts_kv = p.kv_splits > 1 ? L.kv_rows * p.kv_splits * a.head_dim : 0;
+  const auto groups = [&](int64_t n, int splits) {
+    return small ? asc::kv::JoinLanes<64>::groups_of(n, splits) : asc::kv::JoinLanes<128>::groups_of(n, splits);
+  };
+  p.q_join_groups = groups(L.q_rows, p.q_splits);
+  p.kv_join_groups = groups(L.kv_rows, p.kv_splits);
+  const int64_t lanes = a.head_dim / 8;
+  if (L.parts_q > 0) p.q_join = static_cast<uint32_t>(asc::ceil_div(L.q_rows * lanes * p.q_join_groups, 256));
+  if (L.parts_kv > 0) p.kv_join = static_cast<uint32_t>(asc::ceil_div(L.kv_rows * lanes * p.kv_join_groups, 256));
 }
 
 // Floats of a workspace region, so that the next one is 16-byte aligned.
@@ -137,23 +145,15 @@ int32_t launch(const Launch& L, const char* what, hipStream_t stream) {
     hipLaunchKernelGGL((grad_q<D, E>), grid(L.q_grid), dim3(GradQ<D>::kWaves * 64), 0, stream, L.p);
     const int32_t rc = asc::check_launch(what);
     if (rc != ASC_OK) return rc;
-    if (L.parts_q > 0) {
-      const int groups = asc::kv::JoinLanes<D>::groups_of(L.q_rows, L.p.q_splits);
-      hipLaunchKernelGGL((join_grad<D, E>), grid(asc::ceil_div(L.q_rows * (D / 8) * groups, 256)), dim3(256), 0, stream,
-                         L.p, 0, groups);
-    }
   }
   if (L.kv_grid > 0) {
     const auto kernel = L.p.n_q < GradKv<D>::kRows ? grad_kv<D, E, true> : grad_kv<D, E, false>;
     hipLaunchKernelGGL(kernel, grid(L.kv_grid), dim3(GradKv<D>::kWaves * 64), 0, stream, L.p);
     const int32_t rc = asc::check_launch(what);
     if (rc != ASC_OK) return rc;
-    for (int kind = 1; kind < 3 && L.parts_kv > 0; ++kind) {
-      const int groups = asc::kv::JoinLanes<D>::groups_of(L.kv_rows, L.p.kv_splits);
-      hipLaunchKernelGGL((join_grad<D, E>), grid(asc::ceil_div(L.kv_rows * (D / 8) * groups, 256)), dim3(256), 0,
-                         stream, L.p, kind, groups);
-    }
   }
+  const int64_t joins = int64_t{L.p.q_join} + 2 * int64_t{L.p.kv_join};
+  if (joins > 0) hipLaunchKernelGGL((join_grad<D, E>), grid(joins), dim3(256), 0, stream, L.p);
   return asc::check_launch(what);
 }
 

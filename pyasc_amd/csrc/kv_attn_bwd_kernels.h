@@ -51,6 +51,8 @@ struct GradArgs {
   int32_t capacity, kv_heads, group, n_q, rows;
   int32_t q_blocks, q_splits, kv_blocks, kv_splits;
   uint32_t q_units, kv_units;  // batch * kv_heads * splits
+  uint32_t q_join, kv_join;    // workgroups that add up the parts of dq, of dk and of dv
+  int32_t q_join_groups, kv_join_groups;
   float scale, scale_log2, inv_scale;
 };
 
@@ -507,11 +509,14 @@ __device__ __forceinline__ void grad_kv_body(const GradArgs& p) {
   t.store(dv, p.dv + s.b * p.dv_batch + s.head * p.dv_head + key * p.dv_seq, bad ? nan : 1.0f, zero);
 }
 
-// Adds up the parts of rows.  kind 0: dq, 1: dk, 2: dv.
+// Adds up the parts of rows.  kind 0: dq, 1: dk, 2: dv, in q_join, kv_join and kv_join workgroups of one
+// launch.
 template <int D, class E>
-__device__ __forceinline__ void join_grad_body(const GradArgs& p, int kind, int groups) {
+__device__ __forceinline__ void join_grad_body(const GradArgs& p) {
+  const int kind = blockIdx.x < p.q_join ? 0 : (blockIdx.x < p.q_join + p.kv_join ? 1 : 2);
+  const uint32_t block = blockIdx.x - (kind == 0 ? 0 : p.q_join + (kind - 1) * p.kv_join);
   const int per_head = kind == 0 ? p.rows : p.capacity, splits = kind == 0 ? p.q_splits : p.kv_splits;
-  const JoinLanes<D> at(groups);
+  const JoinLanes<D> at(block, kind == 0 ? p.q_join_groups : p.kv_join_groups);
   const int64_t bh = at.row / per_head;
   if (bh >= static_cast<int64_t>((kind == 0 ? p.q_units : p.kv_units) / splits)) return;
   const int row = static_cast<int>(at.row - bh * per_head);

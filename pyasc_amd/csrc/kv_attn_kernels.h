@@ -832,8 +832,8 @@ struct JoinLanes {
   static constexpr int kLanes = D / 8, kMost = 64 / kLanes;
   int64_t row;
   int ch, group, groups;
-  __device__ __forceinline__ explicit JoinLanes(int n_groups) : groups(n_groups) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  __device__ __forceinline__ JoinLanes(uint32_t block, int n_groups) : groups(n_groups) {
+    const int64_t i = static_cast<int64_t>(block) * 256 + threadIdx.x;
     const int64_t all = i / kLanes;
     ch = static_cast<int>(i % kLanes);
     group = static_cast<int>(all & (groups - 1));
@@ -857,7 +857,7 @@ struct JoinLanes {
 // Adds up the splits of a row, relative to the largest reference point.
 template <int D, class E>
 __device__ __forceinline__ void kv_join_body(const KvArgs& p) {
-  const JoinLanes<D> at(p.join_groups);
+  const JoinLanes<D> at(blockIdx.x, p.join_groups);
   const int64_t bh = at.row / p.rows;
   const int row = static_cast<int>(at.row - bh * p.rows);
   Share s;

@@ -196,8 +196,12 @@ struct Tiles {
       for (int w = 0; w < 4; ++w) b[u][w] = E::pack(x[8 * u + 2 * w], x[8 * u + 2 * w + 1]);
   }
 
-  // acc^T (d = 32 db + 8 rq + 4 h + 0..3 of this lane's row) to a row, as values or as fp32 parts.
-  __device__ __forceinline__ void store(const f32x16 (&acc)[kDBlocks], uint16_t* row, float scale, bool zero) const {
+  // acc^T (d = 32 db + 8 rq + 4 h + 0..3 of this lane's row) to rows, as values, through 32 rows of LDS of
+  // this wave: a lane's own 8 bytes of a row at a time would be 32 pieces of 16 bytes per store.  out(r):
+  // where the wave's row r goes, null: nowhere.
+  template <class Out>
+  __device__ __forceinline__ void store(uint8_t* mine, const f32x16 (&acc)[kDBlocks], float scale, bool zero,
+                                        Out out) const {
 #pragma unroll
     for (int db = 0; db < kDBlocks; ++db)
 #pragma unroll
@@ -205,8 +209,17 @@ struct Tiles {
         u32x2 w;
         w[0] = E::pack(acc[db][rq * 4] * scale, acc[db][rq * 4 + 1] * scale);
         w[1] = E::pack(acc[db][rq * 4 + 2] * scale, acc[db][rq * 4 + 3] * scale);
-        *reinterpret_cast<u32x2*>(row + db * 32 + rq * 8 + h * 4) = zero ? u32x2{0, 0} : w;
+        *reinterpret_cast<u32x2*>(mine + tile_off<D>(col, db * 4 + rq) + h * 8) = zero ? u32x2{0, 0} : w;
       }
+    constexpr int kChunks = D / 8;
+#pragma unroll
+    for (int i = 0; i < 32 * kChunks / 64; ++i) {
+      const int at = i * 64 + lane, r = at / kChunks, ch = at % kChunks;
+      uint16_t* row = out(r);
+      if (row != nullptr) {
+        *reinterpret_cast<u32x4*>(row + ch * 8) = *reinterpret_cast<const u32x4*>(mine + tile_off<D>(r, ch));
+      }
+    }
   }
   __device__ __forceinline__ void store_part(const f32x16 (&acc)[kDBlocks], float* row) const {
 #pragma unroll
@@ -232,7 +245,7 @@ struct GradQ {
   static constexpr int kRows = 32 * kWaves;
   static constexpr int kKeys = 64;  // of a tile
 };
-constexpr int kExactTiles = 4;  // up to as many, delta is exact (see grad_q_body)
+constexpr int kExactTiles = 3;  // up to as many, as the ring has stages, delta is exact (see grad_q_body)
 
 template <int D, class E>
 __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
@@ -267,11 +280,8 @@ __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
     t.template load<kKeys>(ring + stage * kTile, kbase, p.ks.seq, j * kKeys, len);
     t.template load<kKeys>(ring + (3 + stage) * kTile, vbase, p.vs.seq, j * kKeys, len);
   };
-  const auto start = [&] {
-    if (begin < end) load(begin, 0);
-    if (begin + 1 < end) load(begin + 1, 1);
-  };
-  start();
+  if (begin < end) load(begin, 0);
+  if (begin + 1 < end) load(begin + 1, 1);
 
   u32x4 q[T::kKSteps], d_o[T::kKSteps];
   t.own_row(at(p.q, p.qs), live, q);
@@ -300,18 +310,20 @@ __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
   const float a = lse == -INFINITY ? INFINITY : lse * p.inv_scale;
   const float neg_l2 = lse == -INFINITY ? -INFINITY : -lse * 1.4426950408889634f;
 
-  // body(tile, block, x, y) for every 32 keys: x the probabilities, y = dP
-  const auto stream = [&](auto body) {
+  // body(tile, x, y) for every 32 keys: x the probabilities, y = dP; loaded: the tiles are in the ring
+  const auto stream = [&](bool loaded, auto body) {
     int c = 0;
     for (int j = begin; j < end; ++j) {
-      // every wave has read the stage that the tile after the next goes to: it was tile j-1's
-      if (j + 1 < end) {
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLoads) : "memory");
-      } else {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      if (!loaded) {
+        // every wave has read the stage that the tile after the next goes to: it was tile j-1's
+        if (j + 1 < end) {
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLoads) : "memory");
+        } else {
+          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        }
+        asm volatile("s_barrier" ::: "memory");
+        if (j + 2 < end) load(j + 2, c == 0 ? 2 : c - 1);
       }
-      asm volatile("s_barrier" ::: "memory");
-      if (j + 2 < end) load(j + 2, c == 0 ? 2 : c - 1);
       const uint32_t kt = fa::lds_addr(ring + c * kTile), vt = fa::lds_addr(ring + (3 + c) * kTile);
 #pragma unroll
       for (int kb = 0; kb < kKeys / 32; ++kb) {
@@ -337,14 +349,11 @@ __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
   // as the sum of p dP in a pass of its own; over many it is left to o.
   if (total <= kExactTiles) {
     delta = 0.f;
-    stream([&](uint32_t, const f32x16& x, const f32x16& y) {
+    stream(false, [&](uint32_t, const f32x16& x, const f32x16& y) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) delta = fmaf(x[r], y[r], delta);
     });
     delta += other_half(delta);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    asm volatile("s_barrier" ::: "memory");  // the first tile goes where another wave may still read
-    start();
   }
 
   f32x16 acc[T::kDBlocks];
@@ -354,16 +363,16 @@ __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
     p.neg_a[row_at] = -a;
     p.neg_d[row_at] = -delta;
   }
-  stream([&](uint32_t kt, f32x16& x, const f32x16& y) {
+  stream(total <= kExactTiles, [&](uint32_t kt, f32x16& x, const f32x16& y) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] *= y[r] - delta;
     u32x4 ds[2];
     T::pack(x, ds);
     t.add_transposed(kt, ds, acc);
   });
-  if (!live) return;
   const float scale = bad ? __builtin_nanf("") : p.scale;
   if (p.q_splits > 1) {
+    if (!live) return;
     const int64_t part = ((static_cast<int64_t>(s.b) * p.kv_heads + s.head) * p.rows + row) * p.q_splits + s.split;
     if (bad) {
 #pragma unroll
@@ -372,7 +381,15 @@ __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
     t.store_part(acc, p.part_q + part * D);
     return;
   }
-  t.store(acc, p.dq + s.b * p.dq_batch + static_cast<int64_t>(head) * p.dq_head + query * p.dq_seq, scale, false);
+  // the rows go where another wave may still read a tile
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  asm volatile("s_barrier" ::: "memory");
+  const int row0 = (s.row0 * kWaves + t.wave) * 32;
+  t.store(ring + t.wave * (32 * D * 2), acc, scale, false, [&](int r) -> uint16_t* {
+    if (row0 + r >= p.rows) return nullptr;
+    const int g = (row0 + r) / p.n_q, query = row0 + r - g * p.n_q;
+    return p.dq + s.b * p.dq_batch + static_cast<int64_t>(s.head * p.group + g) * p.dq_head + query * p.dq_seq;
+  });
 }
 
 template <int D>
@@ -487,9 +504,9 @@ __device__ __forceinline__ void grad_kv_body(const GradArgs& p) {
     t.add_transposed(qt, ds, dk);
     c = c1;
   }
-  if (key >= p.capacity) return;
   const float nan = __builtin_nanf("");
   if (p.kv_splits > 1) {
+    if (key >= p.capacity) return;
     const int64_t part = ((static_cast<int64_t>(s.b) * p.kv_heads + s.head) * p.capacity + key) * p.kv_splits + s.split;
 #pragma unroll
     for (int i = 0; i < T::kDBlocks; ++i) {
@@ -505,8 +522,18 @@ __device__ __forceinline__ void grad_kv_body(const GradArgs& p) {
   }
   // keys behind the length have no part in the results
   const bool zero = !live && !bad;
-  t.store(dk, p.dk + s.b * p.dk_batch + s.head * p.dk_head + key * p.dk_seq, bad ? nan : p.scale, zero);
-  t.store(dv, p.dv + s.b * p.dv_batch + s.head * p.dv_head + key * p.dv_seq, bad ? nan : 1.0f, zero);
+  // the rows go where another wave may still read a tile
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  asm volatile("s_barrier" ::: "memory");
+  uint8_t* mine = ring + t.wave * (32 * D * 2);
+  const auto rows_of = [&](uint16_t* base, int64_t seq) {
+    return [=](int r) -> uint16_t* {
+      const int at = key0 + t.wave * 32 + r;
+      return at < p.capacity ? base + at * seq : nullptr;
+    };
+  };
+  t.store(mine, dk, bad ? nan : p.scale, zero, rows_of(p.dk + s.b * p.dk_batch + s.head * p.dk_head, p.dk_seq));
+  t.store(mine, dv, bad ? nan : 1.0f, zero, rows_of(p.dv + s.b * p.dv_batch + s.head * p.dv_head, p.dv_seq));
 }
 
 // Adds up the parts of rows.  kind 0: dq, 1: dk, 2: dv, in q_join, kv_join and kv_join workgroups of one

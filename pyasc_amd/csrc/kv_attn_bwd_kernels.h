@@ -263,6 +263,7 @@ __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
   const int len = keys_of(p, s.b, bad);
   const int row = (s.row0 * kWaves + t.wave) * 32 + t.col;
   const bool live = row < p.rows;
+  const bool act = (s.row0 * kWaves + t.wave) * 32 < p.rows;  // of the wave; others only load and wait
   const int g = live ? row / p.n_q : 0, query = live ? row - g * p.n_q : 0;
   const uint32_t head = s.head * p.group + g;
   const auto at = [&](const uint8_t* base, const Strides& st) {
@@ -324,7 +325,10 @@ __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
         asm volatile("s_barrier" ::: "memory");
         if (j + 2 < end) load(j + 2, c == 0 ? 2 : c - 1);
       }
-      const uint32_t kt = fa::lds_addr(ring + c * kTile), vt = fa::lds_addr(ring + (3 + c) * kTile);
+      const int at = c;
+      c = c == 2 ? 0 : c + 1;
+      if (!act) continue;
+      const uint32_t kt = fa::lds_addr(ring + at * kTile), vt = fa::lds_addr(ring + (3 + at) * kTile);
 #pragma unroll
       for (int kb = 0; kb < kKeys / 32; ++kb) {
         const uint32_t off = kb * 32 * D * 2;
@@ -340,7 +344,6 @@ __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
         for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], p.scale_log2, neg_l2));
         body(kt + off, x, y);
       }
-      c = c == 2 ? 0 : c + 1;
     }
   };
 
@@ -418,6 +421,7 @@ __device__ __forceinline__ void grad_kv_body(const GradArgs& p) {
   const int key0 = s.row0 * GradKv<D>::kKeys;
   const int key = key0 + t.wave * 32 + t.col;
   const bool live = key < len;
+  const bool act = key0 + t.wave * 32 < len;  // of the wave; others only load and wait
 
   // tiles of rows: every query head of the group, its queries in tiles
   const int per_head = ((kPacked ? p.rows : p.n_q) + kRows - 1) / kRows;
@@ -476,8 +480,11 @@ __device__ __forceinline__ void grad_kv_body(const GradArgs& p) {
     }
     asm volatile("s_barrier" ::: "memory");
     if (j + 2 < end) load(c2);
-    const uint32_t qt = fa::lds_addr(ring + c * kTile), dt = fa::lds_addr(ring + (3 + c) * kTile);
-    const uint32_t vals = fa::lds_addr(reinterpret_cast<const uint8_t*>(values[c])) + t.h * 16;
+    const int at = c;
+    c = c1;
+    if (!act) continue;
+    const uint32_t qt = fa::lds_addr(ring + at * kTile), dt = fa::lds_addr(ring + (3 + at) * kTile);
+    const uint32_t vals = fa::lds_addr(reinterpret_cast<const uint8_t*>(values[at])) + t.h * 16;
     u32x4 ia[4], id[4];  // rows 8 i + 4 h + 0..3
 #pragma unroll
     for (int i = 0; i < 4; ++i) ia[i] = fa::lds_read_b128(vals, i * 32);
@@ -502,7 +509,6 @@ __device__ __forceinline__ void grad_kv_body(const GradArgs& p) {
     T::pack(y, ds);
     t.add_transposed(dt, pb, dv);
     t.add_transposed(qt, ds, dk);
-    c = c1;
   }
   const float nan = __builtin_nanf("");
   if (p.kv_splits > 1) {

@@ -21,8 +21,8 @@
 // parts join_grad adds in order.
 //
 // The matrix units bound both, at the clock that the board's power leaves: 4 sequences, 32 / 8 heads of
-// 128, 2048 queries, 1024 keys, bf16: grad_q (three products) 223 to 240 us, 0.86 to 0.92 PFLOP/s, matrix units
-// busy 40%; grad_kv (four) 271 us, 1.01 PFLOP/s, 47%; join_grad 8 us for each of dk and dv.
+// 128, 2048 queries, 1024 keys, bf16: grad_q (three products) 225 us, 0.92 PFLOP/s, matrix units busy
+// 40%; grad_kv (four) 266 us, 1.03 PFLOP/s, 47%; join_grad 15 us for dk and dv in two parts each (84 MB).
 #pragma once
 
 #include "kv_attn_kernels.h"

@@ -427,3 +427,54 @@ def test_refused_places_and_scales(device):
     want = (do.double().sum(2, keepdim=True) / 8).expand(v.shape)
     # probabilities of 1/8 are exact; sums in fp32, then a rounding
     torch.testing.assert_close(dv.double(), want, rtol=2.0 ** -11 + 2.0 ** -20, atol=1e-6)
+
+
+@pytest.mark.parametrize("seed", range(20))
+def test_random_trees(device, seed):
+    """Caches of any page size or in one piece, ragged lengths, sparse and dense masks, ragged drafts;
+    page numbers behind a sequence's pages are garbage."""
+    r = torch.Generator().manual_seed(seed)
+    g = torch.Generator(device=device).manual_seed(seed)
+
+    def pick(*values):
+        return values[int(torch.randint(len(values), (1,), generator=r))]
+
+    def size(lo, hi):
+        return int(round(math.exp(float(torch.rand(1, generator=r)) * math.log(hi / lo)) * lo))
+
+    dt, D = pick(torch.float16, torch.bfloat16), pick(64, 128)
+    b, hk, group, n = size(1, 6), size(1, 4), pick(1, 2, 4, 8), size(1, 150)
+    page = pick(1, 3, 16, 48, 64, 100, 128, 256)
+    columns = size(1, max(1, 3000 // page))
+    lengths = torch.randint(0, columns * page + 1, (b,), generator=r, dtype=torch.int32)
+    lengths[0] = pick(0, 1, columns * page)
+    drafts = pick(None, torch.randint(0, n + 1, (b,), generator=r, dtype=torch.int32))
+    q, kd, vd = rows((b, hk * group, n, D), dt, g, "bshd"), rows((b, hk, n, D), dt, g, "bshd"), rows((b, hk, n, D), dt, g)
+    kind = pick("chain", "shared", "own")
+    mask = None if kind == "chain" else torch.rand((n, n) if kind == "shared" else (b, n, n), generator=g,
+                                                   device=device) < pick(0.02, 0.5)
+    table = None
+    if pick(True, True, False):
+        pages = b * columns + 3
+        kc, vc = rows((pages, hk, page, D), dt, g), rows((pages, hk, page, D), dt, g, "bshd")
+        table = torch.randperm(pages, generator=r)[:b * columns].view(b, columns).int()
+        keys, values = (x[table.long().to(device)].permute(0, 2, 1, 3, 4).reshape(b, hk, -1, D) for x in (kc, vc))
+        for i in range(b):
+            table[i, -(-int(lengths[i]) // page):] = 2 ** 30
+        table = table.to(device)
+    else:
+        kc, vc = rows((b, hk, columns * page, D), dt, g, "bshd"), rows((b, hk, columns * page, D), dt, g)
+        keys, values = kc, vc
+    o = torch.full_like(q, 7.0)
+    lse = torch.full((b, hk * group, n), 7.0, device=device)
+    kernels.tree_attention(q, kc, vc, lengths.to(device), kd, vd, mask, o, D ** -0.5, block_table=table, lse=lse,
+                           draft_lengths=None if drafts is None else drafts.to(device))
+    chain = torch.ones((n, n), dtype=torch.bool, device=device).tril()
+    for i in range(b):
+        cached, t = int(lengths[i]), n if drafts is None else int(drafts[i])
+        own = (chain if mask is None else mask if mask.dim() == 2 else mask[i])[:t, :t]
+        seen = torch.cat([torch.ones((t, cached), dtype=torch.bool, device=device), own], 1)
+        assert (o[i, :, t:] == 7).all() and (lse[i, :, t:] == 7).all()
+        for j in range(hk * group):
+            k, v = (torch.cat([x[i, j // group, :cached], y[i, j // group, :t]]) for x, y in ((keys, kd), (values, vd)))
+            check(o[i, j, :t], lse[i, j, :t], *attend(q[i, j, :t], k, v, seen, D ** -0.5), dt)

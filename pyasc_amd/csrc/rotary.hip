@@ -128,7 +128,6 @@ template <typename T, int V, bool kInterleaved, Mode kMode>
 __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
   constexpr int kSlots = slots_per_lane<V>();
   __shared__ float2 table[kMaxTokens * kMaxHeadDim / 2];
-  __shared__ float sums[kMode == kNormGrad ? 2 * kMaxHeadDim : 1];
   __shared__ float weights[kMode != kTurn ? 2 * kMaxHeadDim : 1];
 
   const int tid = threadIdx.x;
@@ -381,37 +380,41 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
 
   if (kMode == kNormGrad) {
     // the workgroup's sums: rows of one wave by a butterfly over the lanes above the row's, then
-    // the four waves one after the other, always in the same order
-    const int wave = tid >> 6;
-    for (int i = tid; i < 2 * p.head_dim; i += kThreads) sums[i] = 0.f;
+    // the four waves, always in the same order
+    float* sums = reinterpret_cast<float*>(table);  // [wave][2][head_dim]
+    constexpr int kWaves = kThreads / 64;
+    static_assert(sizeof(table) >= kWaves * 2 * kMaxHeadDim * sizeof(float), "the sums fit the table");
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int i = 0; i < kSlots; ++i)
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            for (int d = p.lanes; d < 64; d <<= 1) dw[t][i][c][e] += __shfl_xor(dw[t][i][c][e], d, 64);
+            for (int d = p.lanes; d < 64; d <<= 1) dw[k][i][c][e] += __shfl_xor(dw[k][i][c][e], d, 64);
           }
-    for (int turn = 0; turn < kThreads / 64; ++turn) {
-      __syncthreads();
-      if (wave != turn || (tid & 63) >= p.lanes) continue;
+    __syncthreads();  // the table's last readers
+    if ((tid & 63) < p.lanes) {
+      float* mine = sums + (tid >> 6) * 2 * p.head_dim;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) {
           if (!live[i]) continue;
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            sums[t * p.head_dim + c0[i] + e] += dw[t][i][0][e];
-            sums[t * p.head_dim + c1[i] + e] += dw[t][i][1][e];
+            mine[k * p.head_dim + c0[i] + e] = dw[k][i][0][e];
+            mine[k * p.head_dim + c1[i] + e] = dw[k][i][1][e];
           }
         }
     }
     __syncthreads();
     for (int i = tid; i < 2 * p.head_dim; i += kThreads) {
-      p.parts[static_cast<int64_t>(blockIdx.x) * 2 * p.head_dim + i] = sums[i];
+      float sum = sums[i];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) sum += sums[w * 2 * p.head_dim + i];
+      p.parts[static_cast<int64_t>(blockIdx.x) * 2 * p.head_dim + i] = sum;
     }
   }
 }
@@ -517,7 +520,8 @@ int32_t check(const asc_rotary_t* a, const char* what, Mode mode) {
 }
 
 // The widest vector (16 bytes at most; four values in a gradient launch, whose two rows in flight and
-// sums would not fit the registers of four waves per SIMD otherwise: 98 us against 46) that
+// sums would not fit the registers of four waves per SIMD otherwise: 127 us against 107 at 4 x 4096 tokens of
+// 32 + 8 heads, bf16) that
 // every row's slots allow: both halves of a pair slot and every stride and address are multiples of it.
 int vector_width(const asc_rotary_t& a, Mode mode) {
   const int64_t size = a.dtype == ASC_DT_FLOAT32 ? 4 : 2;

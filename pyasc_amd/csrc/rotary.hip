@@ -16,7 +16,7 @@
 // row by row, the norm took 74 us where it takes 63).
 //
 // bf16, 4 x 4096 tokens, 32 + 8 heads of 128: positions 60 us (5.6 TB/s), with the norm 63 (5.3), a
-// copy of the same bytes 65; the gradient 107 (4.7), its conversions and sums beside the loads.
+// copy of the same bytes 65; the gradient 105 (4.8), its conversions and sums beside the loads.
 // fp32, half the tokens: 131, 133 and 195 us (5.1 TB/s each).
 #include <type_traits>
 
@@ -217,14 +217,16 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
         h.dy += h.dy_step;
       }
     };
-    // The first rows are asked for ahead of the table, but for the gradient's, whose registers are
-    // full.
-    constexpr bool kAhead = kMode != kNormGrad;
+    // The first rows are asked for ahead of the table; of the gradient's, whose registers are full, the
+    // queries' alone and only in four 16-bit values (8 x 2047 tokens of 32 + 8 heads of 64: 53.4 to 51.3 us).
+    constexpr bool kAhead = kMode != kNormGrad, kQueriesAhead = kAhead || (sizeof(T) == 2 && V == 4);
     Heads heads[2];
     Row first[2];
-    if constexpr (kAhead) {
+    if constexpr (kQueriesAhead) {
       heads[0] = heads_of(std::integral_constant<int, 0>{});
       fetch(heads[0], first[0]);
+    }
+    if constexpr (kAhead) {
       heads[1] = heads_of(std::integral_constant<int, 1>{});
       fetch(heads[1], first[1]);
     }
@@ -363,17 +365,20 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(RotaryArgs p) {
         work(second);
       }
     };
-    if constexpr (kAhead) {
+    const auto fetch_and_work = [&](auto which) {
+      Heads h = heads_of(which);
+      Row m;
+      fetch(h, m);
+      rows_of(which, h, m);
+    };
+    if constexpr (kQueriesAhead) {
       rows_of(std::integral_constant<int, 0>{}, heads[0], first[0]);
+    } else {
+      fetch_and_work(std::integral_constant<int, 0>{});
+    }
+    if constexpr (kAhead) {
       rows_of(std::integral_constant<int, 1>{}, heads[1], first[1]);
     } else {
-      const auto fetch_and_work = [&](auto which) {
-        Heads h = heads_of(which);
-        Row m;
-        fetch(h, m);
-        rows_of(which, h, m);
-      };
-      fetch_and_work(std::integral_constant<int, 0>{});
       fetch_and_work(std::integral_constant<int, 1>{});
     }
   }
@@ -520,7 +525,7 @@ int32_t check(const asc_rotary_t* a, const char* what, Mode mode) {
 }
 
 // The widest vector (16 bytes at most; four values in a gradient launch, whose two rows in flight and
-// sums would not fit the registers of four waves per SIMD otherwise: 127 us against 107 at 4 x 4096 tokens of
+// sums would not fit the registers of four waves per SIMD otherwise: 127 us against 105 at 4 x 4096 tokens of
 // 32 + 8 heads, bf16) that
 // every row's slots allow: both halves of a pair slot and every stride and address are multiples of it.
 int vector_width(const asc_rotary_t& a, Mode mode) {

@@ -526,6 +526,18 @@ int32_t asc_cross_attention_fwd(const asc_attention_t* args, void* workspace,
 int64_t asc_tree_attention_workspace(const asc_attention_t* args);
 int32_t asc_tree_attention(const asc_attention_t* args, void* workspace,
                            int64_t workspace_bytes, asc_stream_t stream);
+/* The launch that asc_cross_attention_fwd (tree 0) or asc_tree_attention makes with
+ * these arguments: kv_wide, whose workgroups stream the keys once for up to 128 (head_dim
+ * 64) or 256 rows, or kv_narrow, up to 32 rows; a row is a query of one of the heads that
+ * share a key / value head.  More than one split: kv_join adds the parts up.  Same checks
+ * and errors. */
+typedef struct asc_attention_plan {
+  char kernel[16]; /* NUL-terminated; empty when there is nothing to launch */
+  int32_t row_blocks; /* workgroups over the rows of one key / value head */
+  int32_t splits;     /* and over the keys of one sequence */
+} asc_attention_plan_t;
+int32_t asc_attention_plan(const asc_attention_t* args, int32_t tree,
+                           asc_attention_plan_t* plan);
 /* The gradients of asc_cross_attention_fwd from q, k, v, its o and lse, and the
  * gradient d_o of o: dq, dk and dv, the latter two summed over the query heads that
  * share a key / value head, in a fixed order; zeros behind a sequence's keys.  The

@@ -76,6 +76,11 @@ class AttentionArgs(ctypes.Structure):
                 ("mask_row_stride", _c_i64), ("d_o", Rows), ("dq", Rows), ("dk", Rows), ("dv", Rows)]
 
 
+class AttentionPlan(ctypes.Structure):
+    """asc_attention_plan_t: the launch of an attention entry over other keys than the queries' own."""
+    _fields_ = [("kernel", ctypes.c_char * 16), ("row_blocks", _c_i32), ("splits", _c_i32)]
+
+
 # name -> argtypes; every entry point returns int32_t (asc_reduce_f32_workspace a byte
 # count, the others a status), those of INT64_FUNCS an int64_t byte count.
 SIGNATURES = {
@@ -133,6 +138,7 @@ SIGNATURES = {
     "asc_cross_attention_bwd": [_c_p, _c_p, _c_i64, _c_p],
     "asc_tree_attention_workspace": [_c_p],
     "asc_tree_attention": [_c_p, _c_p, _c_i64, _c_p],
+    "asc_attention_plan": [_c_p, _c_i32, ctypes.POINTER(AttentionPlan)],
     "asc_unary_f32": [_c_i32, _c_p, _c_p, _c_i64, _c_p],
     "asc_binary": [_c_i32, _c_i32, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_f64, _c_i64, _c_p],
     "asc_where_cmp": [_c_i32, _c_i32, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_f64, _c_i64, _c_f64, _c_f64, _c_p],

@@ -3,6 +3,7 @@
 // it).  The device code is kv_attn_kernels.h; here are the checks, the choice of the kernel and of
 // the split of the keys, and the workspace of the splits.
 #include <cmath>
+#include <cstdio>
 
 #include "kv_attn_host.h"
 #include "kv_attn_kernels.h"
@@ -270,4 +271,15 @@ extern "C" int64_t asc_tree_attention_workspace(const asc_attention_t* args) {
 }
 extern "C" int32_t asc_tree_attention(const asc_attention_t* args, void* ws, int64_t ws_bytes, asc_stream_t stream) {
   return run(args, true, "asc_tree_attention", ws, ws_bytes, stream);
+}
+extern "C" int32_t asc_attention_plan(const asc_attention_t* args, int32_t tree, asc_attention_plan_t* plan) {
+  ASC_REQUIRE(plan, ASC_ERR_INVALID_ARG, "asc_attention_plan: null plan");
+  *plan = asc_attention_plan_t{};
+  Launch L;
+  const int32_t rc = make(args, tree != 0, "asc_attention_plan", L);
+  if (rc != ASC_OK || L.blocks == 0) return rc;
+  snprintf(plan->kernel, sizeof(plan->kernel), "%s", L.wide ? "kv_wide" : "kv_narrow");
+  plan->row_blocks = L.p.row_blocks;
+  plan->splits = L.p.splits;
+  return ASC_OK;
 }

@@ -541,8 +541,8 @@ int32_t asc_attention_plan(const asc_attention_t* args, int32_t tree,
 /* The gradients of asc_cross_attention_fwd from q, k, v, its o and lse, and the
  * gradient d_o of o: dq, dk and dv, the latter two summed over the query heads that
  * share a key / value head, in a fixed order; zeros behind a sequence's keys.  The
- * probabilities and the scores' gradients are rounded to the type for their products,
- * as those of the forward pass are. */
+ * probabilities and the scores' gradients are rounded to the type's precision for their
+ * products, as those of the forward pass are, not to its range. */
 int64_t asc_cross_attention_bwd_workspace(const asc_attention_t* args);
 int32_t asc_cross_attention_bwd(const asc_attention_t* args, void* workspace,
                                 int64_t workspace_bytes, asc_stream_t stream);

@@ -894,8 +894,9 @@ def cross_attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: t
     """The gradients of cross_attention_fwd: from the gradient ``do`` of o, its inputs and its o and
     lse, the gradients of q, k and v.  dk and dv are summed over the query heads that share a key /
     value head, in a fixed order, and are zeros behind a sequence's keys.  The probabilities and the
-    scores' gradients are rounded to the inputs' type for their products; in float16 those below
-    2^-14 lose bits, so small gradients want a scaled loss."""
+    scores' gradients are rounded to the inputs' type for their products: to its precision, whatever
+    their size (in float16 they are held at powers of two that move with the largest of a row or key),
+    but the gradients themselves end at the type's smallest value."""
     device = _current_device()
     q_rows, o_rows, k_rows, v_rows = _kv_rows(q, k, v, o, sm_scale, device, ("k", "v"), written=False)
     dtype, shape = q.dtype, q.shape

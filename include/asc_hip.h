@@ -462,7 +462,9 @@ typedef struct asc_rows {
  *                       `workspace` holds asc_qk_norm_rotary_bwd_workspace bytes.
  * dtype: ASC_DT_FLOAT32 / FLOAT16 / BFLOAT16; computed in fp32, one rounding per
  * value.  head_dim even and at most 512.  k_heads (or q_heads) may be 0.  A result
- * may lie in place of an input with the same strides, and nowhere else over one. */
+ * may lie in place of its own input with the same strides (dq over q or dq_out too);
+ * one that shares a byte with another operand or result is refused
+ * (ASC_ERR_INVALID_ARG), views that interleave are not. */
 typedef struct asc_rotary {
   int32_t dtype, head_dim, rotary_dim, interleaved, backward;
   int32_t positions_int64; /* positions are int64_t (else int32_t) */
@@ -504,6 +506,8 @@ int32_t asc_qk_norm_rotary_bwd(const asc_rotary_t* args, void* workspace,
  *                          written.
  * A length outside the cache, or a page outside it that a length reaches, is not
  * followed: the sequence's results are NaN.
+ * A result that shares a byte with an operand or another result is refused
+ * (ASC_ERR_INVALID_ARG).
  * `workspace` holds the entry's _workspace bytes, 16-byte aligned (0: NULL allowed). */
 typedef struct asc_attention {
   int32_t dtype, head_dim;

@@ -161,6 +161,33 @@ int32_t make(const asc_attention_t* a, bool tree, const char* what, Launch& L) {
   return ASC_OK;
 }
 
+int32_t check_places(const asc_attention_t& a, bool tree, const char* what) {
+  const bool paged = tree && a.block_table != nullptr && a.kv_len > 0;
+  const auto rows = [&](const char* name, const asc_rows_t& r, int64_t batch, int64_t heads, int64_t length) {
+    return asc::region_of(name, r, batch, heads, length, a.head_dim, 2);
+  };
+  const int64_t kv_batch = paged ? a.num_pages : a.batch, kv_rows = paged ? a.page_size : a.kv_len;
+  const asc_rows_t none{};
+  const asc_rows_t table{const_cast<int32_t*>(paged ? a.block_table : nullptr), a.table_stride, 0, 0};
+  const asc_rows_t mask{const_cast<uint8_t*>(tree ? a.tree_mask : nullptr), a.mask_batch_stride, 0, a.mask_row_stride};
+  const int64_t lengths = a.batch * static_cast<int64_t>(sizeof(int32_t));
+  const asc::Region results[] = {
+      rows("o", a.o, a.batch, a.q_heads, a.q_len),
+      asc::region_of("lse", a.lse, a.batch * a.q_heads * a.q_len * static_cast<int64_t>(sizeof(float)))};
+  const asc::Region operands[] = {
+      rows("q", a.q, a.batch, a.q_heads, a.q_len),
+      rows("k", a.k, kv_batch, a.kv_heads, kv_rows),
+      rows("v", a.v, kv_batch, a.kv_heads, kv_rows),
+      rows("k_draft", tree ? a.k_draft : none, a.batch, a.kv_heads, a.q_len),
+      rows("v_draft", tree ? a.v_draft : none, a.batch, a.kv_heads, a.q_len),
+      asc::region_of("kv_lengths", a.kv_lengths, lengths),
+      asc::region_of("draft_lengths", tree ? a.draft_lengths : nullptr, lengths),
+      asc::region_of("block_table", table, a.batch, 1, 1, paged ? asc::ceil_div(a.kv_len, a.page_size) : 0,
+                     sizeof(int32_t)),
+      asc::region_of("tree_mask", mask, a.batch, 1, a.q_len, a.q_len, 1)};
+  return asc::kv::check_places(what, results, operands);
+}
+
 template <int D, class E>
 void launch(const Launch& L, bool tree, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(L.blocks));
@@ -180,11 +207,13 @@ void launch(const Launch& L, bool tree, hipStream_t stream) {
 int32_t run(const asc_attention_t* a, bool tree, const char* what, void* workspace, int64_t workspace_bytes,
             asc_stream_t stream) {
   Launch L;
-  const int32_t rc = make(a, tree, what, L);
+  int32_t rc = make(a, tree, what, L);
   if (rc != ASC_OK || L.blocks == 0) return rc;
   const int64_t need = workspace_of(L, a->head_dim);
   ASC_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && asc::aligned16(workspace)), ASC_ERR_INVALID_ARG,
               "%s: the workspace must hold %lld bytes, 16-byte aligned", what, static_cast<long long>(need));
+  rc = check_places(*a, tree, what);
+  if (rc != ASC_OK) return rc;
   if (need != 0) {
     L.p.part_o = static_cast<float*>(workspace);
     L.p.part_ml = L.p.part_o + L.p.units * static_cast<int64_t>(L.p.rows) * a->head_dim;

@@ -141,6 +141,18 @@ int32_t make(const asc_attention_t* a, const char* what, Launch& L) {
   return ASC_OK;
 }
 
+int32_t check_places(const asc_attention_t& a, const char* what) {
+  const auto rows = [&](const char* name, const asc_rows_t& r, bool q) {
+    return asc::region_of(name, r, a.batch, q ? a.q_heads : a.kv_heads, q ? a.q_len : a.kv_len, a.head_dim, 2);
+  };
+  const asc::Region results[] = {rows("dq", a.dq, true), rows("dk", a.dk, false), rows("dv", a.dv, false)};
+  const asc::Region operands[] = {
+      rows("do", a.d_o, true), rows("q", a.q, true), rows("k", a.k, false), rows("v", a.v, false), rows("o", a.o, true),
+      asc::region_of("lse", a.lse, a.batch * a.q_heads * a.q_len * static_cast<int64_t>(sizeof(float))),
+      asc::region_of("kv_lengths", a.kv_lengths, a.batch * static_cast<int64_t>(sizeof(int32_t)))};
+  return asc::kv::check_places(what, results, operands);
+}
+
 template <int D, class E>
 int32_t launch(const Launch& L, const char* what, hipStream_t stream) {
   const auto grid = [](int64_t n) { return dim3(static_cast<uint32_t>(n)); };
@@ -171,11 +183,13 @@ extern "C" int32_t asc_cross_attention_bwd(const asc_attention_t* args, void* wo
                                            asc_stream_t stream) {
   const char* what = "asc_cross_attention_bwd";
   Launch L;
-  const int32_t rc = make(args, what, L);
+  int32_t rc = make(args, what, L);
   if (rc != ASC_OK || !L.keys) return rc;
   const int64_t need = workspace_of(L);
   ASC_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && asc::aligned16(workspace)), ASC_ERR_INVALID_ARG,
               "%s: the workspace must hold %lld bytes, 16-byte aligned", what, static_cast<long long>(need));
+  rc = check_places(*args, what);
+  if (rc != ASC_OK) return rc;
   float* at = static_cast<float*>(workspace);
   const auto take = [&at](int64_t n) {
     float* r = at;

@@ -3,6 +3,7 @@
 
 #include "common.h"
 #include "kv_attn_kernels.h"
+#include "overlap.h"
 
 namespace asc {
 namespace kv {
@@ -16,6 +17,21 @@ int32_t strides_of(const asc_rows_t& r, int64_t batch, int64_t heads, int64_t ro
 
 // Whether rows can be read and written in 16-byte pieces.
 bool row_operand(const asc_rows_t& r);
+
+// Every result shares no byte with an operand nor with another result.
+template <int kResults, int kOperands>
+int32_t check_places(const char* what, const Region (&results)[kResults], const Region (&operands)[kOperands]) {
+  for (int i = 0; i < kResults; ++i) {
+    for (const Region& x : operands) {
+      ASC_REQUIRE(!overlap(results[i], x), ASC_ERR_INVALID_ARG, "%s: '%s' overlaps '%s'", what, results[i].name, x.name);
+    }
+    for (int j = 0; j < i; ++j) {
+      ASC_REQUIRE(!overlap(results[i], results[j]), ASC_ERR_INVALID_ARG, "%s: '%s' overlaps '%s'", what,
+                  results[i].name, results[j].name);
+    }
+  }
+  return ASC_OK;
+}
 
 }  // namespace kv
 }  // namespace asc

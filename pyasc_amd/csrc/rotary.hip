@@ -22,6 +22,7 @@
 
 #include "common.h"
 #include "numeric.h"
+#include "overlap.h"
 
 namespace {
 
@@ -524,6 +525,47 @@ int32_t check(const asc_rotary_t* a, const char* what, Mode mode) {
   return ASC_OK;
 }
 
+// A result may lie in place of its own input, row by row (a lane reads its values of a row before it
+// writes them), and shares no byte with another operand or result.
+int32_t check_places(const asc_rotary_t& a, const char* what, Mode mode) {
+  const int64_t element = a.dtype == ASC_DT_FLOAT32 ? 4 : 2, weight = a.head_dim * static_cast<int64_t>(sizeof(float));
+  const auto rows = [&](const char* name, const asc_rows_t& r, bool key) {
+    return asc::region_of(name, r, a.batch, key ? a.k_heads : a.q_heads, a.seq, a.head_dim, element);
+  };
+  const bool grad = mode == kNormGrad;
+  const asc_rows_t none{};
+  const asc::Region results[] = {rows(grad ? "dq" : "q_out", a.q_out, false), rows(grad ? "dk" : "k_out", a.k_out, true)};
+  const asc::Region of_q[] = {rows("q", a.q, false), rows("dq_out", grad ? a.dq_out : none, false)};
+  const asc::Region of_k[] = {rows("k", a.k, true), rows("dk_out", grad ? a.dk_out : none, true)};
+  const int64_t position = a.positions_int64 ? 8 : 4;
+  const asc_rows_t at{const_cast<void*>(a.rotary_dim ? a.positions : nullptr), a.position_batch_stride, 0,
+                      a.position_seq_stride};
+  const asc::Region shared[] = {
+      asc::region_of("positions", at, a.batch, 1, a.seq, 1, position),
+      asc::region_of("freqs", a.freqs, a.rotary_dim / 2 * 8),
+      asc::region_of("q_weight", mode != kTurn && a.q_heads ? a.q_weight : nullptr, weight),
+      asc::region_of("k_weight", mode != kTurn && a.k_heads ? a.k_weight : nullptr, weight)};
+  const auto apart = [&](const asc::Region& result, const asc::Region& other) {
+    ASC_REQUIRE(!asc::overlap(result, other), ASC_ERR_INVALID_ARG, "%s: '%s' overlaps '%s'", what, result.name,
+                other.name);
+    return static_cast<int32_t>(ASC_OK);
+  };
+  int32_t rc = ASC_OK;
+  for (int t = 0; t < 2; ++t) {
+    const asc::Region& result = results[t];
+    for (const asc::Region& x : t ? of_k : of_q) {
+      if (!asc::same_place(result, x) && (rc = apart(result, x)) != ASC_OK) return rc;
+    }
+    for (const asc::Region& x : t ? of_q : of_k) {
+      if ((rc = apart(result, x)) != ASC_OK) return rc;
+    }
+    for (const asc::Region& x : shared) {
+      if ((rc = apart(result, x)) != ASC_OK) return rc;
+    }
+  }
+  return apart(results[0], results[1]);
+}
+
 // The widest vector (16 bytes at most; four values in a gradient launch, whose two rows in flight and
 // sums would not fit the registers of four waves per SIMD otherwise: 127 us against 105 at 4 x 4096 tokens of
 // 32 + 8 heads, bf16) that
@@ -549,6 +591,8 @@ void sum_weights(const asc_rotary_t& a, const float* parts, int n_parts, hipStre
 }
 
 int32_t run(const asc_rotary_t* a, const char* what, Mode mode, float* parts, asc_stream_t stream) {
+  const int32_t places = check_places(*a, what, mode);
+  if (places != ASC_OK) return places;
   RotaryArgs p{};
   const auto rows = [](const asc_rows_t& r) { return Rows{r.data, r.batch_stride, r.head_stride, r.seq_stride}; };
   p.x[0] = rows(a->q);

@@ -656,6 +656,15 @@ def _vector(t: torch.Tensor, name: str, dtype: torch.dtype, device: int, shape: 
     return t.data_ptr()
 
 
+def _launch(entry: str, *args: Any) -> None:
+    """Calls an entry; what is left for it to refuse of a call's arguments is an error of their values."""
+    code = getattr(_native._lib or _native.load_library(), entry)(*args)
+    if code == _native.ERR_INVALID_ARG:
+        raise ValueError(_native.last_error())
+    if code != 0:
+        _native.check(code, entry)
+
+
 def _with_workspace(entry: str, args: bytes, device: torch.device, stream: Any) -> None:
     """Calls an entry with the workspace that it asks for, from the launch stream's pool as
     workspace_on's.  Under a capture that torch does not know of the workspace would go to others
@@ -663,7 +672,7 @@ def _with_workspace(entry: str, args: bytes, device: torch.device, stream: Any) 
     handle = _stream(stream)
     nbytes = getattr(_native.load_library(), entry + "_workspace")(args)
     if nbytes == 0:
-        _native.call(entry, args, 0, 0, handle)
+        _launch(entry, args, 0, 0, handle)
         return
     if handle == _native.current_stream_handle(device.index):
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
@@ -674,7 +683,7 @@ def _with_workspace(entry: str, args: bytes, device: torch.device, stream: Any) 
             usable = not torch.cuda.is_current_stream_capturing() or _held_by_a_graph(workspace)
     if not usable:
         raise RuntimeError(f"{entry} needs a workspace: capture it with torch.cuda.graph")
-    _native.call(entry, args, workspace.data_ptr(), nbytes, handle)
+    _launch(entry, args, workspace.data_ptr(), nbytes, handle)
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
@@ -800,8 +809,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     multiplied by ``magnitude``; the other columns are copied.  ``backward`` gives the gradient:
     the turn the other way.  A result may lie in place of its input."""
     device = _current_device()
-    _native.call("asc_rotary", _rotary_args(q, k, positions, freqs, q_out, k_out, interleaved, magnitude, device,
-                                            backward), _stream(stream))
+    _launch("asc_rotary", _rotary_args(q, k, positions, freqs, q_out, k_out, interleaved, magnitude, device, backward),
+            _stream(stream))
 
 
 def qk_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: torch.Tensor,
@@ -811,8 +820,8 @@ def qk_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: torch.T
     """rotary after an RMS norm of each head: x / sqrt(mean(x^2) + epsilon) * weight, the weights
     float32 [head_dim]."""
     device = _current_device()
-    _native.call("asc_qk_norm_rotary", _rotary_args(q, k, positions, freqs, q_out, k_out, interleaved, magnitude,
-                                                    device, False, epsilon, (q_weight, k_weight)), _stream(stream))
+    _launch("asc_qk_norm_rotary", _rotary_args(q, k, positions, freqs, q_out, k_out, interleaved, magnitude, device, False,
+                                               epsilon, (q_weight, k_weight)), _stream(stream))
 
 
 def qk_norm_rotary_bwd(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q: torch.Tensor,

@@ -526,7 +526,8 @@ int32_t check(const asc_rotary_t* a, const char* what, Mode mode) {
 }
 
 // A result may lie in place of its own input, row by row (a lane reads its values of a row before it
-// writes them), and shares no byte with another operand or result.
+// writes them), and shares no byte with another operand or result.  The weights' gradients are written by a
+// launch of their own behind the one that reads the operands, so only other results are in their way.
 int32_t check_places(const asc_rotary_t& a, const char* what, Mode mode) {
   const int64_t element = a.dtype == ASC_DT_FLOAT32 ? 4 : 2, weight = a.head_dim * static_cast<int64_t>(sizeof(float));
   const auto rows = [&](const char* name, const asc_rows_t& r, bool key) {
@@ -545,6 +546,8 @@ int32_t check_places(const asc_rotary_t& a, const char* what, Mode mode) {
       asc::region_of("freqs", a.freqs, a.rotary_dim / 2 * 8),
       asc::region_of("q_weight", mode != kTurn && a.q_heads ? a.q_weight : nullptr, weight),
       asc::region_of("k_weight", mode != kTurn && a.k_heads ? a.k_weight : nullptr, weight)};
+  const asc::Region sums[] = {asc::region_of("dq_weight", grad ? a.dq_weight : nullptr, weight),
+                              asc::region_of("dk_weight", grad ? a.dk_weight : nullptr, weight)};
   const auto apart = [&](const asc::Region& result, const asc::Region& other) {
     ASC_REQUIRE(!asc::overlap(result, other), ASC_ERR_INVALID_ARG, "%s: '%s' overlaps '%s'", what, result.name,
                 other.name);
@@ -562,8 +565,12 @@ int32_t check_places(const asc_rotary_t& a, const char* what, Mode mode) {
     for (const asc::Region& x : shared) {
       if ((rc = apart(result, x)) != ASC_OK) return rc;
     }
+    for (const asc::Region& x : sums) {
+      if ((rc = apart(result, x)) != ASC_OK) return rc;
+    }
   }
-  return apart(results[0], results[1]);
+  if ((rc = apart(results[0], results[1])) != ASC_OK) return rc;
+  return apart(sums[0], sums[1]);
 }
 
 // The widest vector (16 bytes at most; four values in a gradient launch, whose two rows in flight and
@@ -688,6 +695,8 @@ extern "C" int32_t asc_qk_norm_rotary_bwd(const asc_rotary_t* args, void* worksp
   if (rc != ASC_OK) return rc;
   if (empty(*args)) {  // no rows: the weights' gradients are zeros
     if (args->dq_weight == nullptr && args->dk_weight == nullptr) return ASC_OK;
+    const int32_t places = check_places(*args, "asc_qk_norm_rotary_bwd", kNormGrad);
+    if (places != ASC_OK) return places;
     sum_weights(*args, nullptr, 0, static_cast<hipStream_t>(stream));
     return asc::check_launch("asc_qk_norm_rotary_bwd");
   }

@@ -95,6 +95,11 @@ def test_refused(device):
         with pytest.raises(ValueError, match="'q_out' overlaps 'k_out'"):
             kernels.rotary(apart, apart, positions, freqs, rows(0), rows(at))
     kernels.rotary(rows(0), None, positions, freqs, rows(n), None)  # next to each other
+    dw = torch.zeros(127, device=device)
+    for first, second in ((w, w), (dw[:64], dw[63:])):
+        with pytest.raises(ValueError, match="'dq_weight' overlaps 'dk_weight'"):
+            kernels.qk_norm_rotary_bwd(apart, apart.clone(), rows(0), rows(n), w, w, positions, freqs, rows(2 * n),
+                                       rows(3 * n), first, second, 1e-6)
 
     q, k, v, do = (torch.zeros((2, 2, 9, 64), device=device).bfloat16() for _ in range(4))
     lse, lengths = torch.zeros((2, 2, 9), device=device), torch.full((2,), 9, dtype=torch.int32, device=device)

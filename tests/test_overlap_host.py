@@ -80,6 +80,16 @@ def test_rotary_gradients():
     a = rotary_args()
     a.k_out.data = a.dq_out.data + Q_BYTES - 2
     refused(entry, a, "dk", "dq_out", *more)
+    for shift in (0, 4, -252):  # the weights' gradients, of one norm for queries and keys or next to each other
+        a = rotary_args()
+        a.dk_weight = a.dq_weight + shift
+        refused(entry, a, "dq_weight", "dk_weight", *more)
+    a = rotary_args()
+    a.dq_weight = a.k_out.data + K_BYTES - 4
+    refused(entry, a, "dk", "dq_weight", *more)
+    a = rotary_args()  # no rows: the weights' gradients are still written
+    a.seq, a.dk_weight = 0, a.dq_weight
+    refused(entry, a, "dq_weight", "dk_weight", *more)
 
 
 def attention_args():

@@ -503,7 +503,8 @@ int32_t asc_qk_norm_rotary_bwd(const asc_rotary_t* args, void* workspace,
  *                          drafted key j (of q_len) where tree_mask[b][query][j] is not
  *                          0 (NULL: j <= query).  draft_lengths (may be NULL): drafted
  *                          tokens of sequence b; the queries behind them are not
- *                          written.
+ *                          written: none of a negative number (more than q_len:
+ *                          NaN, as other lengths that do not fit).
  * A length outside the cache, or a page outside it that a length reaches, is not
  * followed: the sequence's results are NaN.
  * A result that shares a byte with an operand or another result is refused

@@ -410,7 +410,8 @@ __device__ __forceinline__ bool out_row(const KvArgs& p, const Share& s, int row
   return true;
 }
 
-// Queries of sequence b that are written: those behind its drafted tokens are left as they were.
+// Queries of sequence b that are written: those behind its drafted tokens are left as they were (all, where
+// their number is negative; one above n_q leaves none, and they are NaN).
 __device__ __forceinline__ int written_of(const KvArgs& p, int b) {
   return p.k_draft && p.draft_lengths ? p.draft_lengths[b] : p.n_q;
 }

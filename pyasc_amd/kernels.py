@@ -943,11 +943,11 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     - k_draft, v_draft: [batch, kv_heads, n, head_dim], not in the cache yet.  tree_mask (bool
       [n, n] or [batch, n, n]): whether token i attends token j (its ancestors and itself); None: a
       chain, j <= i.  draft_lengths (int32 [batch]): tokens of each sequence, default n; the rows of
-      o and lse behind them are left as they were.
+      o and lse behind them are left as they were, all of them where the number is negative.
 
     Strides and the last dimension as in cross_attention_fwd.  A token that attends nothing gets zeros
-    and an lse of -inf.  A length outside the cache, or a page outside it that a length reaches, is
-    not followed: the sequence's results are NaN."""
+    and an lse of -inf.  A length outside the cache, a page outside it that a length reaches, or a
+    number of drafted tokens above n is not followed: the sequence's results are NaN."""
     device = _current_device()
     q_rows, o_rows, k_rows, v_rows = _kv_rows(q, k_cache, v_cache, o, sm_scale, device, ("k_cache", "v_cache"),
                                               pages=block_table is not None)

@@ -166,7 +166,6 @@ __device__ __forceinline__ float other_half(float v) {
 // fa_fwd_body does.
 template <int D, int kWaves, int QB, class E = Bf16, bool kXor = false>
 struct FaState {
-  using Element = E;
   static constexpr int kQ = 32 * QB;              // queries per wave
   static constexpr int kChunks = D / 8;           // 16-byte chunks per row
   static constexpr int kTileBytes = BKV * D * 2;  // one K or V tile

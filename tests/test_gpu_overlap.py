@@ -44,6 +44,19 @@ def test_a_projection_in_place(device, b, s, hq, hk):
     assert torch.equal(dws[0], dws[2]) and torch.equal(dws[1], dws[3])
 
 
+def test_weights_gradients_in_place_of_the_weights(device):
+    g = torch.Generator(device=device).manual_seed(1)
+    _, (q, k) = fused(g, 3, 300, (4, 2), 64)
+    _, (dq, dk) = fused(g, 3, 300, (4, 2), 64)
+    freqs, _ = kernels.rotary_frequencies(64)
+    positions = torch.arange(300, device=device)
+    w = [torch.rand(64, generator=g, device=device) for _ in range(2)]
+    outs = [torch.empty_like(t) for t in (q, k, *w, q, k)]
+    kernels.qk_norm_rotary_bwd(dq, dk, q, k, *w, positions, freqs, *outs[:4], 1e-6)
+    kernels.qk_norm_rotary_bwd(dq, dk, q, k, *w, positions, freqs, *outs[4:], *w, 1e-6)
+    assert all(torch.equal(a, b) for a, b in zip(outs[:4], outs[4:] + w))
+
+
 def test_the_two_halves_of_a_head(device):
     """Rows of 64 of every 128 values: the result in the other half of the same rows."""
     g = torch.Generator(device=device).manual_seed(2)

@@ -1,8 +1,8 @@
 """Socket power and graphics clock of the bench workloads on one MI355X -> profiles/power_clock.md.
 
-    python profile_power.py [--out profiles/power_clock.md]
+    python profile_power.py [--out profiles/power_clock.md] [--attention]
 
-Needs the GPU and ``amd-smi``.  Two parts, both sampled with bench.PowerSampler
+Needs the GPU and ``amd-smi``.  Three parts (``--attention``: the third alone, in place of the file's), all sampled with bench.PowerSampler
 (``amd-smi metric -p -c -g 0`` about every 0.4 s; median of the samples after the first
 two):
 
@@ -13,6 +13,8 @@ two):
 2. The same GEMM kernels on one round of 128 output tiles (half of the 256 CUs busy) and
    on one round of 256 tiles (all CUs), launched back to back for three seconds each:
    whether a round's time follows the clock the card settles at.
+3. Attention over other keys than the queries' own, forward and gradients, launched back
+   to back for four seconds each: whether the board's power sets their clock.
 """
 from __future__ import annotations
 
@@ -32,6 +34,12 @@ ROUNDS = [  # (dtype, M, N, K): 128 tiles of 256x256 (half the CUs), then 256 (a
     ("int8", 2048, 4096, 4096), ("int8", 4096, 4096, 4096),
     ("int8", 2048, 4096, 16384), ("int8", 4096, 4096, 16384),
     ("bf16", 2048, 4096, 8192), ("bf16", 4096, 4096, 8192),
+]
+
+
+ATTENTION = [  # batch, query and key / value heads, queries, keys, head_dim, gradients
+    (4, 32, 32, 4096, 2048, 128, False), (4, 32, 8, 2048, 1024, 128, False), (4, 32, 8, 2048, 1024, 128, True),
+    (4, 32, 8, 2048, 1024, 64, True), (4, 32, 32, 4096, 2048, 128, True),
 ]
 
 
@@ -60,6 +68,28 @@ def workloads(dev) -> list:
     return rows
 
 
+def _timed(fn, secs: float) -> tuple:
+    """us per call of calls back to back, and the sampler's summary."""
+    import torch
+    for _ in range(5):
+        fn()
+    torch.cuda.synchronize()
+    s = bench.PowerSampler()
+    s.start()
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    n, t_end = 0, time.time() + secs
+    e0.record()
+    while time.time() < t_end:
+        for _ in range(50):
+            fn()
+        n += 50
+        torch.cuda.synchronize()
+    e1.record()
+    torch.cuda.synchronize()
+    s.stop()
+    return e0.elapsed_time(e1) * 1e3 / n, s.summary()
+
+
 def rounds(dev, secs: float = 3.0) -> list:
     import torch
     from pyasc_amd import kernels
@@ -81,24 +111,7 @@ def rounds(dev, secs: float = 3.0) -> list:
 
             def fn():
                 kernels.matmul(a, b, c)
-        for _ in range(5):
-            fn()
-        torch.cuda.synchronize()
-        s = bench.PowerSampler()
-        s.start()
-        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-        n, t_end = 0, time.time() + secs
-        e0.record()
-        while time.time() < t_end:
-            for _ in range(50):
-                fn()
-            n += 50
-            torch.cuda.synchronize()
-        e1.record()
-        torch.cuda.synchronize()
-        s.stop()
-        p = s.summary()
-        us = e0.elapsed_time(e1) * 1e3 / n
+        us, p = _timed(fn, secs)
         mhz = p.get("gfx_mhz_median")
         k_tiles = K // (64 if dtype == "int8" else 32)
         rows.append({"dtype": dtype, "M": M, "N": N, "K": K, "tiles": (M // 256) * (N // 256), "us": us,
@@ -108,6 +121,55 @@ def rounds(dev, secs: float = 3.0) -> list:
               flush=True)
         del a, b, c
     return rows
+
+
+def attention(dev, secs: float = 4.0) -> list:
+    import torch
+    from pyasc_amd import kernels
+    g = torch.Generator(device=dev).manual_seed(3)
+    rows = []
+    for batch, hq, hk, sq, sk, d, grad in ATTENTION:
+        q, k, v, do = (torch.randn((batch, h, s, d), generator=g, device=dev).bfloat16()
+                       for h, s in ((hq, sq), (hk, sk), (hk, sk), (hq, sq)))
+        o, lse = torch.empty_like(q), torch.empty((batch, hq, sq), device=dev)
+        grads = [torch.empty_like(t) for t in (q, k, v)]
+        kernels.cross_attention_fwd(q, k, v, o, d ** -0.5, lse=lse)
+
+        def fn():
+            if grad:
+                kernels.cross_attention_bwd(do, q, k, v, o, lse, *grads, d ** -0.5)
+            else:
+                kernels.cross_attention_fwd(q, k, v, o, d ** -0.5, lse=lse)
+        us, p = _timed(fn, secs)
+        products = 7 if grad else 2  # each gradient kernel takes s and dP again
+        tflops = 2 * products * batch * hq * sq * sk * d / us * 1e-6
+        name = f"{'gradients' if grad else 'forward'}, {batch}x{hq}/{hk} heads of {d}, {sq} x {sk}"
+        rows.append({"name": name, "us": us, "tflops": tflops, "power": p})
+        print(f"power: {name} {us:.1f} us {tflops:.0f} TFLOP/s {p.get('socket_w_median')} W "
+              f"{p.get('gfx_mhz_median')} MHz", file=sys.stderr, flush=True)
+    return rows
+
+
+def write_attention(path: str, rows: list) -> None:
+    """The third part, in place of the file's or behind it."""
+    with open(path) as f:
+        text = f.read().split("\n## 3. ")[0].rstrip()
+    lines = [
+        "", "", "## 3. Attention over other keys than the queries' own (bf16, about 4 s of calls each)", "",
+        "Made by `python profile_power.py --attention`.  Rates count the products that the kernels take (gradients: "
+        "7, three in `grad_q` and four in `grad_kv`).", "",
+        "| Call | us per call | TFLOP/s | socket W (median, min-max) | GFX MHz | share of the dense peak at this clock |",
+        "|---|---:|---:|---|---:|---:|",
+    ]
+    for r in rows:
+        p = r["power"]
+        mhz = p.get("gfx_mhz_median")
+        share = "-" if mhz is None else f"{r['tflops'] / (2500.0 * mhz / 2400.0):.3f}"
+        lines.append(f"| {r['name']} | {r['us']:.1f} | {r['tflops']:.0f} | {_fmt(p.get('socket_w_median'), 0)} "
+                     f"({_fmt(p.get('socket_w_min'), 0)}-{_fmt(p.get('socket_w_max'), 0)}) | {_fmt(mhz, 0)} | {share} |")
+    lines.append("")
+    with open(path, "w") as f:
+        f.write(text + "\n".join(lines))
 
 
 def write(path: str, wl: list, rd: list) -> None:
@@ -155,6 +217,7 @@ def write(path: str, wl: list, rd: list) -> None:
 def main() -> int:
     ap = argparse.ArgumentParser()
     ap.add_argument("--out", default=os.path.join(REPO, "profiles", "power_clock.md"))
+    ap.add_argument("--attention", action="store_true", help="the third part alone")
     args = ap.parse_args()
     import torch
     from pyasc_amd import _native
@@ -163,9 +226,11 @@ def main() -> int:
         return 1
     _native.load_library()
     dev = torch.device("cuda", 0)
-    wl = workloads(dev)
-    rd = rounds(dev)
-    write(args.out, wl, rd)
+    if not args.attention:
+        wl = workloads(dev)
+        rd = rounds(dev)
+        write(args.out, wl, rd)
+    write_attention(args.out, attention(dev))
     print(f"wrote {args.out}", file=sys.stderr)
     return 0
 

@@ -547,7 +547,8 @@ int32_t asc_attention_plan(const asc_attention_t* args, int32_t tree,
  * gradient d_o of o: dq, dk and dv, the latter two summed over the query heads that
  * share a key / value head, in a fixed order; zeros behind a sequence's keys.  The
  * probabilities and the scores' gradients are rounded to the type's precision for their
- * products, as those of the forward pass are, not to its range. */
+ * products, as those of the forward pass are, not to its range; above 192 keys rowsum(d_o *
+ * o) is of the rounded o. */
 int64_t asc_cross_attention_bwd_workspace(const asc_attention_t* args);
 int32_t asc_cross_attention_bwd(const asc_attention_t* args, void* workspace,
                                 int64_t workspace_bytes, asc_stream_t stream);

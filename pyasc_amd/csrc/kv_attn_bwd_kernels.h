@@ -20,9 +20,11 @@
 // Where rows or keys are few, keys (grad_q) or rows (grad_kv) are split over workgroups, whose fp32
 // parts join_grad adds in order.
 //
-// The matrix units bound both, at the clock that the board's power leaves: 4 sequences, 32 / 8 heads of
-// 128, 2048 queries, 1024 keys, bf16: grad_q (three products) 225 us, 0.92 PFLOP/s, matrix units busy
-// 40%; grad_kv (four) 266 us, 1.03 PFLOP/s, 47%; join_grad 15 us for dk and dv in two parts each (84 MB).
+// Two things bound both.  A wave's products, exp2, packing and sums follow one another, so the matrix units
+// are busy 40 to 47% of the time; and the board is at its power: 1372 to 1400 W of 1400, at 2.0 to 2.1
+// GHz.  4 sequences, 32 / 8 heads of 128, 2048 queries, 1024 keys, bf16: grad_q (three products) 225 us,
+// 0.92 PFLOP/s, matrix units busy 40%; grad_kv (four) 266 us, 1.03 PFLOP/s, 47%; join_grad 15 us for dk and
+// dv in two parts each (84 MB).
 #pragma once
 
 #include "kv_attn_kernels.h"
@@ -385,7 +387,10 @@ __device__ __forceinline__ void grad_q_body(const GradArgs& p) {
 
   // o is rounded to its type, and delta with it.  Over few keys, where o is as large as the values,
   // that shows in the gradients (0.0026 against 0.0024 relative, bf16, 10 keys), and delta is taken
-  // as the sum of p dP in a pass of its own; over many it is left to o.
+  // as the sum of p dP in a pass of its own; over many it is left to o: the pass would add two products
+  // to the nine.  It shows there too where rows give few of the keys most of their probability: 256 rows,
+  // 1024 keys, bf16, dq off by 0.0024 of its norm with a largest probability of 0.02, 0.0033 of
+  // 0.42 and 0.0054 of 0.70 (0.0016 where only the result is rounded).
   if (total <= kExactTiles) {
     delta = 0.f;
     stream(false, [&](uint32_t, const f32x16& x, const f32x16& y) {

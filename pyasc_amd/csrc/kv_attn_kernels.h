@@ -12,10 +12,15 @@
 // direct-to-LDS load takes the places of its rows from those lanes.  Rows past the last key come
 // from a row of zeros, so nothing behind a sequence is read, whatever it holds.
 //
+// The probabilities (unnormalised, fp32 with their sums) are rounded to the element type for the product
+// with the values, as matrix operands have to be: errors of 0.0023 of the results' norm in bf16 where one
+// rounding of exact results leaves 0.0017 (0.00028 and 0.00021 in fp16).  A second product for what
+// the rounding drops would add half to the matrix work.
+//
 //  - kv_wide: a workgroup owns up to 32 rows per wave and streams the keys once for all of them,
 //    through rings of three LDS stages as fa_fwd_body.  The matrix units bound it, at the clock that
-//    the board's power leaves: 4 x 32 heads, 4096 queries, 2048 keys, head_dim 128, bf16: 550 to 565
-//    us, 1.0 PFLOP/s, matrix units busy 46%.  With shared heads and pages a chain of tiles and its
+//    the board's power leaves: 4 x 32 heads, 4096 queries, 2048 keys, head_dim 128, bf16: 547 us,
+//    1.0 PFLOP/s, matrix units busy 46%, at 1400 W of the board's 1400 and 2.0 GHz.  With shared heads and pages a chain of tiles and its
 //    start and end do: 8 sequences of 1024 to 4096 keys, 64 drafted tokens, 32 / 8 heads: 47 us.
 //  - kv_narrow: up to 32 rows; the workgroup's four waves take every fourth tile each.  HBM bounds it
 //    over long caches: 8 sequences of up to 32768 keys in pages, 32 / 8 heads of 128, one token: 671 MB

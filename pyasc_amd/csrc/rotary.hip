@@ -15,9 +15,12 @@
 // weights and the steps of its addresses are registers over all heads (with addresses worked out
 // row by row, the norm took 74 us where it takes 63).
 //
-// bf16, 4 x 4096 tokens, 32 + 8 heads of 128: positions 60 us (5.6 TB/s), with the norm 63 (5.3), a
-// copy of the same bytes 65; the gradient 105 (4.8), its conversions and sums beside the loads.
-// fp32, half the tokens: 131, 133 and 195 us (5.1 TB/s each).
+// Contiguous heads, more bytes than the caches hold: bf16, 4 x 4096 tokens, 32 + 8 heads of 128 (336 MB):
+// positions 64 us (5.2 TB/s), with the norm 66 (5.1), a copy of the same bytes 65; the gradient (503 MB)
+// 106 (4.8), its conversions and sums beside the loads.  fp32 (671 and 1007 MB): 126, 130, a copy 130,
+// and 197 us (5.1 to 5.3 TB/s).  Heads whose slots are no power of two leave lanes idle, and a rotated part that
+// is not a multiple of 16 values narrows the loads: bf16, head_dim 80, 50 us, 52 and 87 (a copy 43);
+// 20 of 80 rotated, 70, 70 and 110; head_dim 130, 121, 127 and 173 (66).
 #include <type_traits>
 
 #include "common.h"

@@ -698,7 +698,9 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
       pair as it is and divides the last one's frequency by the factor;
     - "yarn": pairs that turn at least 32 times in the original length keep their frequency, those
       that turn less than once are divided by the factor, in between linearly in the number of
-      turns; the magnitude is 0.1 ln(factor) + 1 (Peng et al., arXiv:2309.00071, sections 3.2-3.4)."""
+      turns; the magnitude is 0.1 ln(factor) + 1 (Peng et al., arXiv:2309.00071, sections 3.2-3.4).
+      Parity with a trained model's own frequencies is unpinned: programs that ramp over the
+      pairs' numbers between two rounded ends get others, and ``freqs`` can be theirs."""
     rotary_dim = int(rotary_dim)
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be positive and even, got {rotary_dim}")
@@ -831,7 +833,8 @@ def qk_norm_rotary_bwd(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q: 
                        interleaved: bool = False, magnitude: float = 1.0, stream: Any = None) -> None:
     """The gradient of qk_norm_rotary: from the results' gradients and its inputs, the gradients
     of q and k (dq may lie in place of dq_out or q) and of the weights (float32 [head_dim], summed
-    over all rows in a fixed order)."""
+    over all rows in a fixed order, in float32 over a workgroup's rows and float64 over workgroups).
+    A weight that q and k share has two gradients, to be added: one place for both is refused."""
     device = _current_device()
     args = _rotary_args(q, k, positions, freqs, dq, dk, interleaved, magnitude, device, False, epsilon,
                         (q_weight, k_weight), (dq_out, dk_out, dq_weight, dk_weight))
@@ -905,7 +908,9 @@ def cross_attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: t
     value head, in a fixed order, and are zeros behind a sequence's keys.  The probabilities and the
     scores' gradients are rounded to the inputs' type for their products: to its precision, whatever
     their size (in float16 they are held at powers of two that move with the largest of a row or key),
-    but the gradients themselves end at the type's smallest value."""
+    but the gradients themselves end at the type's smallest value.  Above 192 keys the row sums of
+    do * o are of the rounded o: rows that give few of many keys most of their probability have dq
+    and dk off by up to three times a rounding."""
     device = _current_device()
     q_rows, o_rows, k_rows, v_rows = _kv_rows(q, k, v, o, sm_scale, device, ("k", "v"), written=False)
     dtype, shape = q.dtype, q.shape

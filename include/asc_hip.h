@@ -54,6 +54,7 @@ typedef void* asc_stream_t; /* hipStream_t */
 #define ASC_DT_INT32 3
 #define ASC_DT_INT8 4
 #define ASC_DT_INT16 5
+#define ASC_DT_FLOAT8_E4M3 6 /* the OCP format: no infinities, largest value 448 */
 
 /* ---- runtime / platform --------------------------------------------------
  * Replaces rt_wrapper.cpp's device queries (GetDeviceInfoWrapper,
@@ -552,6 +553,137 @@ int32_t asc_attention_plan(const asc_attention_t* args, int32_t tree,
 int64_t asc_cross_attention_bwd_workspace(const asc_attention_t* args);
 int32_t asc_cross_attention_bwd(const asc_attention_t* args, void* workspace,
                                 int64_t workspace_bytes, asc_stream_t stream);
+
+/* ---- a cache held in 8 bits --------------------------------------------------------
+ * No reference function exists; the build defines these next to its attention.
+ * Keys and values as codes of one byte, k and v: num_pages pages of kv_heads heads and
+ * page_size rows of head_dim codes, key j of sequence b in page block_table[b][j /
+ * page_size], row j % page_size.  Without a block_table (NULL): batch pages of kv_len
+ * rows, sequence b's in page b.  kv_len: keys a sequence can have (table width *
+ * page_size).  A scale (fp32, positive and finite) for each head and scale_block rows of a
+ * page: the value of a code c (int8, or float8 e4m3) is c * scale.  k_scales, v_scales:
+ * rows of one element, seq_stride from one block to the next.
+ * head_dim 64 or 128; scale_block a multiple of 16 that divides page_size (kv_len without
+ * pages); codes and 16-bit rows 16-byte aligned, strides multiples of 16 codes or 8
+ * elements; codes within 64 GiB, scales within 8 GiB.
+ *
+ * asc_quantized_cache_append  token i (of n, or new_lengths[b]) of k_new and v_new goes to
+ *     key lengths[b] + i.  A block of no earlier rows gets the scale that it needs, the least
+ *     power of two s >= 2^-126 with |x| <= 127 s (int8) or 448 s (e4m3) for its finite values.
+ *     A block that holds rows keeps its scale where that is enough (s_old >= s); else it
+ *     gets s, and its rows become round(c s_old / s).  Rounded to nearest, ties to even; an
+ *     infinity becomes the largest code, NaN the NaN of e4m3 or 0.  A held scale that is
+ *     not positive and finite counts as 0.  A sequence whose lengths do not fit the cache, and a block
+ *     whose page lies outside it, stay as they are.
+ * asc_quantized_cache_read    k_new[b][.][i], v_new[b][.][i] = the values of key lengths[b] +
+ *     i for i < n, or new_lengths[b]; rows behind these are left as they were.  A sequence
+ *     whose lengths do not fit the cache, and a key whose page lies outside it, give NaN.
+ *     Either of k and v may be left out (k_new.data NULL).  dtype may be ASC_DT_FLOAT32 too.
+ * A result that shares a byte with an operand or another result is refused. */
+typedef struct asc_cache8 {
+  int32_t dtype, cache_dtype; /* of queries, results and new rows; ASC_DT_INT8 or ASC_DT_FLOAT8_E4M3 */
+  int32_t head_dim, page_size, scale_block, causal;
+  float sm_scale;
+  int64_t batch, q_heads, kv_heads, n, kv_len, num_pages;
+  asc_rows_t k, v, k_scales, v_scales;
+  asc_rows_t q, o;         /* attention */
+  asc_rows_t k_new, v_new; /* append and read */
+  float* lse;
+  const int32_t* lengths;
+  const int32_t* new_lengths;
+  const int32_t* block_table;
+  int64_t table_stride;
+} asc_cache8_t;
+int32_t asc_quantized_cache_append(const asc_cache8_t* args, asc_stream_t stream);
+int32_t asc_quantized_cache_read(const asc_cache8_t* args, asc_stream_t stream);
+
+/* ---- pages of a cache -----------------------------------------------------------
+ * Tensors whose first dimension is a cache's pages, of any type: [pages, heads, rows of
+ * row_bytes], strides in bytes, from_stride and to_stride between pages.  rows: page_size, or
+ * what page_size is a multiple of (scales of blocks).
+ *
+ * asc_cache_copy_pages  page to_pages[i] of each `to` becomes page from_pages[i] of `from`
+ *     for i < pairs; pairs with a page outside the tensors are left out.  A page that is
+ *     written must be in no other pair: it holds parts of both then.
+ * asc_cache_fork  the sequences of block_table (batch rows of width pages, lengths) become
+ *     new_batch others: sequence i goes on from sequence parents[i], or (outside the batch)
+ *     holds nothing.  Full pages are shared; the partly filled last page stays with the
+ *     first child of a parent, and each other child gets a free page, into which its rows are
+ *     copied: the free pages from the lowest up, in the children's order, -1 where
+ *     there is none left.  refcounts[page] (num_pages): how many sequences, of these or others, hold it;
+ *     0: free.  Writes table_out (new_batch rows of width; -1 behind a
+ *     sequence's pages), lengths_out and refcounts_out (which may be refcounts).  A length
+ *     outside the table is handed on, with a row of -1.  batch, new_batch: at most 4096.
+ * asc_cache_compact  the pages in use (refcounts > 0), U of them, come to lie at 0 .. U - 1:
+ *     the i-th of those above moves into the i-th free one below.  Writes page_map (num_pages:
+ *     a page's new place, -1 for free ones), table_out (batch rows, may be block_table; -1
+ *     behind a sequence's pages and for pages that are not in use) and refcounts_out (may be
+ *     refcounts).
+ * fork and compact copy within the tensors (`to` must be `from`); `workspace` holds
+ * _workspace bytes, 16-byte aligned. */
+#define ASC_MAX_PAGE_TENSORS 8
+typedef struct asc_page_tensor {
+  const void* from;
+  void* to;
+  int64_t from_stride, to_stride;
+  int64_t heads, rows, row_bytes, head_stride, row_stride;
+} asc_page_tensor_t;
+typedef struct asc_pages {
+  int64_t n_tensors, page_size, num_pages, to_num_pages, pairs, batch, new_batch, width;
+  const int32_t* from_pages;
+  const int32_t* to_pages;
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int32_t* lengths;
+  const int32_t* parents;
+  const int32_t* refcounts;
+  int32_t* table_out;
+  int64_t table_out_stride;
+  int32_t* lengths_out;
+  int32_t* refcounts_out;
+  int32_t* page_map;
+  asc_page_tensor_t tensors[ASC_MAX_PAGE_TENSORS];
+} asc_pages_t;
+int32_t asc_cache_copy_pages(const asc_pages_t* args, asc_stream_t stream);
+int64_t asc_cache_fork_workspace(const asc_pages_t* args);
+int32_t asc_cache_fork(const asc_pages_t* args, void* workspace, int64_t workspace_bytes,
+                       asc_stream_t stream);
+int64_t asc_cache_compact_workspace(const asc_pages_t* args);
+int32_t asc_cache_compact(const asc_pages_t* args, void* workspace, int64_t workspace_bytes,
+                          asc_stream_t stream);
+
+/* ---- logits before a token is chosen ---------------------------------------------
+ * out[r][t] = x of logits[r][t] (float32 / float16 / bfloat16; computed in fp32, each step
+ * rounded, one rounding of the result), in this order:
+ *   a token of the row's history:  x > 0 ? x / repetition[r] : x * repetition[r]
+ *   c times in it behind the prompt:  x - frequency[r] * c - (c > 0 ? presence[r] : 0)
+ *   x + bias[r][t]
+ *   -inf where bit t % 32 of mask[r][t / 32] is 0, whatever x is.
+ * history: the first history_lengths[r] of a row's history_width tokens, int32 or int64; the
+ * first prompt_lengths[r] (NULL: none) are the prompt.  Tokens outside the vocabulary
+ * are passed over.  repetition, frequency, presence, bias and mask may be NULL; bias_stride
+ * 0 shares one row.  A history length outside [0, history_width]: NaN, the mask aside.  out may lie
+ * in place of logits with the same stride; it must not share a byte with another operand. */
+typedef struct asc_logits {
+  int32_t dtype, history_int64;
+  int64_t rows, vocab, history_width;
+  const void* logits;
+  int64_t logits_stride;
+  void* out;
+  int64_t out_stride;
+  const void* history;
+  int64_t history_stride;
+  const int32_t* history_lengths;
+  const int32_t* prompt_lengths;
+  const float* repetition;
+  const float* frequency;
+  const float* presence;
+  const float* bias;
+  int64_t bias_stride;
+  const int32_t* mask;
+  int64_t mask_stride;
+} asc_logits_t;
+int32_t asc_process_logits(const asc_logits_t* args, asc_stream_t stream);
 
 /* ---- element-wise tile operations ------------------------------------------------
  * The generic kernels of the reference's operation tests, one op per launch:

@@ -26,6 +26,7 @@ DT_BFLOAT16 = 2
 DT_INT32 = 3
 DT_INT8 = 4
 DT_INT16 = 5
+DT_FLOAT8_E4M3 = 6
 
 ERR_INVALID_ARG = -1
 ERR_UNSUPPORTED = -2
@@ -79,6 +80,44 @@ class AttentionArgs(ctypes.Structure):
 class AttentionPlan(ctypes.Structure):
     """asc_attention_plan_t: the launch of an attention entry over other keys than the queries' own."""
     _fields_ = [("kernel", ctypes.c_char * 16), ("row_blocks", _c_i32), ("splits", _c_i32)]
+
+
+class Cache8Args(ctypes.Structure):
+    """asc_cache8_t."""
+    _fields_ = [("dtype", _c_i32), ("cache_dtype", _c_i32), ("head_dim", _c_i32), ("page_size", _c_i32),
+                ("scale_block", _c_i32), ("causal", _c_i32), ("sm_scale", _c_f32),
+                ("batch", _c_i64), ("q_heads", _c_i64), ("kv_heads", _c_i64), ("n", _c_i64), ("kv_len", _c_i64),
+                ("num_pages", _c_i64), ("k", Rows), ("v", Rows), ("k_scales", Rows), ("v_scales", Rows), ("q", Rows),
+                ("o", Rows), ("k_new", Rows), ("v_new", Rows), ("lse", _c_p), ("lengths", _c_p),
+                ("new_lengths", _c_p), ("block_table", _c_p), ("table_stride", _c_i64)]
+
+
+MAX_PAGE_TENSORS = 8
+
+
+class PageTensor(ctypes.Structure):
+    """asc_page_tensor_t: strides and rows in bytes."""
+    _fields_ = [("from_", _c_p), ("to", _c_p), ("from_stride", _c_i64), ("to_stride", _c_i64), ("heads", _c_i64),
+                ("rows", _c_i64), ("row_bytes", _c_i64), ("head_stride", _c_i64), ("row_stride", _c_i64)]
+
+
+class PagesArgs(ctypes.Structure):
+    """asc_pages_t."""
+    _fields_ = [("n_tensors", _c_i64), ("page_size", _c_i64), ("num_pages", _c_i64), ("to_num_pages", _c_i64),
+                ("pairs", _c_i64), ("batch", _c_i64), ("new_batch", _c_i64), ("width", _c_i64), ("from_pages", _c_p),
+                ("to_pages", _c_p), ("block_table", _c_p), ("table_stride", _c_i64), ("lengths", _c_p),
+                ("parents", _c_p), ("refcounts", _c_p), ("table_out", _c_p), ("table_out_stride", _c_i64),
+                ("lengths_out", _c_p), ("refcounts_out", _c_p), ("page_map", _c_p),
+                ("tensors", PageTensor * MAX_PAGE_TENSORS)]
+
+
+class LogitsArgs(ctypes.Structure):
+    """asc_logits_t."""
+    _fields_ = [("dtype", _c_i32), ("history_int64", _c_i32), ("rows", _c_i64), ("vocab", _c_i64),
+                ("history_width", _c_i64), ("logits", _c_p), ("logits_stride", _c_i64), ("out", _c_p),
+                ("out_stride", _c_i64), ("history", _c_p), ("history_stride", _c_i64), ("history_lengths", _c_p),
+                ("prompt_lengths", _c_p), ("repetition", _c_p), ("frequency", _c_p), ("presence", _c_p),
+                ("bias", _c_p), ("bias_stride", _c_i64), ("mask", _c_p), ("mask_stride", _c_i64)]
 
 
 # name -> argtypes; every entry point returns int32_t (asc_reduce_f32_workspace a byte
@@ -139,6 +178,14 @@ SIGNATURES = {
     "asc_tree_attention_workspace": [_c_p],
     "asc_tree_attention": [_c_p, _c_p, _c_i64, _c_p],
     "asc_attention_plan": [_c_p, _c_i32, ctypes.POINTER(AttentionPlan)],
+    "asc_quantized_cache_append": [_c_p, _c_p],
+    "asc_quantized_cache_read": [_c_p, _c_p],
+    "asc_cache_copy_pages": [_c_p, _c_p],
+    "asc_cache_fork_workspace": [_c_p],
+    "asc_cache_fork": [_c_p, _c_p, _c_i64, _c_p],
+    "asc_cache_compact_workspace": [_c_p],
+    "asc_cache_compact": [_c_p, _c_p, _c_i64, _c_p],
+    "asc_process_logits": [_c_p, _c_p],
     "asc_unary_f32": [_c_i32, _c_p, _c_p, _c_i64, _c_p],
     "asc_binary": [_c_i32, _c_i32, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_f64, _c_i64, _c_p],
     "asc_where_cmp": [_c_i32, _c_i32, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_f64, _c_i64, _c_f64, _c_f64, _c_p],
@@ -153,7 +200,7 @@ SIGNATURES = {
 }
 INT64_FUNCS = ("asc_qk_norm_rotary_bwd_workspace", "asc_cross_attention_fwd_workspace",
                "asc_cross_attention_bwd_workspace",
-               "asc_tree_attention_workspace")
+               "asc_tree_attention_workspace", "asc_cache_fork_workspace", "asc_cache_compact_workspace")
 # entry points returning a C string
 STRING_FUNCS = ("asc_last_error", "asc_version")
 

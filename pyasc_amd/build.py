@@ -53,6 +53,7 @@ PER_FILE_FLAGS = {
     "elementwise.hip": ["-ffp-contract=off"],
     "asc2_elementwise.hip": ["-ffp-contract=off"],
     "tile_ops.hip": ["-ffp-contract=off"],
+    "logits.hip": ["-ffp-contract=off"],
 }
 
 

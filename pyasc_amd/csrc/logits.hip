@@ -1,0 +1,208 @@
+// Logits before a token is chosen: penalties for tokens of the row's history, a bias, a grammar's
+// mask (asc_process_logits).
+//
+// A workgroup owns a slice of one row's vocabulary.  It counts the history's tokens that fall into the
+// slice in LDS (integers: the order does not matter), then takes the slice through the formula.  The
+// whole history is read for every slice, from L2 after the first.
+#include "common.h"
+#include "numeric.h"
+#include "overlap.h"
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct LogitsArgs {
+  const void* logits;
+  void* out;
+  int64_t logits_stride, out_stride;
+  const void* history;
+  int64_t history_stride;
+  const int32_t* lengths;
+  const int32_t* prompts;
+  const float* repetition;
+  const float* frequency;
+  const float* presence;
+  const float* bias;
+  int64_t bias_stride;
+  const uint32_t* mask;
+  int64_t mask_stride;
+  int32_t history_int64, vocab, width, slices;
+};
+
+struct F32 {
+  typedef float Stored;
+  static __device__ __forceinline__ float load(float x) { return x; }
+  static __device__ __forceinline__ float store(float x) { return x; }
+};
+struct F16 {
+  typedef uint16_t Stored;
+  static __device__ __forceinline__ float load(uint16_t x) { return asc::f16_to_f32(x); }
+  static __device__ __forceinline__ uint16_t store(float x) { return asc::f32_to_f16_rne(x); }
+};
+struct Bf16 {
+  typedef uint16_t Stored;
+  static __device__ __forceinline__ float load(uint16_t x) { return asc::bf16_to_f32(x); }
+  static __device__ __forceinline__ uint16_t store(float x) { return asc::f32_to_bf16_rne(x); }
+};
+
+constexpr int kThreads = 256;
+constexpr uint32_t kInPrompt = 0x80000000u;  // beside the count of a token behind the prompt
+
+// kIters vectors of 16 bytes per thread.  kVec: the rows of logits and out lie at the same offset from 16
+// bytes, so vectors of the slice do, `lead` elements before the row's first; else element by element.
+template <class E, bool kVec, int kIters>
+__global__ void __launch_bounds__(kThreads) process_logits(LogitsArgs p) {
+  typedef typename E::Stored S;
+  constexpr int V = kVec ? 16 / sizeof(S) : 1;
+  constexpr int kPer = 16 / static_cast<int>(sizeof(S));
+  constexpr int kSlice = kThreads * kIters * kPer;
+  constexpr int kVecs = kIters * kPer / V;
+  __shared__ uint32_t counts[kSlice];
+  const int tid = threadIdx.x;
+  const uint32_t row = blockIdx.x / p.slices, slice = blockIdx.x - row * p.slices;
+  const S* x = static_cast<const S*>(p.logits) + row * p.logits_stride;
+  S* y = static_cast<S*>(p.out) + row * p.out_stride;
+  const int lead = kVec ? static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(S)) : 0;
+  const int first = static_cast<int>(slice) * kSlice - lead;  // token of counts[0]
+
+  const int length = p.lengths[row];
+  const bool bad = length < 0 || length > p.width;
+  const int n = bad ? 0 : length;
+  const int prompt = p.prompts ? p.prompts[row] : 0;
+
+#pragma unroll
+  for (int i = 0; i < kSlice / 4 / kThreads; ++i) {
+    reinterpret_cast<u32x4*>(counts)[tid + i * kThreads] = u32x4{0, 0, 0, 0};
+  }
+  __syncthreads();
+  const auto count = [&](int i, int64_t token) {
+    const int64_t at = token - first;
+    if (token < 0 || token >= p.vocab || at < 0 || at >= kSlice) return;
+    if (i < prompt) {
+      atomicOr(&counts[at], kInPrompt);
+    } else {
+      atomicAdd(&counts[at], 1u);
+    }
+  };
+  if (p.history_int64) {
+    const int64_t* h = static_cast<const int64_t*>(p.history) + row * p.history_stride;
+    for (int i = tid; i < n; i += kThreads) count(i, h[i]);
+  } else {
+    const int32_t* h = static_cast<const int32_t*>(p.history) + row * p.history_stride;
+    for (int i = tid; i < n; i += kThreads) count(i, h[i]);
+  }
+  __syncthreads();
+
+  const float repetition = p.repetition ? p.repetition[row] : 1.0f;
+  const float frequency = p.frequency ? p.frequency[row] : 0.0f;
+  const float presence = p.presence ? p.presence[row] : 0.0f;
+  const float* bias = p.bias ? p.bias + row * p.bias_stride : nullptr;
+  const uint32_t* mask = p.mask ? p.mask + row * p.mask_stride : nullptr;
+  const auto process = [&](int token, uint32_t c, float v) {
+    if (c != 0) {
+      v = v > 0.0f ? v / repetition : v * repetition;
+      const float times = static_cast<float>(c & ~kInPrompt);
+      v = v - frequency * times;
+      if (times > 0.0f) v = v - presence;
+    }
+    if (bias) v = v + bias[token];
+    if (bad) v = __builtin_nanf("");
+    if (mask && !((mask[token >> 5] >> (token & 31)) & 1)) v = -INFINITY;
+    return v;
+  };
+#pragma unroll
+  for (int it = 0; it < kVecs; ++it) {
+    const int at = (tid + it * kThreads) * V, token = first + at;
+    if (token >= p.vocab || token + V <= 0) continue;
+    if (V > 1 && token >= 0 && token + V <= p.vocab) {
+      S in[V], out[V];
+      *reinterpret_cast<u32x4*>(in) = *reinterpret_cast<const u32x4*>(x + token);
+#pragma unroll
+      for (int e = 0; e < V; ++e) out[e] = E::store(process(token + e, counts[at + e], E::load(in[e])));
+      *reinterpret_cast<u32x4*>(y + token) = *reinterpret_cast<u32x4*>(out);
+    } else {
+      for (int e = 0; e < V; ++e) {
+        const int t = token + e;
+        if (t >= 0 && t < p.vocab) y[t] = E::store(process(t, counts[at + e], E::load(x[t])));
+      }
+    }
+  }
+}
+
+template <class E, bool kVec>
+void launch(const LogitsArgs& p, int64_t rows, hipStream_t stream) {
+  hipLaunchKernelGGL((process_logits<E, kVec, 8 * sizeof(typename E::Stored) / 4>), dim3(static_cast<uint32_t>(rows * p.slices)),
+                     dim3(kThreads), 0, stream, p);
+}
+
+}  // namespace
+
+extern "C" int32_t asc_process_logits(const asc_logits_t* a, asc_stream_t stream) {
+  const char* what = "asc_process_logits";
+  ASC_REQUIRE(a, ASC_ERR_INVALID_ARG, "%s: null arguments", what);
+  ASC_REQUIRE(a->dtype == ASC_DT_FLOAT32 || a->dtype == ASC_DT_FLOAT16 || a->dtype == ASC_DT_BFLOAT16,
+              ASC_ERR_UNSUPPORTED, "%s: dtype %d not supported (float32, float16, bfloat16)", what, a->dtype);
+  ASC_REQUIRE(a->rows >= 0 && a->vocab >= 0 && a->history_width >= 0, ASC_ERR_INVALID_ARG, "%s: negative shape", what);
+  if (a->rows == 0 || a->vocab == 0) return ASC_OK;
+  ASC_REQUIRE(a->vocab < 1 << 30 && a->history_width < 1 << 30, ASC_ERR_UNSUPPORTED, "%s: shape too large", what);
+  ASC_REQUIRE(a->logits && a->out && a->history_lengths && (a->history || a->history_width == 0), ASC_ERR_INVALID_ARG,
+              "%s: null buffer", what);
+  const int64_t size = a->dtype == ASC_DT_FLOAT32 ? 4 : 2;
+  ASC_REQUIRE(((reinterpret_cast<uintptr_t>(a->logits) | reinterpret_cast<uintptr_t>(a->out)) & (size - 1)) == 0,
+              ASC_ERR_ALIGNMENT, "%s: logits and out must be aligned to their elements", what);
+  const auto rows = [&](const char* name, const void* data, int64_t stride, int64_t row, int64_t element) {
+    return asc::region_of(name, asc_rows_t{const_cast<void*>(data), stride, 0, 0}, a->rows, 1, 1, row, element);
+  };
+  const asc::Region out = rows("out", a->out, a->out_stride, a->vocab, size);
+  const asc::Region logits = rows("logits", a->logits, a->logits_stride, a->vocab, size);
+  const asc::Region operands[] = {
+      rows("history", a->history, a->history_stride, a->history_width, a->history_int64 ? 8 : 4),
+      asc::region_of("history_lengths", a->history_lengths, a->rows * 4),
+      asc::region_of("prompt_lengths", a->prompt_lengths, a->rows * 4),
+      asc::region_of("repetition", a->repetition, a->rows * 4),
+      asc::region_of("frequency", a->frequency, a->rows * 4),
+      asc::region_of("presence", a->presence, a->rows * 4),
+      rows("bias", a->bias, a->bias_stride, a->vocab, 4),
+      rows("mask", a->mask, a->mask_stride, asc::ceil_div(a->vocab, 32), 4)};
+  ASC_REQUIRE(asc::same_place(out, logits) || !asc::overlap(out, logits), ASC_ERR_INVALID_ARG, "%s: 'out' overlaps '%s'",
+              what, "logits");
+  for (const asc::Region& r : operands) {
+    ASC_REQUIRE(!asc::overlap(out, r), ASC_ERR_INVALID_ARG, "%s: 'out' overlaps '%s'", what, r.name);
+  }
+  LogitsArgs p{};
+  p.logits = a->logits;
+  p.out = a->out;
+  p.logits_stride = a->logits_stride;
+  p.out_stride = a->out_stride;
+  p.history = a->history;
+  p.history_stride = a->history_stride;
+  p.history_int64 = a->history_int64;
+  p.lengths = a->history_lengths;
+  p.prompts = a->prompt_lengths;
+  p.repetition = a->repetition;
+  p.frequency = a->frequency;
+  p.presence = a->presence;
+  p.bias = a->bias;
+  p.bias_stride = a->bias_stride;
+  p.mask = reinterpret_cast<const uint32_t*>(a->mask);
+  p.mask_stride = a->mask_stride;
+  p.vocab = static_cast<int32_t>(a->vocab);
+  p.width = static_cast<int32_t>(a->history_width);
+  // room for the lead of a row that does not begin at 16 bytes
+  p.slices = static_cast<int32_t>(asc::ceil_div(a->vocab + 16 / size - 1, 8192));
+  ASC_REQUIRE(a->rows * p.slices < int64_t{1} << 24, ASC_ERR_UNSUPPORTED, "%s: %lld workgroups exceed the launch grid limit",
+              what, static_cast<long long>(a->rows * p.slices));
+  const uintptr_t apart = reinterpret_cast<uintptr_t>(a->logits) ^ reinterpret_cast<uintptr_t>(a->out);
+  const int64_t steps = a->rows > 1 ? (a->logits_stride - a->out_stride) * size : 0;
+  const bool vec = ((apart | static_cast<uintptr_t>(steps)) & 15) == 0;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a->dtype == ASC_DT_FLOAT32) {
+    vec ? launch<F32, true>(p, a->rows, s) : launch<F32, false>(p, a->rows, s);
+  } else if (a->dtype == ASC_DT_FLOAT16) {
+    vec ? launch<F16, true>(p, a->rows, s) : launch<F16, false>(p, a->rows, s);
+  } else {
+    vec ? launch<Bf16, true>(p, a->rows, s) : launch<Bf16, false>(p, a->rows, s);
+  }
+  return asc::check_launch(what);
+}

@@ -1,0 +1,596 @@
+// Pages of a cache: copies between caches, the fork of sequences that share pages, and compaction.
+//
+// What a fork or a compaction does to the pages is worked out by one workgroup, with the reference counts in
+// LDS; a second launch moves the data and writes the tables.  Nothing comes back to the host, so all
+// of them can be captured.  Ranks of free and moving pages are prefix sums and counts are
+// integers: the same result on every call.
+#include "common.h"
+#include "overlap.h"
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kTensors = ASC_MAX_PAGE_TENSORS;
+constexpr int kThreads = 256;
+constexpr int kPiece = 16384;  // bytes of a page that a workgroup copies at a time, where it lies in one piece
+
+// One tensor's share of a page's move: `pieces` parts, of kPiece bytes (flat) or of a head each.
+struct Tensor {
+  const uint8_t* from;
+  uint8_t* to;
+  int64_t from_stride, to_stride;
+  int64_t head_stride, row_stride;
+  int64_t bytes;  // flat: of a page
+  int32_t rows, row_bytes;
+  int32_t flat, pieces;
+  int32_t width;  // bytes that its addresses and sizes are multiples of: 1, 2, 4 or 16
+};
+
+struct CopyArgs {
+  Tensor t[kTensors];
+  int32_t n_tensors, per_move;
+  int32_t page_size;
+  int64_t moves;              // at most
+  const int32_t* count;       // null: moves
+  const int32_t* from;        // pages
+  const int32_t* to;
+  const int32_t* used;        // rows of a page that are copied, null: all
+  int64_t from_pages, to_pages;
+};
+
+template <class T>
+__device__ __forceinline__ void copy_run(const uint8_t* from, uint8_t* to, int64_t bytes) {
+  const T* src = reinterpret_cast<const T*>(from);
+  T* dst = reinterpret_cast<T*>(to);
+  const int n = static_cast<int>(bytes / static_cast<int64_t>(sizeof(T)));
+  int i = threadIdx.x;
+  for (; i + 3 * kThreads < n; i += 4 * kThreads) {
+    T v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = src[i + j * kThreads];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dst[i + j * kThreads] = v[j];
+  }
+  for (; i < n; i += kThreads) dst[i] = src[i];
+}
+
+template <class T>
+__device__ __forceinline__ void copy_rows(const uint8_t* from, uint8_t* to, int rows, int row_bytes, int64_t stride) {
+  const int per = row_bytes / static_cast<int>(sizeof(T));
+  const int64_t n = static_cast<int64_t>(rows) * per;
+  for (int64_t i = threadIdx.x; i < n; i += kThreads) {
+    const int64_t row = i / per;
+    const int64_t at = row * stride + (i - row * per) * static_cast<int64_t>(sizeof(T));
+    *reinterpret_cast<T*>(to + at) = *reinterpret_cast<const T*>(from + at);
+  }
+}
+
+// Item `item` of all: a move, one of its tensors, a piece of that.
+__device__ __forceinline__ void copy_item(const CopyArgs& p, int64_t item) {
+  const int64_t move = item / p.per_move;
+  int piece = static_cast<int>(item - move * p.per_move);
+  const int64_t from_page = p.from[move], to_page = p.to[move];
+  if (from_page < 0 || from_page >= p.from_pages || to_page < 0 || to_page >= p.to_pages) return;
+  int k = 0;
+  while (piece >= p.t[k].pieces) piece -= p.t[k++].pieces;
+  const Tensor& t = p.t[k];
+  const uint8_t* from = t.from + from_page * t.from_stride;
+  uint8_t* to = t.to + to_page * t.to_stride;
+  if (t.flat) {
+    const int64_t at = static_cast<int64_t>(piece) * kPiece;
+    const int64_t n = t.bytes - at < kPiece ? t.bytes - at : kPiece;
+    if (t.width == 16) return copy_run<u32x4>(from + at, to + at, n);
+    if (t.width == 4) return copy_run<uint32_t>(from + at, to + at, n);
+    if (t.width == 2) return copy_run<uint16_t>(from + at, to + at, n);
+    return copy_run<uint8_t>(from + at, to + at, n);
+  }
+  from += piece * t.head_stride;
+  to += piece * t.head_stride;
+  int rows = t.rows;
+  if (p.used) rows = static_cast<int>((static_cast<int64_t>(p.used[move]) * rows + p.page_size - 1) / p.page_size);
+  if (t.row_stride == t.row_bytes) {
+    const int64_t n = static_cast<int64_t>(rows) * t.row_bytes;
+    if (t.width == 16) return copy_run<u32x4>(from, to, n);
+    if (t.width == 4) return copy_run<uint32_t>(from, to, n);
+    if (t.width == 2) return copy_run<uint16_t>(from, to, n);
+    return copy_run<uint8_t>(from, to, n);
+  }
+  if (t.width == 16) return copy_rows<u32x4>(from, to, rows, t.row_bytes, t.row_stride);
+  if (t.width == 4) return copy_rows<uint32_t>(from, to, rows, t.row_bytes, t.row_stride);
+  if (t.width == 2) return copy_rows<uint16_t>(from, to, rows, t.row_bytes, t.row_stride);
+  return copy_rows<uint8_t>(from, to, rows, t.row_bytes, t.row_stride);
+}
+
+__device__ __forceinline__ void copy_items(const CopyArgs& p) {
+  const int64_t moves = p.count ? *p.count : p.moves;
+  for (int64_t item = blockIdx.x; item < moves * p.per_move; item += gridDim.x) copy_item(p, item);
+}
+
+__global__ void __launch_bounds__(kThreads) page_copy(CopyArgs p) { copy_items(p); }
+
+// ------------------------------------------------------------------------------------ plans
+
+constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / asc::kWave;
+constexpr int kMostSequences = 4096;
+
+// Sum of v over the lower threads of the workgroup; total: over all.  `waves`: LDS of its own.
+__device__ __forceinline__ int prefix(int v, int (&waves)[kPlanWaves], int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int sum = v;
+#pragma unroll
+  for (int d = 1; d < asc::kWave; d *= 2) {
+    const int up = __shfl_up(sum, d, asc::kWave);
+    if (lane >= d) sum += up;
+  }
+  __syncthreads();
+  if (lane == 63) waves[wave] = sum;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanWaves; ++w) {
+    if (w < wave) before += waves[w];
+    total += waves[w];
+  }
+  return before + sum - v;
+}
+
+struct PlanArgs {
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* lengths;
+  const int32_t* parents;
+  const int32_t* refcounts;
+  int32_t* table_out;
+  int64_t table_out_stride;
+  int32_t* lengths_out;
+  int32_t* refcounts_out;
+  int32_t* page_map;
+  int32_t* count;  // workspace: moves, and where they go
+  int32_t* from;
+  int32_t* to;
+  int32_t* used;
+  int32_t page_size, pages, batch, new_batch, width;
+};
+
+// Pages that sequence b's row holds, 0 where its length does not fit the table.
+__device__ __forceinline__ int held_of(const PlanArgs& p, int64_t length) {
+  if (length < 0 || length > static_cast<int64_t>(p.width) * p.page_size) return 0;
+  return static_cast<int>((length + p.page_size - 1) / p.page_size);
+}
+
+// The counts change by (children - 1) for a parent's full pages; its last page, partly filled, is given up only
+// by a parent without children.  They go through LDS kCountChunk pages at a time; a page that is
+// free after that has a rank, and goes to the child in need of that rank.
+__global__ void __launch_bounds__(kPlanThreads) fork_plan(PlanArgs p) {
+  constexpr int kCountChunk = 16384, kPer = kCountChunk / kPlanThreads, kRows = kMostSequences / kPlanThreads;
+  __shared__ int counts[kCountChunk];
+  __shared__ int children[kMostSequences];
+  __shared__ int first[kMostSequences];  // child; later 2 * full pages + whether another is partly filled
+  __shared__ int fresh[kMostSequences];  // free page of each rank
+  __shared__ int waves[kPlanWaves];
+  const int tid = threadIdx.x;
+  for (int b = tid; b < p.batch; b += kPlanThreads) {
+    children[b] = 0;
+    first[b] = p.new_batch;
+  }
+  __syncthreads();
+  for (int i = tid; i < p.new_batch; i += kPlanThreads) {
+    const int parent = p.parents[i];
+    if (parent < 0 || parent >= p.batch) continue;
+    atomicAdd(&children[parent], 1);
+    atomicMin(&first[parent], i);
+  }
+  __syncthreads();
+  // children in need of a page
+  int rank[kRows], source[kRows], rows[kRows], mine = 0;
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+    const int i = tid * kRows + k;
+    rank[k] = -1;
+    source[k] = rows[k] = 0;
+    if (i >= p.new_batch) continue;
+    const int parent = p.parents[i];
+    const bool any = parent >= 0 && parent < p.batch;
+    const int length = any ? p.lengths[parent] : 0;
+    p.lengths_out[i] = length;
+    const int held = held_of(p, length);
+    rows[k] = held ? length - length / p.page_size * p.page_size : 0;
+    if (rows[k] == 0 || first[parent] == i) continue;
+    source[k] = p.table[parent * p.table_stride + held - 1];
+    rank[k] = mine++;
+  }
+  int needs;
+  const int before = prefix(mine, waves, needs);
+  for (int b = tid; b < p.batch; b += kPlanThreads) {
+    const int length = p.lengths[b], held = held_of(p, length);
+    const int full = held ? length / p.page_size : 0;
+    first[b] = 2 * full + (held != full);
+  }
+  int given = 0;
+  for (int base = 0; base < p.pages; base += kCountChunk) {
+    const int here = min(kCountChunk, p.pages - base);
+    for (int i = tid; i < here; i += kPlanThreads) counts[i] = p.refcounts[base + i];
+    __syncthreads();
+    const int64_t entries = static_cast<int64_t>(p.batch) * p.width;
+    for (int64_t e = tid; e < entries; e += kPlanThreads) {
+      const int b = static_cast<int>(e / p.width), j = static_cast<int>(e - static_cast<int64_t>(b) * p.width);
+      const int full = first[b] >> 1, c = children[b];
+      const int change = j < full ? c - 1 : (j == full && (first[b] & 1) && c == 0 ? -1 : 0);
+      if (change == 0) continue;
+      const int64_t page = static_cast<int64_t>(p.table[b * p.table_stride + j]) - base;
+      if (page >= 0 && page < here) atomicAdd(&counts[page], change);
+    }
+    __syncthreads();
+    int free = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int i = tid * kPer + k;
+      free += i < here && counts[i] == 0;
+    }
+    int all;
+    int r = given + prefix(free, waves, all);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int i = tid * kPer + k;
+      if (i < here && counts[i] == 0) {
+        if (r < needs) {
+          fresh[r] = base + i;
+          counts[i] = 1;
+        }
+        ++r;
+      }
+    }
+    given += all;
+    __syncthreads();
+    for (int i = tid; i < here; i += kPlanThreads) p.refcounts_out[base + i] = counts[i];
+    __syncthreads();
+  }
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+    const int i = tid * kRows + k;
+    if (i >= p.new_batch) continue;
+    const int r = before + rank[k];
+    p.from[i] = rank[k] >= 0 ? source[k] : -1;
+    p.to[i] = rank[k] >= 0 ? (r < given ? fresh[r] : -1) : -2;  // -2: the parent's own
+    p.used[i] = rows[k];
+  }
+}
+
+// The copies, and the new rows of the table.
+__global__ void __launch_bounds__(kThreads) fork_move(CopyArgs c, PlanArgs p, int row_groups) {
+  if (static_cast<int>(blockIdx.x) >= row_groups) {
+    for (int64_t item = blockIdx.x - row_groups; item < c.moves * c.per_move; item += gridDim.x - row_groups) {
+      copy_item(c, item);
+    }
+    return;
+  }
+  for (int i = blockIdx.x; i < p.new_batch; i += row_groups) {
+    const int parent = p.parents[i];
+    const bool any = parent >= 0 && parent < p.batch;
+    const int held = any ? held_of(p, p.lengths[parent]) : 0;
+    const int to = p.to[i];
+    for (int j = threadIdx.x; j < p.width; j += kThreads) {
+      int page = -1;
+      if (j < held) page = j == held - 1 && to != -2 ? to : p.table[parent * p.table_stride + j];
+      p.table_out[i * p.table_out_stride + j] = page;
+    }
+  }
+}
+
+// Free pages below the number of used ones come before the used pages above it, so both are listed in one
+// pass over the counts.
+__global__ void __launch_bounds__(kPlanThreads) compact_plan(PlanArgs p) {
+  constexpr int kPer = 8, kChunk = kPer * kPlanThreads;
+  __shared__ int waves[kPlanWaves];
+  const int tid = threadIdx.x;
+  int mine = 0, used;
+  for (int i = tid; i < p.pages; i += kPlanThreads) mine += p.refcounts[i] > 0;
+  prefix(mine, waves, used);
+  int holes = 0, movers = 0;
+  for (int base = 0; base < p.pages; base += kChunk) {
+    int refs[kPer], n_holes = 0, n_movers = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int i = base + tid * kPer + k;
+      refs[k] = i < p.pages ? p.refcounts[i] : 0;
+      n_holes += i < used && refs[k] <= 0;
+      n_movers += i >= used && refs[k] > 0;
+    }
+    int all_holes, all_movers;
+    int hole = holes + prefix(n_holes, waves, all_holes);
+    int mover = movers + prefix(n_movers, waves, all_movers);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int i = base + tid * kPer + k;
+      if (i >= p.pages) continue;
+      if (i < used && refs[k] <= 0) p.to[hole++] = i;
+      if (i >= used && refs[k] > 0) {
+        p.from[mover++] = i;
+      } else {
+        p.page_map[i] = refs[k] > 0 ? i : -1;
+        p.refcounts_out[i] = refs[k];
+      }
+    }
+    holes += all_holes;
+    movers += all_movers;
+  }
+  __syncthreads();
+  for (int k = tid; k < movers; k += kPlanThreads) {
+    const int from = p.from[k], to = p.to[k];
+    p.page_map[from] = to;
+    p.refcounts_out[to] = p.refcounts[from];
+    p.refcounts_out[from] = 0;
+  }
+  if (tid == 0) *p.count = movers;
+}
+
+__global__ void __launch_bounds__(kThreads) compact_move(CopyArgs c, PlanArgs p, int row_groups) {
+  if (static_cast<int>(blockIdx.x) >= row_groups) {
+    const int64_t moves = *c.count;
+    for (int64_t item = blockIdx.x - row_groups; item < moves * c.per_move; item += gridDim.x - row_groups) {
+      copy_item(c, item);
+    }
+    return;
+  }
+  for (int b = blockIdx.x; b < p.batch; b += row_groups) {
+    const int held = held_of(p, p.lengths[b]);
+    for (int j = threadIdx.x; j < p.width; j += kThreads) {
+      const int page = j < held ? p.table[b * p.table_stride + j] : -1;
+      p.table_out[b * p.table_out_stride + j] = page >= 0 && page < p.pages ? p.page_map[page] : -1;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------ host
+
+constexpr int64_t kMostGroups = 2048;  // eight workgroups of 256 threads on each of 256 CUs
+
+int width_of(uintptr_t bits) { return (bits & 15) == 0 ? 16 : ((bits & 3) == 0 ? 4 : ((bits & 1) == 0 ? 2 : 1)); }
+
+asc::Region pages_region(const char* name, const void* data, int64_t pages, int64_t stride, const asc_page_tensor_t& t) {
+  const bool any = pages > 0 && t.heads > 0 && t.rows > 0;
+  return asc::spanned({name,
+                       reinterpret_cast<uintptr_t>(data),
+                       {pages, t.heads, t.rows},
+                       {pages > 1 ? stride : 0, t.heads > 1 ? t.head_stride : 0, t.rows > 1 ? t.row_stride : 0},
+                       any ? t.row_bytes : 0,
+                       0,
+                       0});
+}
+
+// The tensors' checks, and their pieces.  partial: a part of a page's rows may be copied.
+int32_t make_copy(const asc_pages_t& a, bool within, bool partial, const char* what, CopyArgs& c) {
+  ASC_REQUIRE(a.n_tensors >= 0 && a.n_tensors <= kTensors, ASC_ERR_INVALID_ARG, "%s: %lld tensors (at most %d)", what,
+              static_cast<long long>(a.n_tensors), kTensors);
+  c.n_tensors = static_cast<int32_t>(a.n_tensors);
+  c.page_size = static_cast<int32_t>(a.page_size);
+  c.from_pages = a.num_pages;
+  c.to_pages = within ? a.num_pages : a.to_num_pages;
+  for (int i = 0; i < c.n_tensors; ++i) {
+    const asc_page_tensor_t& x = a.tensors[i];
+    ASC_REQUIRE(x.from && x.to, ASC_ERR_INVALID_ARG, "%s: null tensor", what);
+    ASC_REQUIRE(!within || (x.from == x.to && x.from_stride == x.to_stride), ASC_ERR_INVALID_ARG,
+                "%s: pages move within a tensor", what);
+    ASC_REQUIRE(x.heads >= 1 && x.rows >= 1 && x.row_bytes >= 1 && x.heads < 1 << 20 && x.rows < 1 << 30 &&
+                    x.row_bytes < 1 << 30 && x.from_stride >= 0 && x.to_stride >= 0 && x.head_stride >= 0 &&
+                    x.row_stride >= 0,
+                ASC_ERR_INVALID_ARG, "%s: invalid shape or stride of a tensor", what);
+    ASC_REQUIRE(!partial || (x.rows <= a.page_size && a.page_size % x.rows == 0), ASC_ERR_INVALID_ARG,
+                "%s: %lld rows of a page of %lld", what, static_cast<long long>(x.rows),
+                static_cast<long long>(a.page_size));
+    Tensor& t = c.t[i];
+    t.from = static_cast<const uint8_t*>(x.from);
+    t.to = static_cast<uint8_t*>(x.to);
+    t.from_stride = x.from_stride;
+    t.to_stride = x.to_stride;
+    t.head_stride = x.heads > 1 ? x.head_stride : 0;
+    t.row_stride = x.rows > 1 ? x.row_stride : x.row_bytes;
+    t.rows = static_cast<int32_t>(x.rows);
+    t.row_bytes = static_cast<int32_t>(x.row_bytes);
+    const bool heads_outside = t.row_stride == x.row_bytes && (x.heads == 1 || x.head_stride == x.rows * x.row_bytes);
+    const bool rows_outside = t.head_stride == x.row_bytes && (x.rows == 1 || x.row_stride == x.heads * x.row_bytes);
+    t.bytes = x.heads * x.rows * x.row_bytes;
+    t.flat = !partial && (heads_outside || rows_outside);
+    const int64_t pieces = t.flat ? asc::ceil_div(t.bytes, kPiece) : x.heads;
+    ASC_REQUIRE(t.bytes < int64_t{1} << 40 && pieces < 1 << 24, ASC_ERR_UNSUPPORTED, "%s: pages too large", what);
+    t.pieces = static_cast<int32_t>(pieces);
+    c.per_move += t.pieces;
+    uintptr_t bits = reinterpret_cast<uintptr_t>(x.from) | reinterpret_cast<uintptr_t>(x.to) |
+                     static_cast<uintptr_t>(x.from_stride | x.to_stride | x.row_bytes);
+    if (!t.flat) bits |= static_cast<uintptr_t>(t.head_stride | t.row_stride);
+    t.width = width_of(bits);
+    // results lie apart from each other and from what is read, unless they are it
+    const asc::Region to = pages_region("a result", x.to, c.to_pages, x.to_stride, x);
+    for (int j = 0; j < c.n_tensors; ++j) {
+      const asc_page_tensor_t& y = a.tensors[j];
+      const asc::Region from = pages_region("a cache", y.from, c.from_pages, y.from_stride, y);
+      const bool same = i == j && x.from == x.to && x.from_stride == x.to_stride;
+      ASC_REQUIRE(same || !asc::overlap(to, from), ASC_ERR_INVALID_ARG, "%s: 'a result' overlaps 'a cache'", what);
+      if (j < i) {
+        ASC_REQUIRE(!asc::overlap(to, pages_region("a result", y.to, c.to_pages, y.to_stride, y)), ASC_ERR_INVALID_ARG,
+                    "%s: two results overlap", what);
+      }
+    }
+  }
+  return ASC_OK;
+}
+
+int32_t check_apart(const asc::Region& r, const asc_pages_t& a, const CopyArgs& c, bool written, const char* what) {
+  for (int i = 0; i < c.n_tensors; ++i) {
+    const asc_page_tensor_t& x = a.tensors[i];
+    ASC_REQUIRE(!asc::overlap(r, pages_region("a cache", x.to, c.to_pages, x.to_stride, x)) &&
+                    (!written || !asc::overlap(r, pages_region("a cache", x.from, c.from_pages, x.from_stride, x))),
+                ASC_ERR_INVALID_ARG, "%s: '%s' overlaps '%s'", what, r.name, "a cache");
+  }
+  return ASC_OK;
+}
+
+int64_t groups_of(int64_t items) { return items < kMostGroups ? items : kMostGroups; }
+
+struct Plan {
+  CopyArgs c{};
+  PlanArgs p{};
+};
+
+int64_t fork_workspace(const asc_pages_t& a) { return 16 + 3 * asc::ceil_div(a.new_batch, 4) * 16; }
+int64_t compact_workspace(const asc_pages_t& a) { return 16 + 2 * asc::ceil_div(a.num_pages, 4) * 16; }
+
+int32_t make_plan(const asc_pages_t* a, bool fork, const char* what, Plan& plan) {
+  ASC_REQUIRE(a, ASC_ERR_INVALID_ARG, "%s: null arguments", what);
+  ASC_REQUIRE(a->page_size >= 1 && a->page_size < 1 << 30 && a->num_pages >= 0 && a->num_pages < 1 << 30 &&
+                  a->width >= 0 && a->width < 1 << 30 && a->batch >= 0 && a->table_stride >= 0 &&
+                  a->table_out_stride >= 0,
+              ASC_ERR_INVALID_ARG, "%s: invalid shape", what);
+  ASC_REQUIRE(a->width * a->page_size < int64_t{1} << 40, ASC_ERR_UNSUPPORTED, "%s: shape too large", what);
+  const int64_t rows = fork ? a->new_batch : a->batch;
+  ASC_REQUIRE(rows >= 0, ASC_ERR_INVALID_ARG, "%s: invalid shape", what);
+  ASC_REQUIRE((!fork && a->batch < 1 << 20) || (a->batch <= kMostSequences && a->new_batch <= kMostSequences),
+              ASC_ERR_UNSUPPORTED, "%s: more than %d sequences", what, fork ? kMostSequences : 1 << 20);
+  const bool table = a->batch > 0 && a->width > 0, counts = a->num_pages > 0;
+  ASC_REQUIRE((!table || a->block_table) && (a->batch == 0 || a->lengths) && (!counts || (a->refcounts && a->refcounts_out)) &&
+                  (rows == 0 || a->width == 0 || a->table_out),
+              ASC_ERR_INVALID_ARG, "%s: null buffer", what);
+  ASC_REQUIRE(fork ? rows == 0 || (a->parents && a->lengths_out) : !counts || a->page_map, ASC_ERR_INVALID_ARG,
+              "%s: null buffer", what);
+  int32_t rc = make_copy(*a, true, fork, what, plan.c);
+  if (rc != ASC_OK) return rc;
+  const auto table_rows = [&](const char* name, const int32_t* data, int64_t stride, int64_t n) {
+    return asc::region_of(name, asc_rows_t{const_cast<int32_t*>(data), stride, 0, 0}, n, 1, 1, a->width, 4);
+  };
+  const asc::Region block_table = table_rows("block_table", a->block_table, a->table_stride, a->batch);
+  const asc::Region refcounts = asc::region_of("refcounts", a->refcounts, a->num_pages * 4);
+  const asc::Region results[] = {
+      table_rows("table_out", a->table_out, a->table_out_stride, rows),
+      asc::region_of("refcounts_out", a->refcounts_out, a->num_pages * 4),
+      fork ? asc::region_of("lengths_out", a->lengths_out, a->new_batch * 4)
+           : asc::region_of("page_map", a->page_map, a->num_pages * 4)};
+  const asc::Region operands[] = {block_table, refcounts, asc::region_of("lengths", a->lengths, a->batch * 4),
+                                  asc::region_of("parents", fork ? a->parents : nullptr, a->new_batch * 4)};
+  for (int i = 0; i < 3; ++i) {
+    for (const asc::Region& x : operands) {
+      const bool in_place = (i == 1 && &x == &operands[1]) || (i == 0 && !fork && &x == &operands[0]);
+      ASC_REQUIRE(!asc::overlap(results[i], x) || (in_place && asc::same_place(results[i], x)), ASC_ERR_INVALID_ARG,
+                  "%s: '%s' overlaps '%s'", what, results[i].name, x.name);
+    }
+    for (int j = 0; j < i; ++j) {
+      ASC_REQUIRE(!asc::overlap(results[i], results[j]), ASC_ERR_INVALID_ARG, "%s: '%s' overlaps '%s'", what,
+                  results[i].name, results[j].name);
+    }
+    rc = check_apart(results[i], *a, plan.c, true, what);
+    if (rc != ASC_OK) return rc;
+  }
+  for (const asc::Region& x : operands) {
+    rc = check_apart(x, *a, plan.c, false, what);
+    if (rc != ASC_OK) return rc;
+  }
+  PlanArgs& p = plan.p;
+  p.table = a->block_table;
+  p.table_stride = a->table_stride;
+  p.lengths = a->lengths;
+  p.parents = a->parents;
+  p.refcounts = a->refcounts;
+  p.table_out = a->table_out;
+  p.table_out_stride = a->table_out_stride;
+  p.lengths_out = a->lengths_out;
+  p.refcounts_out = a->refcounts_out;
+  p.page_map = a->page_map;
+  p.page_size = static_cast<int32_t>(a->page_size);
+  p.pages = static_cast<int32_t>(a->num_pages);
+  p.batch = static_cast<int32_t>(a->batch);
+  p.new_batch = static_cast<int32_t>(a->new_batch);
+  p.width = static_cast<int32_t>(a->width);
+  return ASC_OK;
+}
+
+int32_t check_workspace(const void* workspace, int64_t bytes, int64_t need, const char* what) {
+  ASC_REQUIRE(workspace && bytes >= need && asc::aligned16(workspace), ASC_ERR_INVALID_ARG,
+              "%s: the workspace must hold %lld bytes, 16-byte aligned", what, static_cast<long long>(need));
+  return ASC_OK;
+}
+
+}  // namespace
+
+extern "C" int32_t asc_cache_copy_pages(const asc_pages_t* a, asc_stream_t stream) {
+  const char* what = "asc_cache_copy_pages";
+  ASC_REQUIRE(a, ASC_ERR_INVALID_ARG, "%s: null arguments", what);
+  ASC_REQUIRE(a->pairs >= 0 && a->num_pages >= 0 && a->to_num_pages >= 0, ASC_ERR_INVALID_ARG, "%s: negative shape", what);
+  CopyArgs c{};
+  int32_t rc = make_copy(*a, false, false, what, c);
+  if (rc != ASC_OK || a->pairs == 0 || c.n_tensors == 0) return rc;
+  ASC_REQUIRE(a->from_pages && a->to_pages, ASC_ERR_INVALID_ARG, "%s: null buffer", what);
+  ASC_REQUIRE(a->pairs < int64_t{1} << 31, ASC_ERR_UNSUPPORTED, "%s: too many pairs", what);
+  for (const asc::Region& x : {asc::region_of("from_pages", a->from_pages, a->pairs * 4),
+                               asc::region_of("to_pages", a->to_pages, a->pairs * 4)}) {
+    rc = check_apart(x, *a, c, false, what);
+    if (rc != ASC_OK) return rc;
+  }
+  c.moves = a->pairs;
+  c.from = a->from_pages;
+  c.to = a->to_pages;
+  hipLaunchKernelGGL(page_copy, dim3(static_cast<uint32_t>(groups_of(c.moves * c.per_move))), dim3(kThreads), 0,
+                     static_cast<hipStream_t>(stream), c);
+  return asc::check_launch(what);
+}
+
+extern "C" int64_t asc_cache_fork_workspace(const asc_pages_t* a) {
+  Plan plan;
+  return make_plan(a, true, "asc_cache_fork_workspace", plan) == ASC_OK ? fork_workspace(*a) : 0;
+}
+
+extern "C" int32_t asc_cache_fork(const asc_pages_t* a, void* workspace, int64_t workspace_bytes, asc_stream_t stream) {
+  const char* what = "asc_cache_fork";
+  Plan plan;
+  int32_t rc = make_plan(a, true, what, plan);
+  if (rc == ASC_OK) rc = check_workspace(workspace, workspace_bytes, fork_workspace(*a), what);
+  if (rc != ASC_OK) return rc;
+  const int64_t n = asc::ceil_div(a->new_batch, 4) * 4;
+  plan.p.count = static_cast<int32_t*>(workspace);
+  plan.p.from = plan.p.count + 4;
+  plan.p.to = plan.p.from + n;
+  plan.p.used = plan.p.to + n;
+  CopyArgs& c = plan.c;
+  c.moves = a->new_batch;
+  c.from = plan.p.from;
+  c.to = plan.p.to;
+  c.used = plan.p.used;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(fork_plan, dim3(1), dim3(kPlanThreads), 0, s, plan.p);
+  if (a->new_batch > 0) {
+    const int rows = static_cast<int>(a->new_batch < 256 ? a->new_batch : 256);
+    const int64_t groups = rows + groups_of(c.moves * c.per_move);
+    hipLaunchKernelGGL(fork_move, dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0, s, c, plan.p, rows);
+  }
+  return asc::check_launch(what);
+}
+
+extern "C" int64_t asc_cache_compact_workspace(const asc_pages_t* a) {
+  Plan plan;
+  return make_plan(a, false, "asc_cache_compact_workspace", plan) == ASC_OK ? compact_workspace(*a) : 0;
+}
+
+extern "C" int32_t asc_cache_compact(const asc_pages_t* a, void* workspace, int64_t workspace_bytes,
+                                     asc_stream_t stream) {
+  const char* what = "asc_cache_compact";
+  Plan plan;
+  int32_t rc = make_plan(a, false, what, plan);
+  if (rc == ASC_OK) rc = check_workspace(workspace, workspace_bytes, compact_workspace(*a), what);
+  if (rc != ASC_OK) return rc;
+  plan.p.count = static_cast<int32_t*>(workspace);
+  plan.p.from = plan.p.count + 4;
+  plan.p.to = plan.p.from + asc::ceil_div(a->num_pages, 4) * 4;
+  CopyArgs& c = plan.c;
+  c.moves = a->num_pages / 2;
+  c.count = plan.p.count;
+  c.from = plan.p.from;
+  c.to = plan.p.to;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(compact_plan, dim3(1), dim3(kPlanThreads), 0, s, plan.p);
+  const int rows = static_cast<int>(a->batch < 256 ? a->batch : 256);
+  const int64_t groups = rows + groups_of(c.moves * c.per_move);
+  if (groups > 0) {
+    hipLaunchKernelGGL(compact_move, dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0, s, c, plan.p, rows);
+  }
+  return asc::check_launch(what);
+}

@@ -997,6 +997,375 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _with_workspace("asc_tree_attention", args, q.device, stream)
 
 
+# -------------------------------------------------------------------------- a cache held in 8 bits
+
+_CACHE_CODES = {torch.int8: _native.DT_INT8, torch.float8_e4m3fn: _native.DT_FLOAT8_E4M3}
+_CACHE8 = struct.Struct("@6if6q" + "P3q" * 8 + "4Pq")  # asc_cache8_t
+
+
+def _strided(t: torch.Tensor, name: str, device: int, dims: int, written: bool) -> tuple:
+    """Address, strides and shape of a tensor of this device with so many dimensions."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != device:
+        _here(t, name, device)
+    shape = t.shape
+    if len(shape) != dims:
+        raise ValueError(f"'{name}' must have {dims} dimensions, got {tuple(shape)}")
+    if written and not t.is_contiguous():
+        _apart(t, name)
+    return t.data_ptr(), t.stride(), shape
+
+
+def _codes(t: torch.Tensor, name: str, dtype: torch.dtype, device: int, shape: Optional[tuple], written: bool) -> tuple:
+    """The codes of a cache, [pages, heads, rows, head_dim], as asc_rows_t's fields, and their shape."""
+    at, (s0, s1, s2, s3), size = _strided(t, name, device, 4, written)
+    if t.dtype is not dtype:
+        raise TypeError(f"'{name}' must be {dtype}, got {t.dtype}")
+    if shape is not None and size != shape:
+        raise ValueError(f"'{name}' must be {list(shape)}, got {tuple(size)}")
+    if s3 != 1 and size[3] > 1:
+        raise ValueError(f"the last dimension of '{name}' must be contiguous")
+    if (at | s0 | s1 | s2) & 15:
+        s0, s1, s2 = (s if n > 1 else 0 for s, n in zip((s0, s1, s2), size))
+        if (at | s0 | s1 | s2) & 15:
+            raise ValueError(f"'{name}' must be 16-byte aligned, with strides that are multiples of 16 "
+                             f"(address {at:#x}, strides {t.stride()})")
+    return (at, s0, s1, s2), size
+
+
+def _scales(t: torch.Tensor, name: str, device: int, pages: int, heads: int, rows: int, written: bool) -> tuple:
+    """The scales of a cache, [pages, heads, blocks], as asc_rows_t's fields, and the rows of a block."""
+    at, strides, size = _strided(t, name, device, 3, written)
+    if t.dtype is not torch.float32:
+        raise TypeError(f"'{name}' must be torch.float32, got {t.dtype}")
+    blocks = size[2]
+    if size[0] != pages or size[1] != heads or blocks == 0 and rows or blocks and rows % (16 * blocks):
+        raise ValueError(f"'{name}' must be [{pages}, {heads}, blocks] for blocks of a multiple of 16 rows that divide "
+                         f"the {rows} of a page, got {tuple(size)}")
+    return (at, *strides), rows // blocks if rows else 16
+
+
+def _table(t: torch.Tensor, name: str, device: int, batch: int) -> tuple:
+    """Address, row stride and width of an int32 table of pages."""
+    at, (row, step), size = _strided(t, name, device, 2, False)
+    if t.dtype is not torch.int32 or size[0] != batch:
+        raise ValueError(f"'{name}' must be int32 [{batch}, pages], got {t.dtype} {tuple(size)}")
+    if step != 1 and size[1] > 1:
+        raise ValueError(f"the last dimension of '{name}' must be contiguous")
+    return at, row, size[1]
+
+
+def _cache8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+            block_table: Optional[torch.Tensor], batch: int, device: int, written: bool = False) -> tuple:
+    """Checks a cache of 8 bits: its codes' and scales' rows, (cache dtype, head_dim, page_size, scale_block,
+    kv_heads, kv_len, pages), and the table's address and stride."""
+    if not isinstance(k_cache, torch.Tensor):
+        raise TypeError(f"'k_cache' must be a torch.Tensor, got {type(k_cache).__name__}")
+    dtype = k_cache.dtype
+    if dtype not in _CACHE_CODES:
+        raise TypeError(f"'k_cache' has unsupported dtype {dtype}; expected one of {sorted(map(str, _CACHE_CODES))}")
+    k_rows, shape = _codes(k_cache, "k_cache", dtype, device, None, written)
+    v_rows, _ = _codes(v_cache, "v_cache", dtype, device, shape, written)
+    pages, heads, rows, head_dim = shape
+    if head_dim not in FA_HEAD_DIMS:
+        raise ValueError(f"head_dim {head_dim} not supported (supported: {FA_HEAD_DIMS})")
+    ks_rows, block = _scales(k_scales, "k_scales", device, pages, heads, rows, written)
+    vs_rows, v_block = _scales(v_scales, "v_scales", device, pages, heads, rows, written)
+    if block != v_block:
+        raise ValueError(f"'k_scales' and 'v_scales' have blocks of {block} and {v_block} rows")
+    if block_table is None:
+        if pages != batch:
+            raise ValueError(f"a cache without a block_table must have {batch} sequences, got {pages}")
+        return (*k_rows, *v_rows, *ks_rows, *vs_rows), (_CACHE_CODES[dtype], head_dim, 0, block, heads, rows, pages), (0, 0)
+    table, stride, width = _table(block_table, "block_table", device, batch)
+    if rows == 0:
+        raise ValueError("pages without rows")
+    return ((*k_rows, *v_rows, *ks_rows, *vs_rows), (_CACHE_CODES[dtype], head_dim, rows, block, heads, width * rows, pages),
+            (table, stride))
+
+
+def quantized_cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                           k_scales: torch.Tensor, v_scales: torch.Tensor, cache_lengths: torch.Tensor,
+                           block_table: Optional[torch.Tensor] = None, new_lengths: Optional[torch.Tensor] = None,
+                           stream: Any = None) -> None:
+    """Writes new keys and values into a cache held in 8 bits, behind the tokens that it holds.
+
+    - k, v: float16 or bfloat16 [batch, kv_heads, n, head_dim] (64 or 128), rows 16-byte aligned, strides
+      multiples of 8.  new_lengths (int32 [batch]): new tokens of each sequence, default n.
+    - k_cache, v_cache: int8 or float8_e4m3fn codes, [batch, kv_heads, rows, head_dim], or with ``block_table``
+      (int32 [batch, pages of a sequence]) [pages, kv_heads, page size, head_dim]: key j of sequence b lies in
+      page block_table[b, j // page_size], row j % page_size.  cache_lengths (int32 [batch]): keys
+      before the call; token i becomes key cache_lengths[b] + i.
+    - k_scales, v_scales: float32 [pages, kv_heads, blocks], one for each block of page_size / blocks rows
+      (a multiple of 16) and head; a code stands for itself times its block's scale.
+
+    A block gets the least power of two (at least 2^-126) that holds its new rows' finite values, or keeps its
+    scale where that is enough; where earlier rows' scale has to grow, their codes are rounded
+    to the new one.  Rounded to nearest, ties to even; infinities become the largest code, NaN the NaN of e4m3 or 0
+    of int8.  A sequence whose lengths do not fit the cache, and a block whose page lies outside it, are left
+    as they were.  Pages that two sequences share must not be appended to."""
+    device = _current_device()
+    if not isinstance(k, torch.Tensor):
+        raise TypeError(f"'k' must be a torch.Tensor, got {type(k).__name__}")
+    dtype = k.dtype
+    if dtype not in _HALVES:
+        raise TypeError(f"'k' has unsupported dtype {dtype}; expected one of {sorted(map(str, _HALVES))}")
+    rows = _rows(k, "k", dtype, device, None, False, True)
+    shape = k.shape
+    batch, heads, n, head_dim = shape
+    rows += _rows(v, "v", dtype, device, shape, False, True)
+    cache, sizes, table = _cache8(k_cache, v_cache, k_scales, v_scales, block_table, batch, device, True)
+    if heads != sizes[4] or head_dim != sizes[1]:
+        raise ValueError(f"'k' {tuple(shape)} does not fit the cache {tuple(k_cache.shape)}")
+    lengths = _vector(cache_lengths, "cache_lengths", torch.int32, device, (batch,))
+    news = 0 if new_lengths is None else _vector(new_lengths, "new_lengths", torch.int32, device, (batch,))
+    args = _CACHE8.pack(_DTYPE_CODES[dtype], *sizes[:4], 0, 0.0, batch, 0, heads, n, *sizes[5:], *cache, *_NO_ROWS,
+                        *_NO_ROWS, *rows, 0, lengths, news, *table)
+    _launch("asc_quantized_cache_append", args, _stream(stream))
+
+
+def quantized_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                         starts: torch.Tensor, k_out: Optional[torch.Tensor], v_out: Optional[torch.Tensor],
+                         block_table: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
+                         stream: Any = None) -> None:
+    """The values of keys starts[b] + i (int32 [batch]) of a cache held in 8 bits, as quantized_cache_append's,
+    into k_out[b, :, i] and v_out[b, :, i] for i < counts[b] (int32 [batch], default n): float32, float16 or bfloat16
+    [batch, kv_heads, n, head_dim], either may be None.  Rows behind counts[b] are left as they were.  A
+    sequence whose keys do not fit the cache, and a key whose page lies outside it, give NaN."""
+    device = _current_device()
+    out = k_out if k_out is not None else v_out
+    if not isinstance(out, torch.Tensor):
+        raise TypeError("k_out or v_out must be a torch.Tensor")
+    dtype, shape = out.dtype, out.shape
+    if dtype not in _FLOATS or len(shape) != 4:
+        raise TypeError(f"results must be floats [batch, kv_heads, n, head_dim], got {dtype} {tuple(shape)}")
+    batch, heads, n, head_dim = shape
+    rows = ()
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        at, *strides = _NO_ROWS if t is None else _rows(t, name, dtype, device, shape, True)
+        if (at | (strides[0] | strides[1] | strides[2]) * out.element_size()) & 15:
+            strides = [s if size > 1 else 0 for s, size in zip(strides, shape)]
+            if (at | (strides[0] | strides[1] | strides[2]) * out.element_size()) & 15:
+                raise ValueError(f"'{name}' must be 16-byte aligned, with strides that are multiples of 16 bytes")
+        rows += (at, *strides)
+    cache, sizes, table = _cache8(k_cache, v_cache, k_scales, v_scales, block_table, batch, device)
+    if heads != sizes[4] or head_dim != sizes[1]:
+        raise ValueError(f"results {tuple(shape)} do not fit the cache {tuple(k_cache.shape)}")
+    lengths = _vector(starts, "starts", torch.int32, device, (batch,))
+    news = 0 if counts is None else _vector(counts, "counts", torch.int32, device, (batch,))
+    args = _CACHE8.pack(_DTYPE_CODES[dtype], *sizes[:4], 0, 0.0, batch, 0, heads, n, *sizes[5:], *cache, *_NO_ROWS,
+                        *_NO_ROWS, *rows, 0, lengths, news, *table)
+    _launch("asc_quantized_cache_read", args, _stream(stream))
+
+
+# ------------------------------------------------------------------------------ pages of a cache
+
+_PAGES_HEAD = struct.Struct("@8q3Pq4Pq3P")  # asc_pages_t before its tensors
+_PAGE_TENSOR = struct.Struct("@2P7q")
+_NO_PAGES = bytes(_PAGE_TENSOR.size * _native.MAX_PAGE_TENSORS)
+
+
+def _page_tensors(caches: Any, results: Any, device: int) -> tuple:
+    """The tensors of a cache as asc_page_tensor_t's, their number, and the pages of caches and results."""
+    if isinstance(caches, torch.Tensor):
+        caches = (caches,)
+    if isinstance(results, torch.Tensor):
+        results = (results,)
+    if len(caches) != len(results) or len(caches) > _native.MAX_PAGE_TENSORS:
+        raise ValueError(f"{len(caches)} caches and {len(results)} results (as many, at most {_native.MAX_PAGE_TENSORS})")
+    packed, pages, to_pages = b"", None, None
+    for x, y in zip(caches, results):
+        _here(x, "caches", device)
+        shape = x.shape
+        if len(shape) < 2:
+            raise ValueError(f"a cache must be [pages, heads, rows, ...], got {tuple(shape)}")
+        strides = x.stride()
+        to_shape, to_strides = shape, strides
+        if y is not x:
+            _here(y, "results", device)
+            to_shape, to_strides = y.shape, y.stride()
+            if y.dtype is not x.dtype or to_shape[1:] != shape[1:]:
+                raise ValueError(f"a result {y.dtype} {tuple(to_shape)} does not fit its cache {x.dtype} {tuple(shape)}")
+            if any(a != b for a, b, n in zip(strides[1:], to_strides[1:], shape[1:]) if n > 1):
+                raise ValueError("a cache and its result must have the same strides within a page")
+        if not y.is_contiguous():
+            _apart(y, "results")
+        if pages is None:
+            pages, to_pages = shape[0], to_shape[0]
+        elif shape[0] != pages or to_shape[0] != to_pages:
+            raise ValueError(f"caches of {pages} and {shape[0]} pages, results of {to_pages} and {to_shape[0]}")
+        size = x.element_size()
+        row = size  # what lies behind a row's first element
+        for n, s in zip(reversed(shape[3:]), reversed(strides[3:])):
+            if s * size != row and n > 1:
+                raise ValueError(f"the dimensions of a cache behind its rows must be contiguous (strides {strides})")
+            row *= n
+        if row == 0 or 0 in shape[1:]:
+            raise ValueError(f"a cache without elements: {tuple(shape)}")
+        rows, step = (shape[2], strides[2]) if len(shape) > 2 else (1, 0)
+        packed += _PAGE_TENSOR.pack(x.data_ptr(), y.data_ptr(), strides[0] * size, to_strides[0] * size, shape[1], rows, row,
+                                    strides[1] * size, step * size)
+    return packed + _NO_PAGES[len(packed):], len(caches), pages or 0, to_pages or 0
+
+
+def cache_copy_pages(caches: Any, results: Any, from_pages: torch.Tensor, to_pages: torch.Tensor,
+                     stream: Any = None) -> None:
+    """Page to_pages[i] of each result becomes page from_pages[i] of its cache (both int32 [pairs]): up to eight
+    tensors whose first dimension is the pages (keys, values, their scales), of any type, in one launch.
+    A result may be its cache.  Pairs with a page outside the tensors are left out.  A page that is written
+    must be in no other pair: it would hold parts of both."""
+    device = _current_device()
+    tensors, number, pages, into = _page_tensors(caches, results, device)
+    _here(from_pages, "from_pages", device)
+    if from_pages.dim() != 1:
+        raise ValueError(f"'from_pages' must be a vector, got {tuple(from_pages.shape)}")
+    pairs = from_pages.numel()
+    source = _vector(from_pages, "from_pages", torch.int32, device, (pairs,))
+    target = _vector(to_pages, "to_pages", torch.int32, device, (pairs,))
+    args = _PAGES_HEAD.pack(number, 1, pages, into, pairs, 0, 0, 0, source, target, *(0,) * 10) + tensors
+    _launch("asc_cache_copy_pages", args, _stream(stream))
+
+
+def _books(block_table: torch.Tensor, lengths: torch.Tensor, refcounts: torch.Tensor, refcounts_out: torch.Tensor,
+           page_size: int, pages: Optional[int], device: int) -> tuple:
+    """The bookkeeping that fork and compact share: batch, width, pages, and the addresses."""
+    _here(block_table, "block_table", device)
+    batch = block_table.shape[0] if block_table.dim() == 2 else -1
+    table, stride, width = _table(block_table, "block_table", device, batch)
+    _here(refcounts, "refcounts", device)
+    pages = refcounts.numel() if pages is None else pages
+    counts = _vector(refcounts, "refcounts", torch.int32, device, (pages,))
+    counts_out = _vector(refcounts_out, "refcounts_out", torch.int32, device, (pages,))
+    if page_size < 1:
+        raise ValueError(f"page_size must be positive, got {page_size}")
+    return batch, width, pages, table, stride, _vector(lengths, "lengths", torch.int32, device, (batch,)), counts, counts_out
+
+
+def _table_out(t: torch.Tensor, device: int, rows: int, width: int) -> tuple:
+    at, stride, columns = _table(t, "table_out", device, rows)
+    if columns != width:
+        raise ValueError(f"'table_out' must be [{rows}, {width}], got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        _apart(t, "table_out")
+    return at, stride
+
+
+def cache_fork(caches: Any, block_table: torch.Tensor, lengths: torch.Tensor, parents: torch.Tensor,
+               refcounts: torch.Tensor, page_size: int, table_out: torch.Tensor, lengths_out: torch.Tensor,
+               refcounts_out: torch.Tensor, stream: Any = None) -> None:
+    """The sequences of a paged cache become others: sequence i goes on from sequence parents[i] (int32 [new
+    batch]; outside the batch: it holds nothing, so its pages are free if nobody else has them).
+
+    - caches: up to eight tensors [pages, heads, rows, ...] of any type (keys, values, their scales);
+      page_size is a multiple of each one's rows.
+    - block_table (int32 [batch, width]), lengths (int32 [batch]): the sequences before; table_out (int32
+      [new batch, width], -1 behind a sequence's pages) and lengths_out (int32 [new batch]): after.
+    - refcounts (int32 [pages]): how many sequences hold a page, 0: free; refcounts_out, which may be
+      refcounts: after.
+
+    Full pages are shared.  The last page, where it is partly filled, stays with the first child; each other child
+    gets a free page with its rows: the lowest free ones, in the children's order, -1 where there is none
+    left.  A length outside the table is handed on, with a row of -1.  At most 4096 sequences."""
+    device = _current_device()
+    tensors, number, pages, _ = _page_tensors(caches, caches, device)
+    batch, width, pages, table, stride, length, counts, counts_out = _books(
+        block_table, lengths, refcounts, refcounts_out, page_size, pages if number else None, device)
+    _here(parents, "parents", device)
+    new = parents.numel()
+    parent = _vector(parents, "parents", torch.int32, device, (new,))
+    out, out_stride = _table_out(table_out, device, new, width)
+    args = _PAGES_HEAD.pack(number, page_size, pages, pages, 0, batch, new, width, 0, 0, table, stride, length, parent,
+                            counts, out, out_stride, _vector(lengths_out, "lengths_out", torch.int32, device, (new,)),
+                            counts_out, 0) + tensors
+    _with_workspace("asc_cache_fork", args, block_table.device, stream)
+
+
+def cache_compact(caches: Any, block_table: torch.Tensor, lengths: torch.Tensor, refcounts: torch.Tensor,
+                  page_size: int, table_out: torch.Tensor, refcounts_out: torch.Tensor, page_map: torch.Tensor,
+                  stream: Any = None) -> None:
+    """Brings the pages in use (refcounts > 0), U of them, to the front of a paged cache: the i-th of those at U and
+    above moves into the i-th free one below.  Tensors, tables and counts as cache_fork's; table_out may be
+    block_table, refcounts_out refcounts.  page_map (int32 [pages]) receives each page's new place, -1 for free
+    ones: holders outside the table have it to go by."""
+    device = _current_device()
+    tensors, number, pages, _ = _page_tensors(caches, caches, device)
+    batch, width, pages, table, stride, length, counts, counts_out = _books(
+        block_table, lengths, refcounts, refcounts_out, page_size, pages if number else None, device)
+    out, out_stride = _table_out(table_out, device, batch, width)
+    args = _PAGES_HEAD.pack(number, page_size, pages, pages, 0, batch, 0, width, 0, 0, table, stride, length, 0, counts,
+                            out, out_stride, 0, counts_out,
+                            _vector(page_map, "page_map", torch.int32, device, (pages,))) + tensors
+    _with_workspace("asc_cache_compact", args, block_table.device, stream)
+
+
+# ------------------------------------------------------------------ logits before a token is chosen
+
+_LOGITS = struct.Struct("@2i3qPqPqPq6PqPq")  # asc_logits_t
+
+
+def _matrix(t: torch.Tensor, name: str, dtype: torch.dtype, device: int, shape: tuple, written: bool = False) -> tuple:
+    """Address and row stride of a matrix whose rows are contiguous."""
+    at, (row, step), size = _strided(t, name, device, 2, written)
+    if t.dtype is not dtype:
+        raise TypeError(f"'{name}' must be {dtype}, got {t.dtype}")
+    if size != shape:
+        raise ValueError(f"'{name}' must be {list(shape)}, got {tuple(size)}")
+    if step != 1 and size[1] > 1:
+        raise ValueError(f"the last dimension of '{name}' must be contiguous")
+    return at, row
+
+
+def process_logits(logits: torch.Tensor, out: torch.Tensor, history: torch.Tensor, history_lengths: torch.Tensor,
+                   prompt_lengths: Optional[torch.Tensor] = None, repetition: Optional[torch.Tensor] = None,
+                   frequency: Optional[torch.Tensor] = None, presence: Optional[torch.Tensor] = None,
+                   bias: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None, stream: Any = None) -> None:
+    """Logits [rows, vocabulary] (float32, float16 or bfloat16) before a token is chosen, into ``out`` (which may be
+    logits), computed in float32 in this order:
+
+    - a token of the row's history: x / repetition if x > 0, else x * repetition;
+    - one that comes c times in it behind the prompt: x - frequency * c, and if c > 0 - presence;
+    - x + bias (float32 [vocabulary] or [rows, vocabulary]);
+    - -inf where its bit is 0 in mask (int32 [rows, ceil(vocabulary / 32)]: token t is bit t % 32 of word t // 32),
+      whatever x is; a row whose mask leaves nothing is -inf throughout.
+
+    history (int32 or int64 [rows, width]): the row's first history_lengths (int32 [rows]) tokens, of which the
+    first prompt_lengths (int32 [rows], default none) are the prompt; tokens outside the vocabulary
+    are passed over.  repetition, frequency, presence: float32 [rows].  A history length outside [0, width] gives
+    NaN."""
+    device = _current_device()
+    if not isinstance(logits, torch.Tensor):
+        raise TypeError(f"'logits' must be a torch.Tensor, got {type(logits).__name__}")
+    dtype, shape = logits.dtype, logits.shape
+    if dtype not in _FLOATS:
+        raise TypeError(f"'logits' has unsupported dtype {dtype}; expected one of {sorted(map(str, _FLOATS))}")
+    if len(shape) != 2:
+        raise ValueError(f"'logits' must be [rows, vocabulary], got {tuple(shape)}")
+    rows, vocab = shape
+    x = _matrix(logits, "logits", dtype, device, shape)
+    y = x if out is logits and logits.is_contiguous() else _matrix(out, "out", dtype, device, shape, True)
+    _here(history, "history", device)
+    wide = history.dtype is torch.int64
+    if (not wide and history.dtype is not torch.int32) or history.dim() != 2:
+        raise TypeError(f"'history' must be int32 or int64 [{rows}, width], got {history.dtype} {tuple(history.shape)}")
+    width = history.shape[1]
+    h = _matrix(history, "history", history.dtype, device, (rows, width))
+    per_row = (rows,)
+    lengths = _vector(history_lengths, "history_lengths", torch.int32, device, per_row)
+    prompts = 0 if prompt_lengths is None else _vector(prompt_lengths, "prompt_lengths", torch.int32, device, per_row)
+    r = 0 if repetition is None else _vector(repetition, "repetition", torch.float32, device, per_row)
+    f = 0 if frequency is None else _vector(frequency, "frequency", torch.float32, device, per_row)
+    p = 0 if presence is None else _vector(presence, "presence", torch.float32, device, per_row)
+    b = m = (0, 0)
+    if bias is not None:
+        if isinstance(bias, torch.Tensor) and bias.dim() == 1:
+            b = (_vector(bias, "bias", torch.float32, device, (vocab,)), 0)
+        else:
+            b = _matrix(bias, "bias", torch.float32, device, shape)
+    if mask is not None:
+        m = _matrix(mask, "mask", torch.int32, device, (rows, -(-vocab // 32)))
+    _launch("asc_process_logits", _LOGITS.pack(_DTYPE_CODES[dtype], wide, rows, vocab, width, *x, *y, *h, lengths, prompts, r, f,
+                                               p, *b, *m), _stream(stream))
+
+
 # ------------------------------------------------------------------ element-wise tile operations
 
 UNARY_OPS = ("abs", "ceil", "cos", "cosh", "erf", "exp", "exp2", "floor", "log", "log2", "negative", "relu",

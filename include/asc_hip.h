@@ -579,6 +579,14 @@ int32_t asc_cross_attention_bwd(const asc_attention_t* args, void* workspace,
  *     i for i < n, or new_lengths[b]; rows behind these are left as they were.  A sequence
  *     whose lengths do not fit the cache, and a key whose page lies outside it, give NaN.
  *     Either of k and v may be left out (k_new.data NULL).  dtype may be ASC_DT_FLOAT32 too.
+ * asc_quantized_cache_attention  o = softmax(q k^T sm_scale) v over the first lengths[b] keys,
+ *     fp32 statistics, query head h with key / value head h / (q_heads / kv_heads).  The queries
+ *     are those of the sequence's last new_lengths[b] (NULL: n) keys: with causal != 0
+ *     query i attends the first lengths[b] - new_lengths[b] + i + 1 of them.  Queries
+ *     behind new_lengths[b] are not written, none of a negative number.  A query without
+ *     keys gets zeros, and -inf for its lse (fp32 [batch, q_heads, n], may be NULL).  A
+ *     length outside the cache, a page outside it that a length reaches, or more
+ *     queries than n: NaN.  `workspace` holds _workspace bytes, 16-byte aligned.
  * A result that shares a byte with an operand or another result is refused. */
 typedef struct asc_cache8 {
   int32_t dtype, cache_dtype; /* of queries, results and new rows; ASC_DT_INT8 or ASC_DT_FLOAT8_E4M3 */
@@ -596,6 +604,12 @@ typedef struct asc_cache8 {
 } asc_cache8_t;
 int32_t asc_quantized_cache_append(const asc_cache8_t* args, asc_stream_t stream);
 int32_t asc_quantized_cache_read(const asc_cache8_t* args, asc_stream_t stream);
+int64_t asc_quantized_cache_attention_workspace(const asc_cache8_t* args);
+int32_t asc_quantized_cache_attention(const asc_cache8_t* args, void* workspace,
+                                      int64_t workspace_bytes, asc_stream_t stream);
+/* The launch that asc_quantized_cache_attention makes: cache8_narrow, up to 32 rows a
+ * workgroup, or cache8_wide; a row is a query of one of the heads that share a key / value head. */
+int32_t asc_quantized_cache_attention_plan(const asc_cache8_t* args, asc_attention_plan_t* plan);
 
 /* ---- pages of a cache -----------------------------------------------------------
  * Tensors whose first dimension is a cache's pages, of any type: [pages, heads, rows of

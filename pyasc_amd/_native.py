@@ -180,6 +180,9 @@ SIGNATURES = {
     "asc_attention_plan": [_c_p, _c_i32, ctypes.POINTER(AttentionPlan)],
     "asc_quantized_cache_append": [_c_p, _c_p],
     "asc_quantized_cache_read": [_c_p, _c_p],
+    "asc_quantized_cache_attention_workspace": [_c_p],
+    "asc_quantized_cache_attention": [_c_p, _c_p, _c_i64, _c_p],
+    "asc_quantized_cache_attention_plan": [_c_p, ctypes.POINTER(AttentionPlan)],
     "asc_cache_copy_pages": [_c_p, _c_p],
     "asc_cache_fork_workspace": [_c_p],
     "asc_cache_fork": [_c_p, _c_p, _c_i64, _c_p],
@@ -200,7 +203,8 @@ SIGNATURES = {
 }
 INT64_FUNCS = ("asc_qk_norm_rotary_bwd_workspace", "asc_cross_attention_fwd_workspace",
                "asc_cross_attention_bwd_workspace",
-               "asc_tree_attention_workspace", "asc_cache_fork_workspace", "asc_cache_compact_workspace")
+               "asc_tree_attention_workspace", "asc_cache_fork_workspace", "asc_cache_compact_workspace",
+               "asc_quantized_cache_attention_workspace")
 # entry points returning a C string
 STRING_FUNCS = ("asc_last_error", "asc_version")
 

@@ -1,0 +1,947 @@
+// Attention over a cache held in 8 bits: the device code of asc_quantized_cache_attention.
+//
+// The queries that share a key / value head are its rows: row r is query r % n of the head's query head r / n.
+// With codes c and a scale per block, k_j = ks_j ck_j and v_j = vs_j cv_j, so
+//   s_j = (q . ck_j) (sm_scale ks_j),   o = sum_j (p_j vs_j) cv_j / sum_j p_j,   p_j = exp(s_j - m):
+// the codes go to the matrix units as they are, in fp16, which holds all of them exactly, K's scales go into the
+// scores' factor and V's into the probabilities.  A tile has 64 keys, of 16 of which each group lies in one
+// block and one page, so a lane has four factors per tile.  P^T's values p_j vs_j / R (R: the largest V scale so far)
+// are at most p_j: exp2 takes log2(vs_j / R) with the scores' shift, and the sums over a group are divided by
+// vs_j / R again for the denominator.  Queries of bf16 are brought to fp16's range by a power of two of
+// their row: exact, but for elements 2^-39 and less of the row's largest.
+//
+// The probabilities are rounded to fp16 for the product with the values, as matrix operands have to be:
+// errors of 0.0002 of the results' norm, beside 0.0017 of a bf16 result's own rounding.
+#pragma once
+
+#include "cache8.h"
+#include "flash_attn_kernels.h"
+#include "kv_attn_kernels.h"
+
+namespace asc {
+namespace c8 {
+
+using fa::BKV;
+using fa::F16;
+using fa::f32x16;
+using fa::lds_addr;
+using fa::other_half;
+using kv::f32x4;
+
+constexpr int kGroup = 16, kGroups = BKV / kGroup;
+
+struct AttnArgs {
+  Cache c;
+  const uint16_t* q;
+  uint16_t* o;
+  float* lse;  // [batch, q_heads, n] or null
+  int64_t q_batch, q_head, q_seq, o_batch, o_head, o_seq;  // elements
+  float* part_o;   // [unit][rows][D], unnormalised
+  float* part_ml;  // [unit][rows][2]: reference point (log2), sum
+  int32_t batch, group, rows, row_blocks, splits, join_groups, causal;
+  uint32_t units;  // batch * splits * kv_heads
+  float scale_log2;
+};
+
+// Four codes of a word as two packed pairs of fp16.
+template <class Q>
+__device__ __forceinline__ u32x2 codes_to_f16(uint32_t w) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  if constexpr (__is_same(Q, Int8)) {
+    // 1024 + (c + 128) has c + 128 as its lowest bits
+    w ^= 0x80808080u;
+    const f16x2 lift = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+    const f16x2 lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - lift;
+    const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - lift;
+    return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+  } else {
+    const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
+    const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
+    return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+  }
+}
+template <class Q>
+__device__ __forceinline__ u32x4 operand_of(uint32_t lo, uint32_t hi) {
+  const u32x2 a = codes_to_f16<Q>(lo), b = codes_to_f16<Q>(hi);
+  return u32x4{a[0], a[1], b[0], b[1]};
+}
+
+// One workgroup's share, as kv::Share.
+__device__ __forceinline__ kv::Share share_of(const AttnArgs& p) {
+  const uint32_t slot = blockIdx.x >> 3;
+  const uint32_t per = slot / p.row_blocks;
+  kv::Share s;
+  s.unit = per * 8 + (blockIdx.x & 7);
+  s.live = s.unit < p.units;
+  s.row0 = p.row_blocks - 1 - static_cast<int>(slot - per * p.row_blocks);  // causal: the longest first
+  const uint32_t range = s.unit / p.c.kv_heads;
+  s.head = static_cast<int>(s.unit - range * p.c.kv_heads);
+  s.b = static_cast<int>(range / p.splits);
+  s.split = static_cast<int>(range - static_cast<uint32_t>(s.b) * p.splits);
+  return s;
+}
+
+// What a sequence has: its keys, and its queries among n.
+struct Sequence {
+  int len, news, first;  // query i attends the first min(first + i, len) keys
+  bool bad;
+  __device__ __forceinline__ Sequence(const AttnArgs& p, int b) {
+    bad = false;
+    len = kv::clamped(p.c.lengths[b], p.c.capacity, bad);
+    news = kv::clamped(p.c.news ? p.c.news[b] : p.c.n, p.c.n, bad);
+    first = p.causal ? len - news + 1 : len;
+  }
+  __device__ __forceinline__ int limit(int query) const { return min(max(first + query, 0), len); }
+};
+// Queries of sequence b that are written (more than n: all of them, as NaN).
+__device__ __forceinline__ int written_of(const AttnArgs& p, int b) { return p.c.news ? p.c.news[b] : p.c.n; }
+
+// The most keys that a row of row0 .. row0 + rows - 1 attends.
+__device__ __forceinline__ int limit_of_rows(const AttnArgs& p, const Sequence& s, int row0, int rows) {
+  const int last = min(row0 + rows, p.rows) - 1;
+  const int g = row0 / p.c.n;
+  const int query = last / p.c.n == g ? last - g * p.c.n : p.c.n - 1;
+  const int q = min(query, s.news - 1);
+  return q < 0 ? 0 : s.limit(q);
+}
+
+// The fewest keys that a row of row0 .. row0 + rows - 1 with a query attends.
+__device__ __forceinline__ int least_of_rows(const AttnArgs& p, const Sequence& s, int row0, int rows) {
+  const int last = min(row0 + rows, p.rows) - 1;
+  const int g = row0 / p.c.n, query = row0 - g * p.c.n;
+  // the first row's, where they are of one head; else a head's first query is among them
+  if (last / p.c.n == g) return query < s.news ? s.limit(query) : s.len;
+  return s.news > 0 ? s.limit(0) : s.len;
+}
+
+// Output row `row` of the share, false where nothing is written.
+__device__ __forceinline__ bool out_row(const AttnArgs& p, const kv::Share& s, int row, int written, int64_t& o_at,
+                                        int64_t& lse_at) {
+  if (row >= p.rows) return false;
+  const int g = row / p.c.n, query = row - g * p.c.n;
+  if (query >= written) return false;
+  const int64_t head = s.head * p.group + g;
+  o_at = s.b * p.o_batch + head * p.o_head + query * p.o_seq;
+  lse_at = (static_cast<int64_t>(s.b) * p.c.kv_heads * p.group + head) * p.c.n + query;
+  return true;
+}
+
+// This lane's row: its query (-1: none), its keys, and its elements in fp16.  kPairs: lane half h holds columns
+// 32 t + 16 h + 0..15 in operands 2 t and 2 t + 1 (as K's codes are read), else 16 k + 8 h + 0..7 in operand k.
+template <int D, class E, bool kPairs>
+__device__ __forceinline__ void load_query(const AttnArgs& p, const kv::Share& s, const Sequence& seq, int row, int h,
+                                           u32x4 (&q)[D / 16], int& limit, float& factor) {
+  int query = -1;
+  int64_t at = 0;
+  if (row < p.rows) {
+    const int g = row / p.c.n;
+    query = row - g * p.c.n;
+    at = s.b * p.q_batch + static_cast<int64_t>(s.head * p.group + g) * p.q_head + query * p.q_seq;
+  }
+  if (query >= seq.news) query = -1;
+  limit = query >= 0 ? seq.limit(query) : seq.len;  // a row without a query restricts nothing
+  factor = p.scale_log2;
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) {
+    const int column = kPairs ? (k >> 1) * 32 + h * 16 + (k & 1) * 8 : k * 16 + h * 8;
+    q[k] = u32x4{0, 0, 0, 0};
+    if (query >= 0) q[k] = *reinterpret_cast<const u32x4*>(p.q + at + column);
+  }
+  if constexpr (__is_same(E, fa::Bf16)) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) most = max(most, max(q[k][w] & 0x7fffu, q[k][w] >> 16 & 0x7fffu));
+    most = max(most, __float_as_uint(other_half(__uint_as_float(most))));
+    // the largest lands in [2^14, 2^15)
+    const uint32_t exponent = max(most >> 7, 14u);
+    const int up = exponent == 255 ? 0 : 141 - static_cast<int>(exponent);
+    const float scale = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+    factor = ldexpf(p.scale_log2, -up);
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        q[k][w] = F16::pack(__uint_as_float(q[k][w] << 16) * scale, __uint_as_float(q[k][w] & 0xffff0000u) * scale);
+      }
+  }
+}
+
+// The places of a tile's groups: lane l works out that of group l % 4.
+struct Places {
+  uint32_t k, v;    // of the group's first row, units of 16 bytes
+  uint32_t ks, vs;  // of its block's scales
+};
+
+struct Rows {
+  uint32_t k0, v0, ks0, vs0;  // the sequence's head
+  const int32_t* table;       // null: one piece
+  int len, b;
+  bool poison;
+
+  __device__ __forceinline__ void init(const AttnArgs& p, const kv::Share& s, const Sequence& seq) {
+    k0 = s.head * p.c.ks.head;
+    v0 = s.head * p.c.vs.head;
+    ks0 = s.head * p.c.kss.head;
+    vs0 = s.head * p.c.vss.head;
+    table = p.c.table ? p.c.table + s.b * p.c.table_stride : nullptr;
+    len = seq.len;
+    b = s.b;
+    poison = seq.bad;
+  }
+  // First key of this lane's group of tile j: groups behind the last key are read as its group.
+  __device__ __forceinline__ uint32_t key_of(int j, int lane) const {
+    return min(j * BKV + (lane & (kGroups - 1)) * kGroup, (len - 1) & ~(kGroup - 1));
+  }
+  // Address of the entry of the table: without one of something that can be read.
+  __device__ __forceinline__ const int32_t* entry(const AttnArgs& p, int j, int lane) const {
+    return table ? table + p.c.page.divide(key_of(j, lane)) : p.c.lengths + b;
+  }
+  __device__ __forceinline__ Places places(const AttnArgs& p, int j, int lane, uint32_t id) {
+    const uint32_t key = key_of(j, lane);
+    const uint32_t row = key - p.c.page.divide(key) * p.c.page.d;
+    if (!table) id = b;
+    const bool bad = id >= p.c.pages;
+    poison = poison || __builtin_amdgcn_ballot_w64(bad) != 0;
+    if (bad) id = 0;
+    const uint32_t block = p.c.block.divide(row);
+    Places r;
+    r.k = k0 + id * p.c.ks.page + row * p.c.ks.row;
+    r.v = v0 + id * p.c.vs.page + row * p.c.vs.row;
+    r.ks = ks0 + id * p.c.kss.page + block * p.c.kss.row;
+    r.vs = vs0 + id * p.c.vss.page + block * p.c.vss.row;
+    return r;
+  }
+};
+
+// The online softmax of a wave: lane (row, half h of the keys); register r of score block kb is key 32 kb + 8 (r / 4) +
+// 4 h + r % 4, of group 2 kb + r / 8.
+template <int D>
+struct Softmax {
+  static constexpr int kDBlocks = D / 32;
+  f32x16 acc[kDBlocks];  // in units of R
+  float m, l;            // reference point (log2) and this lane half's sum
+  float factor;          // of the raw scores of a unit scale (log2)
+  float R;               // largest V scale so far
+  int limit;             // keys of the row
+  float a[kGroups];      // factors of the tile's groups
+  float shift[kGroups];  // log2 of V scale / R
+  float undo[kGroups];   // R / V scale
+
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int i = 0; i < kDBlocks; ++i) acc[i] = f32x16{};
+    m = -INFINITY;
+    l = 0.f;
+    R = 0.f;
+  }
+  // The tile's scales, of group l % 4 in lane l.  A V scale below 2^-40 R counts as that: its values times p stay
+  // below fp16's smallest.
+  __device__ __forceinline__ void set_scales(float ks, float vs) {
+    float top = fmaxf(vs, dpp_mov<kDppQuadXor1>(vs));
+    top = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, fmaxf(top, dpp_mov<kDppQuadXor2>(top)))));
+    if (top > R) {
+      const float down = R / top;
+#pragma unroll
+      for (int i = 0; i < kDBlocks; ++i) acc[i] *= down;
+      R = top;
+    }
+    const float ratio = fmaxf(vs / R, 0x1p-40f);
+    const float log_ratio = __builtin_amdgcn_logf(ratio), inverse = 1.0f / ratio;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      // not zero, which times the -inf of a hidden key would be NaN
+      a[g] = fmaxf(factor * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), g)), 0x1p-126f);
+      shift[g] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, log_ratio), g));
+      undo[g] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, inverse), g));
+    }
+  }
+  __device__ __forceinline__ void hide(f32x16 (&s)[2], int j, int h) const {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        if (j * BKV + kb * 32 + (r >> 2) * 8 + h * 4 + (r & 3) >= limit) s[kb][r] = -INFINITY;
+      }
+  }
+  // Largest score of the tile, less fp16's lift.
+  __device__ __forceinline__ float tile_max(const f32x16 (&s)[2]) const {
+    float top = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      float t = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) t = fmaxf(t, s[g >> 1][(g & 1) * 8 + r]);
+      top = fmaxf(top, t * a[g]);
+    }
+    return fmaxf(top, other_half(top)) - F16::kLift;
+  }
+  __device__ __forceinline__ void raise(float top) {
+    const bool up = top > m;
+    const float alpha = up ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
+    if (up) m = top;
+    l *= alpha;
+#pragma unroll
+    for (int i = 0; i < kDBlocks; ++i) acc[i] *= alpha;
+  }
+  __device__ __forceinline__ float reference() const { return m == -INFINITY ? 0.f : -m; }
+  // Values 2 w and 2 w + 1 of group g, and their sum.
+  __device__ __forceinline__ void pair(const f32x16 (&s)[2], int g, int w, float ref, u32x4 (&pb)[2][2], float& sum) const {
+    const int kb = g >> 1, u = g & 1;
+    const float e0 = __builtin_amdgcn_exp2f(fmaf(s[kb][8 * u + 2 * w], a[g], ref + shift[g]));
+    const float e1 = __builtin_amdgcn_exp2f(fmaf(s[kb][8 * u + 2 * w + 1], a[g], ref + shift[g]));
+    sum += e0;
+    sum += e1;
+    pb[kb][u][w] = F16::pack(e0, e1);
+  }
+  // P^T operands of the tile; returns this lane's sum of probabilities.
+  __device__ __forceinline__ float probs(const f32x16 (&s)[2], u32x4 (&pb)[2][2]) const {
+    const float ref = reference();
+    float rs = 0.f;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) pair(s, g, w, ref, pb, sum);
+      rs = fmaf(sum, undo[g], rs);
+    }
+    return rs;
+  }
+  __device__ __forceinline__ bool out_of_range(float sum) const {
+    return __builtin_amdgcn_ballot_w64(sum > F16::kTileSumLimit || m == -INFINITY) != 0;
+  }
+  __device__ __forceinline__ void guard(const f32x16 (&s)[2], u32x4 (&pb)[2][2], float& rs) {
+    if (out_of_range(rs)) {
+      raise(tile_max(s));
+      rs = probs(s, pb);
+    }
+    l += rs;
+  }
+
+  // A NaN among the values of keys that only some rows attend is taken as zero in the products, whose 0 times NaN
+  // would reach all rows (without_nan).  Where that was met, the rows that attend it get it back: tile j, from memory.
+  __device__ __forceinline__ void add_nan(const AttnArgs& p, const kv::Share& s, int j, int h) {
+    for (int i = 0; i < BKV; ++i) {
+      const int key = j * BKV + i;
+      uint32_t page, row;
+      if (__builtin_amdgcn_ballot_w64(key < limit) == 0) return;
+      if (!place(p.c, s.b, key, page, row)) continue;  // NaN already
+      const uint8_t* v = p.c.v + row_at(p.c.vs, page, s.head, row) + h * 4;
+#pragma unroll
+      for (int db = 0; db < kDBlocks; ++db)
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq) {
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(v + db * 32 + rq * 8);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (key < limit && (w >> (8 * e) & 0x7fu) == 0x7fu) acc[db][rq * 4 + e] = __builtin_nanf("");
+          }
+        }
+    }
+  }
+};
+
+// A word of e4m3 codes with zeros in place of NaN, noted in `found`.
+__device__ __forceinline__ uint32_t without_nan(uint32_t w, uint32_t& found) {
+  const uint32_t nan = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+  found |= nan;
+  return w & ~((nan >> 7) * 0xffu);
+}
+
+// ------------------------------------------------------------------------------------ few rows
+
+template <int D>
+struct Narrow {
+  static constexpr int kWaves = 4, kWgPerCu = D == 128 ? 2 : 3;
+  static constexpr int kRows = 32;
+  static constexpr int kTile = BKV * D;           // bytes
+  static constexpr int kLoads = kTile / 1024;     // of a wave
+  static constexpr int kRowsPerLoad = 1024 / D;
+  static constexpr int kScaleBytes = 3 * 256;     // table entries, K's and V's scales of each lane
+};
+
+// One wave's tiles: codes in LDS as they are, in 16-byte chunks whose place in a row is flipped by the row so that 16
+// rows' reads of a chunk (K) and a transposing read's eight rows (V) lie in different banks.
+template <int D, class Q>
+struct NarrowTiles {
+  using N = Narrow<D>;
+  static constexpr int kChunks = D / 16;
+  uint8_t* k;
+  uint8_t* v;
+  uint8_t* meta;
+  int lane, col, h;
+  uint32_t kaddr, vaddr;
+  uint32_t koff[2], voff[2];
+
+  static __device__ __forceinline__ int kflip(int row) { return D == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
+  static __device__ __forceinline__ int vflip(int row) {
+    return D == 128 ? ((row >> 1) & 1) * 2 + ((row >> 3) & 1) * 4 : ((row >> 3) & 1) * 2;
+  }
+  __device__ __forceinline__ void init(const AttnArgs& p) {
+    kaddr = lds_addr(k) + col * D + ((h ^ kflip(col)) << 4);
+    // lane 2 i + half of a group of 16 reads half a chunk of row i; lane i receives column i of eight rows
+    const int i = (lane & 15) >> 1, row = h * 4 + (i & 3) + (i >> 2) * 8;
+    vaddr = lds_addr(v) + row * D + ((((lane >> 4) & 1) ^ vflip(row)) << 4) + (lane & 1) * 8;
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) {
+      const int in_group = (D == 128 ? odd * 8 : 0) + lane / kChunks, pos = lane % kChunks;
+      koff[odd] = in_group * p.c.ks.row * 16 + ((pos ^ kflip(in_group)) << 4);
+      voff[odd] = in_group * p.c.vs.row * 16 + ((pos ^ vflip(in_group)) << 4);
+    }
+  }
+  template <bool kIsV>
+  __device__ __forceinline__ void load(const AttnArgs& p, uint32_t places) const {
+    const uint64_t base = reinterpret_cast<uint64_t>(kIsV ? p.c.v : p.c.k);
+    uint8_t* dst = kIsV ? v : k;
+#pragma unroll
+    for (int i = 0; i < N::kLoads; ++i) {
+      const uint32_t place = __builtin_amdgcn_readlane(places, D == 128 ? i >> 1 : i);
+      const uint8_t* src = reinterpret_cast<const uint8_t*>(base + static_cast<uint64_t>(place) * 16);
+      const uint32_t off = kIsV ? voff[i & 1] : koff[i & 1];
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + off),
+                                       (__attribute__((address_space(3))) void*)(dst + i * 1024), 16, 0, 0);
+    }
+  }
+  // A word per lane into the wave's slot `slot`.
+  __device__ __forceinline__ void load_word(const void* src, int slot) const {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                     (__attribute__((address_space(3))) void*)(meta + slot * 256), 4, 0, 0);
+  }
+  __device__ __forceinline__ uint32_t word(int slot) const {
+    uint32_t r;
+    asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(r) : "v"(lds_addr(meta) + slot * 256 + lane * 4) : "memory");
+    return r;
+  }
+  // Raw scores of the tile.
+  __device__ __forceinline__ void scores(const u32x4 (&q)[D / 16], f32x16 (&s)[2]) const {
+    constexpr int kPairs = D / 32, kReads = 2 * kPairs, kWin = 4;
+    u32x4 x[kReads];
+#pragma unroll
+    for (int r = 0; r < kWin && r < kReads; ++r) x[r] = fa::lds_read_b128(kaddr ^ ((r % kPairs) << 5), r / kPairs * 32 * D);
+    s[0] = f32x16{};
+    s[1] = f32x16{};
+#pragma unroll
+    for (int r = 0; r < kReads; ++r) {
+      fa::lds_wait(x[r], r + kWin <= kReads ? kWin - 1 : kReads - 1 - r);
+      const u32x4 lo = operand_of<Q>(x[r][0], x[r][1]), hi = operand_of<Q>(x[r][2], x[r][3]);
+      if (r + kWin < kReads) {
+        x[r + kWin] = fa::lds_read_b128(kaddr ^ (((r + kWin) % kPairs) << 5), (r + kWin) / kPairs * 32 * D);
+      }
+      f32x16& t = s[r / kPairs];
+      t = F16::mfma(lo, q[r % kPairs * 2], t);
+      t = F16::mfma(hi, q[r % kPairs * 2 + 1], t);
+    }
+  }
+  static __device__ __forceinline__ u32x2 read_tr(uint32_t addr, int off) {
+    u32x2 r;
+    asm volatile("ds_read_b64_tr_b8 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "i"(off));
+    return r;
+  }
+  static __device__ __forceinline__ void wait(u32x2& r, int n) { asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(r) : "i"(n)); }
+  // Operand r: block r / 4 of the columns, keys 16 (r % 4) .. + 15.
+  template <bool kMasked>
+  __device__ __forceinline__ void pv(Softmax<D>& st, const u32x4 (&pb)[2][2], uint32_t& found) const {
+    constexpr int kOps = 4 * (D / 32), kWin = 8;
+    u32x2 x[kOps];
+#pragma unroll
+    for (int r = 0; r < kWin; ++r) x[r] = read_tr(vaddr ^ ((r >> 2) << 5), (r & 3) * 16 * D);
+#pragma unroll
+    for (int r = 0; r < kOps; ++r) {
+      wait(x[r], r + kWin <= kOps ? kWin - 1 : kOps - 1 - r);
+      if constexpr (kMasked) x[r] = u32x2{without_nan(x[r][0], found), without_nan(x[r][1], found)};
+      const u32x4 a = operand_of<Q>(x[r][0], x[r][1]);
+      if (r + kWin < kOps) x[r + kWin] = read_tr(vaddr ^ (((r + kWin) >> 2) << 5), (r & 3) * 16 * D);
+      st.acc[r >> 2] = F16::mfma(a, pb[(r & 3) >> 1][r & 1], st.acc[r >> 2]);
+    }
+  }
+};
+
+// Waves' parts in LDS, or a row's splits, joined and written: eight values of row `row`, relative to their largest
+// reference point m.
+template <class E>
+__device__ __forceinline__ void write_row(const AttnArgs& p, const kv::Share& s, int row, int ch, const float (&o)[8], float m,
+                                          float l, int written) {
+  int64_t o_at, lse_at;
+  if (!out_row(p, s, row, written, o_at, lse_at)) return;
+  *reinterpret_cast<u32x4*>(p.o + o_at + ch * 8) = kv::pack8<E>(o, kv::inverse_sum(l));
+  if (p.lse != nullptr && ch == 0) p.lse[lse_at] = kv::lse_of(m, l);
+}
+
+// Up to 32 rows; the workgroup's four waves take every fourth tile each.
+template <int D, class E, class Q>
+__device__ __forceinline__ void narrow_body(const AttnArgs& p) {
+  using N = Narrow<D>;
+  constexpr int kWaves = N::kWaves, L = N::kLoads, kRow = D * 4;
+  constexpr bool kHasNan = __is_same(Q, E4m3);
+  static_assert(N::kRows * kRow <= 2 * BKV * D, "a wave's part reuses its tiles");
+  __shared__ __attribute__((aligned(256))) uint8_t lds[kWaves * 2 * N::kTile];
+  __shared__ __attribute__((aligned(256))) uint8_t meta[kWaves * N::kScaleBytes];
+  __shared__ float stats[2][kWaves][N::kRows];
+
+  kv::Share s = share_of(p);
+  if (!s.live) return;
+  s.row0 *= N::kRows;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  NarrowTiles<D, Q> t;
+  t.lane = tid & 63;
+  t.col = t.lane & 31;
+  t.h = t.lane >> 5;
+  t.k = lds + wave * 2 * N::kTile;
+  t.v = t.k + N::kTile;
+  t.meta = meta + wave * N::kScaleBytes;
+  t.init(p);
+  const Sequence seq(p, s.b);
+  Rows rows;
+  rows.init(p, s, seq);
+  Softmax<D> st;
+  st.init();
+
+  const int total = (limit_of_rows(p, seq, s.row0, N::kRows) + BKV - 1) / BKV;
+  const int per = (total + p.splits - 1) / p.splits;
+  const int begin = min(total, s.split * per), end = min(total, begin + per);
+  Places at{}, next_at{};
+  int j = begin + wave;
+  if (j < end) {
+    at = rows.places(p, j, t.lane, static_cast<uint32_t>(*rows.entry(p, j, t.lane)));
+    t.load_word(p.c.k_scale + at.ks, 1);
+    t.load_word(p.c.v_scale + at.vs, 2);
+    t.load_word(rows.entry(p, min(j + kWaves, total - 1), t.lane), 0);
+    t.template load<false>(p, at.k);
+    t.template load<true>(p, at.v);
+  }
+  u32x4 q[D / 16];
+  load_query<D, E, true>(p, s, seq, s.row0 + t.col, t.h, q, st.limit, st.factor);
+  int least = st.limit;  // keys that all rows attend
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) least = min(least, __shfl_xor(least, d, 64));
+  least = __builtin_amdgcn_readfirstlane(least);
+  uint32_t found = 0;
+  for (; j < end; j += kWaves) {
+    const bool next = j + kWaves < end;
+    // all but V_j have landed
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");
+    const float ks = __uint_as_float(t.word(1)), vs = __uint_as_float(t.word(2));
+    const uint32_t id = t.word(0);
+    f32x16 sc[2];
+    t.scores(q, sc);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (next) {
+      next_at = rows.places(p, j + kWaves, t.lane, id);
+      t.load_word(p.c.k_scale + next_at.ks, 1);
+      t.load_word(p.c.v_scale + next_at.vs, 2);
+      t.load_word(rows.entry(p, min(j + 2 * kWaves, total - 1), t.lane), 0);
+      t.template load<false>(p, next_at.k);
+    }
+    st.set_scales(ks, vs);
+    const bool masked = (j + 1) * BKV > least;
+    if (masked) st.hide(sc, j, t.h);
+    if (j == begin + wave) st.m = st.tile_max(sc);  // nothing to rescale yet
+    u32x4 pb[2][2];
+    float rs = st.probs(sc, pb);
+    st.guard(sc, pb, rs);
+    if (next) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L + 3) : "memory");  // all but the next tile's K, scales and entry
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    if (kHasNan && masked) {
+      t.template pv<true>(st, pb, found);
+    } else {
+      t.template pv<false>(st, pb, found);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (next) t.template load<true>(p, next_at.v);
+  }
+  if (kHasNan && __builtin_amdgcn_ballot_w64(found != 0) != 0) {
+    for (int i = begin + wave; i < end; i += kWaves) {
+      if ((i + 1) * BKV > least) st.add_nan(p, s, i, t.h);
+    }
+  }
+
+  // the waves' parts, relative to their own reference points, through LDS
+  const auto part_off = [](int row, int c) { return row * kRow + ((c ^ (row & 15)) << 4); };
+  {
+    float l = st.l + other_half(st.l);
+    if (rows.poison) l = __builtin_nanf("");
+    if (t.h == 0) {
+      stats[0][wave][t.col] = st.m;
+      stats[1][wave][t.col] = l;
+    }
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        const f32x16& a = st.acc[db];
+        *reinterpret_cast<f32x4*>(t.k + part_off(t.col, db * 8 + rq * 2 + t.h)) =
+            f32x4{a[rq * 4] * st.R, a[rq * 4 + 1] * st.R, a[rq * 4 + 2] * st.R, a[rq * 4 + 3] * st.R};
+      }
+  }
+  __syncthreads();
+  const int written = written_of(p, s.b);
+#pragma unroll
+  for (int i = 0; i < N::kRows * (D / 8) / (kWaves * 64); ++i) {
+    const int cc = tid + kWaves * 64 * i;
+    const int row = cc / (D / 8), ch = cc % (D / 8);
+    if (s.row0 + row >= p.rows) continue;
+    float m = stats[0][0][row];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, stats[0][w][row]);
+    float f[kWaves], l_run = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float mw = stats[0][w][row];
+      f[w] = mw == m ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
+      l_run += f[w] * stats[1][w][row];
+    }
+    float o[8] = {};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const uint8_t* part = lds + w * 2 * N::kTile;
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(part + part_off(row, 2 * ch));
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(part + part_off(row, 2 * ch + 1));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[e] = fmaf(f[w], lo[e], o[e]);
+        o[4 + e] = fmaf(f[w], hi[e], o[4 + e]);
+      }
+    }
+    if (p.splits > 1) {
+      const int64_t place = static_cast<int64_t>(s.unit) * p.rows + s.row0 + row;
+      if (ch == 0) *reinterpret_cast<float2*>(p.part_ml + place * 2) = make_float2(m, l_run);
+      *reinterpret_cast<f32x4*>(p.part_o + place * D + ch * 8) = f32x4{o[0], o[1], o[2], o[3]};
+      *reinterpret_cast<f32x4*>(p.part_o + place * D + ch * 8 + 4) = f32x4{o[4], o[5], o[6], o[7]};
+      continue;
+    }
+    write_row<E>(p, s, s.row0 + row, ch, o, m, l_run, written);
+  }
+}
+
+// ------------------------------------------------------------------------------------ many rows
+
+template <int D>
+struct Wide {
+  static constexpr int kWaves = D == 128 ? 8 : 4, kWgPerCu = D == 128 ? 1 : 2;
+  static constexpr int kRows = 32 * kWaves;
+  static constexpr int kTile = BKV * D * 2;  // bytes, in fp16
+};
+
+// Each wave loads the codes of 1024 / D rows of a tile, a piece of 16 per lane, and writes them as fp16 to LDS, where
+// all waves read them.
+template <int D, class E, class Q>
+struct WideState : fa::FaState<D, Wide<D>::kWaves, 1, F16, true> {
+  using Base = fa::FaState<D, Wide<D>::kWaves, 1, F16, true>;
+  static constexpr int T = Wide<D>::kTile;
+  Softmax<D> st;
+  Rows rows;
+  uint32_t koff, voff;        // of this lane's piece in its group of rows
+  uint32_t kdst, vdst;        // of its first chunk of fp16 in a tile; the second's differs by one bit
+  int group;                  // of this wave's rows
+  uint32_t found;             // NaN among the values that this lane has loaded, of tiles that not all rows attend
+
+  __device__ __forceinline__ void init_tiles(const AttnArgs& p) {
+    constexpr int kPieces = D / 16;
+    const int lane = this->lane, row = this->wave * (64 / kPieces) + lane / kPieces, piece = lane % kPieces;
+    group = row / kGroup;
+    koff = (row % kGroup) * p.c.ks.row * 16 + piece * 16;
+    voff = (row % kGroup) * p.c.vs.row * 16 + piece * 16;
+    kdst = fa::k_off<D>(row, piece * 2);
+    vdst = fa::v_off<D>(row, piece * 16);
+    group = __builtin_amdgcn_readfirstlane(group);
+    this->kaddr[0] = fa::k_off<D>(this->col, this->h);
+    const int g_lane = lane & 15;
+    this->vaddr[0] = fa::v_off<D>(this->h * 4 + (g_lane >> 2), ((lane >> 4) & 1) * 16 + (g_lane & 3) * 4);
+  }
+  __device__ __forceinline__ u32x4 load(const uint8_t* codes, uint32_t places, uint32_t off) const {
+    const uint32_t place = __builtin_amdgcn_readlane(places, group);
+    return *reinterpret_cast<const u32x4*>(codes + static_cast<uint64_t>(place) * 16 + off);
+  }
+  template <bool kClean>
+  __device__ __forceinline__ void store(uint8_t* tile, uint32_t dst, u32x4 x) {
+    if constexpr (kClean) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = without_nan(x[i], found);
+    }
+    *reinterpret_cast<u32x4*>(tile + dst) = operand_of<Q>(x[0], x[1]);
+    *reinterpret_cast<u32x4*>(tile + (dst ^ 16)) = operand_of<Q>(x[2], x[3]);
+  }
+  // P^T of this tile between the products of the next one's scores, as FaState::scores_probs.
+  __device__ __forceinline__ float scores_probs(const uint8_t* k, f32x16 (&sn)[2], const f32x16 (&sc)[2], u32x4 (&pb)[2][2]) const {
+    const uint32_t base = lds_addr(k);
+    constexpr int kWin = 4, kReads = 2 * Base::kKSteps, kPer = 16 / kReads;
+    const float ref = st.reference();
+    float rs = 0.f, sum = 0.f;
+    u32x4 x[kReads];
+#pragma unroll
+    for (int r = 0; r < kWin; ++r) x[r] = fa::lds_read_b128(this->k_addr(base, r % Base::kKSteps), (r / Base::kKSteps) * 32 * (D * 2));
+    sn[0] = f32x16{};
+    sn[1] = f32x16{};
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int r = 0; r < kReads; ++r) {
+      fa::lds_wait(x[r], r + kWin <= kReads ? kWin - 1 : kReads - 1 - r);
+      sn[r / Base::kKSteps] = F16::mfma(x[r], this->qreg[0][r % Base::kKSteps], sn[r / Base::kKSteps]);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int it = r * kPer + i;
+        st.pair(sc, it / 4, it % 4, ref, pb, sum);
+        if (it % 4 == 3) {
+          rs = fmaf(sum, st.undo[it / 4], rs);
+          sum = 0.f;
+        }
+      }
+      if (r + kWin < kReads) {
+        x[r + kWin] = fa::lds_read_b128(this->k_addr(base, (r + kWin) % Base::kKSteps), ((r + kWin) / Base::kKSteps) * 32 * (D * 2));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return rs;
+  }
+  __device__ __forceinline__ void pv(const uint8_t* v, const u32x4 (&pb)[2][2]) {
+    const uint32_t base = lds_addr(v);
+    constexpr int kWin = 4, kOps = 4 * Base::kDBlocks;
+    u32x4 x[kOps];
+#pragma unroll
+    for (int r = 0; r < kWin; ++r) x[r] = this->vt_read(base, r);
+#pragma unroll
+    for (int r = 0; r < kOps; ++r) {
+      fa::lds_wait(x[r], 2 * (r + kWin <= kOps ? kWin - 1 : kOps - 1 - r));
+      st.acc[r / 4] = F16::mfma(x[r], pb[(r % 4) >> 1][r & 1], st.acc[r / 4]);
+      if (r + kWin < kOps) x[r + kWin] = this->vt_read(base, r + kWin);
+    }
+  }
+};
+
+// What is under way of the next tiles: codes of K (three tiles ahead at the step's end) and V (two), the scales from the
+// current tile on, the entry of the table of the tile after.
+struct WideAhead {
+  u32x4 k, v;
+  uint32_t v_place, id;
+  float ks[3], vs[3];
+};
+
+// Tile j: LDS holds K_{j+1} and V_j, sc the raw scores of tile j, `a` the codes of K_{j+2} and V_{j+1}.
+// kTail false: tile j + 1 exists, and all of the workgroup's rows attend all of it.
+template <bool kTail, int D, class E, class Q>
+__device__ __forceinline__ void wide_step(WideState<D, E, Q>& w, const AttnArgs& p, int j, int end, uint8_t* ring, int most,
+                                          int least, WideAhead& a, f32x16 (&sc1)[1][2], f32x16 (&sn1)[1][2]) {
+  f32x16(&sc)[2] = sc1[0];
+  f32x16(&sn)[2] = sn1[0];
+  constexpr bool kClean = kTail && __is_same(Q, E4m3);
+  constexpr int T = WideState<D, E, Q>::T;
+  Softmax<D>& st = w.st;
+  uint8_t* k_next = ring + ((j + 1) & 1) * T;
+  uint8_t* v_here = ring + (2 + (j & 1)) * T;
+  // codes that have arrived, into the stages that the last step read
+  if (j + 2 < end) w.template store<false>(ring + (j & 1) * T, w.kdst, a.k);
+  if (j + 1 < end) w.template store<kClean>(ring + (2 + ((j + 1) & 1)) * T, w.vdst, a.v);
+  const float ks = a.ks[0], vs = a.vs[0];
+  a.ks[0] = a.ks[1];
+  a.vs[0] = a.vs[1];
+  a.ks[1] = a.ks[2];
+  a.vs[1] = a.vs[2];
+  if (j + 2 < end) a.v = w.load(p.c.v, a.v_place, w.voff);
+  if (j + 3 < end) {
+    const Places at = w.rows.places(p, j + 3, w.lane, a.id);
+    a.k = w.load(p.c.k, at.k, w.koff);
+    a.v_place = at.v;
+    a.ks[2] = p.c.k_scale[at.ks];
+    a.vs[2] = p.c.v_scale[at.vs];
+    a.id = static_cast<uint32_t>(*w.rows.entry(p, min(j + 4, end - 1), w.lane));
+  }
+  const bool act = !kTail || j * BKV < most;
+  if (act) {
+    st.set_scales(ks, vs);
+    u32x4 pb[2][2];
+    float rs;
+    if constexpr (kTail) {
+      if ((j + 1) * BKV > least) st.hide(sc, j, w.h);
+      rs = st.probs(sc, pb);
+    } else {
+      rs = w.scores_probs(k_next, sn, sc, pb);
+    }
+    st.guard(sc, pb, rs);
+    w.pv(v_here, pb);
+    if constexpr (kTail) {
+      if ((j + 1) * BKV < most && j + 1 < end) {
+        w.scores(k_next, sc1);
+      }
+    }
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  asm volatile("s_barrier" ::: "memory");
+}
+
+template <int D, class E, class Q>
+__device__ __forceinline__ void wide_body(const AttnArgs& p) {
+  using W = Wide<D>;
+  constexpr int kWaves = W::kWaves, T = W::kTile, kThreads = kWaves * 64, kChunks = D / 8;
+  constexpr bool kHasNan = __is_same(Q, E4m3);
+  __shared__ __attribute__((aligned(256))) uint8_t ring[4 * T];
+
+  kv::Share s = share_of(p);
+  if (!s.live) return;
+  s.row0 *= W::kRows;
+  WideState<D, E, Q> w;
+  const int tid = threadIdx.x;
+  if (kWaves == 8 && (tid >> 6) < 4) __builtin_amdgcn_s_setprio(1);
+  w.lane = tid & 63;
+  w.wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  w.col = w.lane & 31;
+  w.h = w.lane >> 5;
+  w.init_tiles(p);
+  const Sequence seq(p, s.b);
+  w.rows.init(p, s, seq);
+  Softmax<D>& st = w.st;
+  st.init();
+  const int wave_row = s.row0 + w.wave * 32;
+  load_query<D, E, false>(p, s, seq, wave_row + w.col, w.h, w.qreg[0], st.limit, st.factor);
+  int least = st.limit;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) least = min(least, __shfl_xor(least, d, 64));
+  least = __builtin_amdgcn_readfirstlane(least);
+  const int most = wave_row < p.rows ? limit_of_rows(p, seq, wave_row, 32) : 0;
+
+  const int total = (limit_of_rows(p, seq, s.row0, W::kRows) + BKV - 1) / BKV;
+  const int per = (total + p.splits - 1) / p.splits;
+  const int begin = min(total, s.split * per), end = min(total, begin + per);
+  w.found = 0;
+  // tiles that all rows of the workgroup attend
+  const int whole = min(end, least_of_rows(p, seq, s.row0, W::kRows) / BKV);
+  if (begin < end) {
+    WideAhead a{};
+    Places at[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const int j = min(begin + i, end - 1);
+      at[i] = w.rows.places(p, j, w.lane, static_cast<uint32_t>(*w.rows.entry(p, j, w.lane)));
+      a.ks[i] = p.c.k_scale[at[i].ks];
+      a.vs[i] = p.c.v_scale[at[i].vs];
+    }
+    const u32x4 k0 = w.load(p.c.k, at[0].k, w.koff), v0 = w.load(p.c.v, at[0].v, w.voff);
+    const u32x4 k1 = w.load(p.c.k, at[1].k, w.koff);
+    a.k = w.load(p.c.k, at[2].k, w.koff);
+    a.v = w.load(p.c.v, at[1].v, w.voff);
+    a.v_place = at[2].v;
+    a.id = static_cast<uint32_t>(*w.rows.entry(p, min(begin + 3, end - 1), w.lane));
+    // tile j in stage j % 2
+    w.template store<false>(ring + (begin & 1) * T, w.kdst, k0);
+    w.template store<false>(ring + ((begin + 1) & 1) * T, w.kdst, k1);
+    if (kHasNan && whole <= begin) {
+      w.template store<true>(ring + (2 + (begin & 1)) * T, w.vdst, v0);
+    } else {
+      w.template store<false>(ring + (2 + (begin & 1)) * T, w.vdst, v0);
+    }
+    __syncthreads();
+    f32x16 sa[1][2], sb[1][2];
+    w.scores(ring + (begin & 1) * T, sa);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    asm volatile("s_barrier" ::: "memory");
+    int j = begin;
+    for (; j + 2 < whole; j += 2) {
+      wide_step<false>(w, p, j, end, ring, most, least, a, sa, sb);
+      wide_step<false>(w, p, j + 1, end, ring, most, least, a, sb, sa);
+    }
+    for (; j < end; ++j) wide_step<true>(w, p, j, end, ring, most, least, a, sa, sa);
+  }
+  if (kHasNan && __syncthreads_or(w.found != 0) != 0) {
+    for (int j = max(begin, whole - 2); j < end; ++j) st.add_nan(p, s, j, w.h);  // from the first tile cleaned on
+  }
+
+  float l_run = st.l + other_half(st.l);
+  if (w.rows.poison) l_run = __builtin_nanf("");
+  const int written = written_of(p, s.b);
+  if (p.splits > 1) {
+    // the unnormalised part, from registers: lane (row, half h) holds d = 32 db + 8 rq + 4 h + 0..3
+    const int row = wave_row + w.col;
+    if (row < p.rows) {
+      const int64_t place = static_cast<int64_t>(s.unit) * p.rows + row;
+      if (w.h == 0) *reinterpret_cast<float2*>(p.part_ml + place * 2) = make_float2(st.m, l_run);
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq) {
+          const f32x16& a = st.acc[db];
+          *reinterpret_cast<f32x4*>(p.part_o + place * D + db * 32 + rq * 8 + w.h * 4) =
+              f32x4{a[rq * 4] * st.R, a[rq * 4 + 1] * st.R, a[rq * 4 + 2] * st.R, a[rq * 4 + 3] * st.R};
+        }
+    }
+    return;
+  }
+  // rows of the block through the rings: 64 rows per stage
+  const float inv = kv::inverse_sum(l_run) * st.R;
+  {
+    const int brow = w.wave * 32 + w.col;
+    uint8_t* os = ring + (brow >> 6) * T;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        const f32x16& a = st.acc[db];
+        u32x2 x;
+        x[0] = E::pack(a[rq * 4] * inv, a[rq * 4 + 1] * inv);
+        x[1] = E::pack(a[rq * 4 + 2] * inv, a[rq * 4 + 3] * inv);
+        *reinterpret_cast<u32x2*>(os + fa::k_off<D>(brow & 63, db * 4 + rq) + w.h * 8) = x;
+      }
+    int64_t o_at, lse_at;
+    if (p.lse != nullptr && w.h == 0 && out_row(p, s, s.row0 + brow, written, o_at, lse_at)) {
+      p.lse[lse_at] = kv::lse_of(st.m, l_run);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < W::kRows * kChunks / kThreads; ++i) {
+    const int cc = tid + kThreads * i;
+    const int row = cc / kChunks, ch = cc % kChunks;
+    int64_t o_at, lse_at;
+    if (!out_row(p, s, s.row0 + row, written, o_at, lse_at)) continue;
+    *reinterpret_cast<u32x4*>(p.o + o_at + ch * 8) =
+        *reinterpret_cast<const u32x4*>(ring + (row >> 6) * T + fa::k_off<D>(row & 63, ch));
+  }
+}
+
+// Adds up the splits of a row, relative to the largest reference point.
+template <int D, class E>
+__device__ __forceinline__ void join_body(const AttnArgs& p) {
+  const kv::JoinLanes<D> at(blockIdx.x, p.join_groups);
+  const int64_t bh = at.row / p.rows;
+  const int row = static_cast<int>(at.row - bh * p.rows);
+  kv::Share s;
+  s.b = static_cast<int>(bh / p.c.kv_heads);
+  s.head = static_cast<int>(bh - static_cast<int64_t>(s.b) * p.c.kv_heads);
+  if (s.b >= p.batch) return;
+  const int written = written_of(p, s.b);
+  int64_t o_at, lse_at;
+  if (!out_row(p, s, row, written, o_at, lse_at)) return;  // all lanes of the row
+  const int64_t first = static_cast<int64_t>(s.b) * p.splits * p.c.kv_heads + s.head;  // unit of split 0
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int k = at.group; k < p.splits; k += at.groups) {
+    m = fmaxf(m, p.part_ml[((first + static_cast<int64_t>(k) * p.c.kv_heads) * p.rows + row) * 2]);
+  }
+  m = at.reduce(m, [](float a, float b) { return fmaxf(a, b); });
+  float l_run = 0.f, o[8] = {};
+#pragma unroll 4
+  for (int k = at.group; k < p.splits; k += at.groups) {
+    const int64_t part = (first + static_cast<int64_t>(k) * p.c.kv_heads) * p.rows + row;
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + part * 2);
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(p.part_o + part * D + at.ch * 8);
+    const f32x4 hi = *reinterpret_cast<const f32x4*>(p.part_o + part * D + at.ch * 8 + 4);
+    const float f = ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m);
+    l_run += f * ml.y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[e] = fmaf(f, lo[e], o[e]);
+      o[4 + e] = fmaf(f, hi[e], o[4 + e]);
+    }
+  }
+  const auto sum = [](float a, float b) { return a + b; };
+  l_run = at.reduce(l_run, sum);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = at.reduce(o[e], sum);
+  if (at.group != 0) return;
+  write_row<E>(p, s, row, at.ch, o, m, l_run, written);
+}
+
+}  // namespace c8
+}  // namespace asc

@@ -1157,6 +1157,49 @@ def quantized_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales:
     _launch("asc_quantized_cache_read", args, _stream(stream))
 
 
+def quantized_cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor,
+                              v_scales: torch.Tensor, cache_lengths: torch.Tensor, o: torch.Tensor, sm_scale: float,
+                              block_table: Optional[torch.Tensor] = None, new_lengths: Optional[torch.Tensor] = None,
+                              causal: bool = True, lse: Optional[torch.Tensor] = None, stream: Any = None) -> None:
+    """Attention of each sequence's newest tokens over a cache held in 8 bits that holds them already (as
+    quantized_cache_append leaves it): o = softmax(q k^T * sm_scale) v for float16 or bfloat16 q and o [batch, heads,
+    n, head_dim], heads a multiple of kv_heads.
+
+    - cache_lengths (int32 [batch]): the keys of each sequence, the new ones among them.  new_lengths (int32 [batch]):
+      its queries, default n, those of its last keys: with ``causal`` query i attends the first cache_lengths -
+      new_lengths + i + 1 keys, else all.  Rows of o and lse behind new_lengths are left as they were, all of them
+      where it is negative.
+    - caches, scales and block_table as quantized_cache_append's; scales positive and finite.
+
+    A query without keys gets zeros and an lse (float32 [batch, heads, n]) of -inf.  A length outside the cache and more
+    queries than n are not followed: NaN; a page outside it gives NaN for the queries that attend its keys, and may
+    for others of the sequence."""
+    device = _current_device()
+    if not isinstance(q, torch.Tensor):
+        raise TypeError(f"'q' must be a torch.Tensor, got {type(q).__name__}")
+    dtype = q.dtype
+    if dtype not in _HALVES:
+        raise TypeError(f"'q' has unsupported dtype {dtype}; expected one of {sorted(map(str, _HALVES))}")
+    q_rows = _rows(q, "q", dtype, device, None, False, True)
+    shape = q.shape
+    batch, heads, n, head_dim = shape
+    o_rows = _rows(o, "o", dtype, device, shape, True, True)
+    cache, sizes, table = _cache8(k_cache, v_cache, k_scales, v_scales, block_table, batch, device)
+    kv_heads = sizes[4]
+    if head_dim != sizes[1]:
+        raise ValueError(f"'q' {tuple(shape)} does not fit the cache {tuple(k_cache.shape)}")
+    if kv_heads == 0 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads cannot share {kv_heads} key / value heads")
+    if not 0 < sm_scale < math.inf:
+        raise ValueError(f"sm_scale must be positive and finite, got {sm_scale}")
+    lse_at = 0 if lse is None else _vector(lse, "lse", torch.float32, device, shape[:3])
+    lengths = _vector(cache_lengths, "cache_lengths", torch.int32, device, (batch,))
+    news = 0 if new_lengths is None else _vector(new_lengths, "new_lengths", torch.int32, device, (batch,))
+    args = _CACHE8.pack(_DTYPE_CODES[dtype], *sizes[:4], bool(causal), sm_scale, batch, heads, kv_heads, n, *sizes[5:], *cache,
+                        *q_rows, *o_rows, *_NO_ROWS, *_NO_ROWS, lse_at, lengths, news, *table)
+    _with_workspace("asc_quantized_cache_attention", args, q.device, stream)
+
+
 # ------------------------------------------------------------------------------ pages of a cache
 
 _PAGES_HEAD = struct.Struct("@8q3Pq4Pq3P")  # asc_pages_t before its tensors

@@ -211,3 +211,54 @@ def test_logits_refusals(kw, code):
     assert lib.asc_process_logits(None, None) == INVALID
     assert lib.asc_process_logits(ctypes.byref(logits(rows=0)), None) == 0
     assert lib.asc_process_logits(ctypes.byref(logits(vocab=0)), None) == 0
+
+
+ATTENTION = "asc_quantized_cache_attention"
+
+
+def attention(a, ws=AT + 20 * FAR, nbytes=1 << 40):
+    return _native.load_library().asc_quantized_cache_attention(ctypes.byref(a), ws, nbytes, None)
+
+
+@pytest.mark.parametrize("kw,code", CACHE + [({"q_heads": 9}, INVALID), ({"q_heads": -1}, INVALID), ({"kv_heads": 0}, INVALID),
+                                             ({"sm_scale": 0.0}, INVALID), ({"sm_scale": float("inf")}, INVALID),
+                                             ({"dtype": 0}, UNSUPPORTED), ({"q": Rows()}, INVALID), ({"o": Rows()}, INVALID),
+                                             ({"q": Rows(AT + 4 * FAR + 8, 2560, 320, 64)}, ALIGNMENT),
+                                             ({"o": Rows(AT + 5 * FAR, 2560, 320, 65)}, ALIGNMENT),
+                                             ({"k": Rows(AT, 1 << 27, 1 << 27, 1 << 26)}, UNSUPPORTED),
+                                             ({"n": 1 << 28}, UNSUPPORTED)])
+def test_attention_refusals(kw, code):
+    a = cache8(**kw)
+    assert attention(a) == code and ATTENTION in _native.last_error()
+    assert _native.load_library().asc_quantized_cache_attention_workspace(ctypes.byref(a)) == 0
+
+
+@pytest.mark.parametrize("kw,names", [({"o": Rows(AT + 4 * FAR, 2560, 320, 64)}, "'o' overlaps 'q'"),
+                                      ({"o": Rows(AT + FAR, 2560, 320, 64)}, "'o' overlaps 'v'"),
+                                      ({"lse": AT + 2 * FAR}, "'lse' overlaps 'k_scales'"),
+                                      ({"lse": AT + 5 * FAR}, "'o' overlaps 'lse'"),
+                                      ({"block_table": AT + 8 * FAR}, "'lse' overlaps 'block_table'")])
+def test_attention_places(kw, names):
+    assert attention(cache8(**kw)) == INVALID and names in _native.last_error()
+
+
+def test_attention_plans_and_workspaces():
+    lib = _native.load_library()
+    plan = _native.AttentionPlan()
+    seen = set()
+    for kv_len, n in ((64, 1), (64000, 1), (6400, 5000), (64000, 300), (640, 40000)):
+        a = cache8(kv_len=kv_len, n=n, q=Rows(AT + 4 * FAR, 8 * n * 64, n * 64, 64), o=Rows(AT + 16 * FAR, 8 * n * 64, n * 64, 64),
+                   num_pages=3000, lse=None, k=Rows(AT + 24 * FAR, 4096, 2048, 64), v=Rows(AT + 32 * FAR, 4096, 2048, 64),
+                   k_scales=Rows(AT + 40 * FAR, 4, 2, 1), v_scales=Rows(AT + 41 * FAR, 4, 2, 1))
+        assert lib.asc_quantized_cache_attention_plan(ctypes.byref(a), ctypes.byref(plan)) == 0
+        seen.add((plan.kernel, plan.splits > 1))
+        need = lib.asc_quantized_cache_attention_workspace(ctypes.byref(a))
+        assert (need > 0) == (plan.splits > 1)
+        if need:
+            for ws, nbytes in ((None, need), (AT, need - 1), (AT + 4, need)):
+                assert attention(a, ws, nbytes) == INVALID and "workspace" in _native.last_error()
+    assert {x for x, _ in seen} == {b"cache8_narrow", b"cache8_wide"} and {x for _, x in seen} == {False, True}
+    assert lib.asc_quantized_cache_attention(None, None, 0, None) == INVALID
+    assert lib.asc_quantized_cache_attention_plan(ctypes.byref(cache8()), None) == INVALID
+    for kw in ({"batch": 0}, {"n": 0}, {"q_heads": 0}):
+        assert attention(cache8(**kw), None, 0) == 0

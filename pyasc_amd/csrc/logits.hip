@@ -11,6 +11,7 @@
 namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct LogitsArgs {
   const void* logits;
@@ -49,6 +50,28 @@ struct Bf16 {
 constexpr int kThreads = 256;
 constexpr uint32_t kInPrompt = 0x80000000u;  // beside the count of a token behind the prompt
 
+// Tokens of the history that a thread has under way: one at a time, each waits for memory alone (47 us for 64
+// rows of 131072 with 8000 tokens, 15 with eight).
+constexpr int kAhead = 8;
+
+template <class T, class F>
+__device__ __forceinline__ void for_history(const void* history, int64_t at, int n, const F& count) {
+  const T* h = static_cast<const T*>(history) + at;
+  for (int base = threadIdx.x; base < n; base += kThreads * kAhead) {
+    T token[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = base + k * kThreads;
+      token[k] = h[i < n ? i : base];
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = base + k * kThreads;
+      if (i < n) count(i, token[k]);
+    }
+  }
+}
+
 // kIters vectors of 16 bytes per thread.  kVec: the rows of logits and out lie at the same offset from 16
 // bytes, so vectors of the slice do, `lead` elements before the row's first; else element by element.
 template <class E, bool kVec, int kIters>
@@ -65,6 +88,16 @@ __global__ void __launch_bounds__(kThreads) process_logits(LogitsArgs p) {
   S* y = static_cast<S*>(p.out) + row * p.out_stride;
   const int lead = kVec ? static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(S)) : 0;
   const int first = static_cast<int>(slice) * kSlice - lead;  // token of counts[0]
+  const bool whole = kVec && first >= 0 && first + kSlice <= p.vocab;
+
+  // the slice's logits are under way while the history is counted
+  u32x4 held[kVec ? kVecs : 1];
+  if (whole) {
+#pragma unroll
+    for (int it = 0; it < (kVec ? kVecs : 0); ++it) {
+      held[it] = *reinterpret_cast<const u32x4*>(x + first + (tid + it * kThreads) * V);
+    }
+  }
 
   const int length = p.lengths[row];
   const bool bad = length < 0 || length > p.width;
@@ -86,11 +119,9 @@ __global__ void __launch_bounds__(kThreads) process_logits(LogitsArgs p) {
     }
   };
   if (p.history_int64) {
-    const int64_t* h = static_cast<const int64_t*>(p.history) + row * p.history_stride;
-    for (int i = tid; i < n; i += kThreads) count(i, h[i]);
+    for_history<int64_t>(p.history, row * p.history_stride, n, count);
   } else {
-    const int32_t* h = static_cast<const int32_t*>(p.history) + row * p.history_stride;
-    for (int i = tid; i < n; i += kThreads) count(i, h[i]);
+    for_history<int32_t>(p.history, row * p.history_stride, n, count);
   }
   __syncthreads();
 
@@ -99,18 +130,58 @@ __global__ void __launch_bounds__(kThreads) process_logits(LogitsArgs p) {
   const float presence = p.presence ? p.presence[row] : 0.0f;
   const float* bias = p.bias ? p.bias + row * p.bias_stride : nullptr;
   const uint32_t* mask = p.mask ? p.mask + row * p.mask_stride : nullptr;
-  const auto process = [&](int token, uint32_t c, float v) {
+  const auto process = [&](uint32_t c, float v, float add, bool allowed) {
     if (c != 0) {
       v = v > 0.0f ? v / repetition : v * repetition;
       const float times = static_cast<float>(c & ~kInPrompt);
       v = v - frequency * times;
       if (times > 0.0f) v = v - presence;
     }
-    if (bias) v = v + bias[token];
+    if (bias) v = v + add;
     if (bad) v = __builtin_nanf("");
-    if (mask && !((mask[token >> 5] >> (token & 31)) & 1)) v = -INFINITY;
-    return v;
+    return allowed ? v : -INFINITY;
   };
+  const auto allowed = [&](int token) { return !mask || ((mask[token >> 5] >> (token & 31)) & 1); };
+  if (whole) {
+    if constexpr (kVec) {
+      const bool bias_vec = ((reinterpret_cast<uintptr_t>(bias) >> 2) + first) % 4 == 0;
+      float add[kVecs][V];
+      uint64_t bits[kVecs];
+#pragma unroll
+      for (int it = 0; it < kVecs; ++it) {
+        const int token = first + (tid + it * kThreads) * V;
+        if (bias) {
+          if (bias_vec) {
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+              *reinterpret_cast<f32x4*>(&add[it][e]) = *reinterpret_cast<const f32x4*>(bias + token + e);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) add[it][e] = bias[token + e];
+          }
+        }
+        bits[it] = ~0ull;
+        if (mask) {
+          bits[it] = (static_cast<uint64_t>(mask[(token + V - 1) >> 5]) << 32 | mask[token >> 5]) >> (token & 31);
+          // both words are the same one, unless the vector lies across two
+        }
+      }
+#pragma unroll
+      for (int it = 0; it < kVecs; ++it) {
+        const int at = (tid + it * kThreads) * V;
+        S in[V], out[V];
+        uint32_t c[V];
+        *reinterpret_cast<u32x4*>(in) = held[it];
+#pragma unroll
+        for (int e = 0; e < V; e += 4) *reinterpret_cast<u32x4*>(&c[e]) = *reinterpret_cast<const u32x4*>(&counts[at + e]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) out[e] = E::store(process(c[e], E::load(in[e]), add[it][e], bits[it] >> e & 1));
+        *reinterpret_cast<u32x4*>(y + first + at) = *reinterpret_cast<u32x4*>(out);
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int it = 0; it < kVecs; ++it) {
     const int at = (tid + it * kThreads) * V, token = first + at;
@@ -119,21 +190,34 @@ __global__ void __launch_bounds__(kThreads) process_logits(LogitsArgs p) {
       S in[V], out[V];
       *reinterpret_cast<u32x4*>(in) = *reinterpret_cast<const u32x4*>(x + token);
 #pragma unroll
-      for (int e = 0; e < V; ++e) out[e] = E::store(process(token + e, counts[at + e], E::load(in[e])));
+      for (int e = 0; e < V; ++e) {
+        out[e] = E::store(process(counts[at + e], E::load(in[e]), bias ? bias[token + e] : 0.0f, allowed(token + e)));
+      }
       *reinterpret_cast<u32x4*>(y + token) = *reinterpret_cast<u32x4*>(out);
     } else {
       for (int e = 0; e < V; ++e) {
         const int t = token + e;
-        if (t >= 0 && t < p.vocab) y[t] = E::store(process(t, counts[at + e], E::load(x[t])));
+        if (t >= 0 && t < p.vocab) {
+          y[t] = E::store(process(counts[at + e], E::load(x[t]), bias ? bias[t] : 0.0f, allowed(t)));
+        }
       }
     }
   }
 }
 
+// Tokens of a workgroup's slice: fewer where there are few rows, whose workgroups would leave most of the chip idle.
+constexpr int kLarge = 8192, kSmall = 2048;
+constexpr int64_t kFewGroups = 512;
+
 template <class E, bool kVec>
-void launch(const LogitsArgs& p, int64_t rows, hipStream_t stream) {
-  hipLaunchKernelGGL((process_logits<E, kVec, 8 * sizeof(typename E::Stored) / 4>), dim3(static_cast<uint32_t>(rows * p.slices)),
-                     dim3(kThreads), 0, stream, p);
+void launch(const LogitsArgs& p, int64_t rows, bool small, hipStream_t stream) {
+  constexpr int kPer = kThreads * 16 / static_cast<int>(sizeof(typename E::Stored));
+  const dim3 grid(static_cast<uint32_t>(rows * p.slices));
+  if (small) {
+    hipLaunchKernelGGL((process_logits<E, kVec, kSmall / kPer>), grid, dim3(kThreads), 0, stream, p);
+  } else {
+    hipLaunchKernelGGL((process_logits<E, kVec, kLarge / kPer>), grid, dim3(kThreads), 0, stream, p);
+  }
 }
 
 }  // namespace
@@ -189,8 +273,11 @@ extern "C" int32_t asc_process_logits(const asc_logits_t* a, asc_stream_t stream
   p.mask_stride = a->mask_stride;
   p.vocab = static_cast<int32_t>(a->vocab);
   p.width = static_cast<int32_t>(a->history_width);
-  // room for the lead of a row that does not begin at 16 bytes
-  p.slices = static_cast<int32_t>(asc::ceil_div(a->vocab + 16 / size - 1, 8192));
+  // room for the lead of rows that do not begin at 16 bytes
+  const bool aligned = asc::aligned16(a->logits) && (a->rows == 1 || a->logits_stride * size % 16 == 0);
+  const int64_t tokens = a->vocab + (aligned ? 0 : 16 / size - 1);
+  const bool small = a->rows * asc::ceil_div(tokens, kLarge) < kFewGroups;
+  p.slices = static_cast<int32_t>(asc::ceil_div(tokens, small ? kSmall : kLarge));
   ASC_REQUIRE(a->rows * p.slices < int64_t{1} << 24, ASC_ERR_UNSUPPORTED, "%s: %lld workgroups exceed the launch grid limit",
               what, static_cast<long long>(a->rows * p.slices));
   const uintptr_t apart = reinterpret_cast<uintptr_t>(a->logits) ^ reinterpret_cast<uintptr_t>(a->out);
@@ -198,11 +285,11 @@ extern "C" int32_t asc_process_logits(const asc_logits_t* a, asc_stream_t stream
   const bool vec = ((apart | static_cast<uintptr_t>(steps)) & 15) == 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (a->dtype == ASC_DT_FLOAT32) {
-    vec ? launch<F32, true>(p, a->rows, s) : launch<F32, false>(p, a->rows, s);
+    vec ? launch<F32, true>(p, a->rows, small, s) : launch<F32, false>(p, a->rows, small, s);
   } else if (a->dtype == ASC_DT_FLOAT16) {
-    vec ? launch<F16, true>(p, a->rows, s) : launch<F16, false>(p, a->rows, s);
+    vec ? launch<F16, true>(p, a->rows, small, s) : launch<F16, false>(p, a->rows, small, s);
   } else {
-    vec ? launch<Bf16, true>(p, a->rows, s) : launch<Bf16, false>(p, a->rows, s);
+    vec ? launch<Bf16, true>(p, a->rows, small, s) : launch<Bf16, false>(p, a->rows, small, s);
   }
   return asc::check_launch(what);
 }

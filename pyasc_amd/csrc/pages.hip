@@ -5,6 +5,7 @@
 // of them can be captured.  Ranks of free and moving pages are prefix sums and counts are
 // integers: the same result on every call.
 #include "common.h"
+#include "divisor.h"
 #include "overlap.h"
 
 namespace {
@@ -27,11 +28,13 @@ struct Tensor {
   int32_t width;  // bytes that its addresses and sizes are multiples of: 1, 2, 4 or 16
 };
 
+// A kernel's first argument: the tensors are read from where the arguments lie (tensor_of).
 struct CopyArgs {
   Tensor t[kTensors];
-  int32_t n_tensors, per_move;
-  int32_t page_size;
-  int64_t moves;              // at most
+  asc::Divisor per_move;  // pieces of a move
+  asc::Divisor page_size;
+  int32_t n_tensors;
+  int32_t moves;              // at most
   const int32_t* count;       // null: moves
   const int32_t* from;        // pages
   const int32_t* to;
@@ -66,48 +69,64 @@ __device__ __forceinline__ void copy_rows(const uint8_t* from, uint8_t* to, int 
   }
 }
 
+// Tensor k.  An array of an argument's struct that is indexed at run time would be copied to scratch memory first:
+// 120 us for copies of 268 MB that take 47.
+typedef const __attribute__((address_space(4))) Tensor* TensorAt;
+__device__ __forceinline__ TensorAt tensor_of(int k) {
+  return (TensorAt)__builtin_amdgcn_kernarg_segment_ptr() + k;
+}
+
 // Item `item` of all: a move, one of its tensors, a piece of that.
-__device__ __forceinline__ void copy_item(const CopyArgs& p, int64_t item) {
-  const int64_t move = item / p.per_move;
-  int piece = static_cast<int>(item - move * p.per_move);
+__device__ __forceinline__ void copy_item(const CopyArgs& p, uint32_t item) {
+  const uint32_t move = p.per_move.divide(item);
+  int piece = static_cast<int>(item - move * p.per_move.d);
   const int64_t from_page = p.from[move], to_page = p.to[move];
+  int used = 0;
+  if (p.used) used = p.used[move];
   if (from_page < 0 || from_page >= p.from_pages || to_page < 0 || to_page >= p.to_pages) return;
-  int k = 0;
-  while (piece >= p.t[k].pieces) piece -= p.t[k++].pieces;
-  const Tensor& t = p.t[k];
-  const uint8_t* from = t.from + from_page * t.from_stride;
-  uint8_t* to = t.to + to_page * t.to_stride;
-  if (t.flat) {
+  TensorAt t = tensor_of(0);
+  while (piece >= t->pieces) {
+    piece -= t->pieces;
+    ++t;
+  }
+  const uint8_t* from = t->from + from_page * t->from_stride;
+  uint8_t* to = t->to + to_page * t->to_stride;
+  const int width = t->width;
+  int64_t bytes;
+  if (t->flat) {
     const int64_t at = static_cast<int64_t>(piece) * kPiece;
-    const int64_t n = t.bytes - at < kPiece ? t.bytes - at : kPiece;
-    if (t.width == 16) return copy_run<u32x4>(from + at, to + at, n);
-    if (t.width == 4) return copy_run<uint32_t>(from + at, to + at, n);
-    if (t.width == 2) return copy_run<uint16_t>(from + at, to + at, n);
-    return copy_run<uint8_t>(from + at, to + at, n);
+    bytes = t->bytes - at < kPiece ? t->bytes - at : kPiece;
+    from += at;
+    to += at;
+  } else {
+    from += piece * t->head_stride;
+    to += piece * t->head_stride;
+    int rows = t->rows;
+    if (p.used) {
+      rows = rows == static_cast<int>(p.page_size.d)
+                 ? used
+                 : static_cast<int>(p.page_size.divide(static_cast<uint32_t>(used * rows + p.page_size.d - 1)));
+    }
+    if (t->row_stride != t->row_bytes) {
+      if (width == 16) return copy_rows<u32x4>(from, to, rows, t->row_bytes, t->row_stride);
+      if (width == 4) return copy_rows<uint32_t>(from, to, rows, t->row_bytes, t->row_stride);
+      if (width == 2) return copy_rows<uint16_t>(from, to, rows, t->row_bytes, t->row_stride);
+      return copy_rows<uint8_t>(from, to, rows, t->row_bytes, t->row_stride);
+    }
+    bytes = static_cast<int64_t>(rows) * t->row_bytes;
   }
-  from += piece * t.head_stride;
-  to += piece * t.head_stride;
-  int rows = t.rows;
-  if (p.used) rows = static_cast<int>((static_cast<int64_t>(p.used[move]) * rows + p.page_size - 1) / p.page_size);
-  if (t.row_stride == t.row_bytes) {
-    const int64_t n = static_cast<int64_t>(rows) * t.row_bytes;
-    if (t.width == 16) return copy_run<u32x4>(from, to, n);
-    if (t.width == 4) return copy_run<uint32_t>(from, to, n);
-    if (t.width == 2) return copy_run<uint16_t>(from, to, n);
-    return copy_run<uint8_t>(from, to, n);
-  }
-  if (t.width == 16) return copy_rows<u32x4>(from, to, rows, t.row_bytes, t.row_stride);
-  if (t.width == 4) return copy_rows<uint32_t>(from, to, rows, t.row_bytes, t.row_stride);
-  if (t.width == 2) return copy_rows<uint16_t>(from, to, rows, t.row_bytes, t.row_stride);
-  return copy_rows<uint8_t>(from, to, rows, t.row_bytes, t.row_stride);
+  if (width == 16) return copy_run<u32x4>(from, to, bytes);
+  if (width == 4) return copy_run<uint32_t>(from, to, bytes);
+  if (width == 2) return copy_run<uint16_t>(from, to, bytes);
+  copy_run<uint8_t>(from, to, bytes);
 }
 
-__device__ __forceinline__ void copy_items(const CopyArgs& p) {
-  const int64_t moves = p.count ? *p.count : p.moves;
-  for (int64_t item = blockIdx.x; item < moves * p.per_move; item += gridDim.x) copy_item(p, item);
+__device__ __forceinline__ void copy_items(const CopyArgs& p, uint32_t first, uint32_t step) {
+  const uint32_t items = static_cast<uint32_t>(p.count ? *p.count : p.moves) * p.per_move.d;
+  for (uint32_t item = first; item < items; item += step) copy_item(p, item);
 }
 
-__global__ void __launch_bounds__(kThreads) page_copy(CopyArgs p) { copy_items(p); }
+__global__ void __launch_bounds__(kThreads) page_copy(CopyArgs p) { copy_items(p, blockIdx.x, gridDim.x); }
 
 // ------------------------------------------------------------------------------------ plans
 
@@ -261,9 +280,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan(PlanArgs p) {
 // The copies, and the new rows of the table.
 __global__ void __launch_bounds__(kThreads) fork_move(CopyArgs c, PlanArgs p, int row_groups) {
   if (static_cast<int>(blockIdx.x) >= row_groups) {
-    for (int64_t item = blockIdx.x - row_groups; item < c.moves * c.per_move; item += gridDim.x - row_groups) {
-      copy_item(c, item);
-    }
+    copy_items(c, blockIdx.x - row_groups, gridDim.x - row_groups);
     return;
   }
   for (int i = blockIdx.x; i < p.new_batch; i += row_groups) {
@@ -328,10 +345,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan(PlanArgs p) {
 
 __global__ void __launch_bounds__(kThreads) compact_move(CopyArgs c, PlanArgs p, int row_groups) {
   if (static_cast<int>(blockIdx.x) >= row_groups) {
-    const int64_t moves = *c.count;
-    for (int64_t item = blockIdx.x - row_groups; item < moves * c.per_move; item += gridDim.x - row_groups) {
-      copy_item(c, item);
-    }
+    copy_items(c, blockIdx.x - row_groups, gridDim.x - row_groups);
     return;
   }
   for (int b = blockIdx.x; b < p.batch; b += row_groups) {
@@ -361,11 +375,12 @@ asc::Region pages_region(const char* name, const void* data, int64_t pages, int6
 }
 
 // The tensors' checks, and their pieces.  partial: a part of a page's rows may be copied.
-int32_t make_copy(const asc_pages_t& a, bool within, bool partial, const char* what, CopyArgs& c) {
+int32_t make_copy(const asc_pages_t& a, int64_t moves, bool within, bool partial, const char* what, CopyArgs& c) {
   ASC_REQUIRE(a.n_tensors >= 0 && a.n_tensors <= kTensors, ASC_ERR_INVALID_ARG, "%s: %lld tensors (at most %d)", what,
               static_cast<long long>(a.n_tensors), kTensors);
   c.n_tensors = static_cast<int32_t>(a.n_tensors);
-  c.page_size = static_cast<int32_t>(a.page_size);
+  c.page_size = asc::divisor_of(partial ? static_cast<uint32_t>(a.page_size) : 1);
+  int64_t per_move = 0;
   c.from_pages = a.num_pages;
   c.to_pages = within ? a.num_pages : a.to_num_pages;
   for (int i = 0; i < c.n_tensors; ++i) {
@@ -380,6 +395,8 @@ int32_t make_copy(const asc_pages_t& a, bool within, bool partial, const char* w
     ASC_REQUIRE(!partial || (x.rows <= a.page_size && a.page_size % x.rows == 0), ASC_ERR_INVALID_ARG,
                 "%s: %lld rows of a page of %lld", what, static_cast<long long>(x.rows),
                 static_cast<long long>(a.page_size));
+    ASC_REQUIRE(!partial || x.rows == a.page_size || x.rows * a.page_size < int64_t{1} << 30, ASC_ERR_UNSUPPORTED,
+                "%s: pages too large", what);
     Tensor& t = c.t[i];
     t.from = static_cast<const uint8_t*>(x.from);
     t.to = static_cast<uint8_t*>(x.to);
@@ -396,7 +413,7 @@ int32_t make_copy(const asc_pages_t& a, bool within, bool partial, const char* w
     const int64_t pieces = t.flat ? asc::ceil_div(t.bytes, kPiece) : x.heads;
     ASC_REQUIRE(t.bytes < int64_t{1} << 40 && pieces < 1 << 24, ASC_ERR_UNSUPPORTED, "%s: pages too large", what);
     t.pieces = static_cast<int32_t>(pieces);
-    c.per_move += t.pieces;
+    per_move += t.pieces;
     uintptr_t bits = reinterpret_cast<uintptr_t>(x.from) | reinterpret_cast<uintptr_t>(x.to) |
                      static_cast<uintptr_t>(x.from_stride | x.to_stride | x.row_bytes);
     if (!t.flat) bits |= static_cast<uintptr_t>(t.head_stride | t.row_stride);
@@ -414,6 +431,11 @@ int32_t make_copy(const asc_pages_t& a, bool within, bool partial, const char* w
       }
     }
   }
+  // the last item plus a grid's step stays below 2^31
+  ASC_REQUIRE(moves < int64_t{1} << 30 && moves * per_move < int64_t{1} << 30, ASC_ERR_UNSUPPORTED,
+              "%s: more than 2^30 pieces of pages to copy", what);
+  c.moves = static_cast<int32_t>(moves);
+  c.per_move = asc::divisor_of(per_move > 0 ? static_cast<uint32_t>(per_move) : 1);
   return ASC_OK;
 }
 
@@ -427,6 +449,7 @@ int32_t check_apart(const asc::Region& r, const asc_pages_t& a, const CopyArgs& 
   return ASC_OK;
 }
 
+int64_t items_of(const CopyArgs& c) { return c.n_tensors > 0 ? static_cast<int64_t>(c.moves) * c.per_move.d : 0; }
 int64_t groups_of(int64_t items) { return items < kMostGroups ? items : kMostGroups; }
 
 struct Plan {
@@ -454,7 +477,7 @@ int32_t make_plan(const asc_pages_t* a, bool fork, const char* what, Plan& plan)
               ASC_ERR_INVALID_ARG, "%s: null buffer", what);
   ASC_REQUIRE(fork ? rows == 0 || (a->parents && a->lengths_out) : !counts || a->page_map, ASC_ERR_INVALID_ARG,
               "%s: null buffer", what);
-  int32_t rc = make_copy(*a, true, fork, what, plan.c);
+  int32_t rc = make_copy(*a, fork ? a->new_batch : a->num_pages / 2, true, fork, what, plan.c);
   if (rc != ASC_OK) return rc;
   const auto table_rows = [&](const char* name, const int32_t* data, int64_t stride, int64_t n) {
     return asc::region_of(name, asc_rows_t{const_cast<int32_t*>(data), stride, 0, 0}, n, 1, 1, a->width, 4);
@@ -517,19 +540,17 @@ extern "C" int32_t asc_cache_copy_pages(const asc_pages_t* a, asc_stream_t strea
   ASC_REQUIRE(a, ASC_ERR_INVALID_ARG, "%s: null arguments", what);
   ASC_REQUIRE(a->pairs >= 0 && a->num_pages >= 0 && a->to_num_pages >= 0, ASC_ERR_INVALID_ARG, "%s: negative shape", what);
   CopyArgs c{};
-  int32_t rc = make_copy(*a, false, false, what, c);
+  int32_t rc = make_copy(*a, a->pairs, false, false, what, c);
   if (rc != ASC_OK || a->pairs == 0 || c.n_tensors == 0) return rc;
   ASC_REQUIRE(a->from_pages && a->to_pages, ASC_ERR_INVALID_ARG, "%s: null buffer", what);
-  ASC_REQUIRE(a->pairs < int64_t{1} << 31, ASC_ERR_UNSUPPORTED, "%s: too many pairs", what);
   for (const asc::Region& x : {asc::region_of("from_pages", a->from_pages, a->pairs * 4),
                                asc::region_of("to_pages", a->to_pages, a->pairs * 4)}) {
     rc = check_apart(x, *a, c, false, what);
     if (rc != ASC_OK) return rc;
   }
-  c.moves = a->pairs;
   c.from = a->from_pages;
   c.to = a->to_pages;
-  hipLaunchKernelGGL(page_copy, dim3(static_cast<uint32_t>(groups_of(c.moves * c.per_move))), dim3(kThreads), 0,
+  hipLaunchKernelGGL(page_copy, dim3(static_cast<uint32_t>(groups_of(items_of(c)))), dim3(kThreads), 0,
                      static_cast<hipStream_t>(stream), c);
   return asc::check_launch(what);
 }
@@ -551,7 +572,6 @@ extern "C" int32_t asc_cache_fork(const asc_pages_t* a, void* workspace, int64_t
   plan.p.to = plan.p.from + n;
   plan.p.used = plan.p.to + n;
   CopyArgs& c = plan.c;
-  c.moves = a->new_batch;
   c.from = plan.p.from;
   c.to = plan.p.to;
   c.used = plan.p.used;
@@ -559,7 +579,7 @@ extern "C" int32_t asc_cache_fork(const asc_pages_t* a, void* workspace, int64_t
   hipLaunchKernelGGL(fork_plan, dim3(1), dim3(kPlanThreads), 0, s, plan.p);
   if (a->new_batch > 0) {
     const int rows = static_cast<int>(a->new_batch < 256 ? a->new_batch : 256);
-    const int64_t groups = rows + groups_of(c.moves * c.per_move);
+    const int64_t groups = rows + groups_of(items_of(c));
     hipLaunchKernelGGL(fork_move, dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0, s, c, plan.p, rows);
   }
   return asc::check_launch(what);
@@ -581,14 +601,13 @@ extern "C" int32_t asc_cache_compact(const asc_pages_t* a, void* workspace, int6
   plan.p.from = plan.p.count + 4;
   plan.p.to = plan.p.from + asc::ceil_div(a->num_pages, 4) * 4;
   CopyArgs& c = plan.c;
-  c.moves = a->num_pages / 2;
   c.count = plan.p.count;
   c.from = plan.p.from;
   c.to = plan.p.to;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(compact_plan, dim3(1), dim3(kPlanThreads), 0, s, plan.p);
   const int rows = static_cast<int>(a->batch < 256 ? a->batch : 256);
-  const int64_t groups = rows + groups_of(c.moves * c.per_move);
+  const int64_t groups = rows + groups_of(items_of(c));
   if (groups > 0) {
     hipLaunchKernelGGL(compact_move, dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0, s, c, plan.p, rows);
   }

@@ -3,7 +3,8 @@
 //
 // A workgroup owns a slice of one row's vocabulary.  It counts the history's tokens that fall into the
 // slice in LDS (integers: the order does not matter), then takes the slice through the formula.  The
-// whole history is read for every slice, from L2 after the first.
+// whole history is read for every slice, from L2 after the first.  HBM bounds large calls: 64 rows of 131072 fp32
+// logits with masks: 70.7 MB in 14.1 us (5.0 TB/s), in 17.3 us with 8000 tokens of history; the launch small ones.
 #include "common.h"
 #include "numeric.h"
 #include "overlap.h"
@@ -47,40 +48,38 @@ struct Bf16 {
   static __device__ __forceinline__ uint16_t store(float x) { return asc::f32_to_bf16_rne(x); }
 };
 
-constexpr int kThreads = 256;
 constexpr uint32_t kInPrompt = 0x80000000u;  // beside the count of a token behind the prompt
 
-// Tokens of the history that a thread has under way: one at a time, each waits for memory alone (47 us for 64
-// rows of 131072 with 8000 tokens, 15 with eight).
+// Tokens of the history that a thread has under way: one at a time, each waits for memory alone.
 constexpr int kAhead = 8;
 
-template <class T, class F>
-__device__ __forceinline__ void for_history(const void* history, int64_t at, int n, const F& count) {
-  const T* h = static_cast<const T*>(history) + at;
+// add(i, token) for the history's first n tokens; what is no uint32 becomes one that no vocabulary has.
+template <int kThreads, class T, class F>
+__device__ __forceinline__ void for_history(const T* history, int n, const F& add) {
   for (int base = threadIdx.x; base < n; base += kThreads * kAhead) {
     T token[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int i = base + k * kThreads;
-      token[k] = h[i < n ? i : base];
+      token[k] = history[i < n ? i : base];
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int i = base + k * kThreads;
-      if (i < n) count(i, token[k]);
+      const bool fits = sizeof(T) == 4 || static_cast<uint64_t>(token[k]) >> 32 == 0;
+      if (i < n) add(i, fits ? static_cast<uint32_t>(token[k]) : ~0u);
     }
   }
 }
 
-// kIters vectors of 16 bytes per thread.  kVec: the rows of logits and out lie at the same offset from 16
+// kPerThread tokens per thread.  kVec: the rows of logits and out lie at the same offset from 16
 // bytes, so vectors of the slice do, `lead` elements before the row's first; else element by element.
-template <class E, bool kVec, int kIters>
+template <class E, bool kVec, int kThreads, int kPerThread>
 __global__ void __launch_bounds__(kThreads) process_logits(LogitsArgs p) {
   typedef typename E::Stored S;
   constexpr int V = kVec ? 16 / sizeof(S) : 1;
-  constexpr int kPer = 16 / static_cast<int>(sizeof(S));
-  constexpr int kSlice = kThreads * kIters * kPer;
-  constexpr int kVecs = kIters * kPer / V;
+  constexpr int kSlice = kThreads * kPerThread;
+  constexpr int kVecs = kPerThread / V;
   __shared__ uint32_t counts[kSlice];
   const int tid = threadIdx.x;
   const uint32_t row = blockIdx.x / p.slices, slice = blockIdx.x - row * p.slices;
@@ -88,16 +87,13 @@ __global__ void __launch_bounds__(kThreads) process_logits(LogitsArgs p) {
   S* y = static_cast<S*>(p.out) + row * p.out_stride;
   const int lead = kVec ? static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(S)) : 0;
   const int first = static_cast<int>(slice) * kSlice - lead;  // token of counts[0]
-  const bool whole = kVec && first >= 0 && first + kSlice <= p.vocab;
+  // vectors that lie in the row are taken whole; `some`, the row's first, is read in place of the others
+  const int some = lead == 0 ? 0 : V - lead;
+  const bool vectors = kVec && some + V <= p.vocab;
+  const auto inside = [&](int token) { return token >= 0 && token + V <= p.vocab; };
 
-  // the slice's logits are under way while the history is counted
-  u32x4 held[kVec ? kVecs : 1];
-  if (whole) {
-#pragma unroll
-    for (int it = 0; it < (kVec ? kVecs : 0); ++it) {
-      held[it] = *reinterpret_cast<const u32x4*>(x + first + (tid + it * kThreads) * V);
-    }
-  }
+  const float* bias = p.bias ? p.bias + row * p.bias_stride : nullptr;
+  const uint32_t* mask = p.mask ? p.mask + row * p.mask_stride : nullptr;
 
   const int length = p.lengths[row];
   const bool bad = length < 0 || length > p.width;
@@ -109,9 +105,11 @@ __global__ void __launch_bounds__(kThreads) process_logits(LogitsArgs p) {
     reinterpret_cast<u32x4*>(counts)[tid + i * kThreads] = u32x4{0, 0, 0, 0};
   }
   __syncthreads();
-  const auto count = [&](int i, int64_t token) {
-    const int64_t at = token - first;
-    if (token < 0 || token >= p.vocab || at < 0 || at >= kSlice) return;
+  const uint32_t here = min(kSlice, p.vocab - first);
+  const auto count = [&](int i, uint32_t token) {
+    // what is counted before the row's first token is looked at by nobody
+    const uint32_t at = token - static_cast<uint32_t>(first);
+    if (at >= here) return;
     if (i < prompt) {
       atomicOr(&counts[at], kInPrompt);
     } else {
@@ -119,17 +117,15 @@ __global__ void __launch_bounds__(kThreads) process_logits(LogitsArgs p) {
     }
   };
   if (p.history_int64) {
-    for_history<int64_t>(p.history, row * p.history_stride, n, count);
+    for_history<kThreads>(static_cast<const int64_t*>(p.history) + row * p.history_stride, n, count);
   } else {
-    for_history<int32_t>(p.history, row * p.history_stride, n, count);
+    for_history<kThreads>(static_cast<const int32_t*>(p.history) + row * p.history_stride, n, count);
   }
   __syncthreads();
 
   const float repetition = p.repetition ? p.repetition[row] : 1.0f;
   const float frequency = p.frequency ? p.frequency[row] : 0.0f;
   const float presence = p.presence ? p.presence[row] : 0.0f;
-  const float* bias = p.bias ? p.bias + row * p.bias_stride : nullptr;
-  const uint32_t* mask = p.mask ? p.mask + row * p.mask_stride : nullptr;
   const auto process = [&](uint32_t c, float v, float add, bool allowed) {
     if (c != 0) {
       v = v > 0.0f ? v / repetition : v * repetition;
@@ -142,14 +138,17 @@ __global__ void __launch_bounds__(kThreads) process_logits(LogitsArgs p) {
     return allowed ? v : -INFINITY;
   };
   const auto allowed = [&](int token) { return !mask || ((mask[token >> 5] >> (token & 31)) & 1); };
-  if (whole) {
-    if constexpr (kVec) {
-      const bool bias_vec = ((reinterpret_cast<uintptr_t>(bias) >> 2) + first) % 4 == 0;
+  if constexpr (kVec) {
+    if (vectors) {
+      u32x4 held[kVecs];
       float add[kVecs][V];
       uint64_t bits[kVecs];
+      const bool bias_vec = ((reinterpret_cast<uintptr_t>(bias) >> 2) + some) % 4 == 0;
 #pragma unroll
       for (int it = 0; it < kVecs; ++it) {
-        const int token = first + (tid + it * kThreads) * V;
+        int token = first + (tid + it * kThreads) * V;
+        token = inside(token) ? token : some;
+        held[it] = *reinterpret_cast<const u32x4*>(x + token);
         if (bias) {
           if (bias_vec) {
 #pragma unroll
@@ -163,8 +162,8 @@ __global__ void __launch_bounds__(kThreads) process_logits(LogitsArgs p) {
         }
         bits[it] = ~0ull;
         if (mask) {
-          bits[it] = (static_cast<uint64_t>(mask[(token + V - 1) >> 5]) << 32 | mask[token >> 5]) >> (token & 31);
           // both words are the same one, unless the vector lies across two
+          bits[it] = (static_cast<uint64_t>(mask[(token + V - 1) >> 5]) << 32 | mask[token >> 5]) >> (token & 31);
         }
       }
 #pragma unroll
@@ -177,46 +176,39 @@ __global__ void __launch_bounds__(kThreads) process_logits(LogitsArgs p) {
         for (int e = 0; e < V; e += 4) *reinterpret_cast<u32x4*>(&c[e]) = *reinterpret_cast<const u32x4*>(&counts[at + e]);
 #pragma unroll
         for (int e = 0; e < V; ++e) out[e] = E::store(process(c[e], E::load(in[e]), add[it][e], bits[it] >> e & 1));
-        *reinterpret_cast<u32x4*>(y + first + at) = *reinterpret_cast<u32x4*>(out);
+        if (inside(first + at)) *reinterpret_cast<u32x4*>(y + first + at) = *reinterpret_cast<u32x4*>(out);
       }
     }
-    return;
   }
-#pragma unroll
-  for (int it = 0; it < kVecs; ++it) {
-    const int at = (tid + it * kThreads) * V, token = first + at;
-    if (token >= p.vocab || token + V <= 0) continue;
-    if (V > 1 && token >= 0 && token + V <= p.vocab) {
-      S in[V], out[V];
-      *reinterpret_cast<u32x4*>(in) = *reinterpret_cast<const u32x4*>(x + token);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        out[e] = E::store(process(counts[at + e], E::load(in[e]), bias ? bias[token + e] : 0.0f, allowed(token + e)));
-      }
-      *reinterpret_cast<u32x4*>(y + token) = *reinterpret_cast<u32x4*>(out);
-    } else {
-      for (int e = 0; e < V; ++e) {
-        const int t = token + e;
-        if (t >= 0 && t < p.vocab) {
-          y[t] = E::store(process(counts[at + e], E::load(x[t]), bias ? bias[t] : 0.0f, allowed(t)));
-        }
-      }
+  // element by element: the row's ends, or all of it
+  for (int at = tid * V; at < kSlice; at += kThreads * V) {
+    const int token = first + at;
+    if (token >= p.vocab) break;
+    if (vectors && inside(token)) continue;
+    for (int e = 0; e < V; ++e) {
+      const int t = token + e;
+      if (t < 0 || t >= p.vocab) continue;
+      y[t] = E::store(process(counts[at + e], E::load(x[t]), bias ? bias[t] : 0.0f, allowed(t)));
     }
   }
 }
 
-// Tokens of a workgroup's slice: fewer where there are few rows, whose workgroups would leave most of the chip idle.
-constexpr int kLarge = 8192, kSmall = 2048;
-constexpr int64_t kFewGroups = 512;
+// Workgroups of many threads read the history in few rounds and few times: 64 rows of 131072 fp32 logits with 8000 tokens
+// of history 17.3 us with 1024 threads and 16384 tokens, 18.8 with 256 and 4096, 21.3 with 256 and 2048.  The last where
+// the large would not fill the chip (16 rows: 9.3 us, 10.4 large; 32 rows: 13.2, 12.0) and the history is no longer than what
+// reading it that often costs (4 rows, 30000 tokens: 13.1, 11.1 large).
+constexpr int kLargeThreads = 1024, kLarge = 16384, kSmallThreads = 256, kSmall = 2048;
+constexpr int64_t kFewGroups = 256, kLongHistory = 16384;
 
 template <class E, bool kVec>
 void launch(const LogitsArgs& p, int64_t rows, bool small, hipStream_t stream) {
-  constexpr int kPer = kThreads * 16 / static_cast<int>(sizeof(typename E::Stored));
   const dim3 grid(static_cast<uint32_t>(rows * p.slices));
   if (small) {
-    hipLaunchKernelGGL((process_logits<E, kVec, kSmall / kPer>), grid, dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((process_logits<E, kVec, kSmallThreads, kSmall / kSmallThreads>), grid, dim3(kSmallThreads), 0, stream,
+                       p);
   } else {
-    hipLaunchKernelGGL((process_logits<E, kVec, kLarge / kPer>), grid, dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((process_logits<E, kVec, kLargeThreads, kLarge / kLargeThreads>), grid, dim3(kLargeThreads), 0, stream,
+                       p);
   }
 }
 
@@ -276,9 +268,9 @@ extern "C" int32_t asc_process_logits(const asc_logits_t* a, asc_stream_t stream
   // room for the lead of rows that do not begin at 16 bytes
   const bool aligned = asc::aligned16(a->logits) && (a->rows == 1 || a->logits_stride * size % 16 == 0);
   const int64_t tokens = a->vocab + (aligned ? 0 : 16 / size - 1);
-  const bool small = a->rows * asc::ceil_div(tokens, kLarge) < kFewGroups;
+  const bool small = a->rows * asc::ceil_div(tokens, kLarge) < kFewGroups && a->history_width <= kLongHistory;
   p.slices = static_cast<int32_t>(asc::ceil_div(tokens, small ? kSmall : kLarge));
-  ASC_REQUIRE(a->rows * p.slices < int64_t{1} << 24, ASC_ERR_UNSUPPORTED, "%s: %lld workgroups exceed the launch grid limit",
+  ASC_REQUIRE(a->rows * p.slices < int64_t{1} << 22, ASC_ERR_UNSUPPORTED, "%s: %lld workgroups exceed the launch grid limit",
               what, static_cast<long long>(a->rows * p.slices));
   const uintptr_t apart = reinterpret_cast<uintptr_t>(a->logits) ^ reinterpret_cast<uintptr_t>(a->out);
   const int64_t steps = a->rows > 1 ? (a->logits_stride - a->out_stride) * size : 0;

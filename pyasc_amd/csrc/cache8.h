@@ -57,14 +57,14 @@ struct Int8 {
   static __device__ __forceinline__ float value(uint32_t w, int k) {
     return static_cast<float>(static_cast<int8_t>(w >> (8 * k)));
   }
-  // codes of four values within the format's range, to nearest even
-  static __device__ __forceinline__ uint32_t pack(const float (&x)[4]) {
-    uint32_t w = 0;
+  // codes of four values times `inverse`, a power of two, within the format's range: to nearest even, as the sum with
+  // 1.5 * 2^23 is rounded, whose lowest byte is the code
+  static __device__ __forceinline__ uint32_t pack(const float (&x)[4], float inverse) {
+    uint32_t w[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      w |= (static_cast<uint32_t>(static_cast<int>(rintf(x[k]))) & 0xffu) << (8 * k);
-    }
-    return w;
+    for (int k = 0; k < 4; ++k) w[k] = __float_as_uint(fmaf(x[k], inverse, 12582912.0f));
+    const uint32_t lo = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(w[3], w[2], 0x04000c0cu);
+    return lo | hi;
   }
   static __device__ __forceinline__ float of_nan(float) { return 0.0f; }
 };
@@ -77,9 +77,9 @@ struct E4m3 {
                           : __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), true);
     return v[k & 1];
   }
-  static __device__ __forceinline__ uint32_t pack(const float (&x)[4]) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true));
+  static __device__ __forceinline__ uint32_t pack(const float (&x)[4], float inverse) {
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inverse, x[1] * inverse, 0, false);
+    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inverse, x[3] * inverse, w, true));
   }
   static __device__ __forceinline__ float of_nan(float x) { return x; }
 };

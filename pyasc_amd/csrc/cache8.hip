@@ -13,13 +13,15 @@ namespace {
 using asc::c8::Cache;
 using asc::c8::u32x2;
 using asc::c8::u32x4;
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 struct RowsArgs {
   Cache c;
   uint8_t* k_new;
   uint8_t* v_new;
   int64_t k_batch, k_head, k_seq, v_batch, v_head, v_seq;  // elements
-  int32_t batch, blocks;  // blocks that n tokens can reach
+  asc::Divisor heads, blocks;  // blocks that n tokens can reach (append), or runs of tokens (read)
+  int32_t batch;
 };
 
 template <bool kBf16>
@@ -52,24 +54,19 @@ __device__ __forceinline__ float group_max(float v, float (&waves)[kWaves]) {
 template <int D, class Q, bool kBf16, int kWaves, int kVecs>
 __global__ void __launch_bounds__(kWaves * 64) append(RowsArgs p) {
   constexpr int kThreads = kWaves * 64, kPerRow = D / 8, kChunk = kThreads * kVecs;
-  __shared__ float waves[kWaves];
+  __shared__ float waves[kWaves], waves_special[kWaves], waves_finite[kWaves];
   const Cache& c = p.c;
   uint32_t id = blockIdx.x;
   const bool is_v = id & 1;
   id >>= 1;
-  const uint32_t pair = id / p.blocks;
-  const int slot = static_cast<int>(id - pair * p.blocks);
-  const int b = static_cast<int>(pair / c.kv_heads), head = static_cast<int>(pair - b * c.kv_heads);
+  const uint32_t pair = p.blocks.divide(id);
+  const int slot = static_cast<int>(id - pair * p.blocks.d);
+  const int b = static_cast<int>(p.heads.divide(pair)), head = static_cast<int>(pair - b * p.heads.d);
   const int length = c.lengths[b], n = c.news ? c.news[b] : c.n;
   if (length < 0 || n <= 0 || n > c.n || length > c.capacity - n) return;
   const int size = static_cast<int>(c.block.d);
   const int start = (static_cast<int>(c.block.divide(length)) + slot) * size;  // the block's first key
   if (start >= length + n) return;
-  uint32_t page, row;
-  if (!asc::c8::place(c, b, start, page, row)) return;
-  const auto& strides = is_v ? c.vs : c.ks;
-  uint8_t* codes = (is_v ? c.v : c.k) + asc::c8::row_at(strides, page, head, row);
-  float* scale_place = (is_v ? c.v_scale : c.k_scale) + asc::c8::scale_at(c, is_v ? c.vss : c.kss, page, head, row);
   const uint16_t* x = reinterpret_cast<const uint16_t*>(is_v ? p.v_new : p.k_new) +
                       b * (is_v ? p.v_batch : p.k_batch) + head * (is_v ? p.v_head : p.k_head);
   const int64_t step = is_v ? p.v_seq : p.k_seq;
@@ -78,7 +75,6 @@ __global__ void __launch_bounds__(kWaves * 64) append(RowsArgs p) {
   const int first_vec = max(old, 0) * kPerRow, end_vec = end * kPerRow;
 
   u32x4 held[kVecs];
-  float amax = 0.0f;
   const auto load = [&](int base) {
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
@@ -87,33 +83,60 @@ __global__ void __launch_bounds__(kWaves * 64) append(RowsArgs p) {
       if (vec < end_vec) held[i] = *reinterpret_cast<const u32x4*>(x + (vec / kPerRow - old) * step + vec % kPerRow * 8);
     }
   };
+  // the new rows, the page and the held scale are under way together
+  load(first_vec);
+  uint32_t page, row;
+  const bool good = asc::c8::place(c, b, start, page, row);
+  const auto& strides = is_v ? c.vs : c.ks;
+  float* scale_place = (is_v ? c.v_scale : c.k_scale) + asc::c8::scale_at(c, is_v ? c.vss : c.kss, good ? page : 0, head, row);
+  float before = 0.0f;
+  if (old > 0) before = *scale_place;
+  if (!good) return;
+  uint8_t* codes = (is_v ? c.v : c.k) + asc::c8::row_at(strides, page, head, row);
+
+  // magnitudes are ordered as the integers of their bits, infinities and NaN above all
   const bool once = end_vec - first_vec <= kChunk;
+  u16x2 most = {0, 0};
   for (int base = first_vec; base < end_vec; base += kChunk) {
-    load(base);
+    if (!once) load(base);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = fabsf(to_f32<kBf16>(static_cast<uint16_t>(held[i][e / 2] >> (e % 2 * 16))));
-        amax = v < INFINITY ? fmaxf(amax, v) : amax;
+      for (int w = 0; w < 4; ++w) {
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, held[i][w] & 0x7fff7fffu));
       }
   }
-  amax = group_max(amax, waves);
-  float scale = scale_for<Q>(amax);
-  float before = 0.0f;
-  if (old > 0) {
-    before = *scale_place;
-    if (!(before > 0.0f && before < INFINITY)) before = 0.0f;
+  const uint16_t top = most[0] > most[1] ? most[0] : most[1];
+  const float largest = group_max(kBf16 ? asc::bf16_to_f32(top) : (top >= 0x7c00u ? INFINITY : asc::f16_to_f32(top)), waves);
+  // a bf16 NaN is lost in group_max, but not that a lane had one
+  const bool special = group_max(top >= (kBf16 ? 0x7f80u : 0x7c00u) ? 1.0f : 0.0f, waves_special) != 0.0f;
+  float amax = largest;
+  if (special) {  // of the finite ones
+    amax = 0.0f;
+    for (int base = first_vec; base < end_vec; base += kChunk) {
+      if (!once) load(base);
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = fabsf(to_f32<kBf16>(static_cast<uint16_t>(held[i][e / 2] >> (e % 2 * 16))));
+          amax = v < INFINITY ? fmaxf(amax, v) : amax;
+        }
+    }
+    amax = group_max(amax, waves_finite);
   }
+  float scale = scale_for<Q>(amax);
+  if (!(before > 0.0f && before < INFINITY)) before = 0.0f;
   const bool grows = before < scale;
   if (!grows) scale = before;
 
-  const auto quantize = [&](float v) {
+  const auto in_range = [&](float v) {
     if (v != v) return Q::of_nan(v);
     return fminf(fmaxf(v, -Q::kMost), Q::kMost);
   };
-  // by a power of two the quotient is a product
+  // By a power of two the quotient is a product, and finite values need no bounds.
   const bool power = (__float_as_uint(scale) & 0x7fffffu) == 0 && scale >= 0x1p-126f && scale <= 0x1p126f;
+  const bool plain = power && !special;
   const float inverse = power ? 1.0f / scale : 0.0f;
   for (int base = first_vec; base < end_vec; base += kChunk) {
     if (!once) load(base);
@@ -125,11 +148,14 @@ __global__ void __launch_bounds__(kWaves * 64) append(RowsArgs p) {
       for (int half = 0; half < 2; ++half) {
         float q[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v = to_f32<kBf16>(static_cast<uint16_t>(held[i][half * 2 + e / 2] >> (e % 2 * 16)));
-          q[e] = quantize(power ? v * inverse : v / scale);
+        for (int e = 0; e < 4; ++e) q[e] = to_f32<kBf16>(static_cast<uint16_t>(held[i][half * 2 + e / 2] >> (e % 2 * 16)));
+        if (plain) {
+          w[half] = Q::pack(q, inverse);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[e] = in_range(power ? q[e] * inverse : q[e] / scale);
+          w[half] = Q::pack(q, 1.0f);
         }
-        w[half] = Q::pack(q);
       }
       if (vec < end_vec) *reinterpret_cast<u32x2*>(codes + (vec / kPerRow) * (strides.row * 16u) + vec % kPerRow * 8) = w;
     }
@@ -143,8 +169,8 @@ __global__ void __launch_bounds__(kWaves * 64) append(RowsArgs p) {
       for (int half = 0; half < 2; ++half) {
         float q[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) q[e] = quantize(Q::value(w[half], e) * before / scale);
-        w[half] = Q::pack(q);
+        for (int e = 0; e < 4; ++e) q[e] = in_range(Q::value(w[half], e) * before / scale);
+        w[half] = Q::pack(q, 1.0f);
       }
       *at = w;
     }
@@ -152,44 +178,62 @@ __global__ void __launch_bounds__(kWaves * 64) append(RowsArgs p) {
   if (threadIdx.x == 0 && (old <= 0 || grows)) *scale_place = scale;
 }
 
-// Eight values of a token's head per thread.
+// A workgroup reads a run of tokens of one head, kVecs vectors of eight values per thread, whose pages, codes and scales are
+// under way together.
+constexpr int kReadVecs = 4;
+template <int D>
+constexpr int kReadTokens = 256 * kReadVecs / (D / 8);
+
 template <int D, class Q, class T>
-__global__ void __launch_bounds__(256) read(RowsArgs p, int64_t vecs) {
-  constexpr int kPerRow = D / 8;
+__global__ void __launch_bounds__(256) read(RowsArgs p) {
+  constexpr int kPerRow = D / 8, kStep = 256 / kPerRow;
   const Cache& c = p.c;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= vecs) return;
-  int64_t at = i / kPerRow;
-  const int ch = static_cast<int>(i - at * kPerRow);
-  const int token = static_cast<int>(at % c.n);
-  at /= c.n;
-  const int head = static_cast<int>(at % c.kv_heads);
-  at /= c.kv_heads;
-  const int b = static_cast<int>(at % p.batch);
-  const bool is_v = at >= p.batch || p.k_new == nullptr;
+  uint32_t pair = p.blocks.divide(blockIdx.x);
+  const int first = static_cast<int>(blockIdx.x - pair * p.blocks.d) * kReadTokens<D> + static_cast<int>(threadIdx.x) / kPerRow;
+  const bool is_v = p.k_new == nullptr || pair >= p.heads.d * p.batch;
+  if (is_v && p.k_new) pair -= p.heads.d * p.batch;
+  const int b = static_cast<int>(p.heads.divide(pair)), head = static_cast<int>(pair - b * p.heads.d);
+  const int ch = static_cast<int>(threadIdx.x) % kPerRow;
   const int start = c.lengths[b], n = c.news ? c.news[b] : c.n;
-  if (token >= n) return;
-  bool good = start >= 0 && n <= c.n && start <= c.capacity - n;
-  uint32_t page = 0, row = 0;
-  if (good) good = asc::c8::place(c, b, start + token, page, row);
-  float out[8];
+  const bool fits = start >= 0 && n <= c.n && start <= c.capacity - n;
+  const auto& strides = is_v ? c.vs : c.ks;
+  const uint8_t* codes = is_v ? c.v : c.k;
+  const float* scales = is_v ? c.v_scale : c.k_scale;
+  T* to = reinterpret_cast<T*>(is_v ? p.v_new : p.k_new) + b * (is_v ? p.v_batch : p.k_batch) + head * (is_v ? p.v_head : p.k_head) +
+          ch * 8;
+  const int64_t step = is_v ? p.v_seq : p.k_seq;
+  const int most = min(n, c.n);  // written, whatever the lengths are
+  uint32_t page[kReadVecs], row[kReadVecs];
+  bool good[kReadVecs];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) out[e] = __builtin_nanf("");
-  if (good) {
-    const u32x2 w = *reinterpret_cast<const u32x2*>((is_v ? c.v : c.k) +
-                                                    asc::c8::row_at(is_v ? c.vs : c.ks, page, head, row) + ch * 8);
-    const float scale = (is_v ? c.v_scale : c.k_scale)[asc::c8::scale_at(c, is_v ? c.vss : c.kss, page, head, row)];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] = Q::value(w[e / 4], e % 4) * scale;
+  for (int i = 0; i < kReadVecs; ++i) {
+    const int token = first + i * kStep;
+    page[i] = row[i] = 0;
+    good[i] = fits && token < most;
+    if (good[i]) good[i] = asc::c8::place(c, b, start + token, page[i], row[i]);
   }
-  T* to = reinterpret_cast<T*>(is_v ? p.v_new : p.k_new) + b * (is_v ? p.v_batch : p.k_batch) +
-          head * (is_v ? p.v_head : p.k_head) + token * (is_v ? p.v_seq : p.k_seq) + ch * 8;
-  T packed[8];
+  u32x2 w[kReadVecs];
+  float scale[kReadVecs];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) packed[e] = static_cast<T>(out[e]);
+  for (int i = 0; i < kReadVecs; ++i) {
+    w[i] = u32x2{0, 0};
+    scale[i] = __builtin_nanf("");
+    if (good[i]) {
+      w[i] = *reinterpret_cast<const u32x2*>(codes + asc::c8::row_at(strides, page[i], head, row[i]) + ch * 8);
+      scale[i] = scales[asc::c8::scale_at(c, is_v ? c.vss : c.kss, page[i], head, row[i])];
+    }
+  }
 #pragma unroll
-  for (int e = 0; e < static_cast<int>(sizeof(T)) / 2; ++e) {
-    reinterpret_cast<u32x4*>(to)[e] = reinterpret_cast<const u32x4*>(packed)[e];
+  for (int i = 0; i < kReadVecs; ++i) {
+    const int token = first + i * kStep;
+    if (token >= most) continue;
+    T packed[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) packed[e] = static_cast<T>(Q::value(w[i][e / 4], e % 4) * scale[i]);
+#pragma unroll
+    for (int e = 0; e < static_cast<int>(sizeof(T)) / 2; ++e) {
+      reinterpret_cast<u32x4*>(to + token * step)[e] = reinterpret_cast<const u32x4*>(packed)[e];
+    }
   }
 }
 
@@ -221,6 +265,7 @@ int32_t make(const asc_cache8_t* a, bool reads, const char* what, Launch& L) {
   p.v_head = a->v_new.head_stride;
   p.v_seq = a->v_new.seq_stride;
   p.batch = static_cast<int32_t>(a->batch);
+  p.heads = asc::divisor_of(static_cast<uint32_t>(a->kv_heads));
   L.tensors = (p.k_new != nullptr) + (p.v_new != nullptr);
   asc::Region cache[asc::c8::kRegions];
   asc::c8::regions_of(*a, cache);
@@ -263,14 +308,14 @@ int32_t launch_append(const Launch& L, int64_t units, hipStream_t s) {
 }
 
 template <int D, class Q>
-void launch_read(const Launch& L, int32_t dtype, int64_t vecs, hipStream_t s) {
-  const dim3 grid(static_cast<uint32_t>(asc::ceil_div(vecs, 256)));
+void launch_read(const Launch& L, int32_t dtype, int64_t groups, hipStream_t s) {
+  const dim3 grid(static_cast<uint32_t>(groups));
   if (dtype == ASC_DT_FLOAT32) {
-    hipLaunchKernelGGL((read<D, Q, float>), grid, dim3(256), 0, s, L.p, vecs);
+    hipLaunchKernelGGL((read<D, Q, float>), grid, dim3(256), 0, s, L.p);
   } else if (dtype == ASC_DT_FLOAT16) {
-    hipLaunchKernelGGL((read<D, Q, _Float16>), grid, dim3(256), 0, s, L.p, vecs);
+    hipLaunchKernelGGL((read<D, Q, _Float16>), grid, dim3(256), 0, s, L.p);
   } else {
-    hipLaunchKernelGGL((read<D, Q, __bf16>), grid, dim3(256), 0, s, L.p, vecs);
+    hipLaunchKernelGGL((read<D, Q, __bf16>), grid, dim3(256), 0, s, L.p);
   }
 }
 
@@ -376,8 +421,9 @@ extern "C" int32_t asc_quantized_cache_append(const asc_cache8_t* a, asc_stream_
   const int32_t rc = make(a, false, what, L);
   if (rc != ASC_OK || L.tensors == 0 || L.p.c.capacity == 0) return rc;
   const int64_t block = a->scale_block;
-  L.p.blocks = static_cast<int32_t>((a->n + block - 2) / block + 1);
-  const int64_t units = 2 * a->batch * a->kv_heads * L.p.blocks;
+  const int64_t blocks = (a->n + block - 2) / block + 1;
+  L.p.blocks = asc::divisor_of(static_cast<uint32_t>(blocks));
+  const int64_t units = 2 * a->batch * a->kv_heads * blocks;
   ASC_REQUIRE(units < int64_t{1} << 24, ASC_ERR_UNSUPPORTED, "%s: %lld workgroups exceed the launch grid limit", what,
               static_cast<long long>(units));
   const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -399,15 +445,18 @@ extern "C" int32_t asc_quantized_cache_read(const asc_cache8_t* a, asc_stream_t 
   Launch L;
   const int32_t rc = make(a, true, what, L);
   if (rc != ASC_OK || L.tensors == 0) return rc;
-  const int64_t vecs = L.tensors * a->batch * a->kv_heads * a->n * (a->head_dim / 8);
-  ASC_REQUIRE(vecs < int64_t{1} << 32, ASC_ERR_UNSUPPORTED, "%s: too many rows", what);
+  const int64_t runs = asc::ceil_div(a->n, a->head_dim == 64 ? kReadTokens<64> : kReadTokens<128>);
+  const int64_t groups = L.tensors * a->batch * a->kv_heads * runs;
+  ASC_REQUIRE(groups < int64_t{1} << 24, ASC_ERR_UNSUPPORTED, "%s: %lld workgroups exceed the launch grid limit", what,
+              static_cast<long long>(groups));
+  L.p.blocks = asc::divisor_of(static_cast<uint32_t>(runs));
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (a->cache_dtype == ASC_DT_INT8) {
-    a->head_dim == 64 ? launch_read<64, asc::c8::Int8>(L, a->dtype, vecs, s)
-                      : launch_read<128, asc::c8::Int8>(L, a->dtype, vecs, s);
+    a->head_dim == 64 ? launch_read<64, asc::c8::Int8>(L, a->dtype, groups, s)
+                      : launch_read<128, asc::c8::Int8>(L, a->dtype, groups, s);
   } else {
-    a->head_dim == 64 ? launch_read<64, asc::c8::E4m3>(L, a->dtype, vecs, s)
-                      : launch_read<128, asc::c8::E4m3>(L, a->dtype, vecs, s);
+    a->head_dim == 64 ? launch_read<64, asc::c8::E4m3>(L, a->dtype, groups, s)
+                      : launch_read<128, asc::c8::E4m3>(L, a->dtype, groups, s);
   }
   return asc::check_launch(what);
 }

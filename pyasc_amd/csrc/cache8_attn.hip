@@ -48,6 +48,9 @@ Way way_of(int64_t heads, int64_t row_blocks, int64_t tiles, int64_t slots, int 
   if (shares < slots) w.splits = fill * slots / shares;
   if (w.splits > tiles / least) w.splits = tiles / least;
   if (w.splits > kMaxSplits) w.splits = kMaxSplits;
+#ifdef SPL
+  w.splits = SPL;
+#endif
   if (w.splits < 1) w.splits = 1;
   const int64_t chain = asc::ceil_div(asc::ceil_div(tiles, w.splits), waves);
   w.us = static_cast<double>(asc::ceil_div(shares * w.splits, slots)) * (start + tile * static_cast<double>(chain)) +
@@ -67,6 +70,10 @@ void plan(Launch& L, const asc_cache8_t& a) {
   const Way& w = L.wide ? wide : narrow;
   p.row_blocks = static_cast<int>(w.row_blocks);
   p.splits = static_cast<int>(w.splits);
+  p.by_n = asc::divisor_of(static_cast<uint32_t>(p.c.n));
+  p.by_heads = asc::divisor_of(static_cast<uint32_t>(p.c.kv_heads));
+  p.by_splits = asc::divisor_of(static_cast<uint32_t>(p.splits));
+  p.by_row_blocks = asc::divisor_of(static_cast<uint32_t>(p.row_blocks));
   p.units = static_cast<uint32_t>(heads * p.splits);
   L.rows_all = heads * p.rows;
   p.join_groups = small ? asc::kv::JoinLanes<64>::groups_of(L.rows_all, p.splits)

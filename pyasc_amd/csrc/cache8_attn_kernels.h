@@ -40,7 +40,11 @@ struct AttnArgs {
   float* part_ml;  // [unit][rows][2]: reference point (log2), sum
   int32_t batch, group, rows, row_blocks, splits, join_groups, causal;
   uint32_t units;  // batch * splits * kv_heads
+  Divisor by_n, by_heads, by_splits, by_row_blocks;
   float scale_log2;
+
+  // Tiles of a split of `total` tiles: the last splits may have none.
+  __device__ __forceinline__ int per(int total) const { return static_cast<int>(by_splits.divide(total + splits - 1)); }
 };
 
 // Four codes of a word as two packed pairs of fp16.
@@ -69,14 +73,14 @@ __device__ __forceinline__ u32x4 operand_of(uint32_t lo, uint32_t hi) {
 // One workgroup's share, as kv::Share.
 __device__ __forceinline__ kv::Share share_of(const AttnArgs& p) {
   const uint32_t slot = blockIdx.x >> 3;
-  const uint32_t per = slot / p.row_blocks;
+  const uint32_t per = p.by_row_blocks.divide(slot);
   kv::Share s;
   s.unit = per * 8 + (blockIdx.x & 7);
   s.live = s.unit < p.units;
   s.row0 = p.row_blocks - 1 - static_cast<int>(slot - per * p.row_blocks);  // causal: the longest first
-  const uint32_t range = s.unit / p.c.kv_heads;
+  const uint32_t range = p.by_heads.divide(s.unit);
   s.head = static_cast<int>(s.unit - range * p.c.kv_heads);
-  s.b = static_cast<int>(range / p.splits);
+  s.b = static_cast<int>(p.by_splits.divide(range));
   s.split = static_cast<int>(range - static_cast<uint32_t>(s.b) * p.splits);
   return s;
 }
@@ -99,8 +103,8 @@ __device__ __forceinline__ int written_of(const AttnArgs& p, int b) { return p.c
 // The most keys that a row of row0 .. row0 + rows - 1 attends.
 __device__ __forceinline__ int limit_of_rows(const AttnArgs& p, const Sequence& s, int row0, int rows) {
   const int last = min(row0 + rows, p.rows) - 1;
-  const int g = row0 / p.c.n;
-  const int query = last / p.c.n == g ? last - g * p.c.n : p.c.n - 1;
+  const int g = p.by_n.divide(row0);
+  const int query = static_cast<int>(p.by_n.divide(last)) == g ? last - g * p.c.n : p.c.n - 1;
   const int q = min(query, s.news - 1);
   return q < 0 ? 0 : s.limit(q);
 }
@@ -108,9 +112,9 @@ __device__ __forceinline__ int limit_of_rows(const AttnArgs& p, const Sequence& 
 // The fewest keys that a row of row0 .. row0 + rows - 1 with a query attends.
 __device__ __forceinline__ int least_of_rows(const AttnArgs& p, const Sequence& s, int row0, int rows) {
   const int last = min(row0 + rows, p.rows) - 1;
-  const int g = row0 / p.c.n, query = row0 - g * p.c.n;
+  const int g = p.by_n.divide(row0), query = row0 - g * p.c.n;
   // the first row's, where they are of one head; else a head's first query is among them
-  if (last / p.c.n == g) return query < s.news ? s.limit(query) : s.len;
+  if (static_cast<int>(p.by_n.divide(last)) == g) return query < s.news ? s.limit(query) : s.len;
   return s.news > 0 ? s.limit(0) : s.len;
 }
 
@@ -118,7 +122,7 @@ __device__ __forceinline__ int least_of_rows(const AttnArgs& p, const Sequence& 
 __device__ __forceinline__ bool out_row(const AttnArgs& p, const kv::Share& s, int row, int written, int64_t& o_at,
                                         int64_t& lse_at) {
   if (row >= p.rows) return false;
-  const int g = row / p.c.n, query = row - g * p.c.n;
+  const int g = p.by_n.divide(row), query = row - g * p.c.n;
   if (query >= written) return false;
   const int64_t head = s.head * p.group + g;
   o_at = s.b * p.o_batch + head * p.o_head + query * p.o_seq;
@@ -126,27 +130,28 @@ __device__ __forceinline__ bool out_row(const AttnArgs& p, const kv::Share& s, i
   return true;
 }
 
-// This lane's row: its query (-1: none), its keys, and its elements in fp16.  kPairs: lane half h holds columns
-// 32 t + 16 h + 0..15 in operands 2 t and 2 t + 1 (as K's codes are read), else 16 k + 8 h + 0..7 in operand k.
-template <int D, class E, bool kPairs>
-__device__ __forceinline__ void load_query(const AttnArgs& p, const kv::Share& s, const Sequence& seq, int row, int h,
-                                           u32x4 (&q)[D / 16], int& limit, float& factor) {
-  int query = -1;
-  int64_t at = 0;
-  if (row < p.rows) {
-    const int g = row / p.c.n;
-    query = row - g * p.c.n;
-    at = s.b * p.q_batch + static_cast<int64_t>(s.head * p.group + g) * p.q_head + query * p.q_seq;
-  }
-  if (query >= seq.news) query = -1;
-  limit = query >= 0 ? seq.limit(query) : seq.len;  // a row without a query restricts nothing
-  factor = p.scale_log2;
+// This lane's row: its elements, and its query (-1: none).  kPairs: lane half h holds columns 32 t + 16 h + 0..15 in
+// operands 2 t and 2 t + 1 (as K's codes are read), else 16 k + 8 h + 0..7 in operand k.
+template <int D, bool kPairs>
+__device__ __forceinline__ int load_query(const AttnArgs& p, const kv::Share& s, int row, int h, u32x4 (&q)[D / 16]) {
+  const int r = min(row, p.rows - 1), g = p.by_n.divide(r), query = r - g * p.c.n;
+  const uint16_t* at = p.q + s.b * p.q_batch + static_cast<int64_t>(s.head * p.group + g) * p.q_head + query * p.q_seq;
 #pragma unroll
   for (int k = 0; k < D / 16; ++k) {
     const int column = kPairs ? (k >> 1) * 32 + h * 16 + (k & 1) * 8 : k * 16 + h * 8;
-    q[k] = u32x4{0, 0, 0, 0};
-    if (query >= 0) q[k] = *reinterpret_cast<const u32x4*>(p.q + at + column);
+    q[k] = *reinterpret_cast<const u32x4*>(at + column);
   }
+  return row < p.rows ? query : -1;
+}
+// The keys that it attends (a row without a query restricts nothing), its elements in fp16 and its scores' factor.
+template <int D, class E>
+__device__ __forceinline__ void take_query(const AttnArgs& p, const Sequence& seq, int query, u32x4 (&q)[D / 16], int& limit,
+                                           float& factor) {
+  const bool any = query >= 0 && query < seq.news;
+  limit = any ? seq.limit(query) : seq.len;
+  factor = p.scale_log2;
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) q[k] = any ? q[k] : u32x4{0, 0, 0, 0};
   if constexpr (__is_same(E, fa::Bf16)) {
     uint32_t most = 0;
 #pragma unroll
@@ -180,23 +185,32 @@ struct Rows {
   int len, b;
   bool poison;
 
-  __device__ __forceinline__ void init(const AttnArgs& p, const kv::Share& s, const Sequence& seq) {
+  __device__ __forceinline__ void init(const AttnArgs& p, const kv::Share& s) {
     k0 = s.head * p.c.ks.head;
     v0 = s.head * p.c.vs.head;
     ks0 = s.head * p.c.kss.head;
     vs0 = s.head * p.c.vss.head;
     table = p.c.table ? p.c.table + s.b * p.c.table_stride : nullptr;
-    len = seq.len;
     b = s.b;
-    poison = seq.bad;
   }
-  // First key of this lane's group of tile j: groups behind the last key are read as its group.
+  // First key of this lane's group of tile j: groups behind the last key are read as the tile's first.
   __device__ __forceinline__ uint32_t key_of(int j, int lane) const {
-    return min(j * BKV + (lane & (kGroups - 1)) * kGroup, (len - 1) & ~(kGroup - 1));
+    const int key = j * BKV + (lane & (kGroups - 1)) * kGroup;
+    return key < len ? key : j * BKV;
   }
   // Address of the entry of the table: without one of something that can be read.
   __device__ __forceinline__ const int32_t* entry(const AttnArgs& p, int j, int lane) const {
     return table ? table + p.c.page.divide(key_of(j, lane)) : p.c.lengths + b;
+  }
+  // The entry of a tile whose place in the sequence is not known yet, and what places() takes in its place once
+  // it is: a group behind the last key has the first group's.
+  __device__ __forceinline__ uint32_t early_entry(const AttnArgs& p, int j, int lane) const {
+    const int key = min(j * BKV + (lane & (kGroups - 1)) * kGroup, p.c.capacity - 1);
+    return table && key >= 0 ? static_cast<uint32_t>(table[p.c.page.divide(key)]) : 0;
+  }
+  __device__ __forceinline__ uint32_t settled(int j, int lane, uint32_t id) const {
+    const uint32_t of_first = __builtin_amdgcn_mov_dpp(static_cast<int>(id), 0x00, 0xF, 0xF, true);  // lane 0 of each four
+    return j * BKV + (lane & (kGroups - 1)) * kGroup < len ? id : of_first;
   }
   __device__ __forceinline__ Places places(const AttnArgs& p, int j, int lane, uint32_t id) {
     const uint32_t key = key_of(j, lane);
@@ -491,27 +505,34 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
   t.v = t.k + N::kTile;
   t.meta = meta + wave * N::kScaleBytes;
   t.init(p);
-  const Sequence seq(p, s.b);
+  // what does not wait for the sequence's length is asked for with it
   Rows rows;
-  rows.init(p, s, seq);
+  rows.init(p, s);
+  u32x4 q[D / 16];
+  const int query = load_query<D, true>(p, s, s.row0 + t.col, t.h, q);
+  uint32_t id = 0;
+  if (p.splits == 1) id = rows.early_entry(p, wave, t.lane);
+  const Sequence seq(p, s.b);
+  rows.len = seq.len;
+  rows.poison = seq.bad;
   Softmax<D> st;
   st.init();
 
   const int total = (limit_of_rows(p, seq, s.row0, N::kRows) + BKV - 1) / BKV;
-  const int per = (total + p.splits - 1) / p.splits;
+  const int per = p.per(total);
   const int begin = min(total, s.split * per), end = min(total, begin + per);
   Places at{}, next_at{};
   int j = begin + wave;
   if (j < end) {
-    at = rows.places(p, j, t.lane, static_cast<uint32_t>(*rows.entry(p, j, t.lane)));
+    id = p.splits == 1 ? rows.settled(j, t.lane, id) : static_cast<uint32_t>(*rows.entry(p, j, t.lane));
+    at = rows.places(p, j, t.lane, id);
     t.load_word(p.c.k_scale + at.ks, 1);
     t.load_word(p.c.v_scale + at.vs, 2);
     t.load_word(rows.entry(p, min(j + kWaves, total - 1), t.lane), 0);
     t.template load<false>(p, at.k);
     t.template load<true>(p, at.v);
   }
-  u32x4 q[D / 16];
-  load_query<D, E, true>(p, s, seq, s.row0 + t.col, t.h, q, st.limit, st.factor);
+  take_query<D, E>(p, seq, query, q, st.limit, st.factor);
   int least = st.limit;  // keys that all rows attend
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) least = min(least, __shfl_xor(least, d, 64));
@@ -522,7 +543,7 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
     // all but V_j have landed
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");
     const float ks = __uint_as_float(t.word(1)), vs = __uint_as_float(t.word(2));
-    const uint32_t id = t.word(0);
+    id = t.word(0);
     f32x16 sc[2];
     t.scores(q, sc);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -790,12 +811,15 @@ __device__ __forceinline__ void wide_body(const AttnArgs& p) {
   w.col = w.lane & 31;
   w.h = w.lane >> 5;
   w.init_tiles(p);
+  w.rows.init(p, s);
+  const int wave_row = s.row0 + w.wave * 32;
+  const int query = load_query<D, false>(p, s, wave_row + w.col, w.h, w.qreg[0]);
   const Sequence seq(p, s.b);
-  w.rows.init(p, s, seq);
+  w.rows.len = seq.len;
+  w.rows.poison = seq.bad;
   Softmax<D>& st = w.st;
   st.init();
-  const int wave_row = s.row0 + w.wave * 32;
-  load_query<D, E, false>(p, s, seq, wave_row + w.col, w.h, w.qreg[0], st.limit, st.factor);
+  take_query<D, E>(p, seq, query, w.qreg[0], st.limit, st.factor);
   int least = st.limit;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) least = min(least, __shfl_xor(least, d, 64));
@@ -803,7 +827,7 @@ __device__ __forceinline__ void wide_body(const AttnArgs& p) {
   const int most = wave_row < p.rows ? limit_of_rows(p, seq, wave_row, 32) : 0;
 
   const int total = (limit_of_rows(p, seq, s.row0, W::kRows) + BKV - 1) / BKV;
-  const int per = (total + p.splits - 1) / p.splits;
+  const int per = p.per(total);
   const int begin = min(total, s.split * per), end = min(total, begin + per);
   w.found = 0;
   // tiles that all rows of the workgroup attend
@@ -914,31 +938,32 @@ __device__ __forceinline__ void join_body(const AttnArgs& p) {
   int64_t o_at, lse_at;
   if (!out_row(p, s, row, written, o_at, lse_at)) return;  // all lanes of the row
   const int64_t first = static_cast<int64_t>(s.b) * p.splits * p.c.kv_heads + s.head;  // unit of split 0
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int k = at.group; k < p.splits; k += at.groups) {
-    m = fmaxf(m, p.part_ml[((first + static_cast<int64_t>(k) * p.c.kv_heads) * p.rows + row) * 2]);
-  }
-  m = at.reduce(m, [](float a, float b) { return fmaxf(a, b); });
-  float l_run = 0.f, o[8] = {};
+  // each group of lanes its splits, against the largest so far, then the groups
+  float m = -INFINITY, l_run = 0.f, o[8] = {};
 #pragma unroll 4
   for (int k = at.group; k < p.splits; k += at.groups) {
     const int64_t part = (first + static_cast<int64_t>(k) * p.c.kv_heads) * p.rows + row;
     const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + part * 2);
     const f32x4 lo = *reinterpret_cast<const f32x4*>(p.part_o + part * D + at.ch * 8);
     const f32x4 hi = *reinterpret_cast<const f32x4*>(p.part_o + part * D + at.ch * 8 + 4);
-    const float f = ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m);
-    l_run += f * ml.y;
+    const float top = fmaxf(m, ml.x);
+    const float before = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+    const float f = ml.x == top ? 1.0f : __builtin_amdgcn_exp2f(ml.x - top);
+    m = top;
+    l_run = l_run * before + f * ml.y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      o[e] = fmaf(f, lo[e], o[e]);
-      o[4 + e] = fmaf(f, hi[e], o[4 + e]);
+      o[e] = fmaf(f, lo[e], o[e] * before);
+      o[4 + e] = fmaf(f, hi[e], o[4 + e] * before);
     }
   }
   const auto sum = [](float a, float b) { return a + b; };
-  l_run = at.reduce(l_run, sum);
+  const float top = at.reduce(m, [](float a, float b) { return fmaxf(a, b); });
+  const float f = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+  m = top;
+  l_run = at.reduce(l_run * f, sum);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] = at.reduce(o[e], sum);
+  for (int e = 0; e < 8; ++e) o[e] = at.reduce(o[e] * f, sum);
   if (at.group != 0) return;
   write_row<E>(p, s, row, at.ch, o, m, l_run, written);
 }

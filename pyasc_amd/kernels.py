@@ -1015,33 +1015,21 @@ def _strided(t: torch.Tensor, name: str, device: int, dims: int, written: bool) 
     return t.data_ptr(), t.stride(), shape
 
 
-def _codes(t: torch.Tensor, name: str, dtype: torch.dtype, device: int, shape: Optional[tuple], written: bool) -> tuple:
-    """The codes of a cache, [pages, heads, rows, head_dim], as asc_rows_t's fields, and their shape."""
-    at, (s0, s1, s2, s3), size = _strided(t, name, device, 4, written)
-    if t.dtype is not dtype:
-        raise TypeError(f"'{name}' must be {dtype}, got {t.dtype}")
-    if shape is not None and size != shape:
-        raise ValueError(f"'{name}' must be {list(shape)}, got {tuple(size)}")
-    if s3 != 1 and size[3] > 1:
-        raise ValueError(f"the last dimension of '{name}' must be contiguous")
-    if (at | s0 | s1 | s2) & 15:
-        s0, s1, s2 = (s if n > 1 else 0 for s, n in zip((s0, s1, s2), size))
-        if (at | s0 | s1 | s2) & 15:
-            raise ValueError(f"'{name}' must be 16-byte aligned, with strides that are multiples of 16 "
-                             f"(address {at:#x}, strides {t.stride()})")
-    return (at, s0, s1, s2), size
-
-
 def _scales(t: torch.Tensor, name: str, device: int, pages: int, heads: int, rows: int, written: bool) -> tuple:
     """The scales of a cache, [pages, heads, blocks], as asc_rows_t's fields, and the rows of a block."""
-    at, strides, size = _strided(t, name, device, 3, written)
+    if not isinstance(t, torch.Tensor) or t.get_device() != device:
+        _here(t, name, device)
     if t.dtype is not torch.float32:
         raise TypeError(f"'{name}' must be torch.float32, got {t.dtype}")
-    blocks = size[2]
-    if size[0] != pages or size[1] != heads or blocks == 0 and rows or blocks and rows % (16 * blocks):
-        raise ValueError(f"'{name}' must be [{pages}, {heads}, blocks] for blocks of a multiple of 16 rows that divide "
-                         f"the {rows} of a page, got {tuple(size)}")
-    return (at, *strides), rows // blocks if rows else 16
+    size = t.shape
+    blocks = size[2] if len(size) == 3 else -1
+    if blocks <= 0 or rows % (16 * blocks) or size[0] != pages or size[1] != heads:
+        if blocks != 0 or rows or size[0] != pages or size[1] != heads:
+            raise ValueError(f"'{name}' must be [{pages}, {heads}, blocks] for blocks of a multiple of 16 rows that "
+                             f"divide the {rows} of a page, got {tuple(size)}")
+    if written and not t.is_contiguous():
+        _apart(t, name)
+    return t.data_ptr(), *t.stride(), (rows // blocks if rows else 16)
 
 
 def _table(t: torch.Tensor, name: str, device: int, batch: int) -> tuple:
@@ -1061,26 +1049,47 @@ def _cache8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor
     if not isinstance(k_cache, torch.Tensor):
         raise TypeError(f"'k_cache' must be a torch.Tensor, got {type(k_cache).__name__}")
     dtype = k_cache.dtype
-    if dtype not in _CACHE_CODES:
+    code = _CACHE_CODES.get(dtype)
+    if code is None:
         raise TypeError(f"'k_cache' has unsupported dtype {dtype}; expected one of {sorted(map(str, _CACHE_CODES))}")
-    k_rows, shape = _codes(k_cache, "k_cache", dtype, device, None, written)
-    v_rows, _ = _codes(v_cache, "v_cache", dtype, device, shape, written)
+    shape = k_cache.shape
+    if len(shape) != 4:
+        raise ValueError(f"'k_cache' must be [pages, kv_heads, rows, head_dim], got {tuple(shape)}")
     pages, heads, rows, head_dim = shape
     if head_dim not in FA_HEAD_DIMS:
         raise ValueError(f"head_dim {head_dim} not supported (supported: {FA_HEAD_DIMS})")
-    ks_rows, block = _scales(k_scales, "k_scales", device, pages, heads, rows, written)
-    vs_rows, v_block = _scales(v_scales, "v_scales", device, pages, heads, rows, written)
+    fields = ()
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if not isinstance(t, torch.Tensor) or t.get_device() != device:
+            _here(t, name, device)
+        if t.dtype is not dtype:
+            raise TypeError(f"'{name}' must be {dtype}, got {t.dtype}")
+        if t.shape != shape:
+            raise ValueError(f"'{name}' must be {list(shape)}, got {tuple(t.shape)}")
+        if written and not t.is_contiguous():
+            _apart(t, name)
+        at, (s0, s1, s2, s3) = t.data_ptr(), t.stride()
+        if s3 != 1:
+            raise ValueError(f"the last dimension of '{name}' must be contiguous")
+        if (at | s0 | s1 | s2) & 15:
+            s0, s1, s2 = (s if n > 1 else 0 for s, n in zip((s0, s1, s2), shape))
+            if (at | s0 | s1 | s2) & 15:
+                raise ValueError(f"'{name}' must be 16-byte aligned, with strides that are multiples of 16 "
+                                 f"(address {at:#x}, strides {t.stride()})")
+        fields += (at, s0, s1, s2)
+    *ks_rows, block = _scales(k_scales, "k_scales", device, pages, heads, rows, written)
+    *vs_rows, v_block = _scales(v_scales, "v_scales", device, pages, heads, rows, written)
     if block != v_block:
         raise ValueError(f"'k_scales' and 'v_scales' have blocks of {block} and {v_block} rows")
+    fields += (*ks_rows, *vs_rows)
     if block_table is None:
         if pages != batch:
             raise ValueError(f"a cache without a block_table must have {batch} sequences, got {pages}")
-        return (*k_rows, *v_rows, *ks_rows, *vs_rows), (_CACHE_CODES[dtype], head_dim, 0, block, heads, rows, pages), (0, 0)
+        return fields, (code, head_dim, 0, block, heads, rows, pages), (0, 0)
     table, stride, width = _table(block_table, "block_table", device, batch)
     if rows == 0:
         raise ValueError("pages without rows")
-    return ((*k_rows, *v_rows, *ks_rows, *vs_rows), (_CACHE_CODES[dtype], head_dim, rows, block, heads, width * rows, pages),
-            (table, stride))
+    return fields, (code, head_dim, rows, block, heads, width * rows, pages), (table, stride)
 
 
 def quantized_cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,

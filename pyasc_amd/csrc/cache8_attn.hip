@@ -48,9 +48,6 @@ Way way_of(int64_t heads, int64_t row_blocks, int64_t tiles, int64_t slots, int 
   if (shares < slots) w.splits = fill * slots / shares;
   if (w.splits > tiles / least) w.splits = tiles / least;
   if (w.splits > kMaxSplits) w.splits = kMaxSplits;
-#ifdef SPL
-  w.splits = SPL;
-#endif
   if (w.splits < 1) w.splits = 1;
   const int64_t chain = asc::ceil_div(asc::ceil_div(tiles, w.splits), waves);
   w.us = static_cast<double>(asc::ceil_div(shares * w.splits, slots)) * (start + tile * static_cast<double>(chain)) +

@@ -173,59 +173,91 @@ __device__ __forceinline__ void take_query(const AttnArgs& p, const Sequence& se
   }
 }
 
-// The places of a tile's groups: lane l works out that of group l % 4.
-struct Places {
-  uint32_t k, v;    // of the group's first row, units of 16 bytes
-  uint32_t ks, vs;  // of its block's scales
-};
+// What a wave knows of its tiles' groups: sixteen of its tiles at a time, whose 64 groups its lanes work out together, lane 4 t + g
+// group g of tile first + t * step.  The next sixteen's entries of the table and scales are asked for on the way
+// (kEntries, kScales), as their use waits for all loads before it.
+constexpr int kBatch = 64 / kGroups, kEntries = 4, kScales = 8;
 
-struct Rows {
+struct Groups {
   uint32_t k0, v0, ks0, vs0;  // the sequence's head
   const int32_t* table;       // null: one piece
-  int len, b;
-  bool poison;
+  int len, b, lane, step;
+  int first;                  // of the current tiles
+  bool poison;                // a page or a length outside the cache: the rows' results are NaN
+  uint32_t k, v;              // places of the groups' first rows, units of 16 bytes
+  float ks, vs;               // scales, 0 behind the last key
+  uint32_t next_id, next_k, next_v;
+  float next_ks, next_vs;
 
-  __device__ __forceinline__ void init(const AttnArgs& p, const kv::Share& s) {
+  __device__ __forceinline__ void init(const AttnArgs& p, const kv::Share& s, int lane_, int step_) {
     k0 = s.head * p.c.ks.head;
     v0 = s.head * p.c.vs.head;
     ks0 = s.head * p.c.kss.head;
     vs0 = s.head * p.c.vss.head;
     table = p.c.table ? p.c.table + s.b * p.c.table_stride : nullptr;
     b = s.b;
+    lane = lane_;
+    step = step_;
   }
-  // First key of this lane's group of tile j: groups behind the last key are read as the tile's first.
-  __device__ __forceinline__ uint32_t key_of(int j, int lane) const {
-    const int key = j * BKV + (lane & (kGroups - 1)) * kGroup;
-    return key < len ? key : j * BKV;
+  __device__ __forceinline__ int key_of(int from) const {
+    return (from + (lane / kGroups) * step) * BKV + (lane % kGroups) * kGroup;
   }
-  // Address of the entry of the table: without one of something that can be read.
-  __device__ __forceinline__ const int32_t* entry(const AttnArgs& p, int j, int lane) const {
-    return table ? table + p.c.page.divide(key_of(j, lane)) : p.c.lengths + b;
+  // The entries of the table for the tiles from `from` on; a length that is not known yet is taken for the capacity.
+  __device__ __forceinline__ uint32_t entries(const AttnArgs& p, int from, int end) const {
+    const int key = key_of(from);
+    return table && key < end ? static_cast<uint32_t>(table[p.c.page.divide(key)]) : 0;
   }
-  // The entry of a tile whose place in the sequence is not known yet, and what places() takes in its place once
-  // it is: a group behind the last key has the first group's.
-  __device__ __forceinline__ uint32_t early_entry(const AttnArgs& p, int j, int lane) const {
-    const int key = min(j * BKV + (lane & (kGroups - 1)) * kGroup, p.c.capacity - 1);
-    return table && key >= 0 ? static_cast<uint32_t>(table[p.c.page.divide(key)]) : 0;
-  }
-  __device__ __forceinline__ uint32_t settled(int j, int lane, uint32_t id) const {
-    const uint32_t of_first = __builtin_amdgcn_mov_dpp(static_cast<int>(id), 0x00, 0xF, 0xF, true);  // lane 0 of each four
-    return j * BKV + (lane & (kGroups - 1)) * kGroup < len ? id : of_first;
-  }
-  __device__ __forceinline__ Places places(const AttnArgs& p, int j, int lane, uint32_t id) {
-    const uint32_t key = key_of(j, lane);
+  // Groups behind the last key are read as their tile's first, and those of tiles behind it not at all.
+  __device__ __forceinline__ void places(const AttnArgs& p, int from, uint32_t id, uint32_t& at_k, uint32_t& at_v, float& s_k,
+                                         float& s_v) {
+    const int key = key_of(from);
+    const bool there = key < len;
     const uint32_t row = key - p.c.page.divide(key) * p.c.page.d;
     if (!table) id = b;
-    const bool bad = id >= p.c.pages;
+    const bool bad = there && id >= p.c.pages;
     poison = poison || __builtin_amdgcn_ballot_w64(bad) != 0;
     if (bad) id = 0;
-    const uint32_t block = p.c.block.divide(row);
-    Places r;
-    r.k = k0 + id * p.c.ks.page + row * p.c.ks.row;
-    r.v = v0 + id * p.c.vs.page + row * p.c.vs.row;
-    r.ks = ks0 + id * p.c.kss.page + block * p.c.kss.row;
-    r.vs = vs0 + id * p.c.vss.page + block * p.c.vss.row;
-    return r;
+    s_k = s_v = 0.f;
+    at_k = at_v = 0;
+    if (there) {
+      const uint32_t block = p.c.block.divide(row);
+      at_k = k0 + id * p.c.ks.page + row * p.c.ks.row;
+      at_v = v0 + id * p.c.vs.page + row * p.c.vs.row;
+      s_k = p.c.k_scale[ks0 + id * p.c.kss.page + block * p.c.kss.row];
+      s_v = p.c.v_scale[vs0 + id * p.c.vss.page + block * p.c.vss.row];
+    }
+    // lane 0 of each four: its tile's first
+    const uint32_t tile_k = __builtin_amdgcn_mov_dpp(static_cast<int>(at_k), 0x00, 0xF, 0xF, true);
+    const uint32_t tile_v = __builtin_amdgcn_mov_dpp(static_cast<int>(at_v), 0x00, 0xF, 0xF, true);
+    at_k = there ? at_k : tile_k;
+    at_v = there ? at_v : tile_v;
+  }
+  __device__ __forceinline__ void start(const AttnArgs& p, int from, uint32_t id) {
+    first = from;
+    places(p, from, id, k, v, ks, vs);
+  }
+  // Before tile number t of the current ones (end: keys of the tiles that are worked on).
+  __device__ __forceinline__ void ask(const AttnArgs& p, int t, int end) {
+    const int from = first + kBatch * step;
+    if (t == kEntries && from * BKV < end) next_id = entries(p, from, len);
+    if (t == kScales && from * BKV < end) places(p, from, next_id, next_k, next_v, next_ks, next_vs);
+  }
+  // To the next tiles, where number n is the first of them.
+  __device__ __forceinline__ void advance(int& n) {
+    const bool on = n == kBatch;
+    first += on ? kBatch * step : 0;
+    k = on ? next_k : k;
+    v = on ? next_v : v;
+    ks = on ? next_ks : ks;
+    vs = on ? next_vs : vs;
+    n = on ? 0 : n;
+  }
+  // Place of group g of tile number t, of these tiles or the next.
+  template <bool kIsV>
+  __device__ __forceinline__ uint32_t place(int t, int g) const {
+    const uint32_t now = __builtin_amdgcn_readlane(kIsV ? v : k, (t * kGroups + g) & 63);
+    const uint32_t next = __builtin_amdgcn_readlane(kIsV ? next_v : next_k, (t * kGroups + g) & 63);
+    return t < kBatch ? now : next;
   }
 };
 
@@ -237,11 +269,12 @@ struct Softmax {
   f32x16 acc[kDBlocks];  // in units of R
   float m, l;            // reference point (log2) and this lane half's sum
   float factor;          // of the raw scores of a unit scale (log2)
-  float R;               // largest V scale so far
+  float R;               // largest V scale, so far or of all
   int limit;             // keys of the row
-  float a[kGroups];      // factors of the tile's groups
+  float log_ratio, inverse;  // of this lane's group: log2 of V scale / R, and R / V scale
+  float a[kGroups];      // of the tile's groups: the factors of their scores,
   float shift[kGroups];  // log2 of V scale / R
-  float undo[kGroups];   // R / V scale
+  float undo[kGroups];   // and R / V scale
 
   __device__ __forceinline__ void init() {
 #pragma unroll
@@ -250,25 +283,33 @@ struct Softmax {
     l = 0.f;
     R = 0.f;
   }
-  // The tile's scales, of group l % 4 in lane l.  A V scale below 2^-40 R counts as that: its values times p stay
+  // The V scales of the current tiles, one per lane, in units of R.  One below 2^-40 R counts as that: its values times p stay
   // below fp16's smallest.
-  __device__ __forceinline__ void set_scales(float ks, float vs) {
-    float top = fmaxf(vs, dpp_mov<kDppQuadXor1>(vs));
-    top = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, fmaxf(top, dpp_mov<kDppQuadXor2>(top)))));
-    if (top > R) {
-      const float down = R / top;
-#pragma unroll
-      for (int i = 0; i < kDBlocks; ++i) acc[i] *= down;
-      R = top;
-    }
+  __device__ __forceinline__ void take_ratios(float vs) {
     const float ratio = fmaxf(vs / R, 0x1p-40f);
-    const float log_ratio = __builtin_amdgcn_logf(ratio), inverse = 1.0f / ratio;
+    log_ratio = __builtin_amdgcn_logf(ratio);
+    inverse = 1.0f / ratio;
+  }
+  // Those, where R is the largest so far.
+  __device__ __forceinline__ void take_scales(float vs) {
+    const float top = fmaxf(R, __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, wave_max(vs)))));
+    const float down = top > R ? R / top : 1.0f;
+#pragma unroll
+    for (int i = 0; i < kDBlocks; ++i) acc[i] *= down;
+    R = top;
+    take_ratios(vs);
+  }
+  // Those of tile number t, and its K scales.
+  __device__ __forceinline__ void set_tile(float ks, int t) {
+    const auto lane = [&](float v, int g) {
+      return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), t * kGroups + g));
+    };
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       // not zero, which times the -inf of a hidden key would be NaN
-      a[g] = fmaxf(factor * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), g)), 0x1p-126f);
-      shift[g] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, log_ratio), g));
-      undo[g] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, inverse), g));
+      a[g] = fmaxf(factor * lane(ks, g), 0x1p-126f);
+      shift[g] = lane(log_ratio, g);
+      undo[g] = lane(inverse, g);
     }
   }
   __device__ __forceinline__ void hide(f32x16 (&s)[2], int j, int h) const {
@@ -279,18 +320,18 @@ struct Softmax {
         if (j * BKV + kb * 32 + (r >> 2) * 8 + h * 4 + (r & 3) >= limit) s[kb][r] = -INFINITY;
       }
   }
-  // Largest score of the tile, less fp16's lift.
-  __device__ __forceinline__ float tile_max(const f32x16 (&s)[2]) const {
-    float top = -INFINITY;
+  // Largest score of half kb of a tile, or of all of it, less fp16's lift.
+  __device__ __forceinline__ float half_max(const f32x16& s, int kb) const {
+    float low = -INFINITY, high = -INFINITY;
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      float t = -INFINITY;
-#pragma unroll
-      for (int r = 0; r < 8; ++r) t = fmaxf(t, s[g >> 1][(g & 1) * 8 + r]);
-      top = fmaxf(top, t * a[g]);
+    for (int r = 0; r < 8; ++r) {
+      low = fmaxf(low, s[r]);
+      high = fmaxf(high, s[8 + r]);
     }
+    const float top = fmaxf(low * a[kb * 2], high * a[kb * 2 + 1]);
     return fmaxf(top, other_half(top)) - F16::kLift;
   }
+  __device__ __forceinline__ float tile_max(const f32x16 (&s)[2]) const { return fmaxf(half_max(s[0], 0), half_max(s[1], 1)); }
   __device__ __forceinline__ void raise(float top) {
     const bool up = top > m;
     const float alpha = up ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
@@ -300,39 +341,47 @@ struct Softmax {
     for (int i = 0; i < kDBlocks; ++i) acc[i] *= alpha;
   }
   __device__ __forceinline__ float reference() const { return m == -INFINITY ? 0.f : -m; }
-  // Values 2 w and 2 w + 1 of group g, and their sum.
-  __device__ __forceinline__ void pair(const f32x16 (&s)[2], int g, int w, float ref, u32x4 (&pb)[2][2], float& sum) const {
-    const int kb = g >> 1, u = g & 1;
-    const float e0 = __builtin_amdgcn_exp2f(fmaf(s[kb][8 * u + 2 * w], a[g], ref + shift[g]));
-    const float e1 = __builtin_amdgcn_exp2f(fmaf(s[kb][8 * u + 2 * w + 1], a[g], ref + shift[g]));
+  // Values 2 w and 2 w + 1 of group u of half kb, and their sum.
+  __device__ __forceinline__ void pair(const f32x16& s, int kb, int u, int w, float ref, u32x4 (&pb)[2], float& sum) const {
+    const int g = kb * 2 + u;
+    const float e0 = __builtin_amdgcn_exp2f(fmaf(s[8 * u + 2 * w], a[g], ref + shift[g]));
+    const float e1 = __builtin_amdgcn_exp2f(fmaf(s[8 * u + 2 * w + 1], a[g], ref + shift[g]));
     sum += e0;
     sum += e1;
-    pb[kb][u][w] = F16::pack(e0, e1);
+    pb[u][w] = F16::pack(e0, e1);
   }
-  // P^T operands of the tile; returns this lane's sum of probabilities.
-  __device__ __forceinline__ float probs(const f32x16 (&s)[2], u32x4 (&pb)[2][2]) const {
+  // P^T operands of half kb; returns this lane's sum of probabilities.
+  __device__ __forceinline__ float probs(const f32x16& s, int kb, u32x4 (&pb)[2]) const {
     const float ref = reference();
     float rs = 0.f;
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
+    for (int u = 0; u < 2; ++u) {
       float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) pair(s, g, w, ref, pb, sum);
-      rs = fmaf(sum, undo[g], rs);
+      for (int w = 0; w < 4; ++w) pair(s, kb, u, w, ref, pb, sum);
+      rs = fmaf(sum, undo[kb * 2 + u], rs);
     }
     return rs;
   }
   __device__ __forceinline__ bool out_of_range(float sum) const {
     return __builtin_amdgcn_ballot_w64(sum > F16::kTileSumLimit || m == -INFINITY) != 0;
   }
-  __device__ __forceinline__ void guard(const f32x16 (&s)[2], u32x4 (&pb)[2][2], float& rs) {
+  // Of a half, or a whole tile.
+  __device__ __forceinline__ void guard(const f32x16& s, int kb, u32x4 (&pb)[2], float rs) {
     if (out_of_range(rs)) {
-      raise(tile_max(s));
-      rs = probs(s, pb);
+      raise(half_max(s, kb));
+      rs = probs(s, kb, pb);
     }
     l += rs;
   }
-
+  __device__ __forceinline__ void tile_probs(const f32x16 (&s)[2], u32x4 (&pb)[2][2]) {
+    float rs = probs(s[0], 0, pb[0]) + probs(s[1], 1, pb[1]);
+    if (out_of_range(rs)) {
+      raise(tile_max(s));
+      rs = probs(s[0], 0, pb[0]) + probs(s[1], 1, pb[1]);
+    }
+    l += rs;
+  }
   // A NaN among the values of keys that only some rows attend is taken as zero in the products, whose 0 times NaN
   // would reach all rows (without_nan).  Where that was met, the rows that attend it get it back: tile j, from memory.
   __device__ __forceinline__ void add_nan(const AttnArgs& p, const kv::Share& s, int j, int h) {
@@ -372,7 +421,6 @@ struct Narrow {
   static constexpr int kTile = BKV * D;           // bytes
   static constexpr int kLoads = kTile / 1024;     // of a wave
   static constexpr int kRowsPerLoad = 1024 / D;
-  static constexpr int kScaleBytes = 3 * 256;     // table entries, K's and V's scales of each lane
 };
 
 // One wave's tiles: codes in LDS as they are, in 16-byte chunks whose place in a row is flipped by the row so that 16
@@ -383,7 +431,6 @@ struct NarrowTiles {
   static constexpr int kChunks = D / 16;
   uint8_t* k;
   uint8_t* v;
-  uint8_t* meta;
   int lane, col, h;
   uint32_t kaddr, vaddr;
   uint32_t koff[2], voff[2];
@@ -404,28 +451,19 @@ struct NarrowTiles {
       voff[odd] = in_group * p.c.vs.row * 16 + ((pos ^ vflip(in_group)) << 4);
     }
   }
+  // Tile number t of the current ones or the next.
   template <bool kIsV>
-  __device__ __forceinline__ void load(const AttnArgs& p, uint32_t places) const {
+  __device__ __forceinline__ void load(const AttnArgs& p, const Groups& groups, int t) const {
     const uint64_t base = reinterpret_cast<uint64_t>(kIsV ? p.c.v : p.c.k);
     uint8_t* dst = kIsV ? v : k;
 #pragma unroll
     for (int i = 0; i < N::kLoads; ++i) {
-      const uint32_t place = __builtin_amdgcn_readlane(places, D == 128 ? i >> 1 : i);
+      const uint32_t place = groups.template place<kIsV>(t, D == 128 ? i >> 1 : i);
       const uint8_t* src = reinterpret_cast<const uint8_t*>(base + static_cast<uint64_t>(place) * 16);
       const uint32_t off = kIsV ? voff[i & 1] : koff[i & 1];
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + off),
                                        (__attribute__((address_space(3))) void*)(dst + i * 1024), 16, 0, 0);
     }
-  }
-  // A word per lane into the wave's slot `slot`.
-  __device__ __forceinline__ void load_word(const void* src, int slot) const {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                     (__attribute__((address_space(3))) void*)(meta + slot * 256), 4, 0, 0);
-  }
-  __device__ __forceinline__ uint32_t word(int slot) const {
-    uint32_t r;
-    asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(r) : "v"(lds_addr(meta) + slot * 256 + lane * 4) : "memory");
-    return r;
   }
   // Raw scores of the tile.
   __device__ __forceinline__ void scores(const u32x4 (&q)[D / 16], f32x16 (&s)[2]) const {
@@ -490,7 +528,6 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
   constexpr bool kHasNan = __is_same(Q, E4m3);
   static_assert(N::kRows * kRow <= 2 * BKV * D, "a wave's part reuses its tiles");
   __shared__ __attribute__((aligned(256))) uint8_t lds[kWaves * 2 * N::kTile];
-  __shared__ __attribute__((aligned(256))) uint8_t meta[kWaves * N::kScaleBytes];
   __shared__ float stats[2][kWaves][N::kRows];
 
   kv::Share s = share_of(p);
@@ -503,34 +540,29 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
   t.h = t.lane >> 5;
   t.k = lds + wave * 2 * N::kTile;
   t.v = t.k + N::kTile;
-  t.meta = meta + wave * N::kScaleBytes;
   t.init(p);
   // what does not wait for the sequence's length is asked for with it
-  Rows rows;
-  rows.init(p, s);
+  Groups groups;
+  groups.init(p, s, t.lane, kWaves);
   u32x4 q[D / 16];
   const int query = load_query<D, true>(p, s, s.row0 + t.col, t.h, q);
   uint32_t id = 0;
-  if (p.splits == 1) id = rows.early_entry(p, wave, t.lane);
+  if (p.splits == 1) id = groups.entries(p, wave, p.c.capacity);
   const Sequence seq(p, s.b);
-  rows.len = seq.len;
-  rows.poison = seq.bad;
+  groups.len = seq.len;
+  groups.poison = seq.bad;
   Softmax<D> st;
   st.init();
 
   const int total = (limit_of_rows(p, seq, s.row0, N::kRows) + BKV - 1) / BKV;
   const int per = p.per(total);
   const int begin = min(total, s.split * per), end = min(total, begin + per);
-  Places at{}, next_at{};
   int j = begin + wave;
   if (j < end) {
-    id = p.splits == 1 ? rows.settled(j, t.lane, id) : static_cast<uint32_t>(*rows.entry(p, j, t.lane));
-    at = rows.places(p, j, t.lane, id);
-    t.load_word(p.c.k_scale + at.ks, 1);
-    t.load_word(p.c.v_scale + at.vs, 2);
-    t.load_word(rows.entry(p, min(j + kWaves, total - 1), t.lane), 0);
-    t.template load<false>(p, at.k);
-    t.template load<true>(p, at.v);
+    if (p.splits > 1) id = groups.entries(p, j, groups.len);
+    groups.start(p, j, id);
+    t.template load<false>(p, groups, 0);
+    t.template load<true>(p, groups, 0);
   }
   take_query<D, E>(p, seq, query, q, st.limit, st.factor);
   int least = st.limit;  // keys that all rows attend
@@ -538,31 +570,26 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
   for (int d = 1; d < 32; d *= 2) least = min(least, __shfl_xor(least, d, 64));
   least = __builtin_amdgcn_readfirstlane(least);
   uint32_t found = 0;
-  for (; j < end; j += kWaves) {
+  for (int n = 0; j < end; j += kWaves, ++n) {  // tile number n of the current ones
     const bool next = j + kWaves < end;
+    if (n == 0 || n == kBatch) {
+      groups.advance(n);
+      st.take_scales(groups.vs);
+    }
     // all but V_j have landed
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");
-    const float ks = __uint_as_float(t.word(1)), vs = __uint_as_float(t.word(2));
-    id = t.word(0);
     f32x16 sc[2];
     t.scores(q, sc);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (next) {
-      next_at = rows.places(p, j + kWaves, t.lane, id);
-      t.load_word(p.c.k_scale + next_at.ks, 1);
-      t.load_word(p.c.v_scale + next_at.vs, 2);
-      t.load_word(rows.entry(p, min(j + 2 * kWaves, total - 1), t.lane), 0);
-      t.template load<false>(p, next_at.k);
-    }
-    st.set_scales(ks, vs);
+    if (next) t.template load<false>(p, groups, n + 1);
+    st.set_tile(groups.ks, n);
     const bool masked = (j + 1) * BKV > least;
     if (masked) st.hide(sc, j, t.h);
     if (j == begin + wave) st.m = st.tile_max(sc);  // nothing to rescale yet
     u32x4 pb[2][2];
-    float rs = st.probs(sc, pb);
-    st.guard(sc, pb, rs);
+    st.tile_probs(sc, pb);
     if (next) {
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L + 3) : "memory");  // all but the next tile's K, scales and entry
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");  // all but the next tile's K
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
@@ -572,7 +599,8 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
       t.template pv<false>(st, pb, found);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (next) t.template load<true>(p, next_at.v);
+    groups.ask(p, n, end * BKV);
+    if (next) t.template load<true>(p, groups, n + 1);
   }
   if (kHasNan && __builtin_amdgcn_ballot_w64(found != 0) != 0) {
     for (int i = begin + wave; i < end; i += kWaves) {
@@ -584,7 +612,7 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
   const auto part_off = [](int row, int c) { return row * kRow + ((c ^ (row & 15)) << 4); };
   {
     float l = st.l + other_half(st.l);
-    if (rows.poison) l = __builtin_nanf("");
+    if (groups.poison) l = __builtin_nanf("");
     if (t.h == 0) {
       stats[0][wave][t.col] = st.m;
       stats[1][wave][t.col] = l;
@@ -654,7 +682,7 @@ struct WideState : fa::FaState<D, Wide<D>::kWaves, 1, F16, true> {
   using Base = fa::FaState<D, Wide<D>::kWaves, 1, F16, true>;
   static constexpr int T = Wide<D>::kTile;
   Softmax<D> st;
-  Rows rows;
+  Groups groups;
   uint32_t koff, voff;        // of this lane's piece in its group of rows
   uint32_t kdst, vdst;        // of its first chunk of fp16 in a tile; the second's differs by one bit
   int group;                  // of this wave's rows
@@ -673,8 +701,7 @@ struct WideState : fa::FaState<D, Wide<D>::kWaves, 1, F16, true> {
     const int g_lane = lane & 15;
     this->vaddr[0] = fa::v_off<D>(this->h * 4 + (g_lane >> 2), ((lane >> 4) & 1) * 16 + (g_lane & 3) * 4);
   }
-  __device__ __forceinline__ u32x4 load(const uint8_t* codes, uint32_t places, uint32_t off) const {
-    const uint32_t place = __builtin_amdgcn_readlane(places, group);
+  __device__ __forceinline__ u32x4 load(const uint8_t* codes, uint32_t place, uint32_t off) const {
     return *reinterpret_cast<const u32x4*>(codes + static_cast<uint64_t>(place) * 16 + off);
   }
   template <bool kClean>
@@ -686,111 +713,165 @@ struct WideState : fa::FaState<D, Wide<D>::kWaves, 1, F16, true> {
     *reinterpret_cast<u32x4*>(tile + dst) = operand_of<Q>(x[0], x[1]);
     *reinterpret_cast<u32x4*>(tile + (dst ^ 16)) = operand_of<Q>(x[2], x[3]);
   }
-  // P^T of this tile between the products of the next one's scores, as FaState::scores_probs.
-  __device__ __forceinline__ float scores_probs(const uint8_t* k, f32x16 (&sn)[2], const f32x16 (&sc)[2], u32x4 (&pb)[2][2]) const {
-    const uint32_t base = lds_addr(k);
-    constexpr int kWin = 4, kReads = 2 * Base::kKSteps, kPer = 16 / kReads;
+  // V^T operand r of half kb of a tile: block r / 2 of the columns, its keys 16 (r % 2) .. + 15.
+  __device__ __forceinline__ u32x4 v_operand(uint32_t base, int kb, int r) const {
+    return this->vt_read(base, (r >> 1) * 4 + kb * 2 + (r & 1));
+  }
+  __device__ __forceinline__ u32x4 k_operand(uint32_t base, int kb, int r) const {
+    return fa::lds_read_b128(this->k_addr(base, r), kb * 32 * (D * 2));
+  }
+  static constexpr int kOps = Base::kKSteps;  // of K, and as many of V, for a half of a tile
+  static_assert(kOps == 2 * Base::kDBlocks, "operands of a half");
+
+  // The probabilities of half kb (s[kb], into pb_out) between the products that wait for nothing of it: the raw scores of
+  // the half behind it (into s[1 - kb], of `k`'s rows) and, kPv, the values times the probabilities of the half before it
+  // (pb_in, of `v`'s rows).  Returns the probabilities' sum.
+  template <int kb, bool kPv>
+  __device__ __forceinline__ float half(const uint8_t* k, const uint8_t* v, f32x16 (&s)[2], const u32x4 (&pb_in)[2],
+                                        u32x4 (&pb_out)[2]) {
+    constexpr int kWin = 3, kPer = 8 / kOps, kEach = kPv ? 3 : 1;  // LDS reads in a round
+    const uint32_t kbase = lds_addr(k), vbase = lds_addr(v);
     const float ref = st.reference();
     float rs = 0.f, sum = 0.f;
-    u32x4 x[kReads];
+    u32x4 x[kOps], y[kOps];
 #pragma unroll
-    for (int r = 0; r < kWin; ++r) x[r] = fa::lds_read_b128(this->k_addr(base, r % Base::kKSteps), (r / Base::kKSteps) * 32 * (D * 2));
-    sn[0] = f32x16{};
-    sn[1] = f32x16{};
+    for (int r = 0; r < kWin; ++r) {
+      x[r] = k_operand(kbase, 1 - kb, r);
+      if constexpr (kPv) y[r] = v_operand(vbase, 1 - kb, r);
+    }
+    f32x16 next = {};
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int r = 0; r < kReads; ++r) {
-      fa::lds_wait(x[r], r + kWin <= kReads ? kWin - 1 : kReads - 1 - r);
-      sn[r / Base::kKSteps] = F16::mfma(x[r], this->qreg[0][r % Base::kKSteps], sn[r / Base::kKSteps]);
+    for (int r = 0; r < kOps; ++r) {
+      const int behind = kEach * (r + kWin <= kOps ? kWin - 1 : kOps - 1 - r);
+      fa::lds_wait(x[r], behind + kEach - 1);
+      next = F16::mfma(x[r], this->qreg[0][r], next);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int it = r * kPer + i;
-        st.pair(sc, it / 4, it % 4, ref, pb, sum);
+        st.pair(s[kb], kb, it / 4, it % 4, ref, pb_out, sum);
         if (it % 4 == 3) {
-          rs = fmaf(sum, st.undo[it / 4], rs);
+          rs = fmaf(sum, st.undo[kb * 2 + it / 4], rs);
           sum = 0.f;
         }
       }
-      if (r + kWin < kReads) {
-        x[r + kWin] = fa::lds_read_b128(this->k_addr(base, (r + kWin) % Base::kKSteps), ((r + kWin) / Base::kKSteps) * 32 * (D * 2));
+      if constexpr (kPv) {
+        fa::lds_wait(y[r], behind);
+        st.acc[r >> 1] = F16::mfma(y[r], pb_in[r & 1], st.acc[r >> 1]);
+      }
+      if (r + kWin < kOps) {
+        x[r + kWin] = k_operand(kbase, 1 - kb, r + kWin);
+        if constexpr (kPv) y[r + kWin] = v_operand(vbase, 1 - kb, r + kWin);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    s[1 - kb] = next;
     return rs;
   }
-  __device__ __forceinline__ void pv(const uint8_t* v, const u32x4 (&pb)[2][2]) {
-    const uint32_t base = lds_addr(v);
-    constexpr int kWin = 4, kOps = 4 * Base::kDBlocks;
+  // The scores of half kb of a tile alone, and its values times the probabilities.
+  __device__ __forceinline__ void scores(const uint8_t* k, int kb, f32x16& s) const {
+    constexpr int kWin = 4;
+    const uint32_t base = lds_addr(k);
     u32x4 x[kOps];
 #pragma unroll
-    for (int r = 0; r < kWin; ++r) x[r] = this->vt_read(base, r);
+    for (int r = 0; r < kWin; ++r) x[r] = k_operand(base, kb, r);
+    s = f32x16{};
 #pragma unroll
     for (int r = 0; r < kOps; ++r) {
-      fa::lds_wait(x[r], 2 * (r + kWin <= kOps ? kWin - 1 : kOps - 1 - r));
-      st.acc[r / 4] = F16::mfma(x[r], pb[(r % 4) >> 1][r & 1], st.acc[r / 4]);
-      if (r + kWin < kOps) x[r + kWin] = this->vt_read(base, r + kWin);
+      fa::lds_wait(x[r], r + kWin <= kOps ? kWin - 1 : kOps - 1 - r);
+      s = F16::mfma(x[r], this->qreg[0][r], s);
+      if (r + kWin < kOps) x[r + kWin] = k_operand(base, kb, r + kWin);
+    }
+  }
+  __device__ __forceinline__ void pv(const uint8_t* v, int kb, const u32x4 (&pb)[2]) {
+    constexpr int kWin = 4;
+    const uint32_t base = lds_addr(v);
+    u32x4 y[kOps];
+#pragma unroll
+    for (int r = 0; r < kWin; ++r) y[r] = v_operand(base, kb, r);
+#pragma unroll
+    for (int r = 0; r < kOps; ++r) {
+      fa::lds_wait(y[r], 2 * (r + kWin <= kOps ? kWin - 1 : kOps - 1 - r));
+      st.acc[r >> 1] = F16::mfma(y[r], pb[r & 1], st.acc[r >> 1]);
+      if (r + kWin < kOps) y[r + kWin] = v_operand(base, kb, r + kWin);
     }
   }
 };
 
-// What is under way of the next tiles: codes of K (three tiles ahead at the step's end) and V (two), the scales from the
-// current tile on, the entry of the table of the tile after.
+// The way of the tiles through a wave.  LDS has three stages for each of K and V, tile t in stage t % 3.  In step j: the codes of
+// K_{j+2} and V_{j+1}, asked for in the step before, go into stages that no wave reads any more, and those of K_{j+3}
+// and V_{j+2} are asked for; then, half a tile (32 keys) at a time, the probabilities, between the products of the
+// scores of the half behind and of the values of the half before.
 struct WideAhead {
   u32x4 k, v;
-  uint32_t v_place, id;
-  float ks[3], vs[3];
+  int n;             // number of tile j among the groups' current ones
+  int c;             // j % 3
+  u32x4 pb[2][2];    // probabilities of each half
 };
 
-// Tile j: LDS holds K_{j+1} and V_j, sc the raw scores of tile j, `a` the codes of K_{j+2} and V_{j+1}.
-// kTail false: tile j + 1 exists, and all of the workgroup's rows attend all of it.
-template <bool kTail, int D, class E, class Q>
-__device__ __forceinline__ void wide_step(WideState<D, E, Q>& w, const AttnArgs& p, int j, int end, uint8_t* ring, int most,
-                                          int least, WideAhead& a, f32x16 (&sc1)[1][2], f32x16 (&sn1)[1][2]) {
-  f32x16(&sc)[2] = sc1[0];
-  f32x16(&sn)[2] = sn1[0];
-  constexpr bool kClean = kTail && __is_same(Q, E4m3);
+// kTail false: tile j + 1 exists, and all of the workgroup's rows attend all of tile j; whole: tiles of which they do.  The second
+// half's probabilities are left for the next step, whose kFirst is false, or for the caller.
+template <bool kTail, bool kFirst, int D, class E, class Q>
+__device__ __forceinline__ void wide_step(WideState<D, E, Q>& w, const AttnArgs& p, int j, int end, int whole, uint8_t* ring, int most,
+                                          int least, WideAhead& a, f32x16 (&s)[2]) {
   constexpr int T = WideState<D, E, Q>::T;
   Softmax<D>& st = w.st;
-  uint8_t* k_next = ring + ((j + 1) & 1) * T;
-  uint8_t* v_here = ring + (2 + (j & 1)) * T;
-  // codes that have arrived, into the stages that the last step read
-  if (j + 2 < end) w.template store<false>(ring + (j & 1) * T, w.kdst, a.k);
-  if (j + 1 < end) w.template store<kClean>(ring + (2 + ((j + 1) & 1)) * T, w.vdst, a.v);
-  const float ks = a.ks[0], vs = a.vs[0];
-  a.ks[0] = a.ks[1];
-  a.vs[0] = a.vs[1];
-  a.ks[1] = a.ks[2];
-  a.vs[1] = a.vs[2];
-  if (j + 2 < end) a.v = w.load(p.c.v, a.v_place, w.voff);
-  if (j + 3 < end) {
-    const Places at = w.rows.places(p, j + 3, w.lane, a.id);
-    a.k = w.load(p.c.k, at.k, w.koff);
-    a.v_place = at.v;
-    a.ks[2] = p.c.k_scale[at.ks];
-    a.vs[2] = p.c.v_scale[at.vs];
-    a.id = static_cast<uint32_t>(*w.rows.entry(p, min(j + 4, end - 1), w.lane));
+  const int c1 = a.c == 2 ? 0 : a.c + 1, c2 = a.c == 0 ? 2 : a.c - 1;  // of j + 1, and of j + 2 and j - 1
+  uint8_t *k_here = ring + a.c * T, *k_next = ring + c1 * T, *v_here = ring + (3 + a.c) * T, *v_before = ring + (3 + c2) * T;
+  if (a.n == kBatch) {
+    w.groups.advance(a.n);
+    st.take_ratios(w.groups.vs);
   }
-  const bool act = !kTail || j * BKV < most;
-  if (act) {
-    st.set_scales(ks, vs);
-    u32x4 pb[2][2];
-    float rs;
-    if constexpr (kTail) {
-      if ((j + 1) * BKV > least) st.hide(sc, j, w.h);
-      rs = st.probs(sc, pb);
+  if (j + 2 < end) w.template store<false>(ring + c2 * T, w.kdst, a.k);
+  if (j + 1 < end) {
+    if (__is_same(Q, E4m3) && j + 1 >= whole) {
+      w.template store<true>(ring + (3 + c1) * T, w.vdst, a.v);
     } else {
-      rs = w.scores_probs(k_next, sn, sc, pb);
-    }
-    st.guard(sc, pb, rs);
-    w.pv(v_here, pb);
-    if constexpr (kTail) {
-      if ((j + 1) * BKV < most && j + 1 < end) {
-        w.scores(k_next, sc1);
-      }
+      w.template store<false>(ring + (3 + c1) * T, w.vdst, a.v);
     }
   }
+  w.groups.ask(p, a.n, end * BKV);
+  if (j + 2 < end) a.v = w.load(p.c.v, w.groups.template place<true>(a.n + 2, w.group), w.voff);
+  if (j + 3 < end) a.k = w.load(p.c.k, w.groups.template place<false>(a.n + 3, w.group), w.koff);
+  if constexpr (kTail) {
+    if (j * BKV < most) {
+      st.set_tile(w.groups.ks, a.n);
+      w.scores(k_here, 1, s[1]);
+      if ((j + 1) * BKV > least) st.hide(s, j, w.h);
+      st.guard(s[0], 0, a.pb[0], st.probs(s[0], 0, a.pb[0]));
+      w.pv(v_here, 0, a.pb[0]);
+      st.guard(s[1], 1, a.pb[1], st.probs(s[1], 1, a.pb[1]));
+      w.pv(v_here, 1, a.pb[1]);
+      if ((j + 1) * BKV < most && j + 1 < end) w.scores(k_next, 0, s[0]);
+    }
+  } else {
+    st.set_tile(w.groups.ks, a.n);
+    st.guard(s[0], 0, a.pb[0], w.template half<0, !kFirst>(k_here, v_before, s, a.pb[1], a.pb[0]));
+    st.guard(s[1], 1, a.pb[1], w.template half<1, true>(k_next, v_here, s, a.pb[0], a.pb[1]));
+  }
+  ++a.n;
+  a.c = c1;
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   asm volatile("s_barrier" ::: "memory");
+}
+
+// Largest V scale of keys begin .. end - 1, by the workgroup: to move R as the tiles come would take registers that the tiles'
+// steps do not have.  NaN, and what is not positive, counts as 0.
+template <int kWaves>
+__device__ __forceinline__ float largest_scale(const AttnArgs& p, const kv::Share& s, int begin, int end, int threads,
+                                               float (&waves)[kWaves]) {
+  float top = 0.f;
+  for (int key = begin + static_cast<int>(threadIdx.x) * kGroup; key < end; key += threads * kGroup) {
+    uint32_t page, row;
+    if (!place(p.c, s.b, key, page, row)) continue;
+    top = fmaxf(top, p.c.v_scale[scale_at(p.c, p.c.vss, page, s.head, row)]);
+  }
+  top = wave_max(top);
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) top = fmaxf(top, waves[i]);
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, top)));
 }
 
 template <int D, class E, class Q>
@@ -798,7 +879,8 @@ __device__ __forceinline__ void wide_body(const AttnArgs& p) {
   using W = Wide<D>;
   constexpr int kWaves = W::kWaves, T = W::kTile, kThreads = kWaves * 64, kChunks = D / 8;
   constexpr bool kHasNan = __is_same(Q, E4m3);
-  __shared__ __attribute__((aligned(256))) uint8_t ring[4 * T];
+  __shared__ __attribute__((aligned(256))) uint8_t ring[6 * T];
+  __shared__ float scales[kWaves];
 
   kv::Share s = share_of(p);
   if (!s.live) return;
@@ -811,12 +893,12 @@ __device__ __forceinline__ void wide_body(const AttnArgs& p) {
   w.col = w.lane & 31;
   w.h = w.lane >> 5;
   w.init_tiles(p);
-  w.rows.init(p, s);
+  w.groups.init(p, s, w.lane, 1);
   const int wave_row = s.row0 + w.wave * 32;
   const int query = load_query<D, false>(p, s, wave_row + w.col, w.h, w.qreg[0]);
   const Sequence seq(p, s.b);
-  w.rows.len = seq.len;
-  w.rows.poison = seq.bad;
+  w.groups.len = seq.len;
+  w.groups.poison = seq.bad;
   Softmax<D>& st = w.st;
   st.init();
   take_query<D, E>(p, seq, query, w.qreg[0], st.limit, st.factor);
@@ -833,47 +915,41 @@ __device__ __forceinline__ void wide_body(const AttnArgs& p) {
   // tiles that all rows of the workgroup attend
   const int whole = min(end, least_of_rows(p, seq, s.row0, W::kRows) / BKV);
   if (begin < end) {
-    WideAhead a{};
-    Places at[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      const int j = min(begin + i, end - 1);
-      at[i] = w.rows.places(p, j, w.lane, static_cast<uint32_t>(*w.rows.entry(p, j, w.lane)));
-      a.ks[i] = p.c.k_scale[at[i].ks];
-      a.vs[i] = p.c.v_scale[at[i].vs];
-    }
-    const u32x4 k0 = w.load(p.c.k, at[0].k, w.koff), v0 = w.load(p.c.v, at[0].v, w.voff);
-    const u32x4 k1 = w.load(p.c.k, at[1].k, w.koff);
-    a.k = w.load(p.c.k, at[2].k, w.koff);
-    a.v = w.load(p.c.v, at[1].v, w.voff);
-    a.v_place = at[2].v;
-    a.id = static_cast<uint32_t>(*w.rows.entry(p, min(begin + 3, end - 1), w.lane));
-    // tile j in stage j % 2
-    w.template store<false>(ring + (begin & 1) * T, w.kdst, k0);
-    w.template store<false>(ring + ((begin + 1) & 1) * T, w.kdst, k1);
+    WideAhead a;
+    w.groups.start(p, begin, w.groups.entries(p, begin, seq.len));
+    const auto load_k = [&](int i) { return w.load(p.c.k, w.groups.template place<false>(i, w.group), w.koff); };
+    const auto load_v = [&](int i) { return w.load(p.c.v, w.groups.template place<true>(i, w.group), w.voff); };
+    const int t1 = min(1, end - 1 - begin), t2 = min(2, end - 1 - begin);
+    const u32x4 k0 = load_k(0), v0 = load_v(0), k1 = load_k(t1);
+    a.k = load_k(t2);
+    a.v = load_v(t1);
+    st.R = largest_scale(p, s, begin * BKV, min(end * BKV, seq.len), kThreads, scales);
+    st.take_ratios(w.groups.vs);
+    a.n = a.c = 0;  // tile begin in stage 0
+    w.template store<false>(ring, w.kdst, k0);
+    w.template store<false>(ring + T, w.kdst, k1);
     if (kHasNan && whole <= begin) {
-      w.template store<true>(ring + (2 + (begin & 1)) * T, w.vdst, v0);
+      w.template store<true>(ring + 3 * T, w.vdst, v0);
     } else {
-      w.template store<false>(ring + (2 + (begin & 1)) * T, w.vdst, v0);
+      w.template store<false>(ring + 3 * T, w.vdst, v0);
     }
     __syncthreads();
-    f32x16 sa[1][2], sb[1][2];
-    w.scores(ring + (begin & 1) * T, sa);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    asm volatile("s_barrier" ::: "memory");
+    f32x16 s2[2];
+    w.scores(ring, 0, s2[0]);
     int j = begin;
-    for (; j + 2 < whole; j += 2) {
-      wide_step<false>(w, p, j, end, ring, most, least, a, sa, sb);
-      wide_step<false>(w, p, j + 1, end, ring, most, least, a, sb, sa);
+    if (j < whole && j + 1 < end) {
+      wide_step<false, true>(w, p, j, end, whole, ring, most, least, a, s2);
+      for (++j; j < whole && j + 1 < end; ++j) wide_step<false, false>(w, p, j, end, whole, ring, most, least, a, s2);
+      w.pv(ring + (3 + (a.c == 0 ? 2 : a.c - 1)) * T, 1, a.pb[1]);
     }
-    for (; j < end; ++j) wide_step<true>(w, p, j, end, ring, most, least, a, sa, sa);
+    for (; j < end; ++j) wide_step<true, false>(w, p, j, end, whole, ring, most, least, a, s2);
   }
   if (kHasNan && __syncthreads_or(w.found != 0) != 0) {
-    for (int j = max(begin, whole - 2); j < end; ++j) st.add_nan(p, s, j, w.h);  // from the first tile cleaned on
+    for (int j = max(begin, whole); j < end; ++j) st.add_nan(p, s, j, w.h);
   }
 
   float l_run = st.l + other_half(st.l);
-  if (w.rows.poison) l_run = __builtin_nanf("");
+  if (w.groups.poison) l_run = __builtin_nanf("");
   const int written = written_of(p, s.b);
   if (p.splits > 1) {
     // the unnormalised part, from registers: lane (row, half h) holds d = 32 db + 8 rq + 4 h + 0..3

@@ -34,36 +34,68 @@ struct Launch {
 };
 
 constexpr int kMaxSplits = 64;
-constexpr int64_t kCus = 256;
+constexpr int kCus = 256;
 
 struct Way {
   int64_t row_blocks, splits;
   double us;
 };
 
-Way way_of(int64_t heads, int64_t row_blocks, int64_t tiles, int64_t slots, int fill, int64_t least, int waves, double start,
-           double tile) {
-  Way w{row_blocks, 1, 0.0};
-  const int64_t shares = heads * row_blocks;
-  if (shares < slots) w.splits = fill * slots / shares;
-  if (w.splits > tiles / least) w.splits = tiles / least;
-  if (w.splits > kMaxSplits) w.splits = kMaxSplits;
-  if (w.splits < 1) w.splits = 1;
-  const int64_t chain = asc::ceil_div(asc::ceil_div(tiles, w.splits), waves);
-  w.us = static_cast<double>(asc::ceil_div(shares * w.splits, slots)) * (start + tile * static_cast<double>(chain)) +
-         (w.splits > 1 ? 3.5 : 0.0);
-  return w;
+// What a kernel takes, in us: `start`, and then the longest of its workgroups' chains of tiles (`chain` for each round of
+// `waves` tiles), of what the busiest CU works on (`tile` for each), and of the average CU's work and a part (`last`) of
+// a workgroup's chain where sequences of several lengths end one by one.  A split's parts cost `join` and their bytes.
+// Fitted to 240 shapes of 4 to 2048 rows, 8 heads, 1 to 40 sequences and 512 to 32768 keys, with 1 to 64 splits in either
+// kernel: off by 6 to 19% (root mean square).  The choice from it is 2% slower than the best of each shape on average
+// where the caches were read just before, 4% where they come from memory; as many splits as fill the card's slots
+// twice: 8% and 13%.  8 sequences of 15000 to 32768 keys get their best (16 splits: 72 us, 4: 80, 64: 95).
+struct Cost {
+  int rows, slots, waves;  // slots: workgroups that the card holds
+  double start, chain, tile, last;
+};
+constexpr double kJoinUs = 4.5, kPartBytesPerUs = 3e6;
+template <int D>
+constexpr Cost kNarrowCost{Narrow<D>::kRows, kCus * Narrow<D>::kWgPerCu, Narrow<D>::kWaves, D == 128 ? 7.4 : 6.2,
+                           D == 128 ? 1.85 : 1.28, D == 128 ? 0.48 : 0.28, 0.3};
+template <int D>
+constexpr Cost kWideCost{Wide<D>::kRows, kCus * Wide<D>::kWgPerCu, 1, D == 128 ? 9.2 : 7.2, D == 128 ? 1.75 : 1.03,
+                         D == 128 ? 2.0 : 0.77, 0.0};
+
+// The fastest split: more than another only where they save 3%.
+Way way_of(const Cost& c, int64_t batch, int64_t heads, int64_t rows, int64_t tiles, int head_dim) {
+  Way best{asc::ceil_div(rows, c.rows), 1, INFINITY};
+  heads *= batch;
+  const int64_t shares = heads * best.row_blocks;
+  const double last = batch > 1 ? c.last : 0.0;
+  const auto consider = [&](int64_t splits) {
+    const int64_t all = shares * splits, per = asc::ceil_div(tiles, splits);
+    const double chain = c.chain * static_cast<double>(asc::ceil_div(per, c.waves)), work = c.tile * static_cast<double>(per);
+    const double average = work * static_cast<double>(all) / kCus;
+    const double busiest = all < kCus ? average : work * static_cast<double>(asc::ceil_div(all, kCus));
+    const double chains = chain * static_cast<double>(asc::ceil_div(all, c.slots));
+    double us = c.start + std::fmax(std::fmax(chains, busiest), average + last * chain);
+    if (splits > 1) us += kJoinUs + static_cast<double>(heads * rows * splits * head_dim * 8) / kPartBytesPerUs;
+    if (us < 0.97 * best.us) best = {best.row_blocks, splits, us};
+  };
+  consider(1);
+  if (shares >= 8 * kCus) return best;
+  const int64_t most = tiles / 2 < kMaxSplits ? tiles / 2 : kMaxSplits;
+  for (int64_t splits = 2, step = 1; splits <= most; splits += step) {  // 2, 3, 4, 6, 8, 12, ...
+    if ((splits & (splits - 1)) == 0) step = splits / 2;
+    consider(splits);
+  }
+  for (int64_t fill = kCus; fill <= 2 * kCus; fill += kCus) {  // as many as the CUs hold at a time
+    if (fill / shares > 1 && fill / shares <= most) consider(fill / shares);
+  }
+  return best;
 }
 
 void plan(Launch& L, const asc_cache8_t& a) {
   AttnArgs& p = L.p;
   const bool small = a.head_dim == 64;
   const int64_t heads = a.batch * a.kv_heads, tiles = asc::ceil_div(p.c.capacity, asc::fa::BKV);
-  const Way narrow = way_of(heads, asc::ceil_div(p.rows, 32), tiles, kCus * (small ? Narrow<64>::kWgPerCu : Narrow<128>::kWgPerCu), 2,
-                            8, 4, small ? 4.5 : 5.5, small ? 1.2 : 2.0);
-  const Way wide = way_of(heads, asc::ceil_div(p.rows, small ? Wide<64>::kRows : Wide<128>::kRows), tiles,
-                          kCus * (small ? Wide<64>::kWgPerCu : Wide<128>::kWgPerCu), 1, 4, 1, small ? 8.0 : 9.0, small ? 1.6 : 2.2);
-  L.wide = p.rows > 32 && narrow.us > 0.9 * wide.us;
+  const Way narrow = way_of(small ? kNarrowCost<64> : kNarrowCost<128>, a.batch, a.kv_heads, p.rows, tiles, a.head_dim);
+  const Way wide = way_of(small ? kWideCost<64> : kWideCost<128>, a.batch, a.kv_heads, p.rows, tiles, a.head_dim);
+  L.wide = p.rows > Narrow<128>::kRows && wide.us < 0.95 * narrow.us;
   const Way& w = L.wide ? wide : narrow;
   p.row_blocks = static_cast<int>(w.row_blocks);
   p.splits = static_cast<int>(w.splits);

@@ -1335,8 +1335,8 @@ def cache_compact(caches: Any, block_table: torch.Tensor, lengths: torch.Tensor,
                   page_size: int, table_out: torch.Tensor, refcounts_out: torch.Tensor, page_map: torch.Tensor,
                   stream: Any = None) -> None:
     """Brings the pages in use (refcounts > 0), U of them, to the front of a paged cache: the i-th of those at U and
-    above moves into the i-th free one below.  Tensors, tables and counts as cache_fork's; table_out may be
-    block_table, refcounts_out refcounts.  page_map (int32 [pages]) receives each page's new place, -1 for free
+    above moves into the i-th free one below.  Tensors (whose pages move whole, whatever their rows), tables and counts as
+    cache_fork's; table_out may be block_table, refcounts_out refcounts.  page_map (int32 [pages]) receives each page's new place, -1 for free
     ones: holders outside the table have it to go by."""
     device = _current_device()
     tensors, number, pages, _ = _page_tensors(caches, caches, device)

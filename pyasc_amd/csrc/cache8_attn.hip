@@ -102,12 +102,15 @@ void plan(Launch& L, const asc_cache8_t& a) {
   p.by_n = asc::divisor_of(static_cast<uint32_t>(p.c.n));
   p.by_heads = asc::divisor_of(static_cast<uint32_t>(p.c.kv_heads));
   p.by_splits = asc::divisor_of(static_cast<uint32_t>(p.splits));
-  p.by_row_blocks = asc::divisor_of(static_cast<uint32_t>(p.row_blocks));
+  p.lanes = p.causal && p.row_blocks >= 2 * p.group ? p.group : 1;
+  p.per_lane = asc::ceil_div(p.row_blocks, p.lanes);
+  p.by_lanes = asc::divisor_of(static_cast<uint32_t>(p.lanes));
+  p.by_slots = asc::divisor_of(static_cast<uint32_t>(p.lanes * p.per_lane));
   p.units = static_cast<uint32_t>(heads * p.splits);
   L.rows_all = heads * p.rows;
   p.join_groups = small ? asc::kv::JoinLanes<64>::groups_of(L.rows_all, p.splits)
                         : asc::kv::JoinLanes<128>::groups_of(L.rows_all, p.splits);
-  L.blocks = asc::ceil_div(p.units, 8) * 8 * p.row_blocks;
+  L.blocks = asc::ceil_div(p.units, 8) * 8 * p.lanes * p.per_lane;
 }
 
 // Bytes of the parts: their values and statistics.

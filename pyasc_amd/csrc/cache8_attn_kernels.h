@@ -39,8 +39,9 @@ struct AttnArgs {
   float* part_o;   // [unit][rows][D], unnormalised
   float* part_ml;  // [unit][rows][2]: reference point (log2), sum
   int32_t batch, group, rows, row_blocks, splits, join_groups, causal;
+  int32_t lanes, per_lane;  // of the order of the row blocks
   uint32_t units;  // batch * splits * kv_heads
-  Divisor by_n, by_heads, by_splits, by_row_blocks;
+  Divisor by_n, by_heads, by_splits, by_slots, by_lanes;
   float scale_log2;
 
   // Tiles of a split of `total` tiles: the last splits may have none.
@@ -70,14 +71,16 @@ __device__ __forceinline__ u32x4 operand_of(uint32_t lo, uint32_t hi) {
   return u32x4{a[0], a[1], b[0], b[1]};
 }
 
-// One workgroup's share, as kv::Share.
+// One workgroup's share, as kv::Share.  Causal: the row blocks with most keys first, which are the last ones of each of the
+// group's heads (`lanes` runs of per_lane blocks).
 __device__ __forceinline__ kv::Share share_of(const AttnArgs& p) {
   const uint32_t slot = blockIdx.x >> 3;
-  const uint32_t per = p.by_row_blocks.divide(slot);
+  const uint32_t per = p.by_slots.divide(slot), place = slot - per * p.by_slots.d;
+  const uint32_t back = p.by_lanes.divide(place), run = place - back * p.lanes;
   kv::Share s;
   s.unit = per * 8 + (blockIdx.x & 7);
-  s.live = s.unit < p.units;
-  s.row0 = p.row_blocks - 1 - static_cast<int>(slot - per * p.row_blocks);  // causal: the longest first
+  s.row0 = static_cast<int>(run + 1) * p.per_lane - 1 - static_cast<int>(back);
+  s.live = s.unit < p.units && s.row0 < p.row_blocks;
   const uint32_t range = p.by_heads.divide(s.unit);
   s.head = static_cast<int>(s.unit - range * p.c.kv_heads);
   s.b = static_cast<int>(p.by_splits.divide(range));
@@ -688,6 +691,10 @@ struct WideState : fa::FaState<D, Wide<D>::kWaves, 1, F16, true> {
   int group;                  // of this wave's rows
   uint32_t found;             // NaN among the values that this lane has loaded, of tiles that not all rows attend
 
+  // Neighbouring chunks change places in every other row of 256 bytes, as sixteen lanes write every other chunk of those.
+  static __device__ __forceinline__ uint32_t v_place(int row, int col) {
+    return fa::v_off<D>(row, col) ^ static_cast<uint32_t>((row >> (D == 128 ? 0 : 1) & 1) << 4);
+  }
   __device__ __forceinline__ void init_tiles(const AttnArgs& p) {
     constexpr int kPieces = D / 16;
     const int lane = this->lane, row = this->wave * (64 / kPieces) + lane / kPieces, piece = lane % kPieces;
@@ -695,11 +702,11 @@ struct WideState : fa::FaState<D, Wide<D>::kWaves, 1, F16, true> {
     koff = (row % kGroup) * p.c.ks.row * 16 + piece * 16;
     voff = (row % kGroup) * p.c.vs.row * 16 + piece * 16;
     kdst = fa::k_off<D>(row, piece * 2);
-    vdst = fa::v_off<D>(row, piece * 16);
+    vdst = v_place(row, piece * 16);
     group = __builtin_amdgcn_readfirstlane(group);
     this->kaddr[0] = fa::k_off<D>(this->col, this->h);
     const int g_lane = lane & 15;
-    this->vaddr[0] = fa::v_off<D>(this->h * 4 + (g_lane >> 2), ((lane >> 4) & 1) * 16 + (g_lane & 3) * 4);
+    this->vaddr[0] = v_place(this->h * 4 + (g_lane >> 2), ((lane >> 4) & 1) * 16 + (g_lane & 3) * 4);
   }
   __device__ __forceinline__ u32x4 load(const uint8_t* codes, uint32_t place, uint32_t off) const {
     return *reinterpret_cast<const u32x4*>(codes + static_cast<uint64_t>(place) * 16 + off);

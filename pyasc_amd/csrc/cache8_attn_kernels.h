@@ -10,8 +10,10 @@
 // vs_j / R again for the denominator.  Queries of bf16 are brought to fp16's range by a power of two of
 // their row: exact, but for elements 2^-39 and less of the row's largest.
 //
-// The probabilities are rounded to fp16 for the product with the values, as matrix operands have to be:
-// errors of 0.0002 of the results' norm, beside 0.0017 of a bf16 result's own rounding.
+// The probabilities are rounded to fp16 for the product with the values, as matrix operands have to be: errors of up to 0.0002
+// of the results' norm, beside 0.0017 of a bf16 result's own rounding.  Beside 0.0002 of an fp16 result's they count where a few
+// keys outweigh the rest (0.0003 in all, one row over 500 keys): the kernel for few rows, whose matrix units wait for the cache,
+// multiplies what the rounding leaves as a second term (0.0002; 8 sequences of up to 32768 keys take 74.6 us for 72.3).
 #pragma once
 
 #include "cache8.h"
@@ -377,11 +379,37 @@ struct Softmax {
     }
     l += rs;
   }
-  __device__ __forceinline__ void tile_probs(const f32x16 (&s)[2], u32x4 (&pb)[2][2]) {
-    float rs = probs(s[0], 0, pb[0]) + probs(s[1], 1, pb[1]);
+  // kRest: and what their rounding leaves, rounded.
+  template <bool kRest>
+  __device__ __forceinline__ float both_probs(const f32x16 (&s)[2], u32x4 (&pb)[2][2], u32x4 (&rest)[2][2]) const {
+    if constexpr (!kRest) return probs(s[0], 0, pb[0]) + probs(s[1], 1, pb[1]);
+    const float ref = reference();
+    float rs = 0.f;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int r = 8 * (g & 1) + 2 * w;
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][r], a[g], ref + shift[g]));
+        const float e1 = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][r + 1], a[g], ref + shift[g]));
+        sum += e0;
+        sum += e1;
+        const uint32_t x = F16::pack(e0, e1);
+        const fa::f16x2 rounded = __builtin_bit_cast(fa::f16x2, x);
+        pb[g >> 1][g & 1][w] = x;
+        rest[g >> 1][g & 1][w] = F16::pack(e0 - static_cast<float>(rounded[0]), e1 - static_cast<float>(rounded[1]));
+      }
+      rs = fmaf(sum, undo[g], rs);
+    }
+    return rs;
+  }
+  template <bool kRest>
+  __device__ __forceinline__ void tile_probs(const f32x16 (&s)[2], u32x4 (&pb)[2][2], u32x4 (&rest)[2][2]) {
+    float rs = both_probs<kRest>(s, pb, rest);
     if (out_of_range(rs)) {
       raise(tile_max(s));
-      rs = probs(s[0], 0, pb[0]) + probs(s[1], 1, pb[1]);
+      rs = both_probs<kRest>(s, pb, rest);
     }
     l += rs;
   }
@@ -416,6 +444,10 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t w, uint32_t& found) {
 }
 
 // ------------------------------------------------------------------------------------ few rows
+//
+// Bound by the cache's bytes: 64 sequences of 1024 to 4096 keys (8 heads of 128 columns, int8) are 335 MB in 66 us, 5.1 TB/s with the
+// start and the last sequences' end, 6.0 between (a plain copy: 6.1); one token of each costs nothing beside them.  A wave
+// works on tiles of its own, without barriers, with the next tile's K and V on their way to LDS in the meantime.
 
 template <int D>
 struct Narrow {
@@ -495,8 +527,8 @@ struct NarrowTiles {
   }
   static __device__ __forceinline__ void wait(u32x2& r, int n) { asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(r) : "i"(n)); }
   // Operand r: block r / 4 of the columns, keys 16 (r % 4) .. + 15.
-  template <bool kMasked>
-  __device__ __forceinline__ void pv(Softmax<D>& st, const u32x4 (&pb)[2][2], uint32_t& found) const {
+  template <bool kMasked, bool kRest>
+  __device__ __forceinline__ void pv(Softmax<D>& st, const u32x4 (&pb)[2][2], const u32x4 (&rest)[2][2], uint32_t& found) const {
     constexpr int kOps = 4 * (D / 32), kWin = 8;
     u32x2 x[kOps];
 #pragma unroll
@@ -508,6 +540,7 @@ struct NarrowTiles {
       const u32x4 a = operand_of<Q>(x[r][0], x[r][1]);
       if (r + kWin < kOps) x[r + kWin] = read_tr(vaddr ^ (((r + kWin) >> 2) << 5), (r & 3) * 16 * D);
       st.acc[r >> 2] = F16::mfma(a, pb[(r & 3) >> 1][r & 1], st.acc[r >> 2]);
+      if constexpr (kRest) st.acc[r >> 2] = F16::mfma(a, rest[(r & 3) >> 1][r & 1], st.acc[r >> 2]);
     }
   }
 };
@@ -529,6 +562,7 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
   using N = Narrow<D>;
   constexpr int kWaves = N::kWaves, L = N::kLoads, kRow = D * 4;
   constexpr bool kHasNan = __is_same(Q, E4m3);
+  constexpr bool kRest = __is_same(E, F16);
   static_assert(N::kRows * kRow <= 2 * BKV * D, "a wave's part reuses its tiles");
   __shared__ __attribute__((aligned(256))) uint8_t lds[kWaves * 2 * N::kTile];
   __shared__ float stats[2][kWaves][N::kRows];
@@ -589,17 +623,17 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
     const bool masked = (j + 1) * BKV > least;
     if (masked) st.hide(sc, j, t.h);
     if (j == begin + wave) st.m = st.tile_max(sc);  // nothing to rescale yet
-    u32x4 pb[2][2];
-    st.tile_probs(sc, pb);
+    u32x4 pb[2][2], rest[2][2];
+    st.template tile_probs<kRest>(sc, pb, rest);
     if (next) {
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");  // all but the next tile's K
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
     if (kHasNan && masked) {
-      t.template pv<true>(st, pb, found);
+      t.template pv<true, kRest>(st, pb, rest, found);
     } else {
-      t.template pv<false>(st, pb, found);
+      t.template pv<false, kRest>(st, pb, rest, found);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     groups.ask(p, n, end * BKV);
@@ -670,6 +704,12 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
 }
 
 // ------------------------------------------------------------------------------------ many rows
+//
+// Bound by matrix units, VALU and LDS about equally: 2 sequences of 8192 keys and 2048 new rows (32 query heads on 8, 128
+// columns: 481 GF) in 478 us, 1.0 PF (a large product of matrices: 1.21).  Each of the three is busy for 40 to 50% of the time:
+// the K and V fragments of a wave's 32 rows are read from LDS for those rows only, and codes become fp16 once per workgroup.
+// Half a tile's probabilities are computed between the products of the halves around it (620 us without that), and what a
+// tile's groups need is worked out for sixteen tiles at a time.
 
 template <int D>
 struct Wide {
@@ -894,7 +934,6 @@ __device__ __forceinline__ void wide_body(const AttnArgs& p) {
   s.row0 *= W::kRows;
   WideState<D, E, Q> w;
   const int tid = threadIdx.x;
-  if (kWaves == 8 && (tid >> 6) < 4) __builtin_amdgcn_s_setprio(1);
   w.lane = tid & 63;
   w.wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   w.col = w.lane & 31;

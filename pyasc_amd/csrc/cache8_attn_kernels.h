@@ -705,9 +705,9 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
 
 // ------------------------------------------------------------------------------------ many rows
 //
-// Bound by matrix units, VALU and LDS about equally: 2 sequences of 8192 keys and 2048 new rows (32 query heads on 8, 128
-// columns: 481 GF) in 478 us, 1.0 PF (a large product of matrices: 1.21).  Each of the three is busy for 40 to 50% of the time:
-// the K and V fragments of a wave's 32 rows are read from LDS for those rows only, and codes become fp16 once per workgroup.
+// Bound by what the waves issue: 2 sequences of 8192 keys and 2048 new rows (32 query heads on 8, 128 columns: 481 GF) in
+// 478 us, 1.0 PF (a large product of matrices: 1.21), with the matrix units busy for 44% of the time, the VALU for 54% (a
+// quarter of it exp2) and LDS for 28%: matrix and vector instructions follow one another.
 // Half a tile's probabilities are computed between the products of the halves around it (620 us without that), and what a
 // tile's groups need is worked out for sixteen tiles at a time.
 
@@ -731,20 +731,23 @@ struct WideState : fa::FaState<D, Wide<D>::kWaves, 1, F16, true> {
   int group;                  // of this wave's rows
   uint32_t found;             // NaN among the values that this lane has loaded, of tiles that not all rows attend
 
-  // Neighbouring chunks change places in every other row of 256 bytes, as sixteen lanes write every other chunk of those.
-  static __device__ __forceinline__ uint32_t v_place(int row, int col) {
-    return fa::v_off<D>(row, col) ^ static_cast<uint32_t>((row >> (D == 128 ? 0 : 1) & 1) << 4);
+  // Where a chunk of eight values lies in a tile: a row's second half (D 64: every other row) has neighbours swapped, since eight
+  // lanes write every other chunk of 256 bytes at a time, 128 bytes of banks.
+  static __device__ __forceinline__ uint32_t swapped(int row, int chunk) {
+    return static_cast<uint32_t>(D == 128 ? chunk >> 3 & 1 : row & 1) << 4;
   }
+  static __device__ __forceinline__ uint32_t k_place(int row, int chunk) { return fa::k_off<D>(row, chunk) ^ swapped(row, chunk); }
+  static __device__ __forceinline__ uint32_t v_place(int row, int col) { return fa::v_off<D>(row, col) ^ swapped(row, col >> 3); }
   __device__ __forceinline__ void init_tiles(const AttnArgs& p) {
     constexpr int kPieces = D / 16;
     const int lane = this->lane, row = this->wave * (64 / kPieces) + lane / kPieces, piece = lane % kPieces;
     group = row / kGroup;
     koff = (row % kGroup) * p.c.ks.row * 16 + piece * 16;
     voff = (row % kGroup) * p.c.vs.row * 16 + piece * 16;
-    kdst = fa::k_off<D>(row, piece * 2);
+    kdst = k_place(row, piece * 2);
     vdst = v_place(row, piece * 16);
     group = __builtin_amdgcn_readfirstlane(group);
-    this->kaddr[0] = fa::k_off<D>(this->col, this->h);
+    this->kaddr[0] = k_place(this->col, this->h);
     const int g_lane = lane & 15;
     this->vaddr[0] = v_place(this->h * 4 + (g_lane >> 2), ((lane >> 4) & 1) * 16 + (g_lane & 3) * 4);
   }
@@ -762,10 +765,14 @@ struct WideState : fa::FaState<D, Wide<D>::kWaves, 1, F16, true> {
   }
   // V^T operand r of half kb of a tile: block r / 2 of the columns, its keys 16 (r % 2) .. + 15.
   __device__ __forceinline__ u32x4 v_operand(uint32_t base, int kb, int r) const {
-    return this->vt_read(base, (r >> 1) * 4 + kb * 2 + (r & 1));
+    const int db = r >> 1, row = kb * 32 + (r & 1) * 16;
+    const uint32_t at = (base + this->vaddr[0]) ^ (db << 6) ^ swapped(0, db * 4);
+    const auto lo = fa::lds_read_tr16_b64(at, row * (D * 2)), hi = fa::lds_read_tr16_b64(at, (row + 8) * (D * 2));
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
   }
+  // K operand r: chunks 2 r and 2 r + 1 of its rows.
   __device__ __forceinline__ u32x4 k_operand(uint32_t base, int kb, int r) const {
-    return fa::lds_read_b128(this->k_addr(base, r), kb * 32 * (D * 2));
+    return fa::lds_read_b128((base + this->kaddr[0]) ^ (r << 5) ^ swapped(0, r * 2), kb * 32 * (D * 2));
   }
   static constexpr int kOps = Base::kKSteps;  // of K, and as many of V, for a half of a tile
   static_assert(kOps == 2 * Base::kDBlocks, "operands of a half");

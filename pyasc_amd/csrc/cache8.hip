@@ -93,6 +93,7 @@ __global__ void __launch_bounds__(kWaves * 64) append(RowsArgs p) {
   if (old > 0) before = *scale_place;
   if (!good) return;
   uint8_t* codes = (is_v ? c.v : c.k) + asc::c8::row_at(strides, page, head, row);
+  const uint64_t row_bytes = static_cast<uint64_t>(strides.row) * 16;  // a block's rows may span more than 4 GiB
 
   // magnitudes are ordered as the integers of their bits, infinities and NaN above all
   const bool once = end_vec - first_vec <= kChunk;
@@ -157,13 +158,13 @@ __global__ void __launch_bounds__(kWaves * 64) append(RowsArgs p) {
           w[half] = Q::pack(q, 1.0f);
         }
       }
-      if (vec < end_vec) *reinterpret_cast<u32x2*>(codes + (vec / kPerRow) * (strides.row * 16u) + vec % kPerRow * 8) = w;
+      if (vec < end_vec) *reinterpret_cast<u32x2*>(codes + (vec / kPerRow) * row_bytes + vec % kPerRow * 8) = w;
     }
   }
   if (old > 0 && grows) {
     __syncthreads();  // all have read the scale
     for (int vec = threadIdx.x; vec < first_vec; vec += kThreads) {
-      u32x2* at = reinterpret_cast<u32x2*>(codes + (vec / kPerRow) * (strides.row * 16u) + vec % kPerRow * 8);
+      u32x2* at = reinterpret_cast<u32x2*>(codes + (vec / kPerRow) * row_bytes + vec % kPerRow * 8);
       u32x2 w = *at;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {

@@ -189,6 +189,22 @@ def test_far_rows(device):
     assert (out.float() - x.float()).abs().max() <= scales[5] / 2 + 2.0 ** -10 and not cache[:5].any()
 
 
+@pytest.mark.parametrize("new", [32, 5])
+def test_rows_of_a_block_far_apart(device, new):
+    """Rows outermost: a block that spans 5 GiB, whole, and row by row with scales that grow."""
+    base = torch.zeros((6 << 30,), dtype=torch.int8, device=device)
+    cache = base.as_strided((2, 1, 32, 64), (64, 128, 160 << 20, 1))
+    other = torch.zeros((2, 1, 32, 64), dtype=torch.int8, device=device)
+    scales, near = torch.zeros((2, 2, 1, 1), device=device)
+    x = torch.randn((2, 1, new, 64), device=device).half()
+    lengths = torch.zeros(2, dtype=torch.int32, device=device)
+    for i in range(2 if new < 32 else 1):
+        kernels.quantized_cache_append(x * 2.0 ** i, x * 2.0 ** i, cache, other, scales, near, lengths)
+        lengths += new
+    assert torch.equal(cache, other) and torch.equal(scales, near) and other.any()
+    assert int((base != 0).sum()) == int((other != 0).sum())  # and nothing else
+
+
 def test_another_stream_and_a_captured_step(device):
     g = torch.Generator(device=device).manual_seed(10)
     state, plain = (make(4, 1, 16, 64, 16, torch.int8, torch.Generator(device=device).manual_seed(1)) for _ in range(2))

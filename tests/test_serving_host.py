@@ -158,6 +158,15 @@ def test_fork_and_compact_refusals(entry, kw, code):
     assert getattr(_native.load_library(), entry + "_workspace")(ctypes.byref(a)) == 0
 
 
+def test_pages_whose_heads_are_too_large():
+    """A head of a page that is copied by one workgroup, of 2 GiB."""
+    far = dict(heads=2, rows=1 << 16, row_bytes=1 << 15, head_stride=1 << 32, row_stride=1 << 15)
+    t = _native.PageTensor(1 << 44, 1 << 45, 1 << 34, 1 << 34, 1, 1, 1, 1, 1)
+    for name, value in far.items():
+        setattr(t, name, value)
+    assert call("asc_cache_copy_pages", pages(tensor=t)) == UNSUPPORTED and "too large" in _native.last_error()
+
+
 def test_pages_refusals_of_one_entry():
     assert call("asc_cache_fork", pages(parents=None)) == INVALID
     assert call("asc_cache_fork", pages(lengths_out=None)) == INVALID

@@ -706,8 +706,8 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
 // ------------------------------------------------------------------------------------ many rows
 //
 // Bound by what the waves issue: 2 sequences of 8192 keys and 2048 new rows (32 query heads on 8, 128 columns: 481 GF) in
-// 478 us, 1.0 PF (a large product of matrices: 1.21), with the matrix units busy for 44% of the time, the VALU for 54% (a
-// quarter of it exp2) and LDS for 28%: matrix and vector instructions follow one another.
+// 463 us, 1.04 PF (a large product of matrices: 1.21), with the matrix units busy for 47% of the time, the VALU for 51% (a
+// quarter of it exp2) and LDS for 30%: matrix and vector instructions follow one another.  The clock is 1.8 to 2.0 GHz then.
 // Half a tile's probabilities are computed between the products of the halves around it (620 us without that), and what a
 // tile's groups need is worked out for sixteen tiles at a time.
 
@@ -763,35 +763,47 @@ struct WideState : fa::FaState<D, Wide<D>::kWaves, 1, F16, true> {
     *reinterpret_cast<u32x4*>(tile + dst) = operand_of<Q>(x[0], x[1]);
     *reinterpret_cast<u32x4*>(tile + (dst ^ 16)) = operand_of<Q>(x[2], x[3]);
   }
-  // V^T operand r of half kb of a tile: block r / 2 of the columns, its keys 16 (r % 2) .. + 15.
-  __device__ __forceinline__ u32x4 v_operand(uint32_t base, int kb, int r) const {
-    const int db = r >> 1, row = kb * 32 + (r & 1) * 16;
-    const uint32_t at = (base + this->vaddr[0]) ^ (db << 6) ^ swapped(0, db * 4);
-    const auto lo = fa::lds_read_tr16_b64(at, row * (D * 2)), hi = fa::lds_read_tr16_b64(at, (row + 8) * (D * 2));
+  // V^T operand r of half kb of a tile in stage kStage: block r / 2 of the columns, its keys 16 (r % 2) .. + 15.
+  template <int kStage>
+  __device__ __forceinline__ u32x4 v_operand(uint32_t at, int kb, int r) const {
+    const int off = kStage * T + (kb * 32 + (r & 1) * 16) * (D * 2);
+    const auto lo = fa::lds_read_tr16_b64(at, off), hi = fa::lds_read_tr16_b64(at, off + 8 * (D * 2));
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   }
-  // K operand r: chunks 2 r and 2 r + 1 of its rows.
-  __device__ __forceinline__ u32x4 k_operand(uint32_t base, int kb, int r) const {
-    return fa::lds_read_b128((base + this->kaddr[0]) ^ (r << 5) ^ swapped(0, r * 2), kb * 32 * (D * 2));
+  // Where it lies in a tile at `base`; that of K operand r, chunks 2 r and 2 r + 1 of its rows.
+  __device__ __forceinline__ uint32_t v_at(uint32_t base, int r) const {
+    return (base + this->vaddr[0]) ^ (r >> 1 << 6) ^ swapped(0, (r >> 1) * 4);
+  }
+  __device__ __forceinline__ uint32_t k_at(uint32_t base, int r) const {
+    return (base + this->kaddr[0]) ^ (r << 5) ^ swapped(0, r * 2);
+  }
+  template <int kStage>
+  __device__ __forceinline__ u32x4 k_operand(uint32_t at, int kb, int r) const {
+    return fa::lds_read_b128(at, kStage * T + kb * 32 * (D * 2));
+  }
+  uint32_t kat[Base::kKSteps], vat[Base::kDBlocks];  // of the operands in stage 0
+  __device__ __forceinline__ void init_places(uint8_t* ring) {
+#pragma unroll
+    for (int r = 0; r < Base::kKSteps; ++r) kat[r] = k_at(lds_addr(ring), r);
+#pragma unroll
+    for (int i = 0; i < Base::kDBlocks; ++i) vat[i] = v_at(lds_addr(ring + 3 * T), 2 * i);
   }
   static constexpr int kOps = Base::kKSteps;  // of K, and as many of V, for a half of a tile
   static_assert(kOps == 2 * Base::kDBlocks, "operands of a half");
 
   // The probabilities of half kb (s[kb], into pb_out) between the products that wait for nothing of it: the raw scores of
-  // the half behind it (into s[1 - kb], of `k`'s rows) and, kPv, the values times the probabilities of the half before it
-  // (pb_in, of `v`'s rows).  Returns the probabilities' sum.
-  template <int kb, bool kPv>
-  __device__ __forceinline__ float half(const uint8_t* k, const uint8_t* v, f32x16 (&s)[2], const u32x4 (&pb_in)[2],
-                                        u32x4 (&pb_out)[2]) {
+  // the half behind it (into s[1 - kb], of K's stage kK) and, kPv, the values times the probabilities of the half before it
+  // (pb_in, of V's stage kV).  Returns the probabilities' sum.
+  template <int kb, bool kPv, int kK, int kV>
+  __device__ __forceinline__ float half(f32x16 (&s)[2], const u32x4 (&pb_in)[2], u32x4 (&pb_out)[2]) {
     constexpr int kWin = 3, kPer = 8 / kOps, kEach = kPv ? 3 : 1;  // LDS reads in a round
-    const uint32_t kbase = lds_addr(k), vbase = lds_addr(v);
     const float ref = st.reference();
     float rs = 0.f, sum = 0.f;
     u32x4 x[kOps], y[kOps];
 #pragma unroll
     for (int r = 0; r < kWin; ++r) {
-      x[r] = k_operand(kbase, 1 - kb, r);
-      if constexpr (kPv) y[r] = v_operand(vbase, 1 - kb, r);
+      x[r] = k_operand<kK>(kat[r], 1 - kb, r);
+      if constexpr (kPv) y[r] = v_operand<kV>(vat[r >> 1], 1 - kb, r);
     }
     f32x16 next = {};
     __builtin_amdgcn_sched_barrier(0);
@@ -814,8 +826,8 @@ struct WideState : fa::FaState<D, Wide<D>::kWaves, 1, F16, true> {
         st.acc[r >> 1] = F16::mfma(y[r], pb_in[r & 1], st.acc[r >> 1]);
       }
       if (r + kWin < kOps) {
-        x[r + kWin] = k_operand(kbase, 1 - kb, r + kWin);
-        if constexpr (kPv) y[r + kWin] = v_operand(vbase, 1 - kb, r + kWin);
+        x[r + kWin] = k_operand<kK>(kat[r + kWin], 1 - kb, r + kWin);
+        if constexpr (kPv) y[r + kWin] = v_operand<kV>(vat[(r + kWin) >> 1], 1 - kb, r + kWin);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -828,13 +840,13 @@ struct WideState : fa::FaState<D, Wide<D>::kWaves, 1, F16, true> {
     const uint32_t base = lds_addr(k);
     u32x4 x[kOps];
 #pragma unroll
-    for (int r = 0; r < kWin; ++r) x[r] = k_operand(base, kb, r);
+    for (int r = 0; r < kWin; ++r) x[r] = k_operand<0>(k_at(base, r), kb, r);
     s = f32x16{};
 #pragma unroll
     for (int r = 0; r < kOps; ++r) {
       fa::lds_wait(x[r], r + kWin <= kOps ? kWin - 1 : kOps - 1 - r);
       s = F16::mfma(x[r], this->qreg[0][r], s);
-      if (r + kWin < kOps) x[r + kWin] = k_operand(base, kb, r + kWin);
+      if (r + kWin < kOps) x[r + kWin] = k_operand<0>(k_at(base, r + kWin), kb, r + kWin);
     }
   }
   __device__ __forceinline__ void pv(const uint8_t* v, int kb, const u32x4 (&pb)[2]) {
@@ -842,17 +854,18 @@ struct WideState : fa::FaState<D, Wide<D>::kWaves, 1, F16, true> {
     const uint32_t base = lds_addr(v);
     u32x4 y[kOps];
 #pragma unroll
-    for (int r = 0; r < kWin; ++r) y[r] = v_operand(base, kb, r);
+    for (int r = 0; r < kWin; ++r) y[r] = v_operand<0>(v_at(base, r), kb, r);
 #pragma unroll
     for (int r = 0; r < kOps; ++r) {
       fa::lds_wait(y[r], 2 * (r + kWin <= kOps ? kWin - 1 : kOps - 1 - r));
       st.acc[r >> 1] = F16::mfma(y[r], pb[r & 1], st.acc[r >> 1]);
-      if (r + kWin < kOps) y[r + kWin] = v_operand(base, kb, r + kWin);
+      if (r + kWin < kOps) y[r + kWin] = v_operand<0>(v_at(base, r + kWin), kb, r + kWin);
     }
   }
 };
 
-// The way of the tiles through a wave.  LDS has three stages for each of K and V, tile t in stage t % 3.  In step j: the codes of
+// The way of the tiles through a wave.  LDS has three stages for each of K and V, tile t in stage t % 3, which the clean steps know
+// at compile time: operands lie at registers and constant offsets (478 us where each step adds them up).  In step j: the codes of
 // K_{j+2} and V_{j+1}, asked for in the step before, go into stages that no wave reads any more, and those of K_{j+3}
 // and V_{j+2} are asked for; then, half a tile (32 keys) at a time, the probabilities, between the products of the
 // scores of the half behind and of the values of the half before.
@@ -863,15 +876,17 @@ struct WideAhead {
   u32x4 pb[2][2];    // probabilities of each half
 };
 
-// kTail false: tile j + 1 exists, and all of the workgroup's rows attend all of tile j; whole: tiles of which they do.  The second
-// half's probabilities are left for the next step, whose kFirst is false, or for the caller.
-template <bool kTail, bool kFirst, int D, class E, class Q>
+// kStage: a.c, where tile j + 1 exists and all of the workgroup's rows attend all of tile j (whole: tiles of which they do); the second
+// half's probabilities are left for the next step, whose kFirst is false, or for the caller.  -1: of any other tile.
+template <int kStage, bool kFirst, int D, class E, class Q>
 __device__ __forceinline__ void wide_step(WideState<D, E, Q>& w, const AttnArgs& p, int j, int end, int whole, uint8_t* ring, int most,
                                           int least, WideAhead& a, f32x16 (&s)[2]) {
   constexpr int T = WideState<D, E, Q>::T;
   Softmax<D>& st = w.st;
-  const int c1 = a.c == 2 ? 0 : a.c + 1, c2 = a.c == 0 ? 2 : a.c - 1;  // of j + 1, and of j + 2 and j - 1
-  uint8_t *k_here = ring + a.c * T, *k_next = ring + c1 * T, *v_here = ring + (3 + a.c) * T, *v_before = ring + (3 + c2) * T;
+  constexpr bool kTail = kStage < 0;
+  constexpr int kS1 = (kStage + 1) % 3, kS2 = (kStage + 2) % 3;
+  const int c = kTail ? a.c : kStage;
+  const int c1 = c == 2 ? 0 : c + 1, c2 = c == 0 ? 2 : c - 1;  // of j + 1, and of j + 2 and j - 1
   if (a.n == kBatch) {
     w.groups.advance(a.n);
     st.take_ratios(w.groups.vs);
@@ -889,6 +904,7 @@ __device__ __forceinline__ void wide_step(WideState<D, E, Q>& w, const AttnArgs&
   if (j + 3 < end) a.k = w.load(p.c.k, w.groups.template place<false>(a.n + 3, w.group), w.koff);
   if constexpr (kTail) {
     if (j * BKV < most) {
+      uint8_t *k_here = ring + c * T, *k_next = ring + c1 * T, *v_here = ring + (3 + c) * T;
       st.set_tile(w.groups.ks, a.n);
       w.scores(k_here, 1, s[1]);
       if ((j + 1) * BKV > least) st.hide(s, j, w.h);
@@ -900,8 +916,8 @@ __device__ __forceinline__ void wide_step(WideState<D, E, Q>& w, const AttnArgs&
     }
   } else {
     st.set_tile(w.groups.ks, a.n);
-    st.guard(s[0], 0, a.pb[0], w.template half<0, !kFirst>(k_here, v_before, s, a.pb[1], a.pb[0]));
-    st.guard(s[1], 1, a.pb[1], w.template half<1, true>(k_next, v_here, s, a.pb[0], a.pb[1]));
+    st.guard(s[0], 0, a.pb[0], w.template half<0, !kFirst, kStage, kS2>(s, a.pb[1], a.pb[0]));
+    st.guard(s[1], 1, a.pb[1], w.template half<1, true, kS1, kStage>(s, a.pb[0], a.pb[1]));
   }
   ++a.n;
   a.c = c1;
@@ -987,15 +1003,21 @@ __device__ __forceinline__ void wide_body(const AttnArgs& p) {
       w.template store<false>(ring + 3 * T, w.vdst, v0);
     }
     __syncthreads();
+    w.init_places(ring);
     f32x16 s2[2];
     w.scores(ring, 0, s2[0]);
     int j = begin;
-    if (j < whole && j + 1 < end) {
-      wide_step<false, true>(w, p, j, end, whole, ring, most, least, a, s2);
-      for (++j; j < whole && j + 1 < end; ++j) wide_step<false, false>(w, p, j, end, whole, ring, most, least, a, s2);
-      w.pv(ring + (3 + (a.c == 0 ? 2 : a.c - 1)) * T, 1, a.pb[1]);
+    const int clean = min(whole, end - 1);
+    if (j < clean) {
+      wide_step<0, true>(w, p, j, end, whole, ring, most, least, a, s2);
+      for (++j; j + 2 < clean; j += 3) {
+        wide_step<1, false>(w, p, j, end, whole, ring, most, least, a, s2);
+        wide_step<2, false>(w, p, j + 1, end, whole, ring, most, least, a, s2);
+        wide_step<0, false>(w, p, j + 2, end, whole, ring, most, least, a, s2);
+      }
+      w.pv(ring + 3 * T, 1, a.pb[1]);  // of stage 0
     }
-    for (; j < end; ++j) wide_step<true, false>(w, p, j, end, whole, ring, most, least, a, s2);
+    for (; j < end; ++j) wide_step<-1, false>(w, p, j, end, whole, ring, most, least, a, s2);
   }
   if (kHasNan && __syncthreads_or(w.found != 0) != 0) {
     for (int j = max(begin, whole); j < end; ++j) st.add_nan(p, s, j, w.h);

@@ -610,8 +610,13 @@ def _here(t: torch.Tensor, name: str, device: int) -> torch.Tensor:
 
 def _apart(t: torch.Tensor, name: str) -> None:
     """Refuses a tensor to write to whose elements may share a place."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) == 4 and strides[3] == 1:  # [batch, rows, heads, head_dim] seen as [batch, heads, rows, head_dim]
+        s0, s1, s2, _ = strides
+        if s1 >= shape[3] and s2 >= s1 * shape[1] and s0 >= s2 * shape[2]:
+            return
     span = 0  # of the dimensions so far, from the innermost
-    for stride, size in sorted((t.stride(i), t.shape[i]) for i in range(t.dim()) if t.shape[i] > 1):
+    for stride, size in sorted([x for x in zip(strides, shape) if x[1] > 1]):
         if stride <= span:
             raise ValueError(f"'{name}' is written but its elements overlap (strides {t.stride()})")
         span += stride * (size - 1)

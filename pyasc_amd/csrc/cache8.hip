@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kWaves * 64) append(RowsArgs p) {
 }
 
 // A workgroup reads a run of tokens of one head, kVecs vectors of eight values per thread, whose pages, codes and scales are
-// under way together.  Results are written past the caches.  66 MB (8 sequences of up to 1999 tokens from int8 to fp16) in 11.4 us:
+// under way together.  Results are written past the caches.  50 MB (8 sequences of 500 to 1999 tokens from int8 to fp16) in 11.4 us:
 // with four vectors 15.9, with one 13.2, with stores through the caches 13.3.
 constexpr int kReadVecs = 2;
 template <int D>

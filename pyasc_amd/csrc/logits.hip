@@ -4,7 +4,7 @@
 // A workgroup owns a slice of one row's vocabulary.  It counts the history's tokens that fall into the
 // slice in LDS (integers: the order does not matter), then takes the slice through the formula.  The
 // whole history is read for every slice, from L2 after the first.  HBM bounds large calls: 64 rows of 131072 fp32
-// logits with masks: 70.7 MB in 14.1 us (5.0 TB/s), in 17.3 us with 8000 tokens of history; the launch small ones.
+// logits with masks: 70.7 MB in 14.1 us (5.0 TB/s), in 16 to 17.3 us with 8000 tokens of history; the launch small ones (4 us).
 #include "common.h"
 #include "numeric.h"
 #include "overlap.h"

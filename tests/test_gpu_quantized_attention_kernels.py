@@ -111,3 +111,30 @@ def test_same_results_from_run_to_run_and_from_a_graph(device, name, cache):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("name", LAUNCHES)
+def test_empty_sequences_beside_full_ones(device, name):
+    q, state, table, capacity, _ = operands(name, torch.int8, torch.float16, device, 6)
+    b, _, n, _ = q.shape
+    attend(q, state, [0] + [capacity] * (b - 1), table)
+    attend(q, state, [0] * b, table, [max(0, n - i) for i in range(b)])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("name", LAUNCHES)
+def test_a_query_of_nan_or_infinity_stays_alone(device, name, dtype):
+    q, state, table, capacity, _ = operands(name, torch.float8_e4m3fn, dtype, device, 7)
+    b, _, n, d = q.shape
+    lengths = torch.tensor(lengths_of(b, n, capacity), dtype=torch.int32, device=device)
+    want, got = torch.zeros_like(q), torch.zeros_like(q)
+    kernels.quantized_cache_attention(q, *state, lengths, want, 0.1, block_table=table)
+    bad = q.clone()
+    bad[0, 0, n // 2, 3], bad[0, -1, 0, d - 1] = math.nan, math.inf
+    kernels.quantized_cache_attention(bad, *state, lengths, got, 0.1, block_table=table)
+    hit = torch.zeros(q.shape[:3], dtype=torch.bool, device=device)
+    hit[0, 0, n // 2], hit[0, -1, 0] = True, True
+    assert got[0, 0, n // 2].isnan().all() and torch.equal(got[~hit].isnan(), want[~hit].isnan())
+    # another row of a block may move its reference point: all within a few roundings of the first result
+    a, c = got[~hit].double(), want[~hit].double()
+    assert ((a - c).abs() <= 4 * torch.finfo(dtype).eps * (c.abs() + c.abs().mean(-1, keepdim=True)))[~c.isnan()].all()

@@ -1,10 +1,11 @@
 // Pages of a cache: copies between caches, the fork of sequences that share pages, and compaction.
 //
-// What a fork does to the pages is worked out by one workgroup, with the reference counts in LDS (64 sequences of 4096 tokens to
-// 256: 15 us, bound by chains of loads and ballots), what a compaction does by as many as the pages need (8192: 5.7 us); a
-// second launch moves the data and writes the tables (8192 pages of 65.5 KB, two fifths used: 258 MB in 45.6 us,
-// 5.7 TB/s).  Nothing comes back to the host, so all of them can be captured.  Ranks of free and moving pages are prefix sums and counts are
-// integers: the same result on every call.
+// What a fork does to the pages is worked out by one workgroup, with the reference counts in LDS (64 sequences of 4096
+// tokens to 256: 15 us, bound by its instructions over counts and table: with all its first loads asked for together 15.2),
+// what a compaction does by as many as the pages need (8192: 5.7 us).  A second launch moves the data and writes the
+// tables (8192 pages of 65.5 KB, two fifths used: 258 MB in 45.6 us, 5.7 TB/s).  Nothing comes back to the host, so all of
+// them can be captured.  Ranks of free and moving pages are prefix sums and counts are integers: the same result on every
+// call.
 #include "common.h"
 #include "divisor.h"
 #include "overlap.h"

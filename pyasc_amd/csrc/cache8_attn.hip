@@ -116,7 +116,7 @@ void plan(Launch& L, const asc_cache8_t& a) {
 // Bytes of the parts: their values and statistics.
 int64_t workspace_of(const Launch& L, int head_dim) {
   if (L.blocks == 0 || L.p.splits == 1) return 0;
-  return L.p.units * static_cast<int64_t>(L.p.rows) * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+  return L.p.units * static_cast<int64_t>(L.p.rows) * (head_dim + 4) * static_cast<int64_t>(sizeof(float));
 }
 
 int32_t make(const asc_cache8_t* a, const char* what, Launch& L) {

@@ -5,10 +5,13 @@
 //   s_j = (q . ck_j) (sm_scale ks_j),   o = sum_j (p_j vs_j) cv_j / sum_j p_j,   p_j = exp(s_j - m):
 // the codes go to the matrix units as they are, in fp16, which holds all of them exactly, K's scales go into the
 // scores' factor and V's into the probabilities.  A tile has 64 keys, of 16 of which each group lies in one
-// block and one page, so a lane has four factors per tile.  P^T's values p_j vs_j / R (R: the largest V scale so far)
-// are at most p_j: exp2 takes log2(vs_j / R) with the scores' shift, and the sums over a group are divided by
-// vs_j / R again for the denominator.  Queries of bf16 are brought to fp16's range by a power of two of
-// their row: exact, but for elements 2^-39 and less of the row's largest.
+// block and one page, so a lane has four factors per tile.  P^T's values are e_j = 2^-M p_j vs_j, with a reference point M of
+// their own that follows the row's largest s_j + log2 vs_j as m follows its largest s_j: V scales may lie as far apart as fp32
+// holds, and keys that a row does not attend, or with next to no probability, have no say in it.  exp2 takes log2 vs_j with the
+// scores' shift, and a group's sum of e_j times 2^(M - m) / vs_j is its part of the denominator.  A row's scale that lies 2^-60
+// and more below its 2^(M - m) counts as that: blocks of zeros, with scales of 2^-126, have their share of the denominator.
+// Queries of bf16 are brought to fp16's range by a power of two of their row: exact, but for elements 2^-39 and less of the
+// row's largest.
 //
 // The probabilities are rounded to fp16 for the product with the values, as matrix operands have to be: errors of up to 0.0002
 // of the results' norm, beside 0.0017 of a bf16 result's own rounding.  Beside 0.0002 of an fp16 result's they count where a few
@@ -38,8 +41,8 @@ struct AttnArgs {
   uint16_t* o;
   float* lse;  // [batch, q_heads, n] or null
   int64_t q_batch, q_head, q_seq, o_batch, o_head, o_seq;  // elements
-  float* part_o;   // [unit][rows][D], unnormalised
-  float* part_ml;  // [unit][rows][2]: reference point (log2), sum
+  float* part_o;   // [unit][rows][D], unnormalised, in units of 2^M
+  float* part_ml;  // [unit][rows][4]: m, sum of the probabilities in units of 2^m, M
   int32_t batch, group, rows, row_blocks, splits, join_groups, causal;
   int32_t lanes, per_lane;  // of the order of the row blocks
   uint32_t units;  // batch * splits * kv_heads
@@ -266,43 +269,32 @@ struct Groups {
   }
 };
 
+constexpr float kLeast = 60.0f;  // a row's 2^(M - m) over the least V scale that counts, log2
+
 // The online softmax of a wave: lane (row, half h of the keys); register r of score block kb is key 32 kb + 8 (r / 4) +
 // 4 h + r % 4, of group 2 kb + r / 8.
 template <int D>
 struct Softmax {
   static constexpr int kDBlocks = D / 32;
-  f32x16 acc[kDBlocks];  // in units of R
-  float m, l;            // reference point (log2) and this lane half's sum
+  f32x16 acc[kDBlocks];  // in units of 2^M
+  float m, M;            // reference points (log2): of the scores, and of the scores plus log2 of the V scale
+  float l;               // this lane half's sum of the probabilities in units of 2^m
   float factor;          // of the raw scores of a unit scale (log2)
-  float R;               // largest V scale, so far or of all
   int limit;             // keys of the row
-  float log_ratio, inverse;  // of this lane's group: log2 of V scale / R, and R / V scale
+  float log_scale;       // of this lane's group: log2 of the V scale
   float a[kGroups];      // of the tile's groups: the factors of their scores,
-  float shift[kGroups];  // log2 of V scale / R
-  float undo[kGroups];   // and R / V scale
+  float log_v[kGroups];  // and log2 of the V scale
 
   __device__ __forceinline__ void init() {
 #pragma unroll
     for (int i = 0; i < kDBlocks; ++i) acc[i] = f32x16{};
-    m = -INFINITY;
+    m = M = -INFINITY;
     l = 0.f;
-    R = 0.f;
   }
-  // The V scales of the current tiles, one per lane, in units of R.  One below 2^-40 R counts as that: its values times p stay
-  // below fp16's smallest.
-  __device__ __forceinline__ void take_ratios(float vs) {
-    const float ratio = fmaxf(vs / R, 0x1p-40f);
-    log_ratio = __builtin_amdgcn_logf(ratio);
-    inverse = 1.0f / ratio;
-  }
-  // Those, where R is the largest so far.
+  // The V scales of the current tiles, one per lane.  What is not positive counts as 2^-160, whose values round to zero.
   __device__ __forceinline__ void take_scales(float vs) {
-    const float top = fmaxf(R, __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, wave_max(vs)))));
-    const float down = top > R ? R / top : 1.0f;
-#pragma unroll
-    for (int i = 0; i < kDBlocks; ++i) acc[i] *= down;
-    R = top;
-    take_ratios(vs);
+    const bool small = vs < 0x1p-100f;  // the logarithm takes no subnormal numbers
+    log_scale = fmaxf(__builtin_amdgcn_logf(small ? vs * 0x1p64f : vs) - (small ? 64.0f : 0.0f), -160.0f);
   }
   // Those of tile number t, and its K scales.
   __device__ __forceinline__ void set_tile(float ks, int t) {
@@ -313,8 +305,7 @@ struct Softmax {
     for (int g = 0; g < kGroups; ++g) {
       // not zero, which times the -inf of a hidden key would be NaN
       a[g] = fmaxf(factor * lane(ks, g), 0x1p-126f);
-      shift[g] = lane(log_ratio, g);
-      undo[g] = lane(inverse, g);
+      log_v[g] = lane(log_scale, g);
     }
   }
   __device__ __forceinline__ void hide(f32x16 (&s)[2], int j, int h) const {
@@ -325,74 +316,110 @@ struct Softmax {
         if (j * BKV + kb * 32 + (r >> 2) * 8 + h * 4 + (r & 3) >= limit) s[kb][r] = -INFINITY;
       }
   }
-  // Largest score of half kb of a tile, or of all of it, less fp16's lift.
-  __device__ __forceinline__ float half_max(const f32x16& s, int kb) const {
+  // The largest score of half kb of a tile, or of all of it, and the largest with its V scale, less fp16's lift.
+  struct Tops {
+    float m, M;
+  };
+  __device__ __forceinline__ Tops half_tops(const f32x16& s, int kb) const {
     float low = -INFINITY, high = -INFINITY;
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       low = fmaxf(low, s[r]);
       high = fmaxf(high, s[8 + r]);
     }
-    const float top = fmaxf(low * a[kb * 2], high * a[kb * 2 + 1]);
-    return fmaxf(top, other_half(top)) - F16::kLift;
+    low *= a[kb * 2];
+    high *= a[kb * 2 + 1];
+    const float top = fmaxf(low, high), with_v = fmaxf(low + log_v[kb * 2], high + log_v[kb * 2 + 1]);
+    return {fmaxf(top, other_half(top)) - F16::kLift, fmaxf(with_v, other_half(with_v)) - F16::kLift};
   }
-  __device__ __forceinline__ float tile_max(const f32x16 (&s)[2]) const { return fmaxf(half_max(s[0], 0), half_max(s[1], 1)); }
-  __device__ __forceinline__ void raise(float top) {
-    const bool up = top > m;
-    const float alpha = up ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
-    if (up) m = top;
-    l *= alpha;
+  __device__ __forceinline__ Tops tile_tops(const f32x16 (&s)[2]) const {
+    const Tops x = half_tops(s[0], 0), y = half_tops(s[1], 1);
+    return {fmaxf(x.m, y.m), fmaxf(x.M, y.M)};
+  }
+  // Of a row's first tile.
+  __device__ __forceinline__ void start(const Tops& top) {
+    m = top.m;
+    M = top.M;
+  }
+  __device__ __forceinline__ void raise(const Tops& top) {
+    const bool up = top.m > m, up_v = top.M > M;
+    l *= up ? __builtin_amdgcn_exp2f(m - top.m) : 1.0f;
+    const float alpha = up_v ? __builtin_amdgcn_exp2f(M - top.M) : 1.0f;
+    if (up) m = top.m;
+    if (up_v) M = top.M;
 #pragma unroll
     for (int i = 0; i < kDBlocks; ++i) acc[i] *= alpha;
   }
-  __device__ __forceinline__ float reference() const { return m == -INFINITY ? 0.f : -m; }
+  // What the probabilities are taken against: -M, and M - m.
+  struct Reference {
+    float shift, apart;
+  };
+  __device__ __forceinline__ Reference reference() const {
+    return m == -INFINITY ? Reference{0.f, 0.f} : Reference{-M, M - m};
+  }
+  // The score's shift of group g, and the factor from e_j to p_j.
+  __device__ __forceinline__ float shift_of(const Reference& r, int g) const { return fmaxf(log_v[g], r.apart - kLeast) + r.shift; }
+  __device__ __forceinline__ float undo_of(const Reference& r, int g) const {
+    return __builtin_amdgcn_exp2f(fminf(r.apart - log_v[g], kLeast));
+  }
+  // Sums of a lane over a half, or a whole tile: of the probabilities, and of P^T's values.
+  struct Sums {
+    float p, e;
+  };
   // Values 2 w and 2 w + 1 of group u of half kb, and their sum.
-  __device__ __forceinline__ void pair(const f32x16& s, int kb, int u, int w, float ref, u32x4 (&pb)[2], float& sum) const {
+  __device__ __forceinline__ void pair(const f32x16& s, int kb, int u, int w, const Reference& ref, u32x4 (&pb)[2], float& sum) const {
     const int g = kb * 2 + u;
-    const float e0 = __builtin_amdgcn_exp2f(fmaf(s[8 * u + 2 * w], a[g], ref + shift[g]));
-    const float e1 = __builtin_amdgcn_exp2f(fmaf(s[8 * u + 2 * w + 1], a[g], ref + shift[g]));
+    const float e0 = __builtin_amdgcn_exp2f(fmaf(s[8 * u + 2 * w], a[g], shift_of(ref, g)));
+    const float e1 = __builtin_amdgcn_exp2f(fmaf(s[8 * u + 2 * w + 1], a[g], shift_of(ref, g)));
     sum += e0;
     sum += e1;
     pb[u][w] = F16::pack(e0, e1);
   }
-  // P^T operands of half kb; returns this lane's sum of probabilities.
-  __device__ __forceinline__ float probs(const f32x16& s, int kb, u32x4 (&pb)[2]) const {
-    const float ref = reference();
-    float rs = 0.f;
+  __device__ __forceinline__ void add_group(Sums& sums, const Reference& ref, int g, float sum) const {
+    sums.p = fmaf(sum, undo_of(ref, g), sums.p);
+    sums.e += sum;
+  }
+  // P^T operands of half kb.
+  __device__ __forceinline__ Sums probs(const f32x16& s, int kb, u32x4 (&pb)[2]) const {
+    const Reference ref = reference();
+    Sums sums{0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) pair(s, kb, u, w, ref, pb, sum);
-      rs = fmaf(sum, undo[kb * 2 + u], rs);
+      add_group(sums, ref, kb * 2 + u, sum);
     }
-    return rs;
+    return sums;
   }
-  __device__ __forceinline__ bool out_of_range(float sum) const {
-    return __builtin_amdgcn_ballot_w64(sum > F16::kTileSumLimit || m == -INFINITY) != 0;
+  // The values may not overflow fp16; and where the probabilities grow as far, what counts as the least scale would.
+  __device__ __forceinline__ bool out_of_range(const Sums& sums) const {
+    return __builtin_amdgcn_ballot_w64(fmaxf(sums.p, sums.e) > F16::kTileSumLimit || m == -INFINITY) != 0;
   }
-  // Of a half, or a whole tile.
-  __device__ __forceinline__ void guard(const f32x16& s, int kb, u32x4 (&pb)[2], float rs) {
-    if (out_of_range(rs)) {
-      raise(half_max(s, kb));
-      rs = probs(s, kb, pb);
+  __device__ __forceinline__ void guard(const f32x16& s, int kb, u32x4 (&pb)[2], Sums sums) {
+    if (out_of_range(sums)) {
+      raise(half_tops(s, kb));
+      sums = probs(s, kb, pb);
     }
-    l += rs;
+    l += sums.p;
   }
   // kRest: and what their rounding leaves, rounded.
   template <bool kRest>
-  __device__ __forceinline__ float both_probs(const f32x16 (&s)[2], u32x4 (&pb)[2][2], u32x4 (&rest)[2][2]) const {
-    if constexpr (!kRest) return probs(s[0], 0, pb[0]) + probs(s[1], 1, pb[1]);
-    const float ref = reference();
-    float rs = 0.f;
+  __device__ __forceinline__ Sums both_probs(const f32x16 (&s)[2], u32x4 (&pb)[2][2], u32x4 (&rest)[2][2]) const {
+    if constexpr (!kRest) {
+      const Sums x = probs(s[0], 0, pb[0]), y = probs(s[1], 1, pb[1]);
+      return {x.p + y.p, x.e + y.e};
+    }
+    const Reference ref = reference();
+    Sums sums{0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const int r = 8 * (g & 1) + 2 * w;
-        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][r], a[g], ref + shift[g]));
-        const float e1 = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][r + 1], a[g], ref + shift[g]));
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][r], a[g], shift_of(ref, g)));
+        const float e1 = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][r + 1], a[g], shift_of(ref, g)));
         sum += e0;
         sum += e1;
         const uint32_t x = F16::pack(e0, e1);
@@ -400,18 +427,18 @@ struct Softmax {
         pb[g >> 1][g & 1][w] = x;
         rest[g >> 1][g & 1][w] = F16::pack(e0 - static_cast<float>(rounded[0]), e1 - static_cast<float>(rounded[1]));
       }
-      rs = fmaf(sum, undo[g], rs);
+      add_group(sums, ref, g, sum);
     }
-    return rs;
+    return sums;
   }
   template <bool kRest>
   __device__ __forceinline__ void tile_probs(const f32x16 (&s)[2], u32x4 (&pb)[2][2], u32x4 (&rest)[2][2]) {
-    float rs = both_probs<kRest>(s, pb, rest);
-    if (out_of_range(rs)) {
-      raise(tile_max(s));
-      rs = both_probs<kRest>(s, pb, rest);
+    Sums sums = both_probs<kRest>(s, pb, rest);
+    if (out_of_range(sums)) {
+      raise(tile_tops(s));
+      sums = both_probs<kRest>(s, pb, rest);
     }
-    l += rs;
+    l += sums.p;
   }
   // A NaN among the values of keys that only some rows attend is taken as zero in the products, whose 0 times NaN
   // would reach all rows (without_nan).  Where that was met, the rows that attend it get it back: tile j, from memory.
@@ -545,14 +572,30 @@ struct NarrowTiles {
   }
 };
 
+// What brings sums of values in units of 2^M over one of probabilities in units of 2^m to a result: a factor, and a power of two
+// behind it, as their product may lie outside fp32.
+struct Result {
+  float factor;
+  int power;
+  __device__ __forceinline__ Result(float m, float M, float l) {
+    const float apart = m == -INFINITY ? 0.f : fminf(fmaxf(M - m, -400.0f), 400.0f), whole = floorf(apart);
+    factor = kv::inverse_sum(l) * __builtin_amdgcn_exp2f(apart - whole);
+    power = static_cast<int>(whole);
+  }
+  __device__ __forceinline__ float of(float x) const { return ldexpf(x * factor, power); }
+};
+
 // Waves' parts in LDS, or a row's splits, joined and written: eight values of row `row`, relative to their largest
-// reference point m.
+// reference points m and M.
 template <class E>
-__device__ __forceinline__ void write_row(const AttnArgs& p, const kv::Share& s, int row, int ch, const float (&o)[8], float m,
+__device__ __forceinline__ void write_row(const AttnArgs& p, const kv::Share& s, int row, int ch, float (&o)[8], float m, float M,
                                           float l, int written) {
   int64_t o_at, lse_at;
   if (!out_row(p, s, row, written, o_at, lse_at)) return;
-  *reinterpret_cast<u32x4*>(p.o + o_at + ch * 8) = kv::pack8<E>(o, kv::inverse_sum(l));
+  const Result result(m, M, l);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = result.of(o[e]);
+  *reinterpret_cast<u32x4*>(p.o + o_at + ch * 8) = kv::pack8<E>(o, 1.0f);
   if (p.lse != nullptr && ch == 0) p.lse[lse_at] = kv::lse_of(m, l);
 }
 
@@ -565,7 +608,7 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
   constexpr bool kRest = __is_same(E, F16);
   static_assert(N::kRows * kRow <= 2 * BKV * D, "a wave's part reuses its tiles");
   __shared__ __attribute__((aligned(256))) uint8_t lds[kWaves * 2 * N::kTile];
-  __shared__ float stats[2][kWaves][N::kRows];
+  __shared__ float stats[3][kWaves][N::kRows];
 
   kv::Share s = share_of(p);
   if (!s.live) return;
@@ -622,7 +665,7 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
     st.set_tile(groups.ks, n);
     const bool masked = (j + 1) * BKV > least;
     if (masked) st.hide(sc, j, t.h);
-    if (j == begin + wave) st.m = st.tile_max(sc);  // nothing to rescale yet
+    if (j == begin + wave) st.start(st.tile_tops(sc));  // nothing to rescale yet
     u32x4 pb[2][2], rest[2][2];
     st.template tile_probs<kRest>(sc, pb, rest);
     if (next) {
@@ -653,6 +696,7 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
     if (t.h == 0) {
       stats[0][wave][t.col] = st.m;
       stats[1][wave][t.col] = l;
+      stats[2][wave][t.col] = st.M;
     }
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
@@ -660,7 +704,7 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
       for (int rq = 0; rq < 4; ++rq) {
         const f32x16& a = st.acc[db];
         *reinterpret_cast<f32x4*>(t.k + part_off(t.col, db * 8 + rq * 2 + t.h)) =
-            f32x4{a[rq * 4] * st.R, a[rq * 4 + 1] * st.R, a[rq * 4 + 2] * st.R, a[rq * 4 + 3] * st.R};
+            f32x4{a[rq * 4], a[rq * 4 + 1], a[rq * 4 + 2], a[rq * 4 + 3]};
       }
   }
   __syncthreads();
@@ -670,15 +714,18 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
     const int cc = tid + kWaves * 64 * i;
     const int row = cc / (D / 8), ch = cc % (D / 8);
     if (s.row0 + row >= p.rows) continue;
-    float m = stats[0][0][row];
+    float m = stats[0][0][row], M = stats[2][0][row];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, stats[0][w][row]);
+    for (int w = 1; w < kWaves; ++w) {
+      m = fmaxf(m, stats[0][w][row]);
+      M = fmaxf(M, stats[2][w][row]);
+    }
     float f[kWaves], l_run = 0.f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const float mw = stats[0][w][row];
-      f[w] = mw == m ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
-      l_run += f[w] * stats[1][w][row];
+      const float mw = stats[0][w][row], Mw = stats[2][w][row];
+      l_run += (mw == m ? 1.0f : __builtin_amdgcn_exp2f(mw - m)) * stats[1][w][row];
+      f[w] = Mw == M ? 1.0f : __builtin_amdgcn_exp2f(Mw - M);
     }
     float o[8] = {};
 #pragma unroll
@@ -694,19 +741,20 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
     }
     if (p.splits > 1) {
       const int64_t place = static_cast<int64_t>(s.unit) * p.rows + s.row0 + row;
-      if (ch == 0) *reinterpret_cast<float2*>(p.part_ml + place * 2) = make_float2(m, l_run);
+      if (ch == 0) *reinterpret_cast<f32x4*>(p.part_ml + place * 4) = f32x4{m, l_run, M, 0.f};
       *reinterpret_cast<f32x4*>(p.part_o + place * D + ch * 8) = f32x4{o[0], o[1], o[2], o[3]};
       *reinterpret_cast<f32x4*>(p.part_o + place * D + ch * 8 + 4) = f32x4{o[4], o[5], o[6], o[7]};
       continue;
     }
-    write_row<E>(p, s, s.row0 + row, ch, o, m, l_run, written);
+    write_row<E>(p, s, s.row0 + row, ch, o, m, M, l_run, written);
   }
 }
 
 // ------------------------------------------------------------------------------------ many rows
 //
 // Bound by what the waves issue: 2 sequences of 8192 keys and 2048 new rows (32 query heads on 8, 128 columns: 481 GF) in
-// 463 us, 1.04 PF (a large product of matrices: 1.21), with the matrix units busy for 47% of the time, the VALU for 51% (a
+// 470 us, 1.02 PF (a large product of matrices: 1.21; 463 with V scales in units of one value for all rows, which lost the
+// values of rows whose scales lie 2^-22 and more below it), with the matrix units busy for 47% of the time, the VALU for 51% (a
 // quarter of it exp2) and LDS for 30%: matrix and vector instructions follow one another.  The clock is 1.8 to 2.0 GHz then.
 // Half a tile's probabilities are computed between the products of the halves around it (620 us without that), and what a
 // tile's groups need is worked out for sixteen tiles at a time.
@@ -793,12 +841,13 @@ struct WideState : fa::FaState<D, Wide<D>::kWaves, 1, F16, true> {
 
   // The probabilities of half kb (s[kb], into pb_out) between the products that wait for nothing of it: the raw scores of
   // the half behind it (into s[1 - kb], of K's stage kK) and, kPv, the values times the probabilities of the half before it
-  // (pb_in, of V's stage kV).  Returns the probabilities' sum.
+  // (pb_in, of V's stage kV).  Returns the sums of the probabilities and of their values.
   template <int kb, bool kPv, int kK, int kV>
-  __device__ __forceinline__ float half(f32x16 (&s)[2], const u32x4 (&pb_in)[2], u32x4 (&pb_out)[2]) {
+  __device__ __forceinline__ typename Softmax<D>::Sums half(f32x16 (&s)[2], const u32x4 (&pb_in)[2], u32x4 (&pb_out)[2]) {
     constexpr int kWin = 3, kPer = 8 / kOps, kEach = kPv ? 3 : 1;  // LDS reads in a round
-    const float ref = st.reference();
-    float rs = 0.f, sum = 0.f;
+    const auto ref = st.reference();
+    typename Softmax<D>::Sums sums{0.f, 0.f};
+    float sum = 0.f;
     u32x4 x[kOps], y[kOps];
 #pragma unroll
     for (int r = 0; r < kWin; ++r) {
@@ -817,7 +866,7 @@ struct WideState : fa::FaState<D, Wide<D>::kWaves, 1, F16, true> {
         const int it = r * kPer + i;
         st.pair(s[kb], kb, it / 4, it % 4, ref, pb_out, sum);
         if (it % 4 == 3) {
-          rs = fmaf(sum, st.undo[kb * 2 + it / 4], rs);
+          st.add_group(sums, ref, kb * 2 + it / 4, sum);
           sum = 0.f;
         }
       }
@@ -832,7 +881,7 @@ struct WideState : fa::FaState<D, Wide<D>::kWaves, 1, F16, true> {
       __builtin_amdgcn_sched_barrier(0);
     }
     s[1 - kb] = next;
-    return rs;
+    return sums;
   }
   // The scores of half kb of a tile alone, and its values times the probabilities.
   __device__ __forceinline__ void scores(const uint8_t* k, int kb, f32x16& s) const {
@@ -889,7 +938,7 @@ __device__ __forceinline__ void wide_step(WideState<D, E, Q>& w, const AttnArgs&
   const int c1 = c == 2 ? 0 : c + 1, c2 = c == 0 ? 2 : c - 1;  // of j + 1, and of j + 2 and j - 1
   if (a.n == kBatch) {
     w.groups.advance(a.n);
-    st.take_ratios(w.groups.vs);
+    st.take_scales(w.groups.vs);
   }
   if (j + 2 < end) w.template store<false>(ring + c2 * T, w.kdst, a.k);
   if (j + 1 < end) {
@@ -925,32 +974,12 @@ __device__ __forceinline__ void wide_step(WideState<D, E, Q>& w, const AttnArgs&
   asm volatile("s_barrier" ::: "memory");
 }
 
-// Largest V scale of keys begin .. end - 1, by the workgroup: to move R as the tiles come would take registers that the tiles'
-// steps do not have.  NaN, and what is not positive, counts as 0.
-template <int kWaves>
-__device__ __forceinline__ float largest_scale(const AttnArgs& p, const kv::Share& s, int begin, int end, int threads,
-                                               float (&waves)[kWaves]) {
-  float top = 0.f;
-  for (int key = begin + static_cast<int>(threadIdx.x) * kGroup; key < end; key += threads * kGroup) {
-    uint32_t page, row;
-    if (!place(p.c, s.b, key, page, row)) continue;
-    top = fmaxf(top, p.c.v_scale[scale_at(p.c, p.c.vss, page, s.head, row)]);
-  }
-  top = wave_max(top);
-  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = top;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) top = fmaxf(top, waves[i]);
-  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, top)));
-}
-
 template <int D, class E, class Q>
 __device__ __forceinline__ void wide_body(const AttnArgs& p) {
   using W = Wide<D>;
   constexpr int kWaves = W::kWaves, T = W::kTile, kThreads = kWaves * 64, kChunks = D / 8;
   constexpr bool kHasNan = __is_same(Q, E4m3);
   __shared__ __attribute__((aligned(256))) uint8_t ring[6 * T];
-  __shared__ float scales[kWaves];
 
   kv::Share s = share_of(p);
   if (!s.live) return;
@@ -992,8 +1021,7 @@ __device__ __forceinline__ void wide_body(const AttnArgs& p) {
     const u32x4 k0 = load_k(0), v0 = load_v(0), k1 = load_k(t1);
     a.k = load_k(t2);
     a.v = load_v(t1);
-    st.R = largest_scale(p, s, begin * BKV, min(end * BKV, seq.len), kThreads, scales);
-    st.take_ratios(w.groups.vs);
+    st.take_scales(w.groups.vs);
     a.n = a.c = 0;  // tile begin in stage 0
     w.template store<false>(ring, w.kdst, k0);
     w.template store<false>(ring + T, w.kdst, k1);
@@ -1031,20 +1059,20 @@ __device__ __forceinline__ void wide_body(const AttnArgs& p) {
     const int row = wave_row + w.col;
     if (row < p.rows) {
       const int64_t place = static_cast<int64_t>(s.unit) * p.rows + row;
-      if (w.h == 0) *reinterpret_cast<float2*>(p.part_ml + place * 2) = make_float2(st.m, l_run);
+      if (w.h == 0) *reinterpret_cast<f32x4*>(p.part_ml + place * 4) = f32x4{st.m, l_run, st.M, 0.f};
 #pragma unroll
       for (int db = 0; db < D / 32; ++db)
 #pragma unroll
         for (int rq = 0; rq < 4; ++rq) {
           const f32x16& a = st.acc[db];
           *reinterpret_cast<f32x4*>(p.part_o + place * D + db * 32 + rq * 8 + w.h * 4) =
-              f32x4{a[rq * 4] * st.R, a[rq * 4 + 1] * st.R, a[rq * 4 + 2] * st.R, a[rq * 4 + 3] * st.R};
+              f32x4{a[rq * 4], a[rq * 4 + 1], a[rq * 4 + 2], a[rq * 4 + 3]};
         }
     }
     return;
   }
   // rows of the block through the rings: 64 rows per stage
-  const float inv = kv::inverse_sum(l_run) * st.R;
+  const Result result(st.m, st.M, l_run);
   {
     const int brow = w.wave * 32 + w.col;
     uint8_t* os = ring + (brow >> 6) * T;
@@ -1054,8 +1082,8 @@ __device__ __forceinline__ void wide_body(const AttnArgs& p) {
       for (int rq = 0; rq < 4; ++rq) {
         const f32x16& a = st.acc[db];
         u32x2 x;
-        x[0] = E::pack(a[rq * 4] * inv, a[rq * 4 + 1] * inv);
-        x[1] = E::pack(a[rq * 4 + 2] * inv, a[rq * 4 + 3] * inv);
+        x[0] = E::pack(result.of(a[rq * 4]), result.of(a[rq * 4 + 1]));
+        x[1] = E::pack(result.of(a[rq * 4 + 2]), result.of(a[rq * 4 + 3]));
         *reinterpret_cast<u32x2*>(os + fa::k_off<D>(brow & 63, db * 4 + rq) + w.h * 8) = x;
       }
     int64_t o_at, lse_at;
@@ -1075,7 +1103,7 @@ __device__ __forceinline__ void wide_body(const AttnArgs& p) {
   }
 }
 
-// Adds up the splits of a row, relative to the largest reference point.
+// Adds up the splits of a row, relative to the largest reference points.
 template <int D, class E>
 __device__ __forceinline__ void join_body(const AttnArgs& p) {
   const kv::JoinLanes<D> at(blockIdx.x, p.join_groups);
@@ -1090,18 +1118,19 @@ __device__ __forceinline__ void join_body(const AttnArgs& p) {
   if (!out_row(p, s, row, written, o_at, lse_at)) return;  // all lanes of the row
   const int64_t first = static_cast<int64_t>(s.b) * p.splits * p.c.kv_heads + s.head;  // unit of split 0
   // each group of lanes its splits, against the largest so far, then the groups
-  float m = -INFINITY, l_run = 0.f, o[8] = {};
+  float m = -INFINITY, M = -INFINITY, l_run = 0.f, o[8] = {};
 #pragma unroll 4
   for (int k = at.group; k < p.splits; k += at.groups) {
     const int64_t part = (first + static_cast<int64_t>(k) * p.c.kv_heads) * p.rows + row;
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + part * 2);
+    const f32x4 ml = *reinterpret_cast<const f32x4*>(p.part_ml + part * 4);
     const f32x4 lo = *reinterpret_cast<const f32x4*>(p.part_o + part * D + at.ch * 8);
     const f32x4 hi = *reinterpret_cast<const f32x4*>(p.part_o + part * D + at.ch * 8 + 4);
-    const float top = fmaxf(m, ml.x);
-    const float before = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-    const float f = ml.x == top ? 1.0f : __builtin_amdgcn_exp2f(ml.x - top);
+    const auto weight = [](float x, float top) { return x == top ? 1.0f : __builtin_amdgcn_exp2f(x - top); };
+    const float top = fmaxf(m, ml[0]), top_v = fmaxf(M, ml[2]);
+    l_run = l_run * weight(m, top) + weight(ml[0], top) * ml[1];
+    const float before = weight(M, top_v), f = weight(ml[2], top_v);
     m = top;
-    l_run = l_run * before + f * ml.y;
+    M = top_v;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       o[e] = fmaf(f, lo[e], o[e] * before);
@@ -1109,14 +1138,16 @@ __device__ __forceinline__ void join_body(const AttnArgs& p) {
     }
   }
   const auto sum = [](float a, float b) { return a + b; };
-  const float top = at.reduce(m, [](float a, float b) { return fmaxf(a, b); });
-  const float f = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+  const auto most = [](float a, float b) { return fmaxf(a, b); };
+  const float top = at.reduce(m, most), top_v = at.reduce(M, most);
+  l_run = at.reduce(l_run * (m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top)), sum);
+  const float f = M == top_v ? 1.0f : __builtin_amdgcn_exp2f(M - top_v);
   m = top;
-  l_run = at.reduce(l_run * f, sum);
+  M = top_v;
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = at.reduce(o[e] * f, sum);
   if (at.group != 0) return;
-  write_row<E>(p, s, row, at.ch, o, m, l_run, written);
+  write_row<E>(p, s, row, at.ch, o, m, M, l_run, written);
 }
 
 }  // namespace c8

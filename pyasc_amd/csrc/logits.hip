@@ -6,6 +6,7 @@
 // whole history is read for every slice, from L2 after the first.  HBM bounds large calls: 64 rows of 131072 fp32
 // logits with masks: 70.7 MB in 14.1 us (5.0 TB/s), in 16 to 17.3 us with 8000 tokens of history; the launch small ones (4 us).
 #include "common.h"
+#include "logits_slices.h"
 #include "numeric.h"
 #include "overlap.h"
 
@@ -86,7 +87,9 @@ __global__ void __launch_bounds__(kThreads) process_logits(LogitsArgs p) {
   const S* x = static_cast<const S*>(p.logits) + row * p.logits_stride;
   S* y = static_cast<S*>(p.out) + row * p.out_stride;
   const int lead = kVec ? static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(S)) : 0;
-  const int first = static_cast<int>(slice) * kSlice - lead;  // token of counts[0]
+  const int first = asc::slice_first(static_cast<int>(slice), kSlice, lead);  // token of counts[0]
+  const uint32_t here = asc::slice_places(first, kSlice, p.vocab);
+  if (here == 0) return;  // all of the workgroup
   // vectors that lie in the row are taken whole; `some`, the row's first, is read in place of the others
   const int some = lead == 0 ? 0 : V - lead;
   const bool vectors = kVec && some + V <= p.vocab;
@@ -105,7 +108,6 @@ __global__ void __launch_bounds__(kThreads) process_logits(LogitsArgs p) {
     reinterpret_cast<u32x4*>(counts)[tid + i * kThreads] = u32x4{0, 0, 0, 0};
   }
   __syncthreads();
-  const uint32_t here = min(kSlice, p.vocab - first);
   const auto count = [&](int i, uint32_t token) {
     // what is counted before the row's first token is looked at by nobody
     const uint32_t at = token - static_cast<uint32_t>(first);
@@ -267,9 +269,9 @@ extern "C" int32_t asc_process_logits(const asc_logits_t* a, asc_stream_t stream
   p.width = static_cast<int32_t>(a->history_width);
   // room for the lead of rows that do not begin at 16 bytes
   const bool aligned = asc::aligned16(a->logits) && (a->rows == 1 || a->logits_stride * size % 16 == 0);
-  const int64_t tokens = a->vocab + (aligned ? 0 : 16 / size - 1);
-  const bool small = a->rows * asc::ceil_div(tokens, kLarge) < kFewGroups && a->history_width <= kLongHistory;
-  p.slices = static_cast<int32_t>(asc::ceil_div(tokens, small ? kSmall : kLarge));
+  const auto slices = [&](int of) { return asc::slices_of(a->vocab, of, static_cast<int>(size), aligned); };
+  const bool small = a->rows * slices(kLarge) < kFewGroups && a->history_width <= kLongHistory;
+  p.slices = static_cast<int32_t>(slices(small ? kSmall : kLarge));
   ASC_REQUIRE(a->rows * p.slices < int64_t{1} << 22, ASC_ERR_UNSUPPORTED, "%s: %lld workgroups exceed the launch grid limit",
               what, static_cast<long long>(a->rows * p.slices));
   const uintptr_t apart = reinterpret_cast<uintptr_t>(a->logits) ^ reinterpret_cast<uintptr_t>(a->out);

@@ -574,7 +574,7 @@ int32_t asc_cross_attention_bwd(const asc_attention_t* args, void* workspace,
  *     gets s, and its rows become round(c s_old / s).  Rounded to nearest, ties to even; an
  *     infinity becomes the largest code, NaN the NaN of e4m3 or 0.  A held scale that is
  *     not positive and finite counts as 0.  A sequence whose lengths do not fit the cache, and a block
- *     whose page lies outside it, stay as they are.
+ *     whose page lies outside it, stay as they are.  scale_block: below 2^33 / head_dim.
  * asc_quantized_cache_read    k_new[b][.][i], v_new[b][.][i] = the values of key lengths[b] +
  *     i for i < n, or new_lengths[b]; rows behind these are left as they were.  A sequence
  *     whose lengths do not fit the cache, and a key whose page lies outside it, give NaN.

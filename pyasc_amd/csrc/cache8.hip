@@ -251,6 +251,9 @@ int32_t make(const asc_cache8_t* a, bool reads, const char* what, Launch& L) {
   ASC_REQUIRE(a->dtype == ASC_DT_FLOAT16 || a->dtype == ASC_DT_BFLOAT16 || wide, ASC_ERR_UNSUPPORTED,
               "%s: dtype %d not supported", what, a->dtype);
   if (a->batch == 0 || a->kv_heads == 0 || a->n == 0) return ASC_OK;
+  // a block's vectors of eight values and a step of a workgroup behind them are numbered in 32 bits
+  ASC_REQUIRE(reads || static_cast<int64_t>(a->scale_block) * (a->head_dim / 8) < int64_t{1} << 30, ASC_ERR_UNSUPPORTED,
+              "%s: scale_block %d is too large (below 2^27 rows of 64 values, 2^26 of 128)", what, a->scale_block);
   ASC_REQUIRE(reads ? a->k_new.data || a->v_new.data : a->k_new.data && a->v_new.data, ASC_ERR_INVALID_ARG,
               "%s: null buffer", what);
   const int64_t element = wide ? 4 : 2;

@@ -1110,7 +1110,7 @@ def quantized_cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tens
       page block_table[b, j // page_size], row j % page_size.  cache_lengths (int32 [batch]): keys
       before the call; token i becomes key cache_lengths[b] + i.
     - k_scales, v_scales: float32 [pages, kv_heads, blocks], one for each block of page_size / blocks rows
-      (a multiple of 16) and head; a code stands for itself times its block's scale.
+      (a multiple of 16, below 2^33 / head_dim) and head; a code stands for itself times its block's scale.
 
     A block gets the least power of two (at least 2^-126) that holds its new rows' finite values, or keeps its
     scale where that is enough; where earlier rows' scale has to grow, their codes are rounded

@@ -84,6 +84,19 @@ def test_cache_refusals_of_one_entry():
             assert entry(ctypes.byref(cache8(**kw)), None) == 0
 
 
+@pytest.mark.parametrize("head_dim,most", [(64, 1 << 27), (128, 1 << 26)])
+def test_blocks_whose_vectors_do_not_fit_32_bits(head_dim, most):
+    """An append numbers a block's vectors of eight values: 2^28 rows of 128 codes are -2^31 of them."""
+    bad = Rows(AT + 8, 640, 320, 64)
+    for rows in (1 << 28, most, most - 16):
+        row, scale = Rows(1 << 40, rows * head_dim, rows * head_dim, head_dim), Rows(AT, 1, 1, 1)
+        a = cache8(head_dim=head_dim, block_table=None, batch=1, kv_heads=1, kv_len=rows, scale_block=rows, k=row, v=row, k_scales=scale,
+                   v_scales=scale, k_new=bad, v_new=bad)  # refused all the same
+        code = _native.load_library().asc_quantized_cache_append(ctypes.byref(a), None)
+        assert code == (UNSUPPORTED if rows >= most else ALIGNMENT)
+        assert ("scale_block" in _native.last_error()) == (rows >= most)
+
+
 @pytest.mark.parametrize("entry,kw,names", [
     ("asc_quantized_cache_append", {"k_new": Rows(AT + 64, 640, 320, 64)}, "'k_new' overlaps 'k'"),
     ("asc_quantized_cache_append", {"v_new": Rows(AT + 2 * FAR, 640, 320, 64)}, "'v_new' overlaps 'k_scales'"),

@@ -484,7 +484,9 @@ int32_t make_copy(const asc_pages_t& a, int64_t moves, bool within, bool partial
     t.bytes = x.heads * x.rows * x.row_bytes;
     t.flat = !partial && (heads_outside || rows_outside);
     const int64_t pieces = t.flat ? asc::ceil_div(t.bytes, kPiece) : x.heads;
-    ASC_REQUIRE(t.bytes < int64_t{1} << 40 && pieces < 1 << 24 && (t.flat || x.rows * x.row_bytes < int64_t{1} << 31),
+    // copy_run numbers a head's bytes, and a step of its threads behind them, in 31 bits
+    ASC_REQUIRE(t.bytes < int64_t{1} << 40 && pieces < 1 << 24 &&
+                    (t.flat || x.rows * x.row_bytes <= (int64_t{1} << 31) - 2 * kThreads),
                 ASC_ERR_UNSUPPORTED, "%s: pages too large", what);
     t.pieces = static_cast<int32_t>(pieces);
     per_move += t.pieces;

@@ -180,6 +180,15 @@ def test_pages_whose_heads_are_too_large():
     assert call("asc_cache_copy_pages", pages(tensor=t)) == UNSUPPORTED and "too large" in _native.last_error()
 
 
+def test_pages_whose_heads_end_next_to_2_gib():
+    """A workgroup's numbers of a head's bytes and a step behind them fit 31 bits: 512 bytes less than 2^31 do, rows of odd ones."""
+    for rows, row_bytes, refused in ((4, (1 << 29) - 1, True), (3, 715827713, True), (3, 715827711, False)):
+        t = _native.PageTensor(1 << 44, 1 << 45, 1 << 34, 1 << 34, 2, rows, row_bytes, 1 << 33, row_bytes)
+        code = call("asc_cache_copy_pages", pages(tensor=t, from_pages=None))  # refused all the same
+        assert code == (UNSUPPORTED if refused else INVALID)
+        assert ("too large" in _native.last_error()) == refused
+
+
 def test_pages_refusals_of_one_entry():
     assert call("asc_cache_fork", pages(parents=None)) == INVALID
     assert call("asc_cache_fork", pages(lengths_out=None)) == INVALID

@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(kWaves * 64) append(RowsArgs p) {
   }
   if (old > 0 && grows) {
     __syncthreads();  // all have read the scale
+    const float ratio = before / scale;  // by a power of two; a code times `before` may lie outside fp32
     for (int vec = threadIdx.x; vec < first_vec; vec += kThreads) {
       u32x2* at = reinterpret_cast<u32x2*>(codes + (vec / kPerRow) * row_bytes + vec % kPerRow * 8);
       u32x2 w = *at;
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(kWaves * 64) append(RowsArgs p) {
       for (int half = 0; half < 2; ++half) {
         float q[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) q[e] = in_range(Q::value(w[half], e) * before / scale);
+        for (int e = 0; e < 4; ++e) q[e] = in_range(Q::value(w[half], e) * ratio);
         w[half] = Q::pack(q, 1.0f);
       }
       *at = w;

@@ -142,6 +142,28 @@ def test_held_scales(device, cache, held):
         assert ((got >= torch.minimum(*ends)) & (got <= torch.maximum(*ends))).all()
 
 
+@pytest.mark.parametrize("cache,held", [(torch.int8, 1.5 * 2.0 ** 121), (torch.float8_e4m3fn, 1.75 * 2.0 ** 119)] + [
+    (c, x) for c in FORMATS for x in (1.5 * 2.0 ** 100, 1.5 * 2.0 ** -126, 2.0 ** -140, 1.5 * 2.0 ** -127)])
+def test_codes_are_rescaled_next_to_the_ends_of_fp32(device, cache, held):
+    """Earlier codes times a held scale lie outside fp32, the codes that they become do not: exact products, whose quotients by a
+    power of two are rounded once."""
+    g = torch.Generator(device=device).manual_seed(11)
+    k, v, ks, vs = make(1, 1, 16, 64, 16, cache, g)
+    ks[:], vs[:] = held, held
+    # a largest value that takes a larger scale
+    largest = torch.finfo(torch.bfloat16).max if held > 2.0 ** 110 else (held * 1000 if held > 1 else 2.0 ** -114)
+    x = torch.rand((1, 1, 2, 64), generator=g, device=device).double() * 2 - 1
+    x[0, 0, 0, 0] = 1.0
+    x = (x * largest).bfloat16()
+    ref = [(R.Codes(t), s.double().cpu()) for t, s in ((k, ks), (v, vs))]
+    length = torch.tensor([9], dtype=torch.int32, device=device)
+    kernels.quantized_cache_append(x, x, k, v, ks, vs, length)
+    for (codes, scales), cache_, scales_ in zip(ref, (k, v), (ks, vs)):
+        R.append(x.cpu(), codes, scales, [9], [2], R.Paged(None, 16), 16)
+        assert float(scales[0, 0, 0]) > held
+        assert torch.equal(scales_.double().cpu(), scales) and same(cache_, codes.codes)
+
+
 def test_bad_lengths_and_pages_are_not_followed(device):
     g = torch.Generator(device=device).manual_seed(8)
     state = make(20, 1, 16, 64, 16, torch.int8, g)

@@ -152,7 +152,7 @@ int32_t make(const asc_cache8_t* a, const char* what, Launch& L) {
   p.group = static_cast<int32_t>(a->q_heads / a->kv_heads);
   p.rows = p.group * p.c.n;
   p.causal = a->causal != 0;
-  p.scale_log2 = a->sm_scale * 1.4426950408889634f;
+  p.scale_mantissa = static_cast<float>(std::frexp(a->sm_scale * 1.4426950408889634, &p.scale_power));
   plan(L, *a);
   ASC_REQUIRE(L.blocks < int64_t{1} << 22, ASC_ERR_UNSUPPORTED, "%s: %lld workgroups exceed the launch grid limit", what,
               static_cast<long long>(L.blocks));

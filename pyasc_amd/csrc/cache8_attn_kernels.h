@@ -47,7 +47,10 @@ struct AttnArgs {
   int32_t lanes, per_lane;  // of the order of the row blocks
   uint32_t units;  // batch * splits * kv_heads
   Divisor by_n, by_heads, by_splits, by_slots, by_lanes;
-  float scale_log2;
+  // sm_scale log2(e) as a mantissa, which goes into K's scales, and a power of two, which goes with the queries': neither product
+  // leaves fp32 where the scores do not.
+  float scale_mantissa;
+  int32_t scale_power;
 
   // Tiles of a split of `total` tiles: the last splits may have none.
   __device__ __forceinline__ int per(int total) const { return static_cast<int>(by_splits.divide(total + splits - 1)); }
@@ -151,13 +154,13 @@ __device__ __forceinline__ int load_query(const AttnArgs& p, const kv::Share& s,
   }
   return row < p.rows ? query : -1;
 }
-// The keys that it attends (a row without a query restricts nothing), its elements in fp16 and its scores' factor.
+// The keys that it attends (a row without a query restricts nothing), its elements in fp16 and its scores' power of two.
 template <int D, class E>
 __device__ __forceinline__ void take_query(const AttnArgs& p, const Sequence& seq, int query, u32x4 (&q)[D / 16], int& limit,
-                                           float& factor) {
+                                           int& power) {
   const bool any = query >= 0 && query < seq.news;
   limit = any ? seq.limit(query) : seq.len;
-  factor = p.scale_log2;
+  power = p.scale_power;
 #pragma unroll
   for (int k = 0; k < D / 16; ++k) q[k] = any ? q[k] : u32x4{0, 0, 0, 0};
   if constexpr (__is_same(E, fa::Bf16)) {
@@ -171,7 +174,7 @@ __device__ __forceinline__ void take_query(const AttnArgs& p, const Sequence& se
     const uint32_t exponent = max(most >> 7, 14u);
     const int up = exponent == 255 ? 0 : 141 - static_cast<int>(exponent);
     const float scale = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-    factor = ldexpf(p.scale_log2, -up);
+    power -= up;
 #pragma unroll
     for (int k = 0; k < D / 16; ++k)
 #pragma unroll
@@ -193,7 +196,7 @@ struct Groups {
   int first;                  // of the current tiles
   bool poison;                // a page or a length outside the cache: the rows' results are NaN
   uint32_t k, v;              // places of the groups' first rows, units of 16 bytes
-  float ks, vs;               // scales, 0 behind the last key
+  float ks, vs;               // scales (K's times scale_mantissa), 0 behind the last key
   uint32_t next_id, next_k, next_v;
   float next_ks, next_vs;
 
@@ -231,7 +234,7 @@ struct Groups {
       const uint32_t block = p.c.block.divide(row);
       at_k = k0 + id * p.c.ks.page + row * p.c.ks.row;
       at_v = v0 + id * p.c.vs.page + row * p.c.vs.row;
-      s_k = p.c.k_scale[ks0 + id * p.c.kss.page + block * p.c.kss.row];
+      s_k = p.c.k_scale[ks0 + id * p.c.kss.page + block * p.c.kss.row] * p.scale_mantissa;
       s_v = p.c.v_scale[vs0 + id * p.c.vss.page + block * p.c.vss.row];
     }
     // lane 0 of each four: its tile's first
@@ -279,7 +282,7 @@ struct Softmax {
   f32x16 acc[kDBlocks];  // in units of 2^M
   float m, M;            // reference points (log2): of the scores, and of the scores plus log2 of the V scale
   float l;               // this lane half's sum of the probabilities in units of 2^m
-  float factor;          // of the raw scores of a unit scale (log2)
+  int power;             // of the raw scores, beside K's scales
   int limit;             // keys of the row
   float log_scale;       // of this lane's group: log2 of the V scale
   float a[kGroups];      // of the tile's groups: the factors of their scores,
@@ -304,7 +307,7 @@ struct Softmax {
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       // not zero, which times the -inf of a hidden key would be NaN
-      a[g] = fmaxf(factor * lane(ks, g), 0x1p-126f);
+      a[g] = fmaxf(ldexpf(lane(ks, g), power), 0x1p-126f);
       log_v[g] = lane(log_scale, g);
     }
   }
@@ -644,7 +647,7 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
     t.template load<false>(p, groups, 0);
     t.template load<true>(p, groups, 0);
   }
-  take_query<D, E>(p, seq, query, q, st.limit, st.factor);
+  take_query<D, E>(p, seq, query, q, st.limit, st.power);
   int least = st.limit;  // keys that all rows attend
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) least = min(least, __shfl_xor(least, d, 64));
@@ -999,7 +1002,7 @@ __device__ __forceinline__ void wide_body(const AttnArgs& p) {
   w.groups.poison = seq.bad;
   Softmax<D>& st = w.st;
   st.init();
-  take_query<D, E>(p, seq, query, w.qreg[0], st.limit, st.factor);
+  take_query<D, E>(p, seq, query, w.qreg[0], st.limit, st.power);
   int least = st.limit;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) least = min(least, __shfl_xor(least, d, 64));

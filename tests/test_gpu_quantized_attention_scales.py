@@ -148,3 +148,15 @@ def test_scales_that_rise_and_fall(device, name, dtype):
         e = -60.0 * (keys if i % 2 else capacity - keys) / capacity
         vs[at_keys(vs, table, i, keys, k.shape[2])] = torch.exp2(e.round()).float()[:, None].expand(-1, vs.shape[1])
     attend(q, (k, v, ks, vs), table, [capacity - 3 * i for i in range(b)])
+
+
+@pytest.mark.parametrize("cache", FORMATS)
+@pytest.mark.parametrize("query,key,scale", [(-118, 120, -10), (-118, -14, 127.75), (110, 0, -110), (-60, 60, -8), (-118, 0, 110)])
+@pytest.mark.parametrize("name", LAUNCHES)
+def test_scores_of_factors_of_any_size(device, name, query, key, scale, cache):
+    """Queries, K scales and a factor of the scores near the ends of fp32, each the power of two that is named, with common scores."""
+    q, (k, v, ks, vs), table, capacity, _ = operands(name, cache, torch.bfloat16, device, 13)
+    b, _, n, _ = q.shape
+    q.copy_((q.double() * 2.0 ** query).bfloat16())
+    ks.copy_((ks.double() / 4 * (1.0 if cache is torch.int8 else 0.5) * 2.0 ** key).float())
+    attend(q, (k, v, ks, vs), table, [capacity - 3 * i for i in range(b)], scale=2.0 ** scale)

@@ -353,18 +353,16 @@ struct Softmax {
 #pragma unroll
     for (int i = 0; i < kDBlocks; ++i) acc[i] *= alpha;
   }
-  // What the probabilities are taken against: -M, and M - m.
+  // What the probabilities are taken against: the reference points, and the least log2 of a V scale that counts.
   struct Reference {
-    float shift, apart;
+    float m, M, least;
   };
   __device__ __forceinline__ Reference reference() const {
-    return m == -INFINITY ? Reference{0.f, 0.f} : Reference{-M, M - m};
+    return m == -INFINITY ? Reference{0.f, 0.f, -kLeast} : Reference{m, M, M - m - kLeast};
   }
-  // The score's shift of group g, and the factor from e_j to p_j.
-  __device__ __forceinline__ float shift_of(const Reference& r, int g) const { return fmaxf(log_v[g], r.apart - kLeast) + r.shift; }
-  __device__ __forceinline__ float undo_of(const Reference& r, int g) const {
-    return __builtin_amdgcn_exp2f(fminf(r.apart - log_v[g], kLeast));
-  }
+  // The scores' shift of group g, and the factor from e_j to p_j.
+  __device__ __forceinline__ float shift_of(const Reference& r, int g) const { return fmaxf(log_v[g], r.least) - r.M; }
+  __device__ __forceinline__ float undo_of(const Reference& r, int g) const { return __builtin_amdgcn_exp2f(-r.m - shift_of(r, g)); }
   // Sums of a lane over a half, or a whole tile: of the probabilities, and of P^T's values.
   struct Sums {
     float p, e;

@@ -586,7 +586,9 @@ int32_t asc_cross_attention_bwd(const asc_attention_t* args, void* workspace,
  *     behind new_lengths[b] are not written, none of a negative number.  A query without
  *     keys gets zeros, and -inf for its lse (fp32 [batch, q_heads, n], may be NULL).  A
  *     length outside the cache, a page outside it that a length reaches, or more
- *     queries than n: NaN.  `workspace` holds _workspace bytes, 16-byte aligned.
+ *     queries than n: NaN.  A key's probability times its V scale is rounded by up to 2^-11 of it, or
+ *     2^-33 of the largest that its query attends, and an element of a bf16 query by up to 2^-39 of
+ *     the query's largest.  `workspace` holds _workspace bytes, 16-byte aligned.
  * A result that shares a byte with an operand or another result is refused. */
 typedef struct asc_cache8 {
   int32_t dtype, cache_dtype; /* of queries, results and new rows; ASC_DT_INT8 or ASC_DT_FLOAT8_E4M3 */

@@ -10,13 +10,14 @@
 // holds, and keys that a row does not attend, or with next to no probability, have no say in it.  exp2 takes log2 vs_j with the
 // scores' shift, and a group's sum of e_j times 2^(M - m) / vs_j is its part of the denominator.  A row's scale that lies 2^-60
 // and more below its 2^(M - m) counts as that: blocks of zeros, with scales of 2^-126, have their share of the denominator.
-// Queries of bf16 are brought to fp16's range by a power of two of their row: exact, but for elements 2^-39 and less of the
-// row's largest.
+// Queries of bf16 are brought to fp16's range by a power of two of their row: exact down to 2^-31 of its largest element, and to
+// 2^-39 of that below.
 //
-// The probabilities are rounded to fp16 for the product with the values, as matrix operands have to be: errors of up to 0.0002
-// of the results' norm, beside 0.0017 of a bf16 result's own rounding.  Beside 0.0002 of an fp16 result's they count where a few
-// keys outweigh the rest (0.0003 in all, one row over 500 keys): the kernel for few rows, whose matrix units wait for the cache,
-// multiplies what the rounding leaves as a second term (0.0002; 8 sequences of up to 32768 keys take 74.6 us for 72.3).
+// The e_j are rounded to fp16 for the product with the values, as matrix operands have to be (2^-11 of each, and below 2^-22 of a
+// row's largest 2^-33 of that): errors of up to 0.0002 of the results' norm, beside 0.0017 of a bf16 result's own rounding.
+// Beside 0.0002 of an fp16 result's they count where a few keys outweigh the rest (0.0003 in all, one row over 500 keys): the
+// kernel for few rows, whose matrix units wait for the cache, multiplies what the rounding leaves as a second term (0.0002; 8
+// sequences of up to 32768 keys take 74.6 us for 72.3).
 #pragma once
 
 #include "cache8.h"
@@ -754,9 +755,10 @@ __device__ __forceinline__ void narrow_body(const AttnArgs& p) {
 // ------------------------------------------------------------------------------------ many rows
 //
 // Bound by what the waves issue: 2 sequences of 8192 keys and 2048 new rows (32 query heads on 8, 128 columns: 481 GF) in
-// 470 us, 1.02 PF (a large product of matrices: 1.21; 463 with V scales in units of one value for all rows, which lost the
-// values of rows whose scales lie 2^-22 and more below it), with the matrix units busy for 47% of the time, the VALU for 51% (a
-// quarter of it exp2) and LDS for 30%: matrix and vector instructions follow one another.  The clock is 1.8 to 2.0 GHz then.
+// 465 to 475 us, 1.02 PF (a large product of matrices: 1.21), with the matrix units busy for 46% of the time, the VALU for 54%
+// (a quarter of it exp2) and LDS for 29%: matrix and vector instructions follow one another, at 1.8 to 2.0 GHz.  With 64 columns
+// a tile has the same exponentials for half of the products: 324 us, matrix units 31%, VALU 67%.  V scales in units of one value
+// for all rows took 457 to 466 and 312 us, and lost the values of rows whose scales lie 2^-22 and more below it.
 // Half a tile's probabilities are computed between the products of the halves around it (620 us without that), and what a
 // tile's groups need is worked out for sixteen tiles at a time.
 

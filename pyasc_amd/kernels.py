@@ -1187,7 +1187,8 @@ def quantized_cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
 
     A query without keys gets zeros and an lse (float32 [batch, heads, n]) of -inf.  A length outside the cache and more
     queries than n are not followed: NaN; a page outside it gives NaN for the queries that attend its keys, and may
-    for others of the sequence."""
+    for others of the sequence.  A key's probability times its V scale is rounded by up to 2^-11 of it, or 2^-33 of
+    the largest that its query attends; float32 otherwise."""
     device = _current_device()
     if not isinstance(q, torch.Tensor):
         raise TypeError(f"'q' must be a torch.Tensor, got {type(q).__name__}")
